@@ -16,12 +16,15 @@
 
 #include "../../include/ccglib_amd.h"
 #include "common.h"
+#include "host_util.h"
 
 using namespace ccglib_amd;
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
+
+namespace ccglib_amd {
 
 int fail(int code, const char *fmt, ...) {
   char buf[512];
@@ -36,33 +39,6 @@ int fail(int code, const char *fmt, ...) {
 int fail_hip(hipError_t e, const char *what) {
   return fail(CCGLIB_ERROR_RUNTIME, "%s: %s", what, hipGetErrorString(e));
 }
-
-#define HIP_TRY(expr)                                   \
-  do {                                                  \
-    hipError_t e_ = (expr);                             \
-    if (e_ != hipSuccess) return fail_hip(e_, #expr);   \
-  } while (0)
-
-// Makes `device` current for the lifetime of the guard.
-class DeviceGuard {
- public:
-  explicit DeviceGuard(int device) {
-    if (hipGetDevice(&previous_) != hipSuccess) previous_ = -1;
-    if (previous_ != device) {
-      status_ = hipSetDevice(device);
-      switched_ = (status_ == hipSuccess);
-    }
-  }
-  ~DeviceGuard() {
-    if (switched_ && previous_ >= 0) (void)hipSetDevice(previous_);
-  }
-  hipError_t status() const { return status_; }
-
- private:
-  int previous_ = -1;
-  bool switched_ = false;
-  hipError_t status_ = hipSuccess;
-};
 
 int check_device(int device) {
   int count = 0;
@@ -80,6 +56,10 @@ int check_device(int device) {
   }
   return CCGLIB_OK;
 }
+
+}  // namespace ccglib_amd
+
+namespace {
 
 bool is_enum01(int v) { return v == 0 || v == 1; }
 

@@ -2145,45 +2145,6 @@ template <int N, bool READS = false> __device__ __forceinline__ void wait_vmcnt_
   }
 }
 
-// Both copy helpers write m0 (the LDS base of the copy) and say so in their
-// clobber lists, so that the compiler never assumes a value it put there
-// survives them; clang warns about any mention of m0 there, which is the point.
-// The compiler does not look into an asm statement for the wait states its
-// instructions need after what it placed in front of it: the scalar base of the
-// first helper may have come out of a vector register right before (a spilled
-// scalar register read back with v_readlane), and a vector memory instruction
-// may read such a register five wait states later at the earliest. The helper
-// therefore hands the base on through a scalar move: the scalar ALU may read the
-// register at once, and what it writes the memory instruction may read at once.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load_1k_to_lds(const char *base, unsigned lane_offset,
-                                               unsigned lds_address) {
-  unsigned long long base_here;
-  asm volatile(
-      "s_mov_b64 %0, %3\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, %0"
-      : "=&s"(base_here)
-      : "s"(lds_address), "v"(lane_offset), "s"(base)
-      : "memory", "m0");
-}
-
-// Same, with a full address per lane (planar layout: the 16 rows of a row block
-// are not contiguous in memory).
-__device__ __forceinline__ void load_1k_to_lds_by_lane(const char *lane_address,
-                                                       unsigned lds_address) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off"
-      :
-      : "s"(lds_address), "v"(lane_address)
-      : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 #include "gemm_mfma_wide.h"
 
 template <int DT, int TOUT, int BX, int BY, int WX, int WY, int SLOTS, int WAVES_PER_EU, int LOADER,
