@@ -8,6 +8,14 @@ error behaviour), bound to the C ABI of libccglib_amd.so:
     ccglib::packing::Packing     -> Packing         (include/ccglib/packing/packing.h:25-54)
     ccglib::pipeline::Pipeline   -> Pipeline        (include/ccglib/pipeline/pipeline.h:28-73)
 
+and, without a counterpart in the reference, real products of 8-bit values with
+block scales and orthogonalised updates:
+
+    ccglib::quantize::Quantize            -> Quantize
+    ccglib::mma::ScaledGEMM               -> ScaledGEMM
+    ccglib::pipeline::ScaledLinear        -> ScaledLinear
+    ccglib::orthogonalize::Orthogonalize  -> Orthogonalize
+
 Device buffers are passed as integer device addresses (e.g. ``tensor.data_ptr()``),
 streams as integer ``hipStream_t`` handles (0 = default stream). Every ``Run``
 only enqueues work on the stream. Errors raise ``RuntimeError`` with the
@@ -20,7 +28,9 @@ import enum
 from . import _capi
 
 __all__ = ["ValueType", "ComplexAxisLocation", "Direction", "MemOrder", "Variant",
-           "Precision", "GEMM", "Transpose", "Packing", "Pipeline", "ceildiv", "version"]
+           "Precision", "GEMM", "Transpose", "Packing", "Pipeline", "ScaleGroup", "ScaleType",
+           "Quantize", "ScaledGEMM", "ScaledLinear", "Orthogonalize", "scaled_pitch", "ceildiv",
+           "version"]
 
 
 class ValueType(enum.IntEnum):          # include/ccglib/common/value_type.h:14-22
@@ -51,6 +61,18 @@ class MemOrder(enum.IntEnum):           # include/ccglib/gemm/mem_order.h:6
 class Variant(enum.IntEnum):            # include/ccglib/gemm/variant.h:6
     basic = 0
     opt = 1
+
+
+class ScaleGroup(enum.IntEnum):
+    """Values of an 8-bit matrix that share a scale: 128 of a row, or 128 x 128."""
+    rows = 0
+    blocks = 1
+
+
+class ScaleType(enum.IntEnum):
+    """A scale is a float32 number, or a power of two in one byte: 2^(byte - 127)."""
+    float32 = 0
+    e8m0 = 1
 
 
 _BITS = {ValueType.int1: 1, ValueType.float8e4m3: 8, ValueType.float8e5m2: 8,
@@ -130,8 +152,10 @@ class _Handle:
 
     def __del__(self):
         h = getattr(self, "_h", None)
-        if h is not None and h.value and _capi is not None and ctypes is not None:
-            getattr(_capi.load(), self._destroy)(h)   # (modules are None at interpreter exit)
+        # (modules, or what they hold, are None at interpreter exit)
+        load = getattr(_capi, "load", None)
+        if h is not None and h.value and load is not None and ctypes is not None:
+            getattr(load(), self._destroy)(h)
             self._h = ctypes.c_void_p()
 
 
@@ -266,3 +290,96 @@ def pipeline_run_static(B, M, N, K, device, stream, input_complex_axis_location,
         int(output_complex_axis_location), int(a_mem_order), int(b_mem_order), int(c_mem_order),
         int(input_precision), int(output_precision), int(variant), alpha.real, alpha.imag,
         beta.real, beta.imag, _ptr(d_a), _ptr(d_b), _ptr(d_c)))
+
+
+def scaled_pitch(n):
+    """Distance in elements of rows of n 8-bit values, and of rows of n scales: n rounded up to 16."""
+    return _capi.load().ccglib_scaled_pitch(n)
+
+
+class Quantize(_Handle):
+    """B matrices of M x N to 8 bits with a scale for each group of 128 values (or 128 x 128):
+    as they are, transposed, or both in one pass (formulas and layout: include/ccglib_amd.h)."""
+    _destroy = "ccglib_quantize_destroy"
+
+    def __init__(self, B, M, N, device, stream, input_type, output_type=ValueType.float8e4m3,
+                 group=ScaleGroup.rows, scale_type=ScaleType.float32, input_pitch=0):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_quantize_create(
+            ctypes.byref(self._h), B, M, N, int(device), _ptr(stream), int(input_type), int(output_type),
+            int(group), int(scale_type), int(input_pitch)))
+
+    def Run(self, d_input, d_output, d_scales, d_output_t=0, d_scales_t=0):
+        """d_output [B][M][pitch(N)], d_scales [B][ceil(N/128)][pitch(M or ceil(M/128))]; the
+        transposes' d_output_t [B][N][pitch(M)], d_scales_t likewise. 0: not wanted."""
+        _capi.check(_capi.load().ccglib_quantize_run(
+            self._h, _ptr(d_input), _ptr(d_output), _ptr(d_scales), _ptr(d_output_t), _ptr(d_scales_t)))
+
+
+class ScaledGEMM(_Handle):
+    """C[b] (+)= A[b] B[b]^T of 8-bit operands with a scale for each group of 128 along K.
+
+    A [B][M][pitch_a], B [B][N][pitch_b], C [B][M][pitch_c]; pitches of 0: scaled_pitch(K), N."""
+    _destroy = "ccglib_scaled_gemm_destroy"
+
+    def __init__(self, B, M, N, K, device, stream, a_type=ValueType.float8e4m3,
+                 b_type=ValueType.float8e4m3, c_type=ValueType.bfloat16, a_group=ScaleGroup.rows,
+                 b_group=ScaleGroup.blocks, scale_type=ScaleType.float32, accumulate=False,
+                 pitch_a=0, pitch_b=0, pitch_c=0):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_scaled_gemm_create(
+            ctypes.byref(self._h), B, M, N, K, int(device), _ptr(stream), int(a_type), int(b_type),
+            int(c_type), int(a_group), int(b_group), int(scale_type), int(bool(accumulate)), int(pitch_a),
+            int(pitch_b), int(pitch_c)))
+
+    def Run(self, d_a, d_scales_a, d_b, d_scales_b, d_c):
+        _capi.check(_capi.load().ccglib_scaled_gemm_run(
+            self._h, _ptr(d_a), _ptr(d_scales_a), _ptr(d_b), _ptr(d_scales_b), _ptr(d_c)))
+
+    def KernelName(self):
+        """Which kernel Run launches."""
+        buf = ctypes.create_string_buffer(160)
+        _capi.check(_capi.load().ccglib_scaled_gemm_kernel_name(self._h, buf, len(buf)))
+        return buf.value.decode()
+
+
+class ScaledLinear(_Handle):
+    """A linear layer, y = x W^T, forward and backward, by products of 8-bit copies that the object
+    makes and keeps. x [M][K], W [N][K], y [M][N] and their gradients dx, dy are of `type`, dW is
+    float32."""
+    _destroy = "ccglib_scaled_linear_destroy"
+
+    def __init__(self, M, N, K, device, stream, type=ValueType.bfloat16,
+                 gradient_type=ValueType.float8e5m2, scale_type=ScaleType.float32, training=True):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_scaled_linear_create(
+            ctypes.byref(self._h), M, N, K, int(device), _ptr(stream), int(type), int(gradient_type),
+            int(scale_type), int(bool(training))))
+
+    def SetWeights(self, d_w):
+        _capi.check(_capi.load().ccglib_scaled_linear_set_weights(self._h, _ptr(d_w)))
+
+    def Forward(self, d_x, d_y):
+        _capi.check(_capi.load().ccglib_scaled_linear_forward(self._h, _ptr(d_x), _ptr(d_y)))
+
+    def Backward(self, d_dy, d_dx, d_dw, accumulate_dw=False):
+        """dx = dy W, dW = dy^T x (or dW += ...), with the x and W of the last Forward; 0: not wanted."""
+        _capi.check(_capi.load().ccglib_scaled_linear_backward(
+            self._h, _ptr(d_dy), _ptr(d_dx), _ptr(d_dw), int(bool(accumulate_dw))))
+
+
+class Orthogonalize(_Handle):
+    """B updates of M x N, each made nearly orthogonal by `steps` Newton-Schulz steps
+    X = a X + (b X X^T + c (X X^T)^2) X from X = G / (|G| + epsilon). d_output may be d_input."""
+    _destroy = "ccglib_orthogonalize_destroy"
+
+    def __init__(self, B, M, N, device, stream, type=ValueType.bfloat16, steps=5,
+                 coefficients=(3.4445, -4.7750, 2.0315), epsilon=1e-7, input_pitch=0, output_pitch=0):
+        super().__init__()
+        a, b, c = coefficients
+        _capi.check(_capi.load().ccglib_orthogonalize_create(
+            ctypes.byref(self._h), B, M, N, int(device), _ptr(stream), int(type), int(steps), float(a),
+            float(b), float(c), float(epsilon), int(input_pitch), int(output_pitch)))
+
+    def Run(self, d_input, d_output):
+        _capi.check(_capi.load().ccglib_orthogonalize_run(self._h, _ptr(d_input), _ptr(d_output)))

@@ -40,6 +40,23 @@ SIGNATURES = {
     "ccglib_pipeline_destroy": (_i, [_vp]),
     "ccglib_pipeline_run_static": (_i, [_sz, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
                                         _f, _f, _f, _f, _vp, _vp, _vp]),
+    "ccglib_scaled_pitch": (_sz, [_sz]),
+    "ccglib_quantize_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i, _sz]),
+    "ccglib_quantize_run": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_quantize_destroy": (_i, [_vp]),
+    "ccglib_scaled_gemm_create": (_i, [_pvp, _sz, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _sz,
+                                       _sz, _sz]),
+    "ccglib_scaled_gemm_run": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_scaled_gemm_kernel_name": (_i, [_vp, ctypes.c_char_p, _sz]),
+    "ccglib_scaled_gemm_destroy": (_i, [_vp]),
+    "ccglib_scaled_linear_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i]),
+    "ccglib_scaled_linear_set_weights": (_i, [_vp, _vp]),
+    "ccglib_scaled_linear_forward": (_i, [_vp, _vp, _vp]),
+    "ccglib_scaled_linear_backward": (_i, [_vp, _vp, _vp, _vp, _i]),
+    "ccglib_scaled_linear_destroy": (_i, [_vp]),
+    "ccglib_orthogonalize_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i, _f, _f, _f, _f, _sz, _sz]),
+    "ccglib_orthogonalize_run": (_i, [_vp, _vp, _vp]),
+    "ccglib_orthogonalize_destroy": (_i, [_vp]),
 }
 
 _lib = None

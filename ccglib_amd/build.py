@@ -5,6 +5,7 @@
 """
 import concurrent.futures
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -16,12 +17,10 @@ LIB_PATH = os.path.join(HERE, "libccglib_amd.so")
 # (gemm_mfma.hip is compiled in parts, one per input type, so that they build in parallel)
 SOURCES = ["capi.hip", "gemm_mfma_f16.hip", "gemm_mfma_bf16.hip", "gemm_mfma_f32.hip",
            "gemm_mfma_fp8.hip", "gemm_mfma_int1.hip", "gemm_mfma_dispatch.hip", "gemm_int1.hip",
-           "transpose.hip", "packing.hip", "host_copy.hip"]
-HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_device.h"),
-           os.path.join(CSRC, "gemm_mfma.hip"), os.path.join(CSRC, "gemm_mfma_wide.h"),
-           os.path.join(CSRC, "gemm_mfma_wave.h"),
-           os.path.join(os.path.dirname(HERE), "include", "ccglib_amd.h")]
-
+           "transpose.hip", "packing.hip", "host_copy.hip", "quantize.hip", "scaled_gemm.hip",
+           "scaled_gemm_blocks.hip", "scaled_gemm_rows.hip", "scaled_gemm_e8m0.hip",
+           "scaled_gemm_wide_blocks.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_e8m0.hip",
+           "orthogonalize.hip", "operators_capi.hip"]
 # Packed-fp32 instruction selection is switched off for all device code.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
@@ -48,10 +47,21 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _with_includes(path, found=None):
+    """The source and every file of this tree that it includes, directly or not."""
+    found = [] if found is None else found
+    if path not in found and os.path.exists(path):
+        found.append(path)
+        with open(path) as f:
+            for name in re.findall(r'^#include "([^"]+)"', f.read(), re.M):
+                _with_includes(os.path.normpath(os.path.join(os.path.dirname(path), name)), found)
+    return found
+
+
 def _compile(src, force):
     obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
     path = os.path.join(CSRC, src)
-    if not force and not _stale(obj, [path] + HEADERS):
+    if not force and not _stale(obj, _with_includes(path)):
         return obj, ""
     cmd = [_hipcc()] + HIPCC_FLAGS + _defines() + ["-Rpass-analysis=kernel-resource-usage", "-c", path,
                                                    "-o", obj]
@@ -83,14 +93,15 @@ def _no_scratch_in_gemm_kernels(src, remarks):
     ones of ragged 16-bit pairs two or three, and reload them where a block moves
     to its next C tile (the compiler waits for all memory operations there), and those of 32-bit pairs
     to 16-bit C one address while they look for NaN behind the K loop; anything beyond
-    those few bytes stops the build as well."""
+    those few bytes stops the build as well. The real products (gemm_real) count their copies too
+    and must not spill."""
     name = None
     for l in remarks:
         if "Function Name:" in l:
             name = l.split("Function Name:")[1].split("[")[0].strip()
-        elif "ScratchSize [bytes/lane]:" in l and name and "complex_gemm_mfma" in name:
+        elif "ScratchSize [bytes/lane]:" in l and name and ("complex_gemm_mfma" in name or "gemm_real" in name):
             size = int(l.split("ScratchSize [bytes/lane]:")[1].split("[")[0])
-            if size > (0 if "complex_gemm_mfma_wide" in name else 32):
+            if size > (0 if "complex_gemm_mfma_wide" in name or "gemm_real" in name else 32):
                 os.remove(os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o"))
                 raise RuntimeError("%s: kernel %s spills %d bytes per lane to scratch memory; its "
                                    "explicit vmcnt counts would not hold" % (src, name, size))

@@ -1,0 +1,535 @@
+// C ABI of the operators on 8-bit values with block scales and of the orthogonalised updates (declared in
+// include/ccglib_amd.h): argument checking, object state and workspaces around the kernel launchers. None of them has a
+// counterpart in the reference.
+#include <cstdio>
+#include <cstring>
+#include <new>
+
+#include "host_util.h"
+#include "scaled.h"
+
+using namespace ccglib_amd;
+
+namespace {
+
+constexpr size_t kMostRows = 0x7fffffffu;     // rows, and values of a row, of any matrix here
+constexpr size_t kMostPitch = (size_t)1 << 23;  // bytes: 256 rows are addressed with 32-bit offsets
+constexpr size_t kMostBlocks = 0x7fffffffu;
+
+// Device memory of an object.
+struct Buffer {
+  void *p = nullptr;
+  ~Buffer() {
+    if (p) (void)hipFree(p);
+  }
+  char *at(size_t offset) const { return static_cast<char *>(p) + offset; }
+};
+
+bool is_group(int g) { return g == kScaleRows || g == kScaleBlocks; }
+bool is_scale(int s) { return s == kScaleFloat32 || s == kScaleE8m0; }
+size_t scale_size(int s) { return s == kScaleE8m0 ? 1 : 4; }
+bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
+
+// Allocates `bytes` and clears the first `zeroed`; the memory is cleared when the call returns.
+int allocate(Buffer *b, size_t bytes, size_t zeroed) {
+  if (bytes == 0) return CCGLIB_OK;
+  HIP_TRY(hipMalloc(&b->p, bytes));
+  if (zeroed) {
+    HIP_TRY(hipMemset(b->p, 0, zeroed));
+    HIP_TRY(hipStreamSynchronize(nullptr));
+  }
+  return CCGLIB_OK;
+}
+
+int check_quantize(const QuantizeParams &p, size_t B, size_t M, size_t N) {
+  if (!is_wide_float(p.type_in)) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "Quantize: input is float32, float16 or bfloat16 (type %d)", p.type_in);
+  }
+  if (!is_float8(p.type_out)) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "Quantize: output is float8e4m3 or float8e5m2 (type %d)", p.type_out);
+  }
+  if (!is_group(p.group) || !is_scale(p.scale_type)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "enum argument out of range");
+  }
+  if (B > kMostRows || M > kMostRows || N > kMostRows) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  if (p.in_pitch < N) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Quantize: rows of %zu values at a distance of %zu", N, p.in_pitch);
+  // (groups, and rows of all matrices, are counted in 32 bits)
+  if (B && M && N && (ceil_div(M, 16) > kMostBlocks / B / ceil_div(N, kScaleGroup) || M > 0xffffffffu / B / ceil_div(N, kScaleGroup))) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  }
+  return CCGLIB_OK;
+}
+
+int check_gemm(const ScaledGemmParams &p, size_t B, size_t M, size_t N, size_t K) {
+  if (!is_float8(p.type_a) || !is_float8(p.type_b)) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "ScaledGEMM: operands are float8e4m3 or float8e5m2 (types %d, %d)", p.type_a, p.type_b);
+  }
+  if (!is_wide_float(p.type_c)) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "ScaledGEMM: C is float32, float16 or bfloat16 (type %d)", p.type_c);
+  }
+  if (p.accumulate && p.type_c != kFloat32) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "ScaledGEMM: C that is added to is float32 (type %d)", p.type_c);
+  }
+  if (!is_group(p.group_a) || !is_group(p.group_b) || !is_scale(p.scale_type)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "enum argument out of range");
+  }
+  if (B > kMostRows || M > kMostRows || N > kMostRows || K > kMostPitch) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  }
+  const size_t least = scaled_pitch(K);
+  if (p.pitch_a < least || p.pitch_b < least || p.pitch_a % kScaledPad || p.pitch_b % kScaledPad || p.pitch_a > kMostPitch ||
+      p.pitch_b > kMostPitch) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT,
+                "ScaledGEMM: rows of A and B lie a multiple of %zu bytes apart, %zu to %zu for this K (got %zu, %zu)", kScaledPad,
+                least, kMostPitch, p.pitch_a, p.pitch_b);
+  }
+  if (p.pitch_c < N) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledGEMM: rows of C of %zu values at a distance of %zu", N, p.pitch_c);
+  // (blocks of C times pieces of K, each at least 16 x 64 values, are counted in 32 bits)
+  if (B && M && N && ceil_div(M, 16) > kMostBlocks / 64 / B / ceil_div(N, 64)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  }
+  return CCGLIB_OK;
+}
+
+int check_operand(const char *what, const void *values, const void *scales, int scale_type) {
+  if (!values || !scales) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: %s", what);
+  if (!aligned(values, 16)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "%s: 8-bit values start at a multiple of 16 bytes", what);
+  if (!aligned(scales, scale_size(scale_type))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "%s: misaligned scales", what);
+  return CCGLIB_OK;
+}
+
+size_t element(int type) { return (size_t)bits_of(type) / 8; }
+
+// Allocates what a planned product needs: counters (cleared), then partial sums.
+size_t gemm_workspace(const RealGemmPlan &plan) {
+  return plan.parts > 1 ? ceil_div(plan.counter_bytes, 256) * 256 + plan.partial_bytes : 0;
+}
+
+}  // namespace
+
+struct ccglib_quantize {
+  QuantizeParams p;
+  int device;
+  hipStream_t stream;
+};
+
+struct ccglib_scaled_gemm {
+  ScaledGemmParams p;
+  int device;
+  hipStream_t stream;
+  Buffer workspace;
+};
+
+struct ccglib_scaled_linear {
+  size_t M, N, K;
+  int type, scale_type, device;
+  bool training, have_weights = false, have_forward = false;
+  hipStream_t stream;
+  QuantizeParams x, w, dy;
+  ScaledGemmParams y, dx, dw;
+  Buffer memory;
+};
+
+struct ccglib_orthogonalize {
+  OrthogonalizeParams p;
+  int device;
+  hipStream_t stream;
+  Buffer workspace;
+};
+
+extern "C" {
+
+size_t ccglib_scaled_pitch(size_t n) { return scaled_pitch(n); }
+
+// ---- Quantize ----
+
+int ccglib_quantize_create(ccglib_quantize_t *quantize, size_t B, size_t M, size_t N, int device, void *stream, int type_in,
+                           int type_out, int group, int scale_type, size_t in_pitch) {
+  if (!quantize) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: quantize");
+  *quantize = nullptr;
+  QuantizeParams p = {};
+  p.batch = (unsigned)B;
+  p.m = (unsigned)M;
+  p.n = (unsigned)N;
+  p.in_pitch = in_pitch ? in_pitch : N;
+  p.type_in = type_in;
+  p.type_out = type_out;
+  p.group = group;
+  p.scale_type = scale_type;
+  if (int s = check_quantize(p, B, M, N)) return s;
+  if (int s = check_device(device)) return s;
+  auto *q = new (std::nothrow) ccglib_quantize{p, device, static_cast<hipStream_t>(stream)};
+  if (!q) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
+  *quantize = q;
+  return CCGLIB_OK;
+}
+
+int ccglib_quantize_run(ccglib_quantize_t q, const void *d_in, void *d_out, void *d_scales, void *d_out_t, void *d_scales_t) {
+  if (!q) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  QuantizeParams p = q->p;
+  if (p.batch == 0 || p.m == 0 || p.n == 0) return CCGLIB_OK;
+  if (!d_in) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: input");
+  if (!d_out && !d_out_t) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: output");
+  if (!aligned(d_in, element(p.type_in))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Quantize: misaligned input");
+  if (d_out || d_scales) {
+    if (int s = check_operand("Quantize, output", d_out, d_scales, p.scale_type)) return s;
+  }
+  if (d_out_t || d_scales_t) {
+    if (int s = check_operand("Quantize, transposed output", d_out_t, d_scales_t, p.scale_type)) return s;
+  }
+  p.in = d_in;
+  p.out = d_out;
+  p.scales = d_scales;
+  p.out_t = d_out_t;
+  p.scales_t = d_scales_t;
+  DeviceGuard guard(q->device);
+  HIP_TRY(guard.status());
+  HIP_TRY(launch_quantize(p, q->stream));
+  return CCGLIB_OK;
+}
+
+int ccglib_quantize_destroy(ccglib_quantize_t q) {
+  delete q;
+  return CCGLIB_OK;
+}
+
+// ---- ScaledGEMM ----
+
+int ccglib_scaled_gemm_create(ccglib_scaled_gemm_t *gemm, size_t B, size_t M, size_t N, size_t K, int device, void *stream,
+                              int type_a, int type_b, int type_c, int group_a, int group_b, int scale_type, int accumulate,
+                              size_t pitch_a, size_t pitch_b, size_t pitch_c) {
+  if (!gemm) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: gemm");
+  *gemm = nullptr;
+  ScaledGemmParams p = {};
+  p.batch = (unsigned)B;
+  p.m = (unsigned)M;
+  p.n = (unsigned)N;
+  p.k = (unsigned)K;
+  p.pitch_a = pitch_a ? pitch_a : scaled_pitch(K);
+  p.pitch_b = pitch_b ? pitch_b : scaled_pitch(K);
+  p.pitch_c = pitch_c ? pitch_c : N;
+  p.type_a = type_a;
+  p.type_b = type_b;
+  p.type_c = type_c;
+  p.group_a = group_a;
+  p.group_b = group_b;
+  p.scale_type = scale_type;
+  p.accumulate = accumulate != 0;
+  if (int s = check_gemm(p, B, M, N, K)) return s;
+  if (int s = check_device(device)) return s;
+  DeviceGuard guard(device);
+  HIP_TRY(guard.status());
+  p.plan = plan_scaled_gemm(p);
+  auto *g = new (std::nothrow) ccglib_scaled_gemm{p, device, static_cast<hipStream_t>(stream), {}};
+  if (!g) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
+  if (int s = allocate(&g->workspace, gemm_workspace(p.plan), p.plan.counter_bytes)) {
+    delete g;
+    return s;
+  }
+  g->p.workspace = g->workspace.p;
+  *gemm = g;
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_gemm_run(ccglib_scaled_gemm_t g, const void *d_a, const void *d_scales_a, const void *d_b,
+                           const void *d_scales_b, void *d_c) {
+  if (!g) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  ScaledGemmParams p = g->p;
+  if (p.batch == 0 || p.m == 0 || p.n == 0) return CCGLIB_OK;
+  if (p.k > 0) {
+    if (int s = check_operand("ScaledGEMM, A", d_a, d_scales_a, p.scale_type)) return s;
+    if (int s = check_operand("ScaledGEMM, B", d_b, d_scales_b, p.scale_type)) return s;
+  }
+  if (!d_c) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: ScaledGEMM, C");
+  if (!aligned(d_c, element(p.type_c))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledGEMM: misaligned C");
+  p.a = d_a;
+  p.b = d_b;
+  p.scales_a = d_scales_a;
+  p.scales_b = d_scales_b;
+  p.c = d_c;
+  DeviceGuard guard(g->device);
+  HIP_TRY(guard.status());
+  HIP_TRY(launch_scaled_gemm(p, g->stream));
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_gemm_kernel_name(ccglib_scaled_gemm_t g, char *buffer, size_t size) {
+  if (!g || !buffer || size == 0) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle or buffer");
+  snprintf(buffer, size, "%s", describe_scaled_gemm(g->p));
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_gemm_destroy(ccglib_scaled_gemm_t g) {
+  if (!g) return CCGLIB_OK;
+  DeviceGuard guard(g->device);
+  delete g;
+  return CCGLIB_OK;
+}
+
+// ---- ScaledLinear ----
+
+int ccglib_scaled_linear_create(ccglib_scaled_linear_t *linear, size_t M, size_t N, size_t K, int device, void *stream, int type,
+                                int gradient_type, int scale_type, int training) {
+  if (!linear) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: linear");
+  *linear = nullptr;
+  if (M > kMostPitch || N > kMostPitch || K > kMostPitch) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  auto quantize = [&](size_t m, size_t n, int out, int group) {
+    QuantizeParams p = {};
+    p.batch = 1;
+    p.m = (unsigned)m;
+    p.n = (unsigned)n;
+    p.in_pitch = n;
+    p.type_in = type;
+    p.type_out = out;
+    p.group = group;
+    p.scale_type = scale_type;
+    return p;
+  };
+  auto gemm = [&](size_t m, size_t n, size_t k, int a, int c, int group_b) {
+    ScaledGemmParams p = {};
+    p.batch = 1;
+    p.m = (unsigned)m;
+    p.n = (unsigned)n;
+    p.k = (unsigned)k;
+    p.pitch_a = p.pitch_b = scaled_pitch(k);
+    p.pitch_c = n;
+    p.type_a = a;
+    p.type_b = kFloat8e4m3;
+    p.type_c = c;
+    p.group_a = kScaleRows;
+    p.group_b = group_b;
+    p.scale_type = scale_type;
+    return p;
+  };
+  const QuantizeParams qx = quantize(M, K, kFloat8e4m3, kScaleRows), qw = quantize(N, K, kFloat8e4m3, kScaleBlocks),
+                       qdy = quantize(M, N, gradient_type, kScaleRows);
+  ScaledGemmParams y = gemm(M, N, K, kFloat8e4m3, type, kScaleBlocks), dx = gemm(M, K, N, gradient_type, type, kScaleBlocks),
+                   dw = gemm(N, K, M, gradient_type, kFloat32, kScaleRows);
+  if (int s = check_quantize(qx, 1, M, K)) return s;
+  if (int s = check_quantize(qw, 1, N, K)) return s;
+  if (int s = check_quantize(qdy, 1, M, N)) return s;
+  if (int s = check_gemm(y, 1, M, N, K)) return s;
+  if (int s = check_gemm(dx, 1, M, K, N)) return s;
+  if (int s = check_gemm(dw, 1, N, K, M)) return s;
+  if (int s = check_device(device)) return s;
+  DeviceGuard guard(device);
+  HIP_TRY(guard.status());
+  auto *l = new (std::nothrow) ccglib_scaled_linear;
+  if (!l) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
+  l->M = M;
+  l->N = N;
+  l->K = K;
+  l->type = type;
+  l->scale_type = scale_type;
+  l->device = device;
+  l->training = training != 0;
+  l->stream = static_cast<hipStream_t>(stream);
+  // One allocation: counters and partial sums that the three products share (they run one after the other), then the
+  // 8-bit copies of x, w and dy in both orientations (without training: of x and w as they are).
+  size_t counters = 0, partial = 0, at = 0;
+  ScaledGemmParams *const products[] = {&y, &dx, &dw};
+  for (int i = 0; i < (l->training ? 3 : 1); ++i) {
+    ScaledGemmParams &p = *products[i];
+    p.plan = plan_scaled_gemm(p);
+    if (p.plan.counter_bytes > counters) counters = p.plan.counter_bytes;
+    if (p.plan.partial_bytes > partial) partial = p.plan.partial_bytes;
+  }
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += ceil_div(bytes, 256) * 256;
+    return here;
+  };
+  take(counters);
+  // (a product's partial sums follow its own counters)
+  take(partial);
+  struct Copy {
+    size_t values, scales;
+  };
+  auto copy = [&](size_t rows, size_t k, int group) {
+    Copy c;
+    c.values = take(rows * scaled_pitch(k));
+    c.scales = take(ceil_div(k, kScaleGroup) * scaled_pitch(scale_rows(rows, group)) * scale_size(scale_type));
+    return c;
+  };
+  const Copy cx = copy(M, K, kScaleRows), cw = copy(N, K, kScaleBlocks);
+  Copy cxt{}, cwt{}, cdy{}, cdyt{};
+  if (l->training) {
+    cxt = copy(K, M, kScaleRows);
+    cwt = copy(K, N, kScaleBlocks);
+    cdy = copy(M, N, kScaleRows);
+    cdyt = copy(N, M, kScaleRows);
+  }
+  if (int s = allocate(&l->memory, at, counters)) {
+    delete l;
+    return s;
+  }
+  auto outputs = [&](QuantizeParams p, const Copy &direct, const Copy &transposed) {
+    p.out = l->memory.at(direct.values);
+    p.scales = l->memory.at(direct.scales);
+    if (l->training) {
+      p.out_t = l->memory.at(transposed.values);
+      p.scales_t = l->memory.at(transposed.scales);
+    }
+    return p;
+  };
+  l->x = outputs(qx, cx, cxt);
+  l->w = outputs(qw, cw, cwt);
+  if (l->training) l->dy = outputs(qdy, cdy, cdyt);
+  auto operands = [&](ScaledGemmParams p, const Copy &a, const Copy &b) {
+    p.a = l->memory.at(a.values);
+    p.scales_a = l->memory.at(a.scales);
+    p.b = l->memory.at(b.values);
+    p.scales_b = l->memory.at(b.scales);
+    p.workspace = l->memory.p;
+    return p;
+  };
+  l->y = operands(y, cx, cw);
+  if (l->training) {
+    l->dx = operands(dx, cdy, cwt);
+    l->dw = operands(dw, cdyt, cxt);
+  }
+  *linear = l;
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t l, const void *d_w) {
+  if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  if (!d_w && l->N && l->K) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: weights");
+  if (!aligned(d_w, element(l->type))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned weights");
+  DeviceGuard guard(l->device);
+  HIP_TRY(guard.status());
+  QuantizeParams p = l->w;
+  p.in = d_w;
+  HIP_TRY(launch_quantize(p, l->stream));
+  l->have_weights = true;
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_linear_forward(ccglib_scaled_linear_t l, const void *d_x, void *d_y) {
+  if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  if (!l->have_weights) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: forward before the weights were set");
+  if ((!d_x && l->M && l->K) || (!d_y && l->M && l->N)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: x or y");
+  if (!aligned(d_x, element(l->type)) || !aligned(d_y, element(l->type))) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned x or y");
+  }
+  DeviceGuard guard(l->device);
+  HIP_TRY(guard.status());
+  QuantizeParams q = l->x;
+  q.in = d_x;
+  HIP_TRY(launch_quantize(q, l->stream));
+  ScaledGemmParams p = l->y;
+  p.c = d_y;
+  HIP_TRY(launch_scaled_gemm(p, l->stream));
+  l->have_forward = true;
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_linear_backward(ccglib_scaled_linear_t l, const void *d_dy, void *d_dx, void *d_dw, int accumulate_dw) {
+  if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  if (!l->training) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward of a layer that was created without training");
+  if (!l->have_forward) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward before forward");
+  if (!d_dx && !d_dw) return CCGLIB_OK;
+  if (!d_dy && l->M && l->N) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: dy");
+  if (!aligned(d_dy, element(l->type)) || !aligned(d_dx, element(l->type)) || !aligned(d_dw, 4)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned dy, dx or dw");
+  }
+  DeviceGuard guard(l->device);
+  HIP_TRY(guard.status());
+  QuantizeParams q = l->dy;
+  q.in = d_dy;
+  if (!d_dx) q.out = q.scales = nullptr;
+  if (!d_dw) q.out_t = q.scales_t = nullptr;
+  HIP_TRY(launch_quantize(q, l->stream));
+  if (d_dx) {
+    ScaledGemmParams p = l->dx;
+    p.c = d_dx;
+    HIP_TRY(launch_scaled_gemm(p, l->stream));
+  }
+  if (d_dw) {
+    ScaledGemmParams p = l->dw;
+    p.c = d_dw;
+    p.accumulate = accumulate_dw != 0;
+    HIP_TRY(launch_scaled_gemm(p, l->stream));
+  }
+  return CCGLIB_OK;
+}
+
+int ccglib_scaled_linear_destroy(ccglib_scaled_linear_t l) {
+  if (!l) return CCGLIB_OK;
+  DeviceGuard guard(l->device);
+  delete l;
+  return CCGLIB_OK;
+}
+
+// ---- Orthogonalize ----
+
+int ccglib_orthogonalize_create(ccglib_orthogonalize_t *orthogonalize, size_t B, size_t M, size_t N, int device, void *stream,
+                                int type, int steps, float a, float b, float c, float epsilon, size_t in_pitch,
+                                size_t out_pitch) {
+  if (!orthogonalize) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: orthogonalize");
+  *orthogonalize = nullptr;
+  if (!is_wide_float(type)) {
+    return fail(CCGLIB_ERROR_UNSUPPORTED, "Orthogonalize: matrices are float32, float16 or bfloat16 (type %d)", type);
+  }
+  if (steps < 1 || steps > 1000) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: 1 to 1000 steps (got %d)", steps);
+  if (!(epsilon >= 0.f)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: epsilon is not negative (got %g)", epsilon);
+  constexpr size_t kMost = (size_t)1 << 21;   // (rows of 2^22 bytes)
+  if (B > 65535 || M > kMost || N > kMost || (B && M && N && M * N > ((size_t)1 << 40) / B)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
+  }
+  OrthogonalizeParams p = {};
+  p.batch = (unsigned)B;
+  p.m = (unsigned)M;
+  p.n = (unsigned)N;
+  p.in_pitch = in_pitch ? in_pitch : N;
+  p.out_pitch = out_pitch ? out_pitch : N;
+  if (p.in_pitch < N || p.out_pitch < N) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: rows of %zu values at a distance of %zu and %zu", N, p.in_pitch,
+                p.out_pitch);
+  }
+  p.type = type;
+  p.steps = steps;
+  p.a = a;
+  p.b = b;
+  p.c = c;
+  p.epsilon = epsilon;
+  if (int s = check_device(device)) return s;
+  DeviceGuard guard(device);
+  HIP_TRY(guard.status());
+  auto *o = new (std::nothrow) ccglib_orthogonalize{p, device, static_cast<hipStream_t>(stream), {}};
+  if (!o) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
+  if (B && M && N) {
+    if (int s = allocate(&o->workspace, orthogonalize_workspace_bytes(p), orthogonalize_zeroed_bytes(p))) {
+      delete o;
+      return s;
+    }
+  }
+  o->p.workspace = o->workspace.p;
+  *orthogonalize = o;
+  return CCGLIB_OK;
+}
+
+int ccglib_orthogonalize_run(ccglib_orthogonalize_t o, const void *d_in, void *d_out) {
+  if (!o) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
+  OrthogonalizeParams p = o->p;
+  if (p.batch == 0 || p.m == 0 || p.n == 0) return CCGLIB_OK;
+  if (!d_in || !d_out) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: input or output");
+  if (!aligned(d_in, element(p.type)) || !aligned(d_out, element(p.type))) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: misaligned input or output");
+  }
+  p.in = d_in;
+  p.out = d_out;
+  DeviceGuard guard(o->device);
+  HIP_TRY(guard.status());
+  HIP_TRY(launch_orthogonalize(p, o->stream));
+  return CCGLIB_OK;
+}
+
+int ccglib_orthogonalize_destroy(ccglib_orthogonalize_t o) {
+  if (!o) return CCGLIB_OK;
+  DeviceGuard guard(o->device);
+  delete o;
+  return CCGLIB_OK;
+}
+
+}  // extern "C"

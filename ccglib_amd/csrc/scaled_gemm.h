@@ -1,0 +1,131 @@
+// C[m][n] (+)= sum over groups g of 128 of K: scale_a[g][m] scale_b[g][n] sum over k in g of A[m][k] B[n][k], 8-bit operands.
+//
+// B's rows (n, the contiguous axis of C) are X of the product kernel, A's rows Y. With float scales the instruction
+// sums one group from zero, and the vector ALU adds it to C's sum with the product of the two scales: one fused operation
+// for each element and group where B has a scale for 128 x 128 values (a lane's scale of A times a uniform one), two where
+// each row of B has its own. Powers of two (e8m0) are what the matrix instruction takes as its own scales.
+// Sums are held in 32 bits throughout, and rounded once, to the type of C; a 32-bit C is multiplied by the fp16
+// instruction, since the 8-bit one does not sum to 32 bits (kWide* in real_gemm.h).
+#ifndef CCGLIB_AMD_SCALED_GEMM_H_
+#define CCGLIB_AMD_SCALED_GEMM_H_
+
+#include "real_gemm.h"
+#include "scaled.h"
+
+namespace ccglib_amd {
+namespace real {
+
+// Block shapes: BX (columns of C) x BY (rows), waves, ring.
+struct ShapeInfo {
+  unsigned bx, by;
+  const char *name;
+};
+#define CCGLIB_SCALED_SHAPES(DO) \
+  DO(0, 256, 256, 2, 4, 2, 2)    \
+  DO(1, 128, 128, 2, 2, 2, 2)    \
+  DO(2, 64, 64, 2, 2, 4, 2)      \
+  DO(3, 64, 32, 4, 1, 6, 2)
+// (fp16 operands take twice the registers)
+#define CCGLIB_WIDE_SHAPES(DO) \
+  DO(0, 128, 256, 2, 4, 2, 2)  \
+  DO(1, 128, 128, 2, 2, 2, 2)  \
+  DO(2, 64, 64, 2, 2, 4, 2)    \
+  DO(3, 64, 32, 4, 1, 6, 2)
+
+struct StoreC {
+  struct Params {
+    char *c;
+    size_t pitch, batch;     // elements from row to row, from matrix to matrix
+    unsigned nx, ny;
+    int type, accumulate;
+  };
+  const Params &p;
+  __device__ explicit StoreC(const Params &params) : p(params) {}
+
+  template <typename T, int N> __device__ __forceinline__ void put(size_t at, unsigned left, const float (&v)[N]) const {
+    typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T) < N ? 16 / sizeof(T) : N)));
+    typedef piece_t piece_unaligned_t __attribute__((aligned(sizeof(T))));
+    constexpr int E = sizeof(piece_t) / sizeof(T);
+    T *to = reinterpret_cast<T *>(p.c) + at;
+    if (left >= (unsigned)N) {
+#pragma unroll
+      for (int i = 0; i < N; i += E) {
+        piece_t w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = (T)v[i + e];
+        *reinterpret_cast<piece_unaligned_t *>(to + i) = w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if ((unsigned)e < left) to[e] = (T)v[e];
+      }
+    }
+  }
+
+  template <int N>
+  __device__ __forceinline__ void store(unsigned b, unsigned y, unsigned x, const float (&v)[N], bool) const {
+    const size_t at = (size_t)b * p.batch + (size_t)y * p.pitch + x;
+    const unsigned left = p.nx - x;
+    if (p.accumulate) {   // (32-bit C)
+      const float *old = reinterpret_cast<const float *>(p.c) + at;
+      float w[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = (unsigned)e < left ? v[e] + old[e] : 0.f;
+      put<float>(at, left, w);
+    } else if (p.type == kFloat32) {
+      put<float>(at, left, v);
+    } else if (p.type == kFloat16) {
+      put<_Float16>(at, left, v);
+    } else {
+      put<__bf16>(at, left, v);
+    }
+  }
+};
+
+template <int MODE> hipError_t launch_scaled_mode(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kScaledBlocks>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kScaledRows>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kScaledE8m0>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kWideBlocks>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kWideRows>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+template <> hipError_t launch_scaled_mode<kWideE8m0>(const ScaledGemmParams &p, const Args &a, hipStream_t stream);
+
+#ifdef CCGLIB_SCALED_MODE
+template <int MODE, int FX, int FY>
+hipError_t launch_scaled(int shape, unsigned grid, const Args &a, const StoreC::Params &e, hipStream_t stream) {
+#define CCGLIB_CASE(ID, BX, BY, WX, WY, SLOTS, EU)                                                       \
+  case ID:                                                                                               \
+    gemm_real<MODE, FX, FY, BX, BY, WX, WY, SLOTS, EU, StoreC><<<grid, 64 * WX * WY, 0, stream>>>(a, e); \
+    break;
+  if constexpr (ModeTraits<MODE>::kWide) {
+    switch (shape) { CCGLIB_WIDE_SHAPES(CCGLIB_CASE) }
+  } else {
+    switch (shape) { CCGLIB_SCALED_SHAPES(CCGLIB_CASE) }
+  }
+#undef CCGLIB_CASE
+  return hipGetLastError();
+}
+
+template <> hipError_t launch_scaled_mode<CCGLIB_SCALED_MODE>(const ScaledGemmParams &p, const Args &a, hipStream_t stream) {
+  constexpr int MODE = CCGLIB_SCALED_MODE;
+  StoreC::Params e;
+  e.c = static_cast<char *>(p.c);
+  e.pitch = p.pitch_c;
+  e.batch = (size_t)p.m * p.pitch_c;
+  e.nx = p.n;
+  e.ny = p.m;
+  e.type = p.type_c;
+  e.accumulate = p.accumulate;
+  const unsigned grid = a.batch * a.parts * a.blocks_x * a.blocks_y;
+  const bool a4 = p.type_a == kFloat8e4m3, b4 = p.type_b == kFloat8e4m3;
+  if (a4 && b4) return launch_scaled<MODE, 0, 0>(p.plan.shape, grid, a, e, stream);
+  if (b4) return launch_scaled<MODE, 0, 1>(p.plan.shape, grid, a, e, stream);
+  if (a4) return launch_scaled<MODE, 1, 0>(p.plan.shape, grid, a, e, stream);
+  return launch_scaled<MODE, 1, 1>(p.plan.shape, grid, a, e, stream);
+}
+#endif
+
+}  // namespace real
+}  // namespace ccglib_amd
+#endif  // CCGLIB_AMD_SCALED_GEMM_H_

@@ -20,6 +20,11 @@ enum ValueType { int1 = 0, int32 = 1, bfloat16 = 2, float8e4m3 = 3, float8e5m2 =
 enum ComplexAxisLocation { complex_planar = 0, complex_interleaved = 1 };
 enum Direction { forward = 0, backward = 1 };
 
+// 8-bit values with block scales (no counterpart in the reference): values that share a scale - 128 of a row, or
+// 128 x 128 - and what a scale is, a float or a power of two in a byte.
+enum ScaleGroup { scale_rows = 0, scale_blocks = 1 };
+enum ScaleType { scale_float32 = 0, scale_e8m0 = 1 };
+
 namespace mma {
 enum MemOrder { row_major = 0, col_major = 1 };
 enum Variant { basic = 0, opt = 1 };

@@ -337,6 +337,94 @@ CCGLIB_API int ccglib_pipeline_run_static(
     int output_type, int variant, float alpha_re, float alpha_im, float beta_re,
     float beta_im, const void *d_a, const void *d_b, void *d_c);
 
+/* ------------------------------------------------------------------------
+ * Real products of 8-bit values with block scales, what makes their operands,
+ * a linear layer of them, and orthogonalised updates of weights. No
+ * counterpart in the reference.
+ *
+ * Layout of an 8-bit matrix of R rows of C values (e4m3 or e5m2): the rows
+ * lie ccglib_scaled_pitch(C) bytes apart (a multiple of 16), the bytes behind
+ * a row's end are zero. Its scales are numbered first by the group of 128
+ * values along the row, then by the row (SCALE_ROWS) or by 128 rows
+ * (SCALE_BLOCKS):
+ *     scales[ceil(C / 128)][ccglib_scaled_pitch(R or ceil(R / 128))]
+ * float, or one byte that holds a power of two (e8m0: 2^(byte - 127); the byte
+ * 255 would be NaN). A batch is such matrices one after the other. Values start
+ * at a multiple of 16 bytes.
+ * ---------------------------------------------------------------------- */
+/* Groups of values that share a scale: 128 of a row, or 128 x 128 */
+enum { CCGLIB_SCALE_ROWS = 0, CCGLIB_SCALE_BLOCKS = 1 };
+/* What a scale is */
+enum { CCGLIB_SCALE_FLOAT32 = 0, CCGLIB_SCALE_E8M0 = 1 };
+
+typedef struct ccglib_quantize *ccglib_quantize_t;
+typedef struct ccglib_scaled_gemm *ccglib_scaled_gemm_t;
+typedef struct ccglib_scaled_linear *ccglib_scaled_linear_t;
+typedef struct ccglib_orthogonalize *ccglib_orthogonalize_t;
+
+/* n rounded up to the distance of rows, of values and of scales. */
+CCGLIB_API size_t ccglib_scaled_pitch(size_t n);
+
+/* B matrices of M x N (float32, float16, bfloat16; rows in_pitch values apart,
+ * 0: N) to 8 bits. For each group, t the type's largest value (448, 57344):
+ *     amax = max(2^-100, largest finite |x|)
+ *     float32 scales: scale = amax / t, q = round(x * (t / amax))
+ *     e8m0 scales:    scale = 2^ceil(log2(amax / t)), q = round(x / scale)
+ * in 32 bits, q rounded to nearest, ties to even. NaN stays NaN; an infinity
+ * stays one in e5m2 and is NaN in e4m3. run writes the matrix as it is
+ * (d_out, d_scales), its transpose (d_out_t, d_scales_t: N rows of M values,
+ * groups along M), or both; a pair that is not wanted is null. */
+CCGLIB_API int ccglib_quantize_create(ccglib_quantize_t *quantize, size_t B, size_t M, size_t N, int device, void *stream,
+                                      int type_in, int type_out, int group, int scale_type, size_t in_pitch);
+CCGLIB_API int ccglib_quantize_run(ccglib_quantize_t quantize, const void *d_in, void *d_out, void *d_scales, void *d_out_t,
+                                   void *d_scales_t);
+CCGLIB_API int ccglib_quantize_destroy(ccglib_quantize_t quantize);
+
+/* C[m][n] (+)= sum over groups g of 128 of K of
+ *     scale_a[g][m] scale_b[g][n] sum over k in g of A[m][k] B[n][k]
+ * for B matrices each of M x K and N x K, C M x N row-major (float32, float16,
+ * bfloat16). Sums are held in 32 bits and rounded once. accumulate: C, which is
+ * float32 then, is added to. pitch_a, pitch_b: bytes between rows where they
+ * are not ccglib_scaled_pitch(K) (0; multiples of 16); pitch_c: elements
+ * between rows of C (0: N). K may be 0 (a sum of nothing). */
+CCGLIB_API int ccglib_scaled_gemm_create(ccglib_scaled_gemm_t *gemm, size_t B, size_t M, size_t N, size_t K, int device,
+                                         void *stream, int type_a, int type_b, int type_c, int group_a, int group_b,
+                                         int scale_type, int accumulate, size_t pitch_a, size_t pitch_b, size_t pitch_c);
+CCGLIB_API int ccglib_scaled_gemm_run(ccglib_scaled_gemm_t gemm, const void *d_a, const void *d_scales_a, const void *d_b,
+                                      const void *d_scales_b, void *d_c);
+CCGLIB_API int ccglib_scaled_gemm_kernel_name(ccglib_scaled_gemm_t gemm, char *buffer, size_t size);
+CCGLIB_API int ccglib_scaled_gemm_destroy(ccglib_scaled_gemm_t gemm);
+
+/* A linear layer of K inputs and N outputs on M rows, y = x W^T, by products of
+ * 8-bit copies: x (M x K) and dy (M x N) with scales for 128 values along the
+ * summed index, W (N x K) for 128 x 128; x and W in e4m3, dy in gradient_type.
+ * x, y, W, dy and dx are of `type`, dw is float32. set_weights keeps 8-bit
+ * copies of W until it is called again, forward those of x until the next one;
+ * backward, with the x and W of then, computes
+ *     dx = dy W,  dw = dy^T x  (accumulate_dw: dw += dy^T x);
+ * d_dx or d_dw may be null. training = 0: forward only, half the work of
+ * making the copies. */
+CCGLIB_API int ccglib_scaled_linear_create(ccglib_scaled_linear_t *linear, size_t M, size_t N, size_t K, int device, void *stream,
+                                           int type, int gradient_type, int scale_type, int training);
+CCGLIB_API int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t linear, const void *d_w);
+CCGLIB_API int ccglib_scaled_linear_forward(ccglib_scaled_linear_t linear, const void *d_x, void *d_y);
+CCGLIB_API int ccglib_scaled_linear_backward(ccglib_scaled_linear_t linear, const void *d_dy, void *d_dx, void *d_dw,
+                                             int accumulate_dw);
+CCGLIB_API int ccglib_scaled_linear_destroy(ccglib_scaled_linear_t linear);
+
+/* B updates G of M x N (float32, float16, bfloat16; rows in_pitch and out_pitch
+ * values apart, 0: N), each made nearly orthogonal by a Newton-Schulz iteration:
+ *     X = G / (|G| + epsilon), |.| the Frobenius norm
+ *     steps times:  S = X X^T,  X = a X + (b S + c S S) X      (M <= N; else of G^T)
+ * d_out may be d_in. bfloat16 updates are multiplied in fp16 (11 bits), others
+ * in two fp16 for each value (22 bits); sums are 32 bits. A matrix that holds
+ * NaN or an infinity becomes NaN. */
+CCGLIB_API int ccglib_orthogonalize_create(ccglib_orthogonalize_t *orthogonalize, size_t B, size_t M, size_t N, int device,
+                                           void *stream, int type, int steps, float a, float b, float c, float epsilon,
+                                           size_t in_pitch, size_t out_pitch);
+CCGLIB_API int ccglib_orthogonalize_run(ccglib_orthogonalize_t orthogonalize, const void *d_in, void *d_out);
+CCGLIB_API int ccglib_orthogonalize_destroy(ccglib_orthogonalize_t orthogonalize);
+
 #ifdef __cplusplus
 }
 #endif
