@@ -473,7 +473,7 @@ int ccglib_orthogonalize_create(ccglib_orthogonalize_t *orthogonalize, size_t B,
   }
   if (steps < 1 || steps > 1000) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: 1 to 1000 steps (got %d)", steps);
   if (!(epsilon >= 0.f)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "Orthogonalize: epsilon is not negative (got %g)", epsilon);
-  constexpr size_t kMost = (size_t)1 << 21;   // (rows of 2^22 bytes)
+  constexpr size_t kMost = (size_t)1 << 20;   // (rows of 2^21 bytes)
   if (B > 65535 || M > kMost || N > kMost || (B && M && N && M * N > ((size_t)1 << 40) / B)) {
     return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
   }

@@ -18,7 +18,6 @@ namespace ccglib_amd {
 namespace {
 
 constexpr unsigned kUnits = 256;
-constexpr unsigned kNormBlocks = 128;     // partial sums of squares a matrix, at most
 constexpr size_t kAlign = 256;
 size_t up(size_t n, size_t to) { return ceil_div(n, to) * to; }
 
@@ -33,31 +32,58 @@ template <> struct Value<kFloat32> { using type = float; };
 template <> struct Value<kFloat16> { using type = _Float16; };
 template <> struct Value<kBfloat16> { using type = __bf16; };
 
-// partial[b][block] = sum of the squares of a part of matrix b
+// partial[b][block] = sum of the squares of a part of matrix b: a block has `rows` x kNormColumns values, a thread eight
+// neighbours at a time
+constexpr unsigned kNormColumns = 2048;
 template <int TYPE>
 __global__ __launch_bounds__(256) void sum_of_squares(const typename Value<TYPE>::type *in, size_t pitch, unsigned m, unsigned n,
-                                                      double *partial) {
-  const unsigned b = blockIdx.y;
-  const typename Value<TYPE>::type *g = in + (size_t)b * m * pitch;
+                                                      unsigned rows, double *partial) {
+  using V = typename Value<TYPE>::type;
+  typedef V eight_t __attribute__((ext_vector_type(8), aligned(sizeof(V))));
+  const unsigned b = blockIdx.z, c = blockIdx.x * kNormColumns + threadIdx.x * 8, r0 = blockIdx.y * rows;
+  const V *g = in + ((size_t)b * m + r0) * pitch + c;
   double sum = 0.0;
-  for (unsigned r = blockIdx.x; r < m; r += gridDim.x) {
-    for (unsigned c = threadIdx.x; c < n; c += 256) {
-      const double v = (double)(float)g[(size_t)r * pitch + c];
-      sum = __builtin_fma(v, v, sum);
+  if (c + 8 <= n) {
+#pragma unroll 8
+    for (unsigned r = 0; r < rows; ++r) {
+      if (r0 + r >= m) break;
+      const eight_t v = *reinterpret_cast<const eight_t *>(g + (size_t)r * pitch);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double d = (double)(float)v[e];
+        sum = __builtin_fma(d, d, sum);
+      }
+    }
+  } else if (c < n) {
+    for (unsigned r = 0; r < rows && r0 + r < m; ++r) {
+      for (unsigned e = 0; c + e < n; ++e) {
+        const double d = (double)(float)g[(size_t)r * pitch + e];
+        sum = __builtin_fma(d, d, sum);
+      }
     }
   }
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   __shared__ double waves[4];
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) partial[(size_t)b * gridDim.x + blockIdx.x] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
+  if (threadIdx.x == 0) {
+    partial[((size_t)b * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
+  }
+}
+
+// The sum of `count` partial sums, by 256 threads, in all of them.
+__device__ __forceinline__ double sum_of(const double *partial, unsigned count, double *waves) {
+  double sum = 0.0;
+  for (unsigned i = threadIdx.x; i < count; i += 256) sum += partial[i];
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  return (waves[0] + waves[1]) + (waves[2] + waves[3]);
 }
 
 // The exponent e of the power of two that X0 is G times, and the factor that is left: 2^-e / (|G| + epsilon).
 // (|G| 2^e is 128 to 256: far from what fp16 cannot hold at either end)
-__device__ __forceinline__ int exponent_and_factor(const double *partial, unsigned count, float epsilon, float *factor) {
-  double sum = 0.0;
-  for (unsigned i = 0; i < count; ++i) sum += partial[i];
+__device__ __forceinline__ int exponent_and_factor(double sum, float epsilon, float *factor) {
   const double norm = __builtin_sqrt(sum);
   if (!(norm < __builtin_inf())) {   // an infinity or a NaN among the values: the result is NaN
     *factor = __builtin_nanf("");
@@ -78,15 +104,11 @@ __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::typ
                                                  const double *partial, unsigned count, float epsilon, float *factor) {
   using H = real::Halves<PAIRS>;
   __shared__ float tile[64][65];
-  __shared__ int exponent;
+  __shared__ double waves[4];
   const unsigned b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  if (threadIdx.x == 0) {
-    float f;
-    exponent = exponent_and_factor(partial + (size_t)b * count, count, epsilon, &f);
-    if (blockIdx.x == 0 && blockIdx.y == 0) factor[b] = f;
-  }
-  __syncthreads();
-  const int e = exponent;
+  float f;
+  const int e = exponent_and_factor(sum_of(partial + (size_t)b * count, count, waves), epsilon, &f);
+  if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) factor[b] = f;
   const int c = threadIdx.x & 63;
   for (int r = threadIdx.x >> 6; r < 64; r += 4) {
     if (r0 + r < m && c0 + c < n) {
@@ -112,7 +134,7 @@ struct Layout {
   size_t x_plane, t_plane, a_plane;        // elements of one plane of one matrix
   size_t counters, partial, norm, factor, diagonal, x, t0, t1, a, p, bytes;
   size_t zeroed;
-  unsigned norm_blocks;
+  unsigned norm_x, norm_y, norm_rows;      // partial sums of squares, rows of one
 };
 
 struct Product {
@@ -163,7 +185,10 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.x_plane = l.m * l.np;
   l.t_plane = l.n * l.mp;
   l.a_plane = l.m * l.mp;
-  l.norm_blocks = (unsigned)std::min<size_t>(std::min<size_t>(p.m, kNormBlocks), std::max<size_t>(1, (size_t)p.m * p.n / 4096));
+  l.norm_x = (unsigned)ceil_div(p.n, (size_t)kNormColumns);
+  // (at least 16 rows, and at most about 2048 partial sums, which every block of to_halves adds up)
+  l.norm_rows = (unsigned)std::max<size_t>(16, ceil_div((size_t)p.m * l.norm_x, 2048));
+  l.norm_y = (unsigned)ceil_div(p.m, (size_t)l.norm_rows);
   size_t counters = 0, partial = 0;
   const real::HalfShape *shapes = pairs ? kPairsShapes : kHalfShapes;
   const Product products[] = {plan_product(pairs, p.batch, l.m, l.m, l.n, true), plan_product(pairs, p.batch, l.m, l.m, l.m, true),
@@ -190,7 +215,7 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.p = take(l.a_plane * h);
   l.zeroed = at;
   l.partial = take(partial);
-  l.norm = take(p.batch * l.norm_blocks * sizeof(double));
+  l.norm = take((size_t)p.batch * l.norm_x * l.norm_y * sizeof(double));
   l.factor = take(p.batch * sizeof(float));
   l.diagonal = take(2 * p.batch * l.mp * sizeof(float));
   l.bytes = at;
@@ -238,14 +263,14 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
   const size_t pl = PAIRS ? 2 : 1;
   const size_t xb = l.x_plane * pl, tb = l.t_plane * pl, ab = l.a_plane * pl;
 
-  sum_of_squares<TYPE><<<dim3(l.norm_blocks, p.batch), 256, 0, stream>>>(in, p.in_pitch, p.m, p.n, norm);
+  sum_of_squares<TYPE><<<dim3(l.norm_x, l.norm_y, p.batch), 256, 0, stream>>>(in, p.in_pitch, p.m, p.n, l.norm_rows, norm);
   const dim3 tiles((unsigned)ceil_div(p.n, (size_t)64), (unsigned)ceil_div(p.m, (size_t)64), p.batch);
   if (l.tall) {
     to_halves<TYPE, PAIRS><<<tiles, 256, 0, stream>>>(in, p.in_pitch, p.m, p.n, t, l.mp, tb, l.t_plane, x, l.np, xb, l.x_plane,
-                                                      norm, l.norm_blocks, p.epsilon, factor);
+                                                      norm, l.norm_x * l.norm_y, p.epsilon, factor);
   } else {
     to_halves<TYPE, PAIRS><<<tiles, 256, 0, stream>>>(in, p.in_pitch, p.m, p.n, x, l.np, xb, l.x_plane, t, l.mp, tb, l.t_plane,
-                                                      norm, l.norm_blocks, p.epsilon, factor);
+                                                      norm, l.norm_x * l.norm_y, p.epsilon, factor);
   }
   HIP_PASS(hipGetLastError());
 

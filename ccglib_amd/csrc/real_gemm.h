@@ -19,6 +19,7 @@
 #define CCGLIB_AMD_REAL_GEMM_H_
 
 #include <type_traits>
+#include <utility>
 
 #include "gemm_device.h"
 
@@ -102,51 +103,47 @@ template <int N> __device__ __forceinline__ void wait_copies_then_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-struct Fragment {
-  int4_t v[2];
-};
-
-__device__ __forceinline__ int8x_t joined(const Fragment &f) {
-  return int8x_t{f.v[0][0], f.v[0][1], f.v[0][2], f.v[0][3], f.v[1][0], f.v[1][1], f.v[1][2], f.v[1][3]};
+// 32 bytes of a row: two 16-byte chunks
+typedef int8x_t Fragment;
+__device__ __forceinline__ half8_t half_of(const Fragment &f, int q) {
+  const int4_t v = q == 0 ? __builtin_shufflevector(f, f, 0, 1, 2, 3) : __builtin_shufflevector(f, f, 4, 5, 6, 7);
+  return __builtin_bit_cast(half8_t, v);
 }
 
 // FX, FY: format codes of 8-bit operands (0 e4m3, 1 e5m2)
 template <int FX, int FY>
 __device__ __forceinline__ float4_t mfma8(const Fragment &x, const Fragment &y, float4_t c, int sx, int sy) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(joined(x), joined(y), c, FX, FY, 0, sx, 0, sy);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, FX, FY, 0, sx, 0, sy);
 }
+
 // A lane's 32 values of 8 bits as fp16, four operands of the fp16 instruction
 struct WideFragment {
   half8_t v[4];
 };
-template <int FORMAT> __device__ __forceinline__ WideFragment widened(const Fragment &f) {
+template <int FORMAT> __device__ __forceinline__ void widen_quarter(const Fragment &f, WideFragment &to, int q) {
   typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const unsigned word = (unsigned)f[2 * q + w];
+    half2_t lo, hi;
+    if constexpr (FORMAT == 0) {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true);
+    } else {   // (e5m2 is the upper half of fp16)
+      lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x010c000cu));
+      hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x030c020cu));
+    }
+    to.v[q][4 * w] = lo[0];
+    to.v[q][4 * w + 1] = lo[1];
+    to.v[q][4 * w + 2] = hi[0];
+    to.v[q][4 * w + 3] = hi[1];
+  }
+}
+template <int FORMAT> __device__ __forceinline__ WideFragment widened(const Fragment &f) {
   WideFragment r;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const unsigned word = (unsigned)f.v[q / 2][q % 2 * 2 + w];
-      half2_t lo, hi;
-      if constexpr (FORMAT == 0) {
-        lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false);
-        hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true);
-      } else {   // (e5m2 is the upper half of fp16)
-        lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x010c000cu));
-        hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x030c020cu));
-      }
-      r.v[q][4 * w] = lo[0];
-      r.v[q][4 * w + 1] = lo[1];
-      r.v[q][4 * w + 2] = hi[0];
-      r.v[q][4 * w + 3] = hi[1];
-    }
-  }
+  for (int q = 0; q < 4; ++q) widen_quarter<FORMAT>(f, r, q);
   return r;
-}
-__device__ __forceinline__ float4_t mfma_wide(const WideFragment &x, const WideFragment &y, float4_t c) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v[q], y.v[q], c, 0, 0, 0);
-  return c;
 }
 // 2^(byte - 127); 255 stands for NaN
 __device__ __forceinline__ float power_of_two(unsigned byte) {
@@ -154,15 +151,38 @@ __device__ __forceinline__ float power_of_two(unsigned byte) {
   return byte == 255 ? __builtin_nanf("") : p;
 }
 
-__device__ __forceinline__ float4_t mfma16(const Fragment &x, const Fragment &y, float4_t c) {
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, x.v[s]), __builtin_bit_cast(half8_t, y.v[s]),
-                                               c, 0, 0, 0);
-  }
-  return c;
+__device__ __forceinline__ float4_t mfma16(const Fragment &x, const Fragment &y, float4_t c, int q) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(half_of(x, q), half_of(y, q), c, 0, 0, 0);
 }
 
+// Nothing moves across: neither instructions, when they are put in order, nor reads of LDS, when they are selected
+#define CCGLIB_PIN                      \
+  do {                                  \
+    asm volatile("" ::: "memory");      \
+    __builtin_amdgcn_sched_barrier(0);  \
+  } while (0)
+// What computes the value comes before this place, what uses it comes behind it (arithmetic has no other order than that of
+// its operands until the instructions have been selected)
+template <typename T> __device__ __forceinline__ void pin(T &value) { asm volatile("" : "+v"(value)); }
+__device__ __forceinline__ void pin(WideFragment &value) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(value.v[q]));
+}
+
+template <int N, typename F, int... I> __device__ __forceinline__ void static_for(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void static_for(F &&f) {
+  static_for<N>(f, std::make_integer_sequence<int, N>{});
+}
+
+// (the same in every lane: say so where it goes to a scalar register of an asm statement)
+__device__ __forceinline__ const char *uniform(const char *p) {
+  const unsigned long long u = (unsigned long long)p;
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)u);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
+  return (const char *)(((unsigned long long)hi << 32) | lo);
+}
 // Which block of D, and which piece of K, a workgroup has.
 struct Place {
   unsigned b, bx, by, part, tile;
@@ -266,29 +286,37 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     scale_base = (of_x ? args.x_scales : args.y_scales) + (size_t)at.b * args.pieces * scale_step;
     scale_lds = j * 256;
   }
-  auto copy = [&](unsigned piece, unsigned slot) {
+  // Copies `from_copy` to `to_copy` - 1 of the wave's COPIES of a piece
+  auto copy_some = [&](unsigned piece, unsigned slot, auto from_copy, auto to_copy) {
     const unsigned to = lds_base + slot * S::kSlotBytes;
     const size_t k = (size_t)piece * kPieceBytes;
     const bool whole = (piece + 1) * (unsigned)kPieceBytes <= args.k_bytes;
+    // (values, so that choosing one of them is no choice of an address of this function's variables)
+    const char *const xk = x_base + k, *const yk = y_base + k;
+    const size_t x_plane = args.x_plane, y_plane = args.y_plane;
 #pragma unroll
-    for (int n = 0; n < OPERAND_COPIES; ++n) {
+    for (int n = from_copy; n < to_copy; ++n) {
+      if (T::kScaled && n == OPERAND_COPIES) {
+        load_scales_to_lds<T::kScaleBytes>(
+            uniform(scale_base + (size_t)piece * scale_step), scale_offset,
+            (unsigned)__builtin_amdgcn_readfirstlane((int)(to + S::kXBytes + S::kYBytes + scale_lds)));
+        continue;
+      }
       const int q = wave + n * WAVES;
       const bool of_x = q < X_COPIES;
       const int plane = PLANES == 1 ? 0 : of_x ? q / (BX / 8) : (q - X_COPIES) / (BY / 8);
-      const char *from = (of_x ? x_base : y_base) + k;
-      if (PLANES > 1 && plane) from += of_x ? args.x_plane : args.y_plane;
+      const char *from = of_x ? xk : yk;
+      if (PLANES > 1 && plane) from += of_x ? x_plane : y_plane;
+      const unsigned at_lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(to + q * 1024));
       if (whole) {
-        load_1k_to_lds(from, offset[n], to + q * 1024);
+        load_1k_to_lds(uniform(from), offset[n], at_lds);
       } else {
-        load_1k_to_lds_by_lane(k + chunk * 16 < args.k_bytes ? from + offset[n] : g_zeros, to + q * 1024);
+        load_1k_to_lds_by_lane(k + chunk * 16 < args.k_bytes ? from + offset[n] : g_zeros, at_lds);
       }
     }
-    if constexpr (T::kScaled) {
-      const size_t s = (size_t)piece * scale_step;
-      if constexpr (BX % 64 == 0) {
-        load_scales_to_lds<T::kScaleBytes>(scale_base + s, scale_offset, to + S::kXBytes + S::kYBytes + scale_lds);
-      }
-    }
+  };
+  auto copy = [&](unsigned piece, unsigned slot) {
+    copy_some(piece, slot, std::integral_constant<int, 0>{}, std::integral_constant<int, COPIES>{});
   };
   static_assert(!T::kScaled || BX % 64 == 0, "scales of X fill whole copies");
 
@@ -297,10 +325,8 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   const unsigned frag0 = fr * kPieceBytes + ((g ^ (fr & 7)) << 4), frag1 = fr * kPieceBytes + (((g + 4) ^ (fr & 7)) << 4);
   auto read = [&](unsigned slot, int from) {
     const char *p = lds + slot * S::kSlotBytes + from;
-    Fragment f;
-    f.v[0] = *reinterpret_cast<const int4_t *>(p + frag0);
-    f.v[1] = *reinterpret_cast<const int4_t *>(p + frag1);
-    return f;
+    const int4_t a = *reinterpret_cast<const int4_t *>(p + frag0), b = *reinterpret_cast<const int4_t *>(p + frag1);
+    return Fragment(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
   const int x_rows = wx * TX * kPieceBytes, y_rows = S::kXBytes + wy * TY * kPieceBytes;
 
@@ -315,110 +341,281 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   }
   const float4_t zero = {0.f, 0.f, 0.f, 0.f};
 
-  auto multiply = [&](unsigned slot) {
-    Fragment y[PLANES][NY];
+  // ---- K loop ----
+  // A step is the products of one X tile with JJ Y tiles. Everything that a step needs is read while the ones before it
+  // run: the fragment of X tile i + 1 behind the first products of tile i; the fragments of Y, the scales and the first X
+  // fragment of the next piece behind the products of the last tile, at whose start the wave waits for its copies of that
+  // piece and passes the barrier. With float scales the sums of a step are added to C's LAG steps later. The order is
+  // written out; left to itself the compiler reads, multiplies, waits and adds one tile after the other (8192^3: 587 us).
+  constexpr bool FLOAT_SCALES = T::kScaled && MODE != kScaledE8m0;
+  constexpr int JJ = MODE <= kScaledE8m0 ? 1 : 2;     // (two sums in turn where several instructions add to one)
+  constexpr int SPT = NY / JJ, STEPS = NX * SPT;
+  constexpr int LAG = T::kWide ? 1 : 2, RING = 2 * LAG;
+  constexpr bool CARRY = STEPS % RING == 0;           // the last sums of a piece are added during the next one
+  // Copies go out behind the products before the last tile's, a few at a time: all of them lie in front of the wait there,
+  // which counts on it
+  constexpr int COPY_STEPS = STEPS - SPT, PER_STEP = COPY_STEPS > 0 ? (COPIES + COPY_STEPS - 1) / COPY_STEPS : 0;
+  static_assert(NY % JJ == 0 && (!FLOAT_SCALES || SPT >= LAG), "steps");
+  const unsigned n = last > first ? last - first : 0;
+  if (n > 0) {
 #pragma unroll
-    for (int p = 0; p < PLANES; ++p) {
-#pragma unroll
-      for (int j = 0; j < NY; ++j) y[p][j] = read(slot, y_rows + p * BY * kPieceBytes + j * 16 * kPieceBytes);
+    for (int t = 0; t < SLOTS - 1; ++t) {
+      if ((unsigned)t < n) copy(first + t, t);
     }
-    const char *scales = lds + slot * S::kSlotBytes + S::kXBytes + S::kYBytes;
-    if constexpr (T::kScaled && MODE != kScaledE8m0) {
-      const float *const sx = reinterpret_cast<const float *>(scales) + wx * TX;
-      const float *const sy = reinterpret_cast<const float *>(scales) + BX + wy * TY;
-      auto scale = [](float stored) {
-        return T::kScaleBytes == 1 ? power_of_two(__builtin_bit_cast(unsigned, stored)) : stored;
-      };
-      float s[NY];
-      typename std::conditional<T::kWide, WideFragment, int>::type y16[NY];
+    using Operand = typename std::conditional<T::kWide, WideFragment, Fragment>::type;
+    Operand y[PLANES][NY], x[2][PLANES];
+    Fragment raw_x, raw_y[2];           // (8 bits that become fp16)
+    float s[NY], s_next[NY], s_old[RING * JJ];   // scales of Y (times X's where that is one number)
+    int e8[NY], e8_next[NY], e8x[2];    // e8m0: bytes for the instruction
+    float4_t sx[2];                     // scales of a lane's rows of X tile i
+    float4_t part[RING][JJ];
+    (void)s, (void)s_next, (void)s_old, (void)e8, (void)e8_next, (void)e8x, (void)sx, (void)part, (void)raw_x, (void)raw_y;
+    auto scale = [](float stored) {
+      return T::kScaleBytes == 1 ? power_of_two(__builtin_bit_cast(unsigned, stored)) : stored;
+    };
+    auto scales_at = [&](unsigned slot) { return lds + slot * S::kSlotBytes + S::kXBytes + S::kYBytes; };
+    auto read_scales_y = [&](unsigned slot) {
+      const float *const sxp = reinterpret_cast<const float *>(scales_at(slot)) + wx * TX;
+      const float *const syp = reinterpret_cast<const float *>(scales_at(slot)) + BX + wy * TY;
 #pragma unroll
       for (int j = 0; j < NY; ++j) {
-        s[j] = scale(sy[j * 16 + fr]);
-        if (T::kBlocks) s[j] *= scale(sx[0]);
-        if constexpr (T::kWide) y16[j] = widened<FY>(y[0][j]);
-      }
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const Fragment x = read(slot, x_rows + i * 16 * kPieceBytes);
-        typename std::conditional<T::kWide, WideFragment, int>::type x16;
-        if constexpr (T::kWide) x16 = widened<FX>(x);
-        float4_t sx4 = zero;
-        if (!T::kBlocks) {
-          sx4 = *reinterpret_cast<const float4_t *>(sx + i / NT * GROUP_ROWS + g * 4 * NT + i % NT * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sx4[e] = scale(sx4[e]);
+        if constexpr (FLOAT_SCALES) {
+          s_next[j] = scale(syp[j * 16 + fr]);
+          if (T::kBlocks) s_next[j] *= scale(sxp[0]);
+        } else if constexpr (MODE == kScaledE8m0) {
+          e8_next[j] = __builtin_bit_cast(int, syp[j * 16 + fr]);
         }
+      }
+    };
+    auto take_scales_y = [&]() {
 #pragma unroll
-        for (int j = 0; j < NY; ++j) {
-          float4_t part;
-          if constexpr (T::kWide) {
-            part = mfma_wide(x16, y16[j], zero);
-          } else {
-            part = mfma8<FX, FY>(x, y[0][j], zero, 0x7f, 0x7f);
-          }
+      for (int j = 0; j < NY; ++j) {
+        if constexpr (FLOAT_SCALES) s[j] = s_next[j];
+        if constexpr (MODE == kScaledE8m0) e8[j] = e8_next[j];
+      }
+    };
+    auto read_scales_x = [&](int to, unsigned slot, int i) {
+      if constexpr (FLOAT_SCALES && !T::kBlocks) {
+        const float *const sxp = reinterpret_cast<const float *>(scales_at(slot)) + wx * TX;
+        sx[to] = *reinterpret_cast<const float4_t *>(sxp + i / NT * GROUP_ROWS + g * 4 * NT + i % NT * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sx[to][e] = scale(sx[to][e]);
+      } else if constexpr (MODE == kScaledE8m0) {
+        const int *const sxp = reinterpret_cast<const int *>(scales_at(slot)) + wx * TX;
+        e8x[to] = sxp[i / NT * GROUP_ROWS + (fr >> 2) * 4 * NT + i % NT * 4 + (fr & 3)];
+      }
+    };
+    auto read_x = [&](int to, unsigned slot, int i) {
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p) {
+        const Fragment f = read(slot, x_rows + p * BX * kPieceBytes + i * 16 * kPieceBytes);
+        if constexpr (T::kWide) {
+          raw_x = f;
+        } else {
+          x[to][p] = f;
+        }
+      }
+    };
+    auto read_y = [&](unsigned slot, int j) {
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p) {
+        const Fragment f = read(slot, y_rows + p * BY * kPieceBytes + j * 16 * kPieceBytes);
+        if constexpr (T::kWide) {
+          raw_y[j % 2] = f;
+        } else {
+          y[p][j] = f;
+        }
+      }
+    };
+    // C's sums of step m, with Y's scales (or, a piece later, the ones kept of that step)
+    auto add = [&](auto step, bool late) {
+      if constexpr (FLOAT_SCALES) {
+        constexpr int m = decltype(step)::value, i = m / SPT;
+#pragma unroll
+        for (int h = 0; h < JJ; ++h) {
+          const int j = m % SPT * JJ + h;
+          const float sy = late ? s_old[m % RING * JJ + h] : s[j];
+          pin(part[m % RING][h]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
+            const float v = part[m % RING][h][e];
             if (T::kBlocks) {
-              acc[0][j][i][e] = __builtin_fmaf(part[e], s[j], acc[0][j][i][e]);
+              acc[0][j][i][e] = __builtin_fmaf(v, sy, acc[0][j][i][e]);
             } else {
-              acc[0][j][i][e] = __builtin_fmaf(part[e] * s[j], sx4[e], acc[0][j][i][e]);
+              acc[0][j][i][e] = __builtin_fmaf(v * sy, sx[i % 2][e], acc[0][j][i][e]);
+            }
+          }
+          pin(acc[0][j][i]);
+        }
+      }
+    };
+    auto products = [&](auto step) {
+      constexpr int m = decltype(step)::value, i = m / SPT, j0 = m % SPT * JJ, b = i % 2;
+      if constexpr (MODE == kScaledE8m0) {
+        acc[0][j0][i] = mfma8<FX, FY>(x[b][0], y[0][j0], acc[0][j0][i], e8x[b], e8[j0]);
+      } else if constexpr (T::kWide) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) {
+            part[m % RING][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][0].v[q], y[0][j0 + h].v[q],
+                                                                       q == 0 ? zero : part[m % RING][h], 0, 0, 0);
+          }
+        }
+      } else if constexpr (T::kScaled) {
+        part[m % RING][0] = mfma8<FX, FY>(x[b][0], y[0][j0], zero, 0x7f, 0x7f);
+      } else if constexpr (MODE == kHalf) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) acc[0][j0 + h][i] = mfma16(x[b][0], y[0][j0 + h], acc[0][j0 + h][i], q);
+        }
+      } else {
+        constexpr int L = PLANES - 1;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) acc[0][j0 + h][i] = mfma16(x[b][0], y[0][j0 + h], acc[0][j0 + h][i], q);
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) acc[L][j0 + h][i] = mfma16(x[b][0], y[L][j0 + h], acc[L][j0 + h][i], q);
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) acc[L][j0 + h][i] = mfma16(x[b][L], y[0][j0 + h], acc[L][j0 + h][i], q);
+        }
+      }
+    };
+
+    // (SLOTS - 2 later pieces are on their way, if there are as many)
+    auto wait = [&](unsigned t) {
+      if (t + SLOTS - 1 < n + (SLOTS > 2 ? 1 : 0)) {
+        wait_copies_then_barrier<COPIES * (SLOTS - 2)>();
+      } else {
+        wait_copies_then_barrier<0>();
+      }
+    };
+    unsigned slot = 0, refill = SLOTS - 1;
+    wait(0);
+    read_scales_y(0);
+    take_scales_y();
+    read_scales_x(0, 0, 0);
+    read_x(0, 0, 0);
+    if constexpr (T::kWide) x[0][0] = widened<FX>(raw_x);
+#pragma unroll
+    for (int j = 0; j < NY; ++j) {
+      read_y(0, j);
+      if constexpr (T::kWide) y[0][j] = widened<FY>(raw_y[j % 2]);
+    }
+    if constexpr (FLOAT_SCALES && CARRY) {   // (nothing to add yet)
+#pragma unroll
+      for (int r = 0; r < RING * JJ; ++r) s_old[r] = 0.f;
+#pragma unroll
+      for (int r = 0; r < RING; ++r) {
+#pragma unroll
+        for (int h = 0; h < JJ; ++h) part[r][h] = 0.f;
+      }
+      if constexpr (!T::kBlocks) sx[1] = 0.f;
+    }
+#pragma unroll 1
+    for (unsigned t = 0; t < n; ++t) {
+      const unsigned next = slot + 1 == SLOTS ? 0 : slot + 1;
+      const bool more = t + SLOTS - 1 < n;
+      static_for<STEPS>([&](auto step) {
+        constexpr int m = step, i = m / SPT, js = m % SPT, to = (i + 1) % 2;
+        constexpr bool at_end = i == NX - 1;
+        CCGLIB_PIN;
+        if constexpr (COPY_STEPS == 0 && m == 0) {
+          if (more) copy(first + t + SLOTS - 1, refill);
+        }
+        if constexpr (at_end && js == 0) {
+          if (t + 1 < n) wait(t + 1);
+          read_scales_y(next);
+        }
+        if constexpr (js == 0) {
+          read_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
+          if constexpr (MODE == kScaledE8m0) read_scales_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
+        }
+        if constexpr (at_end && T::kWide) {
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) {
+            if (js * JJ + h < 2) read_y(next, js * JJ + h);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < JJ; ++h) pin(y[0][js * JJ + h]);
+        products(step);
+#pragma unroll
+        for (int h = 0; h < JJ; ++h) {
+          if constexpr (FLOAT_SCALES) {
+            pin(part[m % RING][h]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < T::kSums; ++k) pin(acc[k][js * JJ + h][i]);
+          }
+        }
+        CCGLIB_PIN;
+        if constexpr (at_end && !T::kWide) {
+#pragma unroll
+          for (int h = 0; h < JJ; ++h) read_y(next, js * JJ + h);
+        }
+        constexpr int c0 = m * PER_STEP < COPIES ? m * PER_STEP : COPIES;
+        constexpr int c1 = (m + 1) * PER_STEP < COPIES ? (m + 1) * PER_STEP : COPIES;
+        static_assert(c0 == c1 || m < COPY_STEPS, "copies lie in front of the wait");
+        if constexpr (c0 < c1) {
+          if (more) {
+            copy_some(first + t + SLOTS - 1, refill, std::integral_constant<int, c0>{}, std::integral_constant<int, c1>{});
+          }
+        }
+        if constexpr (m >= LAG) {
+          add(std::integral_constant<int, m - LAG>{}, false);
+        } else if constexpr (CARRY) {
+          add(std::integral_constant<int, m - LAG + STEPS>{}, true);
+        }
+        if constexpr (FLOAT_SCALES && !T::kBlocks && js == LAG - 1) {
+          read_scales_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
+        }
+        if constexpr (T::kWide) {
+          // the next X fragment becomes fp16 a part at a time; a Y fragment of the next piece where the last products
+          // with its predecessor have been issued
+          static_for<4>([&](auto quarter) {
+            constexpr int q = quarter;
+            if constexpr ((q * SPT) / 4 == js) widen_quarter<FX>(raw_x, x[to][0], q);
+          });
+          if constexpr (at_end) {
+#pragma unroll
+            for (int h = 0; h < JJ; ++h) {
+              const int j = js * JJ + h;
+              y[0][j] = widened<FY>(raw_y[j % 2]);
+              if (j + 2 < NY) read_y(next, j + 2);
             }
           }
         }
-      }
-    } else if constexpr (MODE == kScaledE8m0) {
-      const int *const sx = reinterpret_cast<const int *>(scales) + wx * TX;
-      const int *const sy = reinterpret_cast<const int *>(scales) + BX + wy * TY;
-      int s[NY];
+      });
+      if constexpr (FLOAT_SCALES) {
+        if constexpr (CARRY) {
 #pragma unroll
-      for (int j = 0; j < NY; ++j) s[j] = sy[j * 16 + fr];
+          for (int r = 0; r < LAG; ++r) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const Fragment x = read(slot, x_rows + i * 16 * kPieceBytes);
-        const int t = sx[i / NT * GROUP_ROWS + (fr >> 2) * 4 * NT + i % NT * 4 + (fr & 3)];
-#pragma unroll
-        for (int j = 0; j < NY; ++j) acc[0][j][i] = mfma8<FX, FY>(x, y[0][j], acc[0][j][i], t, s[j]);
-      }
-    } else if constexpr (MODE == kHalf) {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const Fragment x = read(slot, x_rows + i * 16 * kPieceBytes);
-#pragma unroll
-        for (int j = 0; j < NY; ++j) acc[0][j][i] = mfma16(x, y[0][j], acc[0][j][i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const Fragment xh = read(slot, x_rows + i * 16 * kPieceBytes);
-        const Fragment xl = read(slot, x_rows + BX * kPieceBytes + i * 16 * kPieceBytes);
-#pragma unroll
-        for (int j = 0; j < NY; ++j) {
-          acc[0][j][i] = mfma16(xh, y[0][j], acc[0][j][i]);
-          acc[T::kSums - 1][j][i] = mfma16(xh, y[PLANES - 1][j], acc[T::kSums - 1][j][i]);
-          acc[T::kSums - 1][j][i] = mfma16(xl, y[0][j], acc[T::kSums - 1][j][i]);
+            for (int h = 0; h < JJ; ++h) {
+              const int m = STEPS - LAG + r;
+              s_old[m % RING * JJ + h] = s[m % SPT * JJ + h];
+            }
+          }
+        } else {
+          static_for<LAG>([&](auto r) { add(std::integral_constant<int, STEPS - LAG + r>{}, false); });
         }
       }
-    }
-  };
-
-  // ---- K loop ----
-  const unsigned n = last > first ? last - first : 0;
+      if constexpr (NX % 2 == 1) {   // (the next piece's first tile, where its predecessor was in use)
 #pragma unroll
-  for (int t = 0; t < SLOTS - 1; ++t) {
-    if ((unsigned)t < n) copy(first + t, t);
-  }
-  unsigned slot = 0, refill = SLOTS - 1;
-#pragma unroll 1
-  for (unsigned t = 0; t < n; ++t) {
-    if (t + SLOTS - 1 < n + (SLOTS > 2 ? 1 : 0)) {   // (SLOTS - 2 later pieces are on their way)
-      wait_copies_then_barrier<COPIES * (SLOTS - 2)>();
-    } else {
-      wait_copies_then_barrier<0>();
+        for (int p = 0; p < PLANES; ++p) x[0][p] = x[1][p];
+        sx[0] = sx[1];
+        e8x[0] = e8x[1];
+      }
+      take_scales_y();
+      refill = slot;
+      slot = next;
     }
-    if (t + SLOTS - 1 < n) copy(first + t + SLOTS - 1, refill);
-    multiply(slot);
-    refill = slot;
-    slot = slot + 1 == SLOTS ? 0 : slot + 1;
+    if constexpr (FLOAT_SCALES && CARRY) {
+      static_for<LAG>([&](auto r) { add(std::integral_constant<int, STEPS - LAG + r>{}, true); });
+    }
   }
 
   if constexpr (MODE == kHalfPairs) {
@@ -429,20 +626,33 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     }
   }
 
-  // ---- pieces of K joined: in the order of the pieces, whichever block arrives last ----
+  // ---- parts of K joined: in the order of the parts, whichever block arrives last ----
+  // The sums go past the L2 of this XCD and are read past the reader's (stores and loads of agent scope), so that no
+  // cache has to be written back or emptied: with fences of agent scope in their place a product in two parts took 55 us
+  // where this takes
   if (args.parts > 1) {
-    constexpr size_t BLOCK = (size_t)BX * BY;   // floats
-    float4_t *const mine = reinterpret_cast<float4_t *>(args.partial + ((size_t)at.tile * args.parts + at.part) * BLOCK);
+    typedef unsigned long long piece_t;
+    constexpr int PIECES = 2;     // of a lane's four sums
+    constexpr size_t BLOCK = (size_t)BX * BY / PIECES;
+    piece_t *const all = reinterpret_cast<piece_t *>(args.partial) + (size_t)at.tile * args.parts * BLOCK;
+    piece_t *const mine = all + at.part * BLOCK + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < NY; ++j) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) mine[(j * NX + i) * (64 * WAVES) + threadIdx.x] = acc[0][j][i];
+      for (int i = 0; i < NX; ++i) {
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+          const float pair[2] = {acc[0][j][i][2 * h], acc[0][j][i][2 * h + 1]};
+          __hip_atomic_store(mine + ((j * NX + i) * PIECES + h) * (64 * WAVES), __builtin_bit_cast(piece_t, pair), __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
     }
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stores have arrived
     __syncthreads();
     unsigned *const flag = reinterpret_cast<unsigned *>(lds);
     if (threadIdx.x == 0) {
-      const unsigned before = __hip_atomic_fetch_add(args.arrived + at.tile, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+      const unsigned before = __hip_atomic_fetch_add(args.arrived + at.tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       *flag = before + 1 == args.parts;
       if (before + 1 == args.parts) {
         __hip_atomic_store(args.arrived + at.tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -450,20 +660,27 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     }
     __syncthreads();
     if (!*flag) return;
-    __threadfence();
-    const float4_t *from = reinterpret_cast<const float4_t *>(args.partial + (size_t)at.tile * args.parts * BLOCK);
-#pragma unroll
-    for (int j = 0; j < NY; ++j) {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) acc[0][j][i] = from[(j * NX + i) * (64 * WAVES) + threadIdx.x];
-    }
+    const piece_t *from = all + threadIdx.x;
 #pragma unroll 1
-    for (unsigned p = 1; p < args.parts; ++p) {
-      from += BLOCK / 4;
+    for (unsigned p = 0; p < args.parts; ++p, from += BLOCK) {
 #pragma unroll
       for (int j = 0; j < NY; ++j) {
 #pragma unroll
-        for (int i = 0; i < NX; ++i) acc[0][j][i] += from[(j * NX + i) * (64 * WAVES) + threadIdx.x];
+        for (int i = 0; i < NX; ++i) {
+#pragma unroll
+          for (int h = 0; h < PIECES; ++h) {
+            const piece_t u = __hip_atomic_load(from + ((j * NX + i) * PIECES + h) * (64 * WAVES), __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+            const unsigned lo = (unsigned)u, hi = (unsigned)(u >> 32);
+            if (p == 0) {
+              acc[0][j][i][2 * h] = __builtin_bit_cast(float, lo);
+              acc[0][j][i][2 * h + 1] = __builtin_bit_cast(float, hi);
+            } else {
+              acc[0][j][i][2 * h] += __builtin_bit_cast(float, lo);
+              acc[0][j][i][2 * h + 1] += __builtin_bit_cast(float, hi);
+            }
+          }
+        }
       }
     }
   }

@@ -49,7 +49,7 @@ def test_scaled_linear_refuses(change, message):
 @pytest.mark.parametrize("change,message", [
     (dict(type=VT.float8e4m3), "matrices are float32"), (dict(steps=0), "1 to 1000 steps"), (dict(epsilon=-1.0), "epsilon"),
     (dict(epsilon=float("nan")), "epsilon"), (dict(input_pitch=7), "at a distance"), (dict(output_pitch=7), "at a distance"),
-    (dict(B=65536), "size out of range"), (dict(M=(1 << 21) + 1), "size out of range")])
+    (dict(B=65536), "size out of range"), (dict(M=(1 << 20) + 1), "size out of range")])
 def test_orthogonalize_refuses(change, message):
     args = dict(B=1, M=8, N=8, device=0, stream=0)
     args.update(change)
