@@ -183,6 +183,8 @@ __device__ __forceinline__ const char *uniform(const char *p) {
   const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
   return (const char *)(((unsigned long long)hi << 32) | lo);
 }
+__device__ __forceinline__ unsigned uniform(unsigned u) { return (unsigned)__builtin_amdgcn_readfirstlane((int)u); }
+
 // Which block of D, and which piece of K, a workgroup has.
 struct Place {
   unsigned b, bx, by, part, tile;
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   constexpr int OPERAND_COPIES = COPIES_ALL / WAVES;
   constexpr int SCALE_COPIES = T::kScaled ? (BX + BY + 63) / 64 : 0;
   constexpr int COPIES = OPERAND_COPIES + (T::kScaled ? 1 : 0);
-  static_assert(COPIES_ALL % WAVES == 0 && SCALE_COPIES <= WAVES && NX % NT == 0, "shape");
+  static_assert(BX / 8 % WAVES == 0 && BY / 8 % WAVES == 0 && SCALE_COPIES <= WAVES && NX % NT == 0, "shape");
   __shared__ __attribute__((aligned(256))) char lds[S::kLdsBytes];
 
   const int lane = threadIdx.x & 63;
@@ -259,9 +261,9 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   unsigned offset[OPERAND_COPIES];
 #pragma unroll
   for (int n = 0; n < OPERAND_COPIES; ++n) {
-    int q = wave + n * WAVES;
-    const bool of_x = q < X_COPIES;
-    if (!of_x) q -= X_COPIES;
+    // (a wave's n-th copy of a piece: of which operand is known beforehand)
+    const bool of_x = n < X_COPIES / WAVES;
+    const int q = wave + (of_x ? n : n - X_COPIES / WAVES) * WAVES;
     const int row = (q % ((of_x ? BX : BY) / 8)) * 8 + (lane >> 3);
     unsigned want = row;
     if (of_x) {   // row `row` of LDS holds this row of the block
@@ -286,38 +288,38 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     scale_base = (of_x ? args.x_scales : args.y_scales) + (size_t)at.b * args.pieces * scale_step;
     scale_lds = j * 256;
   }
-  // Copies `from_copy` to `to_copy` - 1 of the wave's COPIES of a piece
-  auto copy_some = [&](unsigned piece, unsigned slot, auto from_copy, auto to_copy) {
+  // Where the next piece to be copied is, and the slot of LDS that it goes to
+  const char *x_next = x_base + (size_t)first * kPieceBytes, *y_next = y_base + (size_t)first * kPieceBytes;
+  const char *scales_next = scale_base + (size_t)first * scale_step;
+  unsigned piece_next = first;
+  // Copy n of the wave's COPIES of that piece. `end`: the piece may end inside its 128 bytes; what lies beyond is zero
+  // (the copies of a piece have no branch, and of the two kinds of loop below only the last one asks).
+  auto copy_one = [&](unsigned slot, auto copy, auto end) {
+    constexpr int n = decltype(copy)::value;
     const unsigned to = lds_base + slot * S::kSlotBytes;
-    const size_t k = (size_t)piece * kPieceBytes;
-    const bool whole = (piece + 1) * (unsigned)kPieceBytes <= args.k_bytes;
-    // (values, so that choosing one of them is no choice of an address of this function's variables)
-    const char *const xk = x_base + k, *const yk = y_base + k;
-    const size_t x_plane = args.x_plane, y_plane = args.y_plane;
-#pragma unroll
-    for (int n = from_copy; n < to_copy; ++n) {
-      if (T::kScaled && n == OPERAND_COPIES) {
-        load_scales_to_lds<T::kScaleBytes>(
-            uniform(scale_base + (size_t)piece * scale_step), scale_offset,
-            (unsigned)__builtin_amdgcn_readfirstlane((int)(to + S::kXBytes + S::kYBytes + scale_lds)));
-        continue;
-      }
-      const int q = wave + n * WAVES;
-      const bool of_x = q < X_COPIES;
-      const int plane = PLANES == 1 ? 0 : of_x ? q / (BX / 8) : (q - X_COPIES) / (BY / 8);
-      const char *from = of_x ? xk : yk;
-      if (PLANES > 1 && plane) from += of_x ? x_plane : y_plane;
-      const unsigned at_lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(to + q * 1024));
-      if (whole) {
+    if constexpr (T::kScaled && n == OPERAND_COPIES) {
+      load_scales_to_lds<T::kScaleBytes>(uniform(scales_next), scale_offset, uniform(to + S::kXBytes + S::kYBytes + scale_lds));
+    } else {
+      constexpr bool of_x = n < X_COPIES / WAVES;
+      constexpr int in = of_x ? n : n - X_COPIES / WAVES, plane = in / ((of_x ? BX : BY) / 8 / WAVES);
+      const char *from = of_x ? x_next : y_next;
+      if constexpr (plane > 0) from += of_x ? args.x_plane : args.y_plane;
+      const unsigned at_lds = uniform(to + (wave + n * WAVES) * 1024);
+      if constexpr (!decltype(end)::value) {
         load_1k_to_lds(uniform(from), offset[n], at_lds);
       } else {
-        load_1k_to_lds_by_lane(k + chunk * 16 < args.k_bytes ? from + offset[n] : g_zeros, at_lds);
+        load_1k_to_lds_by_lane((size_t)piece_next * kPieceBytes + chunk * 16 < args.k_bytes ? from + offset[n] : g_zeros, at_lds);
       }
     }
   };
-  auto copy = [&](unsigned piece, unsigned slot) {
-    copy_some(piece, slot, std::integral_constant<int, 0>{}, std::integral_constant<int, COPIES>{});
+  auto advance = [&]() {
+    x_next += kPieceBytes;
+    y_next += kPieceBytes;
+    if constexpr (T::kScaled) scales_next += scale_step;
+    ++piece_next;
   };
+  const std::true_type may_end{};
+  const std::false_type whole{};
   static_assert(!T::kScaled || BX % 64 == 0, "scales of X fill whole copies");
 
   // ---- fragments ----
@@ -360,7 +362,10 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   if (n > 0) {
 #pragma unroll
     for (int t = 0; t < SLOTS - 1; ++t) {
-      if ((unsigned)t < n) copy(first + t, t);
+      if ((unsigned)t < n) {
+        static_for<COPIES>([&](auto c) { copy_one(t, c, may_end); });
+        advance();
+      }
     }
     using Operand = typename std::conditional<T::kWide, WideFragment, Fragment>::type;
     Operand y[PLANES][NY], x[2][PLANES];
@@ -484,16 +489,12 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
       }
     };
 
-    // (SLOTS - 2 later pieces are on their way, if there are as many)
-    auto wait = [&](unsigned t) {
-      if (t + SLOTS - 1 < n + (SLOTS > 2 ? 1 : 0)) {
-        wait_copies_then_barrier<COPIES * (SLOTS - 2)>();
-      } else {
-        wait_copies_then_barrier<0>();
-      }
-    };
     unsigned slot = 0, refill = SLOTS - 1;
-    wait(0);
+    if (n >= (unsigned)SLOTS - 1) {   // (SLOTS - 2 later pieces are on their way)
+      wait_copies_then_barrier<COPIES * (SLOTS - 2)>();
+    } else {
+      wait_copies_then_barrier<0>();
+    }
     read_scales_y(0);
     take_scales_y();
     read_scales_x(0, 0, 0);
@@ -514,19 +515,20 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
       }
       if constexpr (!T::kBlocks) sx[1] = 0.f;
     }
-#pragma unroll 1
-    for (unsigned t = 0; t < n; ++t) {
+    // One piece. REFILL: 0 no further piece is copied; 1 one is, a whole one; 2 one is, perhaps the last, partial one
+    auto piece = [&](auto refill_kind) {
+      constexpr int REFILL = decltype(refill_kind)::value;
       const unsigned next = slot + 1 == SLOTS ? 0 : slot + 1;
-      const bool more = t + SLOTS - 1 < n;
+      const typename std::conditional<REFILL == 2, std::true_type, std::false_type>::type end{};
       static_for<STEPS>([&](auto step) {
         constexpr int m = step, i = m / SPT, js = m % SPT, to = (i + 1) % 2;
         constexpr bool at_end = i == NX - 1;
         CCGLIB_PIN;
-        if constexpr (COPY_STEPS == 0 && m == 0) {
-          if (more) copy(first + t + SLOTS - 1, refill);
-        }
+        if constexpr (COPY_STEPS == 0 && m == 0 && REFILL > 0) static_for<COPIES>([&](auto c) { copy_one(refill, c, end); });
         if constexpr (at_end && js == 0) {
-          if (t + 1 < n) wait(t + 1);
+          // (as many later pieces are on their way; behind the last copies all of them have to have arrived)
+          constexpr int LATER = REFILL != 0 ? COPIES * (SLOTS - 2) : 0;
+          wait_copies_then_barrier<LATER>();
           read_scales_y(next);
         }
         if constexpr (js == 0) {
@@ -559,10 +561,8 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
         constexpr int c0 = m * PER_STEP < COPIES ? m * PER_STEP : COPIES;
         constexpr int c1 = (m + 1) * PER_STEP < COPIES ? (m + 1) * PER_STEP : COPIES;
         static_assert(c0 == c1 || m < COPY_STEPS, "copies lie in front of the wait");
-        if constexpr (c0 < c1) {
-          if (more) {
-            copy_some(first + t + SLOTS - 1, refill, std::integral_constant<int, c0>{}, std::integral_constant<int, c1>{});
-          }
+        if constexpr (c0 < c1 && REFILL > 0) {
+          static_for<c1 - c0>([&](auto c) { copy_one(refill, std::integral_constant<int, c0 + decltype(c)::value>{}, end); });
         }
         if constexpr (m >= LAG) {
           add(std::integral_constant<int, m - LAG>{}, false);
@@ -610,9 +610,21 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
         e8x[0] = e8x[1];
       }
       take_scales_y();
+      if constexpr (REFILL > 0) advance();
       refill = slot;
       slot = next;
+    };
+    // (the piece that K ends in, if it is this block's)
+    const unsigned n_whole = (size_t)last * kPieceBytes <= args.k_bytes ? n : n - 1;
+    unsigned t = 0;
+#pragma unroll 1
+    for (; t + SLOTS - 1 < n_whole; ++t) piece(std::integral_constant<int, 1>{});
+    if (t + SLOTS - 1 < n) {
+      piece(std::integral_constant<int, 2>{});
+      ++t;
     }
+#pragma unroll 1
+    for (; t < n; ++t) piece(std::integral_constant<int, 0>{});
     if constexpr (FLOAT_SCALES && CARRY) {
       static_for<LAG>([&](auto r) { add(std::integral_constant<int, STEPS - LAG + r>{}, true); });
     }
