@@ -117,6 +117,7 @@ class Option(enum.IntEnum):
     gemm_block_tile = 3
     expect_unaligned = 4
     pipeline_route = 5
+    real_block = 6
 
 
 def set_option(option, value):

@@ -17,6 +17,7 @@
 #include "../../include/ccglib_amd.h"
 #include "common.h"
 #include "host_util.h"
+#include "scaled.h"
 
 using namespace ccglib_amd;
 
@@ -25,6 +26,8 @@ thread_local std::string g_last_error;
 }  // namespace
 
 namespace ccglib_amd {
+
+size_t real_block_option = 0;
 
 int fail(int code, const char *fmt, ...) {
   char buf[512];
@@ -174,7 +177,7 @@ struct ccglib_pipeline {
 namespace {
 
 // Process-wide options (ccglib_amd_set_option), read when an object is created.
-size_t g_options[CCGLIB_AMD_OPTION_COUNT] = {0, 1, 0, 0, 0, 0};
+size_t g_options[CCGLIB_AMD_OPTION_COUNT] = {0, 1, 0, 0, 0, 0, 0};
 
 // Largest buffer of 1-bit tiles a pipeline allocates; beyond it the pipeline
 // runs the reference's sequence of kernels on its packed / transposed buffers.
@@ -386,6 +389,12 @@ int ccglib_amd_set_option(int option, size_t value) {
   }
   if (option == CCGLIB_AMD_OPTION_PIPELINE_ROUTE && value > 2) {
     return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "PIPELINE_ROUTE is 0, 1 or 2 (got %zu)", value);
+  }
+  if (option == CCGLIB_AMD_OPTION_REAL_BLOCK) {
+    if (value && (value % 256 < 1 || value % 256 > 16 || value / 256 > 65535)) {
+      return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "REAL_BLOCK is 0, or 1 to 16 plus 256 times at most 65535 (got %zu)", value);
+    }
+    real_block_option = value;
   }
   g_options[option] = value;
   return CCGLIB_OK;

@@ -8,16 +8,46 @@
 namespace ccglib_amd {
 namespace real {
 
-// Matrices of the chain: fp16, or two fp16 for each value (v = first + second * 2^-11), a plane each.
+// Matrices of the chain: fp16, or two fp16 for each value (v = first + second * 2^-11), a plane each. Rows are padded to a
+// whole 128 bytes, with zeros.
 template <bool PAIRS> struct Halves {
-  static __device__ __forceinline__ float get(const _Float16 *p, size_t at, size_t plane) {
-    const float h = (float)p[at];
-    return PAIRS ? __builtin_fmaf((float)p[at + plane], 0x1p-11f, h) : h;
-  }
-  static __device__ __forceinline__ void put(_Float16 *p, size_t at, size_t plane, float v) {
+  static __device__ __forceinline__ _Float16 part(float v, int plane) {
     const _Float16 h = (_Float16)v;
-    p[at] = h;
-    if (PAIRS) p[at + plane] = (_Float16)((v - (float)h) * 0x1p11f);
+    return plane == 0 ? h : (_Float16)((v - (float)h) * 0x1p11f);
+  }
+  static __device__ __forceinline__ void put(_Float16 *p, size_t plane, float v) {
+    p[0] = part(v, 0);
+    if (PAIRS) p[plane] = part(v, 1);
+  }
+  // N (4, 8 or 16) neighbours, at a multiple of N
+  template <int N> static __device__ __forceinline__ void load(const _Float16 *p, size_t plane, float (&v)[N]) {
+    constexpr int E = N < 8 ? N : 8;
+    typedef _Float16 piece_t __attribute__((ext_vector_type(E)));
+#pragma unroll
+    for (int i = 0; i < N; i += E) {
+      const piece_t h = *reinterpret_cast<const piece_t *>(p + i);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i + e] = (float)h[e];
+      if constexpr (PAIRS) {
+        const piece_t l = *reinterpret_cast<const piece_t *>(p + plane + i);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i + e] = __builtin_fmaf((float)l[e], 0x1p-11f, v[i + e]);
+      }
+    }
+  }
+  template <int N> static __device__ __forceinline__ void store(_Float16 *p, size_t plane, const float (&v)[N]) {
+    constexpr int E = N < 8 ? N : 8;
+    typedef _Float16 piece_t __attribute__((ext_vector_type(E)));
+#pragma unroll
+    for (int k = 0; k < (PAIRS ? 2 : 1); ++k) {
+#pragma unroll
+      for (int i = 0; i < N; i += E) {
+        piece_t w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = part(v[i + e], k);
+        *reinterpret_cast<piece_t *>(p + k * plane + i) = w;
+      }
+    }
   }
 };
 
@@ -50,77 +80,105 @@ template <bool PAIRS, int STEP> struct StoreChain {
   const Params &p;
   __device__ explicit StoreChain(const Params &params) : p(params) {}
 
-  template <int N>
-  __device__ __forceinline__ void store(unsigned b, unsigned y, unsigned x, const float (&v)[N], bool mirror) const {
+  // The group's transpose, through LDS into rows of whole pieces of 16 bytes: two lanes with neighbouring y exchange the other's
+  // half of each pair of x, so that LDS is written 4 bytes at a time.
+  template <int NY, int N>
+  __device__ __forceinline__ void store_transposed(const Group &g, const float (&v)[NY][N], _Float16 *t, size_t pitch, size_t plane) const {
     using H = Halves<PAIRS>;
-    const float f = p.factor ? p.factor[b] : 1.f;
-    const unsigned left = p.nx - x;
-    float *const diagonal = p.diagonal + (size_t)b * p.diagonal_pitch;
-    float *const diagonal_p = p.diagonal_p + (size_t)b * p.diagonal_pitch;
-    const _Float16 *const old = p.old + (size_t)b * p.old_batch + (size_t)y * p.old_pitch + x;
-    float w[N];
-    if constexpr (STEP == kGram) {
+    constexpr int PITCH = kGroupPitch<NY>, CHUNKS = NY * 2;      // pieces of a row
+    const int fr = g.lane & 15;
+    const bool odd = fr & 1;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        w[e] = f * f * v[e];
-        if (x + e == y) {
-          diagonal[y] = w[e];
-          w[e] = 0.f;
+    for (int k = 0; k < (PAIRS ? 2 : 1); ++k) {
+#pragma unroll
+      for (int j = 0; j < NY; ++j) {
+        const bool inside = g.y + j * 16 + fr < p.ny;           // (behind the rows' end: zeros)
+        char *const to = g.lds + ((g.lane >> 4) * N + odd) * PITCH + (j * 16 + (fr & ~1)) * 2;
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+          const half2_t two = {H::part(v[j][e], k), H::part(v[j][e + 1], k)};
+          const unsigned mine = inside ? __builtin_bit_cast(unsigned, two) : 0u;
+          const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)mine, 0xb1, 0xf, 0xf, true);   // lane ^ 1
+          // even y: x = e of both; odd y: x = e + 1 of both
+          *reinterpret_cast<unsigned *>(to + e * PITCH) = __builtin_amdgcn_perm(mine, other, odd ? 0x07060302u : 0x01000504u);
         }
       }
-    } else if constexpr (STEP == kSquare) {
-      const float dy = diagonal[y];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if ((unsigned)e < left) {
-          if (x + e == y) {
-            diagonal_p[y] = __builtin_fmaf(p.c, __builtin_fmaf(dy, dy, v[e]), p.b * dy);
-            w[e] = 0.f;
-          } else {
-            const float o = H::get(old, e, p.old_plane);
-            w[e] = __builtin_fmaf(p.c, __builtin_fmaf(dy + diagonal[x + e], o, v[e]), p.b * o);
-          }
-        }
+      for (int r = 0; r < 4 * N * CHUNKS / 64; ++r) {
+        const int at = r * 64 + g.lane, row = at / CHUNKS, chunk = at % CHUNKS;
+        const int4_t piece = *reinterpret_cast<const int4_t *>(g.lds + row * PITCH + chunk * 16);
+        const unsigned x = g.x + row, y = g.y + chunk * 8;
+        if (x < p.nx && y < p.ny) *reinterpret_cast<int4_t *>(t + k * plane + (size_t)x * pitch + y) = piece;
       }
-    } else {
-      const float dy = STEP == kUpdate ? p.a + diagonal_p[y] : 0.f;
+    }
+  }
+
+  template <int NY, int N> __device__ __forceinline__ void store(const Group &g, float (&v)[NY][N]) const {
+    using H = Halves<PAIRS>;
+    const float f = p.factor ? p.factor[g.b] : 1.f;
+    const unsigned x = g.x + (g.lane >> 4) * N, left = x < p.nx ? p.nx - x : 0;
+    float *const diagonal = p.diagonal + (size_t)g.b * p.diagonal_pitch;
+    float *const diagonal_p = p.diagonal_p + (size_t)g.b * p.diagonal_pitch;
+    float dx[N];           // of the columns; (rows of diagonals are as long as rows of A, and zero behind their end)
+    if constexpr (STEP == kSquare || STEP == kUpdateT) {
+      const float *const d = (STEP == kSquare ? diagonal : diagonal_p) + x;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if ((unsigned)e < left) {
-          const float d = STEP == kUpdate ? dy : p.a + diagonal_p[x + e];
-          w[e] = f * __builtin_fmaf(d, H::get(old, e, p.old_plane), v[e]);
-        }
-      }
-      if (p.out) {
-        const size_t at = (size_t)b * p.out_batch + (size_t)y * p.out_pitch + x;
+      for (int e = 0; e < N; ++e) dx[e] = left > 0 ? d[e] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NY; ++j) {
+      const unsigned y = g.y + j * 16 + (g.lane & 15);
+      float(&w)[N] = v[j];
+      if (y >= p.ny || left == 0) continue;
+      float old[N];
+      if constexpr (STEP != kGram) H::load(p.old + (size_t)g.b * p.old_batch + (size_t)y * p.old_pitch + x, p.old_plane, old);
+      if constexpr (STEP == kGram) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          if ((unsigned)e < left) {
-            if (p.out_type == kFloat32) {
-              static_cast<float *>(p.out)[at + e] = w[e];
-            } else if (p.out_type == kFloat16) {
-              static_cast<_Float16 *>(p.out)[at + e] = (_Float16)w[e];
-            } else {
-              static_cast<__bf16 *>(p.out)[at + e] = (__bf16)w[e];
-            }
+          w[e] *= f * f;
+          if (x + e == y) {
+            diagonal[y] = w[e];
+            w[e] = 0.f;
           }
         }
-        return;
-      }
-    }
-    _Float16 *const to = p.to + (size_t)b * p.to_batch;
+      } else if constexpr (STEP == kSquare) {
+        const float dy = diagonal[y];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if ((unsigned)e < left) H::put(to, (size_t)y * p.to_pitch + x + e, p.to_plane, w[e]);
-    }
-    if (STEP == kUpdate || mirror) {
-      _Float16 *const t = STEP == kUpdate ? p.to_t + (size_t)b * p.to_t_batch : to;
-      const unsigned pitch = STEP == kUpdate ? p.to_t_pitch : p.to_pitch;
-      const size_t plane = STEP == kUpdate ? p.to_t_plane : p.to_plane;
+        for (int e = 0; e < N; ++e) {
+          if (x + e == y) {
+            diagonal_p[y] = __builtin_fmaf(p.c, __builtin_fmaf(dy, dy, w[e]), p.b * dy);
+            w[e] = 0.f;
+          } else {
+            w[e] = __builtin_fmaf(p.c, __builtin_fmaf(dy + dx[e], old[e], w[e]), p.b * old[e]);
+          }
+        }
+      } else {
+        const float dy = STEP == kUpdate ? diagonal_p[y] : 0.f;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if ((unsigned)e < left) H::put(t, (size_t)(x + e) * pitch + y, plane, w[e]);
+        for (int e = 0; e < N; ++e) w[e] = f * __builtin_fmaf(p.a + (STEP == kUpdate ? dy : dx[e]), old[e], w[e]);
+        if (STEP == kUpdateT || p.out) {
+          const size_t at = (size_t)g.b * p.out_batch + (size_t)y * p.out_pitch + x;
+          if (p.out_type == kFloat32) {
+            store_row(static_cast<float *>(p.out) + at, left, w);
+          } else if (p.out_type == kFloat16) {
+            store_row(static_cast<_Float16 *>(p.out) + at, left, w);
+          } else {
+            store_row(static_cast<__bf16 *>(p.out) + at, left, w);
+          }
+          continue;
+        }
       }
+      if (left < (unsigned)N) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = (unsigned)e < left ? w[e] : 0.f;
+      }
+      H::store(p.to + (size_t)g.b * p.to_batch + (size_t)y * p.to_pitch + x, p.to_plane, w);
+    }
+    if constexpr (STEP == kUpdate) {
+      if (!p.out) store_transposed(g, v, p.to_t + (size_t)g.b * p.to_t_batch, p.to_t_pitch, p.to_t_plane);
+    } else if constexpr (STEP != kUpdateT) {
+      if (g.mirror) store_transposed(g, v, p.to + (size_t)g.b * p.to_batch, p.to_pitch, p.to_plane);
     }
   }
 };
@@ -132,10 +190,6 @@ template <bool PAIRS, int STEP> struct StoreChain {
 #define CCGLIB_HALF_PAIRS_SHAPES(DO) \
   DO(0, 128, 128, 2, 4, 2, 2)        \
   DO(1, 64, 64, 2, 2, 2, 2)
-
-struct HalfShape {
-  unsigned bx, by;
-};
 
 }  // namespace real
 }  // namespace ccglib_amd

@@ -13,11 +13,11 @@
 #include <algorithm>
 
 #include "orthogonalize.h"
+#include "real_plan.h"
 
 namespace ccglib_amd {
 namespace {
 
-constexpr unsigned kUnits = 256;
 constexpr size_t kAlign = 256;
 size_t up(size_t n, size_t to) { return ceil_div(n, to) * to; }
 
@@ -114,13 +114,13 @@ __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::typ
     if (r0 + r < m && c0 + c < n) {
       const float v = __builtin_ldexpf((float)in[((size_t)b * m + r0 + r) * in_pitch + c0 + c], e);
       tile[r][c] = v;
-      H::put(to + (size_t)b * to_batch, (size_t)(r0 + r) * to_pitch + c0 + c, to_plane, v);
+      H::put(to + (size_t)b * to_batch + (size_t)(r0 + r) * to_pitch + c0 + c, to_plane, v);
     }
   }
   __syncthreads();
   for (int r = threadIdx.x >> 6; r < 64; r += 4) {
     if (c0 + r < n && r0 + c < m) {
-      H::put(to_t + (size_t)b * to_t_batch, (size_t)(c0 + r) * to_t_pitch + r0 + c, to_t_plane, tile[c][r]);
+      H::put(to_t + (size_t)b * to_t_batch + (size_t)(c0 + r) * to_t_pitch + r0 + c, to_t_plane, tile[c][r]);
     }
   }
 }
@@ -138,36 +138,29 @@ struct Layout {
 };
 
 struct Product {
-  int shape;
-  unsigned parts, pieces_per_part, blocks_x, blocks_y;
+  RealGemmPlan plan;
+  unsigned blocks_x, blocks_y;
   size_t blocks;                           // in all
 };
 
-constexpr real::HalfShape kHalfShapes[] = {
-#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY},
+constexpr RealShape kHalfShapes[] = {
+#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY, 64 * WX * WY, #BY "x" #BX},
     CCGLIB_HALF_SHAPES(CCGLIB_INFO)
 };
-constexpr real::HalfShape kPairsShapes[] = {
+constexpr RealShape kPairsShapes[] = {
     CCGLIB_HALF_PAIRS_SHAPES(CCGLIB_INFO)
 #undef CCGLIB_INFO
 };
 
 Product plan_product(bool pairs, size_t batch, size_t nx, size_t ny, size_t k, bool symmetric) {
-  const real::HalfShape *shapes = pairs ? kPairsShapes : kHalfShapes;
-  const int count = pairs ? 2 : 3;
+  const RealShape *const shapes = pairs ? kPairsShapes : kHalfShapes;
+  const int count = pairs ? (int)(sizeof kPairsShapes / sizeof kPairsShapes[0]) : (int)(sizeof kHalfShapes / sizeof kHalfShapes[0]);
   Product r = {};
-  const size_t pieces = ceil_div(k, (size_t)64);
-  for (int s = 0; s < count; ++s) {
-    r.shape = s;
-    r.blocks_x = (unsigned)ceil_div(nx, shapes[s].bx);
-    r.blocks_y = (unsigned)ceil_div(ny, shapes[s].by);
-    r.blocks = batch * (symmetric ? (size_t)r.blocks_y * (r.blocks_y + 1) / 2 : (size_t)r.blocks_x * r.blocks_y);
-    if (r.blocks >= (s == 0 ? kUnits : kUnits / 2)) break;
-  }
-  size_t parts = 1;
-  while (r.blocks * parts < kUnits && pieces / (parts * 2) >= 4) parts *= 2;
-  r.pieces_per_part = (unsigned)ceil_div(pieces, parts);
-  r.parts = (unsigned)ceil_div(pieces, (size_t)r.pieces_per_part);
+  r.plan = plan_real_gemm(shapes, count, batch, nx, ny, ceil_div(k, (size_t)64), symmetric);
+  const RealShape &s = shapes[r.plan.shape];
+  r.blocks_x = (unsigned)ceil_div(nx, s.bx);
+  r.blocks_y = (unsigned)ceil_div(ny, s.by);
+  r.blocks = real_blocks(s, batch, nx, ny, symmetric);
   return r;
 }
 
@@ -190,14 +183,12 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.norm_rows = (unsigned)std::max<size_t>(16, ceil_div((size_t)p.m * l.norm_x, 2048));
   l.norm_y = (unsigned)ceil_div(p.m, (size_t)l.norm_rows);
   size_t counters = 0, partial = 0;
-  const real::HalfShape *shapes = pairs ? kPairsShapes : kHalfShapes;
   const Product products[] = {plan_product(pairs, p.batch, l.m, l.m, l.n, true), plan_product(pairs, p.batch, l.m, l.m, l.m, true),
                               plan_product(pairs, p.batch, l.n, l.m, l.m, false),
                               plan_product(pairs, p.batch, l.m, l.n, l.m, false)};
   for (const Product &r : products) {
-    if (r.parts < 2) continue;
-    counters = std::max(counters, r.blocks * sizeof(unsigned));
-    partial = std::max(partial, r.blocks * r.parts * shapes[r.shape].bx * shapes[r.shape].by * sizeof(float));
+    counters = std::max(counters, r.plan.counter_bytes);
+    partial = std::max(partial, r.plan.partial_bytes);
   }
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -207,17 +198,17 @@ Layout layout_of(const OrthogonalizeParams &p) {
   };
   const size_t h = sizeof(_Float16) * l.planes * p.batch;
   l.counters = take(counters);
-  // (the ends of rows, up to a whole 16 bytes of K, are read and never written)
+  // (the ends of rows, up to a whole 16 bytes of K, are read and hold zeros; so do those of diagonals)
   l.x = take(l.x_plane * h);
   l.t0 = take(l.t_plane * h);
   l.t1 = take(l.t_plane * h);
   l.a = take(l.a_plane * h);
   l.p = take(l.a_plane * h);
+  l.diagonal = take(2 * p.batch * l.mp * sizeof(float));
   l.zeroed = at;
   l.partial = take(partial);
   l.norm = take((size_t)p.batch * l.norm_x * l.norm_y * sizeof(double));
   l.factor = take(p.batch * sizeof(float));
-  l.diagonal = take(2 * p.batch * l.mp * sizeof(float));
   l.bytes = at;
   return l;
 }
@@ -226,9 +217,9 @@ template <bool PAIRS, int STEP>
 hipError_t launch_product(const Product &r, const real::Args &a, const typename real::StoreChain<PAIRS, STEP>::Params &e,
                           hipStream_t stream) {
   using Store = real::StoreChain<PAIRS, STEP>;
-  const unsigned grid = (unsigned)(r.blocks * r.parts);
+  const unsigned grid = (unsigned)(r.blocks * r.plan.parts);
   if constexpr (PAIRS) {
-    switch (r.shape) {
+    switch (r.plan.shape) {
 #define CCGLIB_CASE(ID, BX, BY, WX, WY, SLOTS, EU)                                                                        \
   case ID:                                                                                                                \
     real::gemm_real<real::kHalfPairs, 0, 0, BX, BY, WX, WY, SLOTS, EU, Store><<<grid, 64 * WX * WY, 0, stream>>>(a, e); \
@@ -237,7 +228,7 @@ hipError_t launch_product(const Product &r, const real::Args &a, const typename 
 #undef CCGLIB_CASE
     }
   } else {
-    switch (r.shape) {
+    switch (r.plan.shape) {
 #define CCGLIB_CASE(ID, BX, BY, WX, WY, SLOTS, EU)                                                                   \
   case ID:                                                                                                           \
     real::gemm_real<real::kHalf, 0, 0, BX, BY, WX, WY, SLOTS, EU, Store><<<grid, 64 * WX * WY, 0, stream>>>(a, e); \
@@ -298,8 +289,8 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
     g.blocks_x = r.blocks_x;
     g.blocks_y = r.blocks_y;
     g.symmetric = symmetric;
-    g.parts = r.parts;
-    g.pieces_per_part = r.pieces_per_part;
+    g.parts = r.plan.parts;
+    g.pieces_per_part = r.plan.pieces_per_part;
     g.arrived = reinterpret_cast<unsigned *>(ws + l.counters);
     g.partial = reinterpret_cast<float *>(ws + l.partial);
     return g;

@@ -228,9 +228,41 @@ template <int MODE, int BX, int BY, int WX, int WY, int SLOTS> struct Shape {
   static constexpr int kLdsBytes = SLOTS * kSlotBytes;
 };
 
+// N neighbouring values of type T from `to` on, of which `left` are inside the row; `to` is aligned to its element only.
+template <typename T, int N> __device__ __forceinline__ void store_row(T *to, unsigned left, const float (&v)[N]) {
+  constexpr int E = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
+  typedef T piece_t __attribute__((ext_vector_type(E)));
+  typedef piece_t piece_unaligned_t __attribute__((aligned(sizeof(T))));
+  if (left >= (unsigned)N) {
+#pragma unroll
+    for (int i = 0; i < N; i += E) {
+      piece_t w;
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = (T)v[i + e];
+      *reinterpret_cast<piece_unaligned_t *>(to + i) = w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if ((unsigned)e < left) to[e] = (T)v[e];
+    }
+  }
+}
+
+// What an epilogue is given: 16 NT columns of a wave's tile, from x on, of rows y + 16 j + lane % 16; a lane's values are
+// N = 4 NT neighbours from x + N (lane / 16) on. `lds`: kGroupLds bytes for this wave alone.
+struct Group {
+  unsigned b, y, x;
+  int lane;
+  bool mirror;      // D is symmetric, and this block's transpose has no block of its own
+  char *lds;
+};
+// Rows of a wave's group in LDS, transposed, of 16-bit values: 16 bytes apart from a multiple of 128 bytes, which spreads the
+// pieces of a column over the banks
+template <int NY> constexpr int kGroupPitch = NY * 16 * 2 + 16;
+
 // Epilogue: has `Params`, a constructor from them, and
-//   template <int N> void store(unsigned b, unsigned y, unsigned x, const float (&v)[N], bool mirror)
-// for N consecutive x of row y (which may lie beyond D); mirror: D[x][y] is wanted as well.
+//   template <int NY, int N> void store(const Group &, float (&v)[NY][N])
 template <int MODE, int FX, int FY, int BX, int BY, int WX, int WY, int SLOTS, int WAVES_PER_EU, class Epilogue>
 __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args args, typename Epilogue::Params params) {
   using S = Shape<MODE, BX, BY, WX, WY, SLOTS>;
@@ -671,7 +703,9 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
       }
     }
     __syncthreads();
-    if (!*flag) return;
+    const bool is_last = *flag != 0;
+    __syncthreads();   // (the epilogue uses the LDS that the flag is in)
+    if (!is_last) return;
     const piece_t *from = all + threadIdx.x;
 #pragma unroll 1
     for (unsigned p = 0; p < args.parts; ++p, from += BLOCK) {
@@ -699,21 +733,27 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
 
   // ---- epilogue ----
   const Epilogue epilogue(params);
-  const bool mirror = args.symmetric && at.bx != at.by;
+  constexpr int GROUP_LDS = GROUP_ROWS * kGroupPitch<NY>;
+  static_assert(WAVES * GROUP_LDS <= S::kLdsBytes, "the ring holds a group of every wave");
+  Group group;
+  group.b = at.b;
+  group.y = y0 + wy * TY;
+  group.lane = lane;
+  group.mirror = args.symmetric && at.bx != at.by;
+  group.lds = lds + wave * GROUP_LDS;
 #pragma unroll
-  for (int j = 0; j < NY; ++j) {
-    const unsigned y = y0 + wy * TY + j * 16 + fr;
+  for (int i = 0; i < NX; i += NT) {
+    group.x = x0 + wx * TX + i / NT * GROUP_ROWS;
+    float v[NY][4 * NT];
 #pragma unroll
-    for (int i = 0; i < NX; i += NT) {
-      const unsigned x = x0 + wx * TX + i / NT * GROUP_ROWS + g * 4 * NT;
-      float v[4 * NT];
+    for (int j = 0; j < NY; ++j) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * t + e] = acc[0][j][i + t][e];
+        for (int e = 0; e < 4; ++e) v[j][4 * t + e] = acc[0][j][i + t][e];
       }
-      if (y < args.ny && x < args.nx) epilogue.template store<4 * NT>(at.b, y, x, v, mirror);
     }
+    if (group.y < args.ny && group.x < args.nx) epilogue.store(group, v);
   }
 }
 

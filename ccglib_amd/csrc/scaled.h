@@ -36,6 +36,14 @@ struct RealGemmPlan {
   size_t partial_bytes = 0, counter_bytes = 0;
 };
 
+// A block shape of the real products' kernel: columns and rows of a block, threads.
+struct RealShape {
+  unsigned bx, by, threads;
+  const char *name;
+};
+// The option REAL_BLOCK: 0, or a shape's number + 1, plus 256 times the number of parts that K is cut into (0: chosen).
+extern size_t real_block_option;
+
 struct ScaledGemmParams {
   const void *a, *b, *scales_a, *scales_b;
   void *c;

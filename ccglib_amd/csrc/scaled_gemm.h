@@ -15,11 +15,7 @@
 namespace ccglib_amd {
 namespace real {
 
-// Block shapes: BX (columns of C) x BY (rows), waves, ring.
-struct ShapeInfo {
-  unsigned bx, by;
-  const char *name;
-};
+// Block shapes: BX (columns of C) x BY (rows), waves, ring, waves a SIMD
 #define CCGLIB_SCALED_SHAPES(DO) \
   DO(0, 256, 256, 2, 4, 2, 2)    \
   DO(1, 128, 128, 2, 2, 2, 2)    \
@@ -42,43 +38,25 @@ struct StoreC {
   const Params &p;
   __device__ explicit StoreC(const Params &params) : p(params) {}
 
-  template <typename T, int N> __device__ __forceinline__ void put(size_t at, unsigned left, const float (&v)[N]) const {
-    typedef T piece_t __attribute__((ext_vector_type(16 / sizeof(T) < N ? 16 / sizeof(T) : N)));
-    typedef piece_t piece_unaligned_t __attribute__((aligned(sizeof(T))));
-    constexpr int E = sizeof(piece_t) / sizeof(T);
-    T *to = reinterpret_cast<T *>(p.c) + at;
-    if (left >= (unsigned)N) {
+  template <int NY, int N> __device__ __forceinline__ void store(const Group &g, float (&v)[NY][N]) const {
+    const unsigned x = g.x + (g.lane >> 4) * N, left = x < p.nx ? p.nx - x : 0;
 #pragma unroll
-      for (int i = 0; i < N; i += E) {
-        piece_t w;
+    for (int j = 0; j < NY; ++j) {
+      const unsigned y = g.y + j * 16 + (g.lane & 15);
+      if (y >= p.ny || left == 0) continue;
+      const size_t at = (size_t)g.b * p.batch + (size_t)y * p.pitch + x;
+      if (p.accumulate) {   // (32-bit C)
+        float *const c = reinterpret_cast<float *>(p.c) + at;
 #pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = (T)v[i + e];
-        *reinterpret_cast<piece_unaligned_t *>(to + i) = w;
+        for (int e = 0; e < N; ++e) v[j][e] += (unsigned)e < left ? c[e] : 0.f;
+        store_row(c, left, v[j]);
+      } else if (p.type == kFloat32) {
+        store_row(reinterpret_cast<float *>(p.c) + at, left, v[j]);
+      } else if (p.type == kFloat16) {
+        store_row(reinterpret_cast<_Float16 *>(p.c) + at, left, v[j]);
+      } else {
+        store_row(reinterpret_cast<__bf16 *>(p.c) + at, left, v[j]);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if ((unsigned)e < left) to[e] = (T)v[e];
-      }
-    }
-  }
-
-  template <int N>
-  __device__ __forceinline__ void store(unsigned b, unsigned y, unsigned x, const float (&v)[N], bool) const {
-    const size_t at = (size_t)b * p.batch + (size_t)y * p.pitch + x;
-    const unsigned left = p.nx - x;
-    if (p.accumulate) {   // (32-bit C)
-      const float *old = reinterpret_cast<const float *>(p.c) + at;
-      float w[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = (unsigned)e < left ? v[e] + old[e] : 0.f;
-      put<float>(at, left, w);
-    } else if (p.type == kFloat32) {
-      put<float>(at, left, v);
-    } else if (p.type == kFloat16) {
-      put<_Float16>(at, left, v);
-    } else {
-      put<__bf16>(at, left, v);
     }
   }
 };

@@ -2,18 +2,18 @@
 #include <algorithm>
 #include <cstdio>
 
+#include "real_plan.h"
 #include "scaled_gemm.h"
 
 namespace ccglib_amd {
 namespace {
 
-constexpr real::ShapeInfo kShapes[2][4] = {
-#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY, #BY "x" #BX},
+constexpr RealShape kShapes[2][4] = {
+#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY, 64 * WX * WY, #BY "x" #BX},
     {CCGLIB_SCALED_SHAPES(CCGLIB_INFO)},
     {CCGLIB_WIDE_SHAPES(CCGLIB_INFO)}
 #undef CCGLIB_INFO
 };
-constexpr unsigned kUnits = 256;
 
 bool is_wide(const ScaledGemmParams &p) { return p.type_c == kFloat32; }
 
@@ -25,21 +25,7 @@ int mode_of(const ScaledGemmParams &p) {
 }  // namespace
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
-  RealGemmPlan plan;
-  const size_t pieces = std::max<size_t>(1, ceil_div(p.k, (size_t)real::kPieceBytes));
-  const real::ShapeInfo *const shapes = kShapes[is_wide(p)];
-  auto blocks = [&](int s) { return (size_t)p.batch * ceil_div(p.n, shapes[s].bx) * ceil_div(p.m, shapes[s].by); };
-  plan.shape = p.m <= 32 ? 3 : blocks(0) >= kUnits ? 0 : blocks(1) >= kUnits / 2 ? 1 : 2;
-  const size_t n = blocks(plan.shape);
-  size_t parts = 1;
-  while (n * parts < kUnits && pieces / (parts * 2) >= 4) parts *= 2;
-  plan.pieces_per_part = (unsigned)ceil_div(pieces, parts);
-  plan.parts = (unsigned)ceil_div(pieces, (size_t)plan.pieces_per_part);
-  if (plan.parts > 1) {
-    plan.partial_bytes = n * plan.parts * shapes[plan.shape].bx * shapes[plan.shape].by * sizeof(float);
-    plan.counter_bytes = n * sizeof(unsigned);
-  }
-  return plan;
+  return plan_real_gemm(kShapes[is_wide(p)], 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {
@@ -52,7 +38,7 @@ const char *describe_scaled_gemm(const ScaledGemmParams &p) {
 
 hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
-  const real::ShapeInfo &shape = kShapes[is_wide(p)][p.plan.shape];
+  const RealShape &shape = kShapes[is_wide(p)][p.plan.shape];
   const int mode = mode_of(p);
   real::Args a = {};
   a.x = static_cast<const char *>(p.b);

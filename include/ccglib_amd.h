@@ -120,6 +120,11 @@ CCGLIB_API const char *ccglib_version(void);
  *                    wherever the GEMM can; 2: always through the transposes.
  *                    ccglib_pipeline_reads_in_place tells which one an object
  *                    took.
+ *   REAL_BLOCK       0 (default): the block shape of a real product (ScaledGEMM,
+ *                    ScaledLinear, Orthogonalize) and the parts that its K is
+ *                    cut into are chosen by its sizes; otherwise 1 plus the
+ *                    shape's number (the last one where there are fewer), plus
+ *                    256 times the number of parts (0: chosen).
  * ---------------------------------------------------------------------- */
 enum {
   CCGLIB_AMD_OPTION_INT1_POPCOUNT = 0,
@@ -128,7 +133,8 @@ enum {
   CCGLIB_AMD_OPTION_GEMM_BLOCK_TILE = 3,
   CCGLIB_AMD_OPTION_EXPECT_UNALIGNED = 4,
   CCGLIB_AMD_OPTION_PIPELINE_ROUTE = 5,
-  CCGLIB_AMD_OPTION_COUNT = 6
+  CCGLIB_AMD_OPTION_REAL_BLOCK = 6,
+  CCGLIB_AMD_OPTION_COUNT = 7
 };
 CCGLIB_API int ccglib_amd_set_option(int option, size_t value);
 CCGLIB_API int ccglib_amd_get_option(int option, size_t *value);
