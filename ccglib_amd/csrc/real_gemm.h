@@ -120,36 +120,32 @@ __device__ __forceinline__ float4_t mfma8(const Fragment &x, const Fragment &y, 
 struct WideFragment {
   half8_t v[4];
 };
-template <int FORMAT> __device__ __forceinline__ void widen_quarter(const Fragment &f, WideFragment &to, int q) {
+// (word w, of eight: four values)
+template <int FORMAT> __device__ __forceinline__ void widen_word(const Fragment &f, WideFragment &to, int w) {
   typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const unsigned word = (unsigned)f[2 * q + w];
-    half2_t lo, hi;
-    if constexpr (FORMAT == 0) {
-      lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false);
-      hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true);
-    } else {   // (e5m2 is the upper half of fp16)
-      lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x010c000cu));
-      hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x030c020cu));
-    }
-    to.v[q][4 * w] = lo[0];
-    to.v[q][4 * w + 1] = lo[1];
-    to.v[q][4 * w + 2] = hi[0];
-    to.v[q][4 * w + 3] = hi[1];
+  const unsigned word = (unsigned)f[w];
+  half2_t lo, hi;
+  if constexpr (FORMAT == 0) {
+    lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true);
+  } else {   // (e5m2 is the upper half of fp16)
+    lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x010c000cu));
+    hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(word, word, 0x030c020cu));
   }
+  const int q = w / 2, at = w % 2 * 4;
+  to.v[q][at] = lo[0];
+  to.v[q][at + 1] = lo[1];
+  to.v[q][at + 2] = hi[0];
+  to.v[q][at + 3] = hi[1];
 }
 template <int FORMAT> __device__ __forceinline__ WideFragment widened(const Fragment &f) {
   WideFragment r;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) widen_quarter<FORMAT>(f, r, q);
+  for (int w = 0; w < 8; ++w) widen_word<FORMAT>(f, r, w);
   return r;
 }
-// 2^(byte - 127); 255 stands for NaN
-__device__ __forceinline__ float power_of_two(unsigned byte) {
-  const float p = __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte << 23);
-  return byte == 255 ? __builtin_nanf("") : p;
-}
+// 2^(byte - 127); infinity for 255, which stands for no number
+__device__ __forceinline__ float power_of_two(unsigned byte) { return __builtin_ldexpf(0x1p-127f, (int)byte); }
 
 __device__ __forceinline__ float4_t mfma16(const Fragment &x, const Fragment &y, float4_t c, int q) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(half_of(x, q), half_of(y, q), c, 0, 0, 0);
@@ -402,44 +398,46 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     using Operand = typename std::conditional<T::kWide, WideFragment, Fragment>::type;
     Operand y[PLANES][NY], x[2][PLANES];
     Fragment raw_x, raw_y[2];           // (8 bits that become fp16)
-    float s[NY], s_next[NY], s_old[RING * JJ];   // scales of Y (times X's where that is one number)
-    int e8[NY], e8_next[NY], e8x[2];    // e8m0: bytes for the instruction
+    // (scales are read a while before they are needed, and turned into what is needed only then)
+    float s[NY], s_old[RING * JJ];      // scales of Y (times X's where that is one number)
+    float sy_read[NY], sx_read = 0.f;
     float4_t sx[2];                     // scales of a lane's rows of X tile i
+    int e8[NY], e8x[2];                 // e8m0: bytes for the instruction
     float4_t part[RING][JJ];
-    (void)s, (void)s_next, (void)s_old, (void)e8, (void)e8_next, (void)e8x, (void)sx, (void)part, (void)raw_x, (void)raw_y;
+    (void)s, (void)s_old, (void)sy_read, (void)sx_read, (void)e8, (void)e8x, (void)sx, (void)part, (void)raw_x, (void)raw_y;
     auto scale = [](float stored) {
       return T::kScaleBytes == 1 ? power_of_two(__builtin_bit_cast(unsigned, stored)) : stored;
     };
     auto scales_at = [&](unsigned slot) { return lds + slot * S::kSlotBytes + S::kXBytes + S::kYBytes; };
     auto read_scales_y = [&](unsigned slot) {
-      const float *const sxp = reinterpret_cast<const float *>(scales_at(slot)) + wx * TX;
-      const float *const syp = reinterpret_cast<const float *>(scales_at(slot)) + BX + wy * TY;
+      if constexpr (T::kScaled) {
+        const float *const sxp = reinterpret_cast<const float *>(scales_at(slot)) + wx * TX;
+        const float *const syp = reinterpret_cast<const float *>(scales_at(slot)) + BX + wy * TY;
 #pragma unroll
-      for (int j = 0; j < NY; ++j) {
-        if constexpr (FLOAT_SCALES) {
-          s_next[j] = scale(syp[j * 16 + fr]);
-          if (T::kBlocks) s_next[j] *= scale(sxp[0]);
-        } else if constexpr (MODE == kScaledE8m0) {
-          e8_next[j] = __builtin_bit_cast(int, syp[j * 16 + fr]);
-        }
+        for (int j = 0; j < NY; ++j) sy_read[j] = syp[j * 16 + fr];
+        if constexpr (T::kBlocks) sx_read = sxp[0];
       }
     };
     auto take_scales_y = [&]() {
 #pragma unroll
       for (int j = 0; j < NY; ++j) {
-        if constexpr (FLOAT_SCALES) s[j] = s_next[j];
-        if constexpr (MODE == kScaledE8m0) e8[j] = e8_next[j];
+        if constexpr (FLOAT_SCALES) s[j] = T::kBlocks ? scale(sy_read[j]) * scale(sx_read) : scale(sy_read[j]);
+        if constexpr (MODE == kScaledE8m0) e8[j] = __builtin_bit_cast(int, sy_read[j]);
       }
     };
     auto read_scales_x = [&](int to, unsigned slot, int i) {
       if constexpr (FLOAT_SCALES && !T::kBlocks) {
         const float *const sxp = reinterpret_cast<const float *>(scales_at(slot)) + wx * TX;
         sx[to] = *reinterpret_cast<const float4_t *>(sxp + i / NT * GROUP_ROWS + g * 4 * NT + i % NT * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sx[to][e] = scale(sx[to][e]);
       } else if constexpr (MODE == kScaledE8m0) {
         const int *const sxp = reinterpret_cast<const int *>(scales_at(slot)) + wx * TX;
         e8x[to] = sxp[i / NT * GROUP_ROWS + (fr >> 2) * 4 * NT + i % NT * 4 + (fr & 3)];
+      }
+    };
+    auto take_scales_x = [&](int at) {
+      if constexpr (FLOAT_SCALES && !T::kBlocks && T::kScaleBytes == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sx[at][e] = scale(sx[at][e]);
       }
     };
     auto read_x = [&](int to, unsigned slot, int i) {
@@ -464,41 +462,51 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
         }
       }
     };
-    // C's sums of step m, with Y's scales (or, a piece later, the ones kept of that step)
-    auto add = [&](auto step, bool late) {
+    // Element `of` (4 JJ of them) of C's sums of step m, with Y's scales (or, a piece later, the ones kept of that step)
+    auto add_one = [&](auto step, auto of, bool late) {
       if constexpr (FLOAT_SCALES) {
-        constexpr int m = decltype(step)::value, i = m / SPT;
-#pragma unroll
-        for (int h = 0; h < JJ; ++h) {
-          const int j = m % SPT * JJ + h;
-          const float sy = late ? s_old[m % RING * JJ + h] : s[j];
-          pin(part[m % RING][h]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = part[m % RING][h][e];
-            if (T::kBlocks) {
-              acc[0][j][i][e] = __builtin_fmaf(v, sy, acc[0][j][i][e]);
-            } else {
-              acc[0][j][i][e] = __builtin_fmaf(v * sy, sx[i % 2][e], acc[0][j][i][e]);
-            }
-          }
-          pin(acc[0][j][i]);
+        constexpr int m = decltype(step)::value, i = m / SPT, h = decltype(of)::value / 4, e = decltype(of)::value % 4;
+        constexpr int j = m % SPT * JJ + h;
+        const float sy = late ? s_old[m % RING * JJ + h] : s[j];
+        if constexpr (e == 0) pin(part[m % RING][h]);
+        const float v = part[m % RING][h][e];
+        if (T::kBlocks) {
+          acc[0][j][i][e] = __builtin_fmaf(v, sy, acc[0][j][i][e]);
+        } else {
+          acc[0][j][i][e] = __builtin_fmaf(v * sy, sx[i % 2][e], acc[0][j][i][e]);
         }
+        if constexpr (e == 3) pin(acc[0][j][i]);
       }
+    };
+    auto add = [&](auto step, bool late) {
+      static_for<4 * JJ>([&](auto of) { add_one(step, of, late); });
     };
     auto products = [&](auto step) {
       constexpr int m = decltype(step)::value, i = m / SPT, j0 = m % SPT * JJ, b = i % 2;
       if constexpr (MODE == kScaledE8m0) {
         acc[0][j0][i] = mfma8<FX, FY>(x[b][0], y[0][j0], acc[0][j0][i], e8x[b], e8[j0]);
       } else if constexpr (T::kWide) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-          for (int h = 0; h < JJ; ++h) {
-            part[m % RING][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][0].v[q], y[0][j0 + h].v[q],
-                                                                       q == 0 ? zero : part[m % RING][h], 0, 0, 0);
+        // between these products, which take 16 clocks each: what of the step before is added, and of the next X
+        // fragment becomes fp16
+        static_for<4 * JJ>([&](auto product) {
+          constexpr int k = decltype(product)::value, q = k / JJ, h = k % JJ;
+          part[m % RING][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][0].v[q], y[0][j0 + h].v[q],
+                                                                     q == 0 ? zero : part[m % RING][h], 0, 0, 0);
+          pin(part[m % RING][h]);
+          CCGLIB_PIN;
+          if constexpr (m >= LAG) {
+            add_one(std::integral_constant<int, m - LAG>{}, product, false);
+          } else if constexpr (CARRY) {
+            add_one(std::integral_constant<int, m - LAG + STEPS>{}, product, true);
           }
-        }
+          if constexpr (m % SPT > 0 && k % 2 == 1) {     // (its reads have had a step's time)
+            constexpr int WORDS = 8, SLICES = (SPT > 1 ? SPT - 1 : 1) * 4, PER = (WORDS + SLICES - 1) / SLICES, w0 = ((m % SPT - 1) * 4 + k / 2) * PER;
+            static_for<PER>([&](auto w) {
+              if constexpr (w0 + decltype(w)::value < WORDS) widen_word<FX>(raw_x, x[1 - b][0], w0 + decltype(w)::value);
+            });
+          }
+          CCGLIB_PIN;
+        });
       } else if constexpr (T::kScaled) {
         part[m % RING][0] = mfma8<FX, FY>(x[b][0], y[0][j0], zero, 0x7f, 0x7f);
       } else if constexpr (MODE == kHalf) {
@@ -530,6 +538,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     read_scales_y(0);
     take_scales_y();
     read_scales_x(0, 0, 0);
+    if constexpr (LAG == 2) take_scales_x(0);
     read_x(0, 0, 0);
     if constexpr (T::kWide) x[0][0] = widened<FX>(raw_x);
 #pragma unroll
@@ -596,22 +605,20 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
         if constexpr (c0 < c1 && REFILL > 0) {
           static_for<c1 - c0>([&](auto c) { copy_one(refill, std::integral_constant<int, c0 + decltype(c)::value>{}, end); });
         }
-        if constexpr (m >= LAG) {
-          add(std::integral_constant<int, m - LAG>{}, false);
-        } else if constexpr (CARRY) {
-          add(std::integral_constant<int, m - LAG + STEPS>{}, true);
+        if constexpr (!T::kWide) {
+          if constexpr (m >= LAG) {
+            add(std::integral_constant<int, m - LAG>{}, false);
+          } else if constexpr (CARRY) {
+            add(std::integral_constant<int, m - LAG + STEPS>{}, true);
+          }
         }
         if constexpr (FLOAT_SCALES && !T::kBlocks && js == LAG - 1) {
+          if constexpr (LAG == 1) take_scales_x(i % 2);
           read_scales_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
         }
         if constexpr (T::kWide) {
-          // the next X fragment becomes fp16 a part at a time; a Y fragment of the next piece where the last products
-          // with its predecessor have been issued
-          static_for<4>([&](auto quarter) {
-            constexpr int q = quarter;
-            if constexpr ((q * SPT) / 4 == js) widen_quarter<FX>(raw_x, x[to][0], q);
-          });
-          if constexpr (at_end) {
+          if constexpr (SPT == 1) x[to][0] = widened<FX>(raw_x);
+          if constexpr (at_end) {   // (a Y fragment of the next piece, where the last products with its predecessor have been issued)
 #pragma unroll
             for (int h = 0; h < JJ; ++h) {
               const int j = js * JJ + h;
