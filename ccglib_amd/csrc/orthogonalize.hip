@@ -284,7 +284,7 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
     g.y_batch = my.batch * 2;
     g.x_plane = mx.plane * 2;
     g.y_plane = my.plane * 2;
-    g.k_bytes = (unsigned)up(k, 8) * 2;
+    g.k_bytes = (unsigned)up(k, 64) * 2;   // (rows are padded to whole pieces, with zeros)
     g.pieces = (unsigned)ceil_div(g.k_bytes, (size_t)real::kPieceBytes);
     g.blocks_x = r.blocks_x;
     g.blocks_y = r.blocks_y;

@@ -165,6 +165,8 @@ __device__ __forceinline__ void pin(WideFragment &value) {
   for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(value.v[q]));
 }
 
+__device__ __forceinline__ void pin_scalar(const char *&p) { asm volatile("" : "+s"(p)); }
+
 template <int N, typename F, int... I> __device__ __forceinline__ void static_for(F &&f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
 }
@@ -316,6 +318,9 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     scale_base = (of_x ? args.x_scales : args.y_scales) + (size_t)at.b * args.pieces * scale_step;
     scale_lds = j * 256;
   }
+  // (kept in registers: its address is a scalar load, behind which the LDS reads would be waited for all together)
+  const char *zeros = g_zeros;
+  pin_scalar(zeros);
   // Where the next piece to be copied is, and the slot of LDS that it goes to
   const char *x_next = x_base + (size_t)first * kPieceBytes, *y_next = y_base + (size_t)first * kPieceBytes;
   const char *scales_next = scale_base + (size_t)first * scale_step;
@@ -336,7 +341,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
       if constexpr (!decltype(end)::value) {
         load_1k_to_lds(uniform(from), offset[n], at_lds);
       } else {
-        load_1k_to_lds_by_lane((size_t)piece_next * kPieceBytes + chunk * 16 < args.k_bytes ? from + offset[n] : g_zeros, at_lds);
+        load_1k_to_lds_by_lane((size_t)piece_next * kPieceBytes + chunk * 16 < args.k_bytes ? from + offset[n] : zeros, at_lds);
       }
     }
   };
@@ -347,7 +352,6 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     ++piece_next;
   };
   const std::true_type may_end{};
-  const std::false_type whole{};
   static_assert(!T::kScaled || BX % 64 == 0, "scales of X fill whole copies");
 
   // ---- fragments ----
@@ -397,7 +401,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
     }
     using Operand = typename std::conditional<T::kWide, WideFragment, Fragment>::type;
     Operand y[PLANES][NY], x[2][PLANES];
-    Fragment raw_x, raw_y[2];           // (8 bits that become fp16)
+    Fragment raw_x, raw_y[T::kWide ? NY : 1];   // (8 bits that become fp16)
     // (scales are read a while before they are needed, and turned into what is needed only then)
     float s[NY], s_old[RING * JJ];      // scales of Y (times X's where that is one number)
     float sy_read[NY], sx_read = 0.f;
@@ -456,7 +460,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
       for (int p = 0; p < PLANES; ++p) {
         const Fragment f = read(slot, y_rows + p * BY * kPieceBytes + j * 16 * kPieceBytes);
         if constexpr (T::kWide) {
-          raw_y[j % 2] = f;
+          raw_y[j] = f;
         } else {
           y[p][j] = f;
         }
@@ -544,7 +548,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
 #pragma unroll
     for (int j = 0; j < NY; ++j) {
       read_y(0, j);
-      if constexpr (T::kWide) y[0][j] = widened<FY>(raw_y[j % 2]);
+      if constexpr (T::kWide) y[0][j] = widened<FY>(raw_y[j]);
     }
     if constexpr (FLOAT_SCALES && CARRY) {   // (nothing to add yet)
 #pragma unroll
@@ -576,11 +580,10 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
           read_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
           if constexpr (MODE == kScaledE8m0) read_scales_x(to, at_end ? next : slot, at_end ? 0 : i + 1);
         }
-        if constexpr (at_end && T::kWide) {
+        if constexpr (at_end && T::kWide && js == 0) {
+          // (all at once: in turn with what is made of them they cost a round trip through LDS each, 240 against 2xx us)
 #pragma unroll
-          for (int h = 0; h < JJ; ++h) {
-            if (js * JJ + h < 2) read_y(next, js * JJ + h);
-          }
+          for (int j = 0; j < NY; ++j) read_y(next, j);
         }
 #pragma unroll
         for (int h = 0; h < JJ; ++h) pin(y[0][js * JJ + h]);
@@ -622,8 +625,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
 #pragma unroll
             for (int h = 0; h < JJ; ++h) {
               const int j = js * JJ + h;
-              y[0][j] = widened<FY>(raw_y[j % 2]);
-              if (j + 2 < NY) read_y(next, j + 2);
+              y[0][j] = widened<FY>(raw_y[j]);
             }
           }
         }
