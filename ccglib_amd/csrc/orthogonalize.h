@@ -19,7 +19,7 @@ template <bool PAIRS> struct Halves {
     p[0] = part(v, 0);
     if (PAIRS) p[plane] = part(v, 1);
   }
-  // N (4, 8 or 16) neighbours, at a multiple of N
+  // N (4 or 8) neighbours, at a multiple of N
   template <int N> static __device__ __forceinline__ void load(const _Float16 *p, size_t plane, float (&v)[N]) {
     constexpr int E = N < 8 ? N : 8;
     typedef _Float16 piece_t __attribute__((ext_vector_type(E)));
