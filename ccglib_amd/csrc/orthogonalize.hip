@@ -143,14 +143,21 @@ struct Product {
   size_t blocks;                           // in all
 };
 
-constexpr RealShape kHalfShapes[] = {
-#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY, 64 * WX * WY, #BY "x" #BX},
-    CCGLIB_HALF_SHAPES(CCGLIB_INFO)
-};
-constexpr RealShape kPairsShapes[] = {
-    CCGLIB_HALF_PAIRS_SHAPES(CCGLIB_INFO)
-#undef CCGLIB_INFO
-};
+// (the shapes of orthogonalize.h, in their order; see real_plan.h for the figures)
+constexpr RealShape kHalfShapes[] = {{256, 256, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
+                                     {128, 128, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
+                                     {64, 64, 2, 0.18f, 0.30f, 5.0f, 2.6f, "64x64"}};
+constexpr RealShape kPairsShapes[] = {{128, 128, 1, 1.15f, 1.40f, 7.0f, 1.3f, "128x128"},
+                                      {64, 64, 2, 0.50f, 0.80f, 6.0f, 2.6f, "64x64"}};
+#define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
+  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
+#define CCGLIB_TABLE kHalfShapes
+CCGLIB_HALF_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#define CCGLIB_TABLE kPairsShapes
+CCGLIB_HALF_PAIRS_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#undef CCGLIB_SAME
 
 Product plan_product(bool pairs, size_t batch, size_t nx, size_t ny, size_t k, bool symmetric) {
   const RealShape *const shapes = pairs ? kPairsShapes : kHalfShapes;

@@ -36,9 +36,12 @@ struct RealGemmPlan {
   size_t partial_bytes = 0, counter_bytes = 0;
 };
 
-// A block shape of the real products' kernel: columns and rows of a block, threads.
+// A block shape of the real products' kernel: columns and rows of a block, blocks that a compute unit holds, and what it costs
+// (us): a piece of K where a unit has one block, and where every unit has as many as it holds; a block's start and end;
+// joining parts of K, for each 64 x 64 sums.
 struct RealShape {
-  unsigned bx, by, threads;
+  unsigned bx, by, per_unit;
+  float alone_us, full_us, block_us, join_us;
   const char *name;
 };
 // The option REAL_BLOCK: 0, or a shape's number + 1, plus 256 times the number of parts that K is cut into (0: chosen).

@@ -8,12 +8,31 @@
 namespace ccglib_amd {
 namespace {
 
-constexpr RealShape kShapes[2][4] = {
-#define CCGLIB_INFO(ID, BX, BY, WX, WY, SLOTS, EU) {BX, BY, 64 * WX * WY, #BY "x" #BX},
-    {CCGLIB_SCALED_SHAPES(CCGLIB_INFO)},
-    {CCGLIB_WIDE_SHAPES(CCGLIB_INFO)}
-#undef CCGLIB_INFO
-};
+// (the shapes of scaled_gemm.h, in their order; see real_plan.h for the figures)
+constexpr RealShape kFloatShapes[] = {{256, 256, 1, 0.84f, 1.87f, 7.0f, 0.90f, "256x256"},
+                                      {128, 128, 2, 0.73f, 1.78f, 1.5f, 1.32f, "128x128"},
+                                      {64, 64, 2, 0.235f, 0.456f, 2.5f, 2.6f, "64x64"},
+                                      {64, 32, 2, 0.185f, 0.321f, 2.2f, 6.0f, "32x64"}};
+constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.76f, 1.71f, 6.9f, 0.81f, "256x256"},
+                                     {128, 128, 2, 0.70f, 1.67f, 1.4f, 1.32f, "128x128"},
+                                     {64, 64, 2, 0.20f, 0.44f, 2.4f, 2.7f, "64x64"},
+                                     {64, 32, 2, 0.18f, 0.31f, 2.1f, 6.4f, "32x64"}};
+constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.25f, 2.71f, 6.3f, 0.70f, "256x128"},
+                                     {128, 128, 2, 1.12f, 2.80f, 4.9f, 1.35f, "128x128"},
+                                     {64, 64, 2, 0.465f, 0.80f, 2.8f, 2.5f, "64x64"},
+                                     {64, 32, 2, 0.31f, 0.53f, 2.2f, 5.0f, "32x64"}};
+#define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
+  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
+#define CCGLIB_TABLE kFloatShapes
+CCGLIB_SCALED_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#define CCGLIB_TABLE kE8m0Shapes
+CCGLIB_SCALED_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#define CCGLIB_TABLE kWideShapes
+CCGLIB_WIDE_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#undef CCGLIB_SAME
 
 bool is_wide(const ScaledGemmParams &p) { return p.type_c == kFloat32; }
 
@@ -22,23 +41,27 @@ int mode_of(const ScaledGemmParams &p) {
   return is_wide(p) ? mode + real::kWideBlocks : mode;
 }
 
+const RealShape *shapes_of(const ScaledGemmParams &p) {
+  return is_wide(p) ? kWideShapes : p.scale_type == kScaleE8m0 ? kE8m0Shapes : kFloatShapes;
+}
+
 }  // namespace
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
-  return plan_real_gemm(kShapes[is_wide(p)], 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false);
+  return plan_real_gemm(shapes_of(p), 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {
   static thread_local char name[96];
   static const char *const scales[] = {"float scales, 128 x 128", "float scales", "e8m0 scales"};
   snprintf(name, sizeof name, "gemm_real<8 bits%s, %s> %s block, K in %u", is_wide(p) ? " as fp16" : "", scales[mode_of(p) % 3],
-           kShapes[is_wide(p)][p.plan.shape].name, p.plan.parts);
+           shapes_of(p)[p.plan.shape].name, p.plan.parts);
   return name;
 }
 
 hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
-  const RealShape &shape = kShapes[is_wide(p)][p.plan.shape];
+  const RealShape &shape = shapes_of(p)[p.plan.shape];
   const int mode = mode_of(p);
   real::Args a = {};
   a.x = static_cast<const char *>(p.b);

@@ -52,6 +52,18 @@ def test_sizes(t):
 
 
 @pytest.mark.parametrize("t", list(WIDE))
+@pytest.mark.parametrize("shape,parts", [(1, 1), (1, 3), (2, 1), (2, 2), (3, 1), (3, 5)])
+def test_every_block_shape(t, shape, parts):
+    """The shapes that the sizes would not choose, K in one part and in several."""
+    gen = torch.Generator().manual_seed(10)
+    for B, M, N in [(2, 5, 9), (1, 70, 260), (2, 280, 130), (1, 400, 330)]:
+        g = update(B, M, N, t, gen)
+        with cc.option(cc.Option.real_block, shape + 256 * parts):
+            got, _ = run(g, t)
+        assert near(got, orthogonalized(g), t), (B, M, N)
+
+
+@pytest.mark.parametrize("t", list(WIDE))
 @pytest.mark.parametrize("M,N", [(2100, 2300), (3000, 520), (520, 3000)])
 def test_large_blocks(t, M, N):
     g = update(1, M, N, t, torch.Generator().manual_seed(2))

@@ -88,10 +88,13 @@ def test_large_blocks_and_frobenius_error(tc, gb, st):
 
 
 @pytest.mark.parametrize("tc", [VT.float32, VT.bfloat16])
-@pytest.mark.parametrize("M,N,K", [(1, 64, 8192), (5, 1000, 5000), (64, 64, 16384), (100, 130, 9000), (256, 256, 12800)])
-def test_long_sums_of_few_blocks_are_the_same_every_time(tc, M, N, K):
+@pytest.mark.parametrize("M,N,K,parts", [(1, 64, 8192, 16), (5, 1000, 5000, 3), (64, 64, 16384, 32), (100, 130, 9000, 7),
+                                         (256, 256, 12800, 2)])
+@pytest.mark.parametrize("shape", [1, 2, 3, 4])
+def test_long_sums_in_parts_are_the_same_every_time(tc, M, N, K, parts, shape):
     """K is cut into parts that different blocks sum: same bits on every run."""
-    op, c, want, buffers = product(1, M, N, K, tc=tc)
+    with cc.option(cc.Option.real_block, shape + 256 * parts):
+        op, c, want, buffers = product(1, M, N, K, tc=tc)
     assert not op.KernelName().endswith("K in 1")
     first = c.clone()
     for _ in range(5):
@@ -99,6 +102,17 @@ def test_long_sums_of_few_blocks_are_the_same_every_time(tc, M, N, K):
         op.Run(*(t.data_ptr() for t in buffers), c.data_ptr())
         torch.cuda.synchronize()
         assert torch.equal(c, first)
+
+
+@pytest.mark.parametrize("tc", list(WIDE))
+@pytest.mark.parametrize("gb", list(SG))
+@pytest.mark.parametrize("st", list(ST))
+@pytest.mark.parametrize("shape", [1, 2, 3, 4])
+def test_every_block_shape(tc, gb, st, shape):
+    """The shapes that the sizes would not choose, at sizes that end inside blocks, one to five pieces of K among them."""
+    with cc.option(cc.Option.real_block, shape):
+        for B, M, N, K in [(1, 1, 5, 16), (2, 70, 140, 130), (1, 270, 261, 384), (1, 33, 300, 515), (1, 140, 70, 640)]:
+            product(B, M, N, K, tc=tc, gb=gb, st=st)
 
 
 @pytest.mark.parametrize("M,N,K", [(3, 100, 200), (140, 260, 1000), (64, 64, 20000)])
@@ -203,7 +217,8 @@ def test_graph_of_a_product_in_parts():
     M, N, K = 20, 200, 6000
     gen = torch.Generator().manual_seed(8)
     side = torch.cuda.Stream()
-    op = cc.ScaledGEMM(1, M, N, K, 0, side.cuda_stream, c_type=VT.float32)
+    with cc.option(cc.Option.real_block, 4 + 256 * 5):
+        op = cc.ScaledGEMM(1, M, N, K, 0, side.cuda_stream, c_type=VT.float32)
     assert not op.KernelName().endswith("K in 1")
 
     def operands():
