@@ -493,6 +493,7 @@ int ccglib_orthogonalize_create(ccglib_orthogonalize_t *orthogonalize, size_t B,
   p.b = b;
   p.c = c;
   p.epsilon = epsilon;
+  p.block_option = real_block_option;
   if (int s = check_device(device)) return s;
   DeviceGuard guard(device);
   HIP_TRY(guard.status());

@@ -21,6 +21,9 @@ namespace {
 constexpr size_t kAlign = 256;
 size_t up(size_t n, size_t to) { return ceil_div(n, to) * to; }
 
+// Whether a value of the chain is two fp16.
+bool as_pairs(int type) { return type != kBfloat16; }
+
 #define HIP_PASS(expr)                         \
   do {                                         \
     const hipError_t e_ = (expr);              \
@@ -125,6 +128,317 @@ __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::typ
   }
 }
 
+// ---- small matrices: all steps in one launch ----
+// A workgroup of 16 waves has one matrix, whose chain stays in LDS: X and X^T, A and P, rows 16 bytes longer than a multiple of
+// 64 bytes, so that the fragment reads of 16 rows fall on different banks. A wave computes 32 x 32 sums at a time; every
+// product is at most two rounds of them. What bounds it is latency: 15 products one after the other, three barriers a step.
+// 16 x 128 x 96 bf16: 80 us as 17 launches, 28 in one.
+constexpr unsigned kSmallWaves = 16, kSmallRounds = 2, kSmallPieces = 4, kSmallLds = 156 * 1024;
+struct SmallSizes {
+  unsigned mp, np;                 // extents padded to 32
+  unsigned x_pitch, t_pitch;       // halves: rows of X (np + 8); rows of X^T, A and P (mp + 8)
+  unsigned x_plane, t_plane, a_plane;
+  unsigned bytes;
+};
+constexpr SmallSizes small_sizes(unsigned m, unsigned n, unsigned planes) {
+  SmallSizes s = {};
+  s.mp = (m + 31) / 32 * 32;
+  s.np = (n + 31) / 32 * 32;
+  s.x_pitch = s.np + 8;
+  s.t_pitch = s.mp + 8;
+  s.x_plane = s.mp * s.x_pitch;
+  s.t_plane = s.np * s.t_pitch;
+  s.a_plane = s.mp * s.t_pitch;
+  s.bytes = planes * 2 * (s.x_plane + s.t_plane + 2 * s.a_plane) + 2 * s.mp * 4;
+  return s;
+}
+bool fits_small(size_t m, size_t n, unsigned planes) {
+  if (m > 256 || n > 4096) return false;
+  const SmallSizes s = small_sizes((unsigned)m, (unsigned)n, planes);
+  return s.bytes <= kSmallLds && (s.mp / 32) * (s.np / 32) <= kSmallWaves * kSmallRounds &&
+         s.mp * s.np / 8 <= kSmallPieces * 64 * kSmallWaves;
+}
+
+struct SmallArgs {
+  const void *in;
+  void *out;
+  size_t in_pitch, out_pitch;
+  unsigned rows, cols;             // of the input
+  int steps;
+  float a, b, c, epsilon;
+};
+
+template <int TYPE>
+__global__ __launch_bounds__(64 * kSmallWaves) void orthogonalize_small(SmallArgs args) {
+  constexpr bool PAIRS = TYPE != kBfloat16;
+  constexpr int PLANES = PAIRS ? 2 : 1;
+  using H = real::Halves<PAIRS>;
+  using V = typename Value<TYPE>::type;
+  typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
+  __shared__ double sums[kSmallWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  int fr = lane & 15, g = lane >> 4;
+  const bool tall = args.rows > args.cols;
+  const unsigned m = tall ? args.cols : args.rows, n = tall ? args.rows : args.cols;
+  const SmallSizes z = small_sizes(m, n, PLANES);
+  _Float16 *const x = reinterpret_cast<_Float16 *>(lds), *const t = x + PLANES * z.x_plane, *const a = t + PLANES * z.t_plane,
+                  *const p = a + PLANES * z.a_plane;
+  float *const diagonal = reinterpret_cast<float *>(p + PLANES * z.a_plane), *const diagonal_p = diagonal + z.mp;
+  const V *const in = static_cast<const V *>(args.in) + (size_t)blockIdx.x * args.rows * args.in_pitch;
+
+  // G, eight neighbours of a row at a time, neighbouring lanes in neighbouring rows (which spreads the transpose's writes over
+  // the banks); read once
+  typedef V eight_t __attribute__((ext_vector_type(8), aligned(sizeof(V))));
+  const unsigned pieces = args.rows * ((args.cols + 7) / 8);
+  float v[kSmallPieces][8];
+  double sum = 0.0;
+#pragma unroll
+  for (unsigned q = 0; q < kSmallPieces; ++q) {
+    const unsigned id = threadIdx.x + q * 64 * kSmallWaves;
+    const unsigned c8 = id / args.rows, r = id - c8 * args.rows, c = c8 * 8;
+    const V *const from = in + (size_t)r * args.in_pitch + c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
+    if (id < pieces) {
+      if (c + 8 <= args.cols) {
+        const eight_t got = *reinterpret_cast<const eight_t *>(from);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = (float)got[e];
+      } else {
+#pragma unroll
+        for (unsigned e = 0; e < 8; ++e) {
+          if (c + e < args.cols) v[q][e] = (float)from[e];
+        }
+      }
+    }
+  }
+  // zeros behind the ends of rows and columns
+  for (unsigned i = threadIdx.x; i < z.bytes / 16; i += 64 * kSmallWaves) reinterpret_cast<int4_t *>(lds)[i] = int4_t{0, 0, 0, 0};
+#pragma unroll
+  for (unsigned q = 0; q < kSmallPieces; ++q) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)v[q][e], (double)v[q][e], sum);
+  }
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (unsigned w = 0; w < kSmallWaves; ++w) sum += sums[w];
+  float factor;
+  const int e2 = exponent_and_factor(sum, args.epsilon, &factor);
+  {
+    _Float16 *const same = tall ? t : x, *const turned = tall ? x : t;
+    const unsigned same_pitch = tall ? z.t_pitch : z.x_pitch, turned_pitch = tall ? z.x_pitch : z.t_pitch;
+    const unsigned same_plane = tall ? z.t_plane : z.x_plane, turned_plane = tall ? z.x_plane : z.t_plane;
+#pragma unroll
+    for (unsigned q = 0; q < kSmallPieces; ++q) {
+      const unsigned id = threadIdx.x + q * 64 * kSmallWaves;
+      const unsigned c8 = id / args.rows, r = id - c8 * args.rows, c = c8 * 8;
+      if (id < pieces) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = __builtin_ldexpf(v[q][e], e2);
+        H::store(same + r * same_pitch + c, same_plane, v[q]);       // (behind the row's end: zeros)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) H::put(turned + (c + e) * turned_pitch + r, turned_plane, v[q][e]);
+      }
+    }
+  }
+  __syncthreads();
+
+  // 32 x 32 sums D[y][x] of rows of `rx` (x) and of `ry` (y), over k: [16 of y][16 of x]
+  auto multiply = [&](const _Float16 *rx, unsigned px, unsigned planex, const _Float16 *ry, unsigned py, unsigned planey, unsigned k,
+                      real::float4_t (&d)[2][2]) __attribute__((always_inline)) {
+    real::float4_t lo[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        d[j][i] = 0.f;
+        lo[j][i] = 0.f;
+      }
+    }
+#pragma unroll PAIRS ? 2 : 4
+    for (unsigned at = 0; at < k; at += 32) {
+      real::half8_t fx[PLANES][2], fy[PLANES][2];
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fx[q][i] = *reinterpret_cast<const real::half8_t *>(rx + q * planex + (i * 16 + fr) * px + at + g * 8);
+          fy[q][i] = *reinterpret_cast<const real::half8_t *>(ry + q * planey + (i * 16 + fr) * py + at + g * 8);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) d[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx[0][i], fy[0][j], d[j][i], 0, 0, 0);
+      }
+      if constexpr (PAIRS) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            lo[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx[0][i], fy[PLANES - 1][j], lo[j][i], 0, 0, 0);
+            lo[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx[PLANES - 1][i], fy[0][j], lo[j][i], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if constexpr (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) d[j][i] += lo[j][i] * 0x1p-11f;
+      }
+    }
+  };
+  auto load4 = [&](const _Float16 *from, unsigned plane, float (&v)[4]) {
+    const half4_t h = *reinterpret_cast<const half4_t *>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)h[e];
+    if constexpr (PAIRS) {
+      const half4_t l = *reinterpret_cast<const half4_t *>(from + plane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)l[e], 0x1p-11f, v[e]);
+    }
+  };
+  auto store4 = [&](_Float16 *to, unsigned plane, const float (&v)[4]) {
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q) {
+      const half4_t h = {H::part(v[0], q), H::part(v[1], q), H::part(v[2], q), H::part(v[3], q)};
+      *reinterpret_cast<half4_t *>(to + q * plane) = h;
+    }
+  };
+
+  const unsigned bm = z.mp / 32, bn = z.np / 32;
+  float f = factor;
+  real::float4_t d[kSmallRounds][2][2];
+  // X's new values of piece (i, j) of a round
+  auto updated = [&](unsigned round, unsigned block, int j, int i, float (&w)[4]) __attribute__((always_inline)) {
+    const unsigned y = block / bn * 32 + j * 16 + fr, c = block % bn * 32 + i * 16 + g * 4;
+    const float dy = args.a + diagonal_p[y];
+    float old[4];
+    load4(x + y * z.x_pitch + c, z.x_plane, old);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = f * __builtin_fmaf(dy, old[e], d[round][j][i][e]);
+  };
+#pragma unroll 1
+  for (int step = 0;;) {
+    // (addresses are worked out anew in every step: kept through the loop they fill the registers)
+    asm volatile("" : "+v"(fr), "+v"(g));
+    // A: its diagonal apart (all of it: the mirrored half costs no round more)
+#pragma unroll 1
+    for (unsigned block = wave; block < bm * bm; block += kSmallWaves) {
+      const unsigned y0 = block / bm * 32, x0 = block % bm * 32;
+      real::float4_t v[2][2];
+      multiply(x + x0 * z.x_pitch, z.x_pitch, z.x_plane, x + y0 * z.x_pitch, z.x_pitch, z.x_plane, z.np, v);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned y = y0 + j * 16 + fr, c = x0 + i * 16 + g * 4;
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = f * f * v[j][i][e];
+            if (c + e == y) {
+              diagonal[y] = w[e];
+              w[e] = 0.f;
+            }
+          }
+          store4(a + y * z.t_pitch + c, z.a_plane, w);
+        }
+      }
+    }
+    __syncthreads();
+    // P
+#pragma unroll 1
+    for (unsigned block = wave; block < bm * bm; block += kSmallWaves) {
+      const unsigned y0 = block / bm * 32, x0 = block % bm * 32;
+      real::float4_t v[2][2];
+      multiply(a + x0 * z.t_pitch, z.t_pitch, z.a_plane, a + y0 * z.t_pitch, z.t_pitch, z.a_plane, z.mp, v);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned y = y0 + j * 16 + fr;
+        const float dy = diagonal[y];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned c = x0 + i * 16 + g * 4;
+          float old[4], w[4];
+          load4(a + y * z.t_pitch + c, z.a_plane, old);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = __builtin_fmaf(args.c, __builtin_fmaf(dy + diagonal[c + e], old[e], v[j][i][e]), args.b * old[e]);
+            if (c + e == y) {
+              diagonal_p[y] = __builtin_fmaf(args.c, __builtin_fmaf(dy, dy, v[j][i][e]), args.b * dy);
+              w[e] = 0.f;
+            }
+          }
+          store4(p + y * z.t_pitch + c, z.a_plane, w);
+        }
+      }
+    }
+    __syncthreads();
+    // X and X^T, which are written only when everybody has read them
+#pragma unroll
+    for (unsigned round = 0; round < kSmallRounds; ++round) {
+      const unsigned block = wave + round * kSmallWaves;
+      if (block < bm * bn) {
+        const unsigned y0 = block / bn * 32, x0 = block % bn * 32;
+        multiply(t + x0 * z.t_pitch, z.t_pitch, z.t_plane, p + y0 * z.t_pitch, z.t_pitch, z.a_plane, z.mp, d[round]);
+      }
+    }
+    if (++step == args.steps) break;
+    __syncthreads();
+#pragma unroll
+    for (unsigned round = 0; round < kSmallRounds; ++round) {
+      const unsigned block = wave + round * kSmallWaves;
+      if (block < bm * bn) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const unsigned y = block / bn * 32 + j * 16 + fr, c = block % bn * 32 + i * 16 + g * 4;
+            float w[4];
+            updated(round, block, j, i, w);
+            store4(x + y * z.x_pitch + c, z.x_plane, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) H::put(t + (c + e) * z.t_pitch + y, z.t_plane, w[e]);
+          }
+        }
+      }
+    }
+    f = 1.f;
+    __syncthreads();
+  }
+  V *const out = static_cast<V *>(args.out) + (size_t)blockIdx.x * args.rows * args.out_pitch;
+#pragma unroll
+  for (unsigned round = 0; round < kSmallRounds; ++round) {
+    const unsigned block = wave + round * kSmallWaves;
+    if (block < bm * bn) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned y = block / bn * 32 + j * 16 + fr, c = block % bn * 32 + i * 16 + g * 4;
+          float w[4];
+          updated(round, block, j, i, w);
+          if (y >= m || c >= n) continue;
+          if (tall) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (c + e < n) out[(size_t)(c + e) * args.out_pitch + y] = (V)w[e];
+            }
+          } else {
+            real::store_row(out + (size_t)y * args.out_pitch + c, n - c, w);
+          }
+        }
+      }
+    }
+  }
+}
+
 // Where things are in the workspace.
 struct Layout {
   size_t m, n;                             // shorter and longer extent
@@ -159,19 +473,19 @@ CCGLIB_HALF_PAIRS_SHAPES(CCGLIB_SAME)
 #undef CCGLIB_TABLE
 #undef CCGLIB_SAME
 
-Product plan_product(bool pairs, size_t batch, size_t nx, size_t ny, size_t k, bool symmetric) {
+Product plan_product(const OrthogonalizeParams &p, size_t nx, size_t ny, size_t k, bool symmetric) {
+  const bool pairs = as_pairs(p.type);
+  const size_t batch = p.batch;
   const RealShape *const shapes = pairs ? kPairsShapes : kHalfShapes;
   const int count = pairs ? (int)(sizeof kPairsShapes / sizeof kPairsShapes[0]) : (int)(sizeof kHalfShapes / sizeof kHalfShapes[0]);
   Product r = {};
-  r.plan = plan_real_gemm(shapes, count, batch, nx, ny, ceil_div(k, (size_t)64), symmetric);
+  r.plan = plan_real_gemm(shapes, count, batch, nx, ny, ceil_div(k, (size_t)64), symmetric, p.block_option);
   const RealShape &s = shapes[r.plan.shape];
   r.blocks_x = (unsigned)ceil_div(nx, s.bx);
   r.blocks_y = (unsigned)ceil_div(ny, s.by);
   r.blocks = real_blocks(s, batch, nx, ny, symmetric);
   return r;
 }
-
-bool as_pairs(int type) { return type != kBfloat16; }
 
 Layout layout_of(const OrthogonalizeParams &p) {
   Layout l = {};
@@ -190,9 +504,9 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.norm_rows = (unsigned)std::max<size_t>(16, ceil_div((size_t)p.m * l.norm_x, 2048));
   l.norm_y = (unsigned)ceil_div(p.m, (size_t)l.norm_rows);
   size_t counters = 0, partial = 0;
-  const Product products[] = {plan_product(pairs, p.batch, l.m, l.m, l.n, true), plan_product(pairs, p.batch, l.m, l.m, l.m, true),
-                              plan_product(pairs, p.batch, l.n, l.m, l.m, false),
-                              plan_product(pairs, p.batch, l.m, l.n, l.m, false)};
+  const Product products[] = {plan_product(p, l.m, l.m, l.n, true), plan_product(p, l.m, l.m, l.m, true),
+                              plan_product(p, l.n, l.m, l.m, false),
+                              plan_product(p, l.m, l.n, l.m, false)};
   for (const Product &r : products) {
     counters = std::max(counters, r.plan.counter_bytes);
     partial = std::max(partial, r.plan.partial_bytes);
@@ -218,6 +532,10 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.factor = take(p.batch * sizeof(float));
   l.bytes = at;
   return l;
+}
+
+bool is_small(const OrthogonalizeParams &p) {
+  return !p.block_option && fits_small(std::min(p.m, p.n), std::max(p.m, p.n), as_pairs(p.type) ? 2 : 1);
 }
 
 template <bool PAIRS, int STEP>
@@ -250,6 +568,11 @@ hipError_t launch_product(const Product &r, const real::Args &a, const typename 
 template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t stream) {
   constexpr bool PAIRS = TYPE != kBfloat16;
   using V = typename Value<TYPE>::type;
+  if (is_small(p)) {
+    SmallArgs a = {p.in, p.out, p.in_pitch, p.out_pitch, p.m, p.n, p.steps, p.a, p.b, p.c, p.epsilon};
+    orthogonalize_small<TYPE><<<p.batch, 64 * kSmallWaves, 0, stream>>>(a);
+    return hipGetLastError();
+  }
   const Layout l = layout_of(p);
   char *const ws = static_cast<char *>(p.workspace);
   auto halves = [&](size_t at) { return reinterpret_cast<_Float16 *>(ws + at); };
@@ -276,8 +599,8 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
     const _Float16 *at;
     size_t rows, pitch, plane, batch;
   };
-  const Product gram = plan_product(PAIRS, p.batch, l.m, l.m, l.n, true), square = plan_product(PAIRS, p.batch, l.m, l.m, l.m, true);
-  const Product update = plan_product(PAIRS, p.batch, l.n, l.m, l.m, false), narrow = plan_product(PAIRS, p.batch, l.m, l.n, l.m, false);
+  const Product gram = plan_product(p, l.m, l.m, l.n, true), square = plan_product(p, l.m, l.m, l.m, true);
+  const Product update = plan_product(p, l.n, l.m, l.m, false), narrow = plan_product(p, l.m, l.n, l.m, false);
   auto args = [&](const Matrix &mx, const Matrix &my, size_t k, const Product &r, bool symmetric) {
     real::Args g = {};
     g.x = reinterpret_cast<const char *>(mx.at);
@@ -366,8 +689,8 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
 
 }  // namespace
 
-size_t orthogonalize_workspace_bytes(const OrthogonalizeParams &p) { return layout_of(p).bytes; }
-size_t orthogonalize_zeroed_bytes(const OrthogonalizeParams &p) { return layout_of(p).zeroed; }
+size_t orthogonalize_workspace_bytes(const OrthogonalizeParams &p) { return is_small(p) ? 0 : layout_of(p).bytes; }
+size_t orthogonalize_zeroed_bytes(const OrthogonalizeParams &p) { return is_small(p) ? 0 : layout_of(p).zeroed; }
 
 hipError_t launch_orthogonalize(const OrthogonalizeParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;

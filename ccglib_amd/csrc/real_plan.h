@@ -35,12 +35,13 @@ inline double real_gemm_us(const RealShape &s, size_t blocks, size_t pieces, siz
   return us;
 }
 
+// option: REAL_BLOCK
 inline RealGemmPlan plan_real_gemm(const RealShape *shapes, int count, size_t batch, size_t nx, size_t ny, size_t pieces,
-                                   bool symmetric) {
+                                   bool symmetric, size_t option) {
   RealGemmPlan plan;
   pieces = std::max<size_t>(1, pieces);
-  const int first = real_block_option ? (int)std::min<size_t>(real_block_option % 256 - 1, count - 1) : 0;
-  const int end = real_block_option ? first + 1 : count;
+  const int first = option ? (int)std::min<size_t>(option % 256 - 1, count - 1) : 0;
+  const int end = option ? first + 1 : count;
   double best = 0.0;
   size_t parts = 0;
   for (int s = first; s < end; ++s) {
@@ -55,7 +56,7 @@ inline RealGemmPlan plan_real_gemm(const RealShape *shapes, int count, size_t ba
       if (blocks * p > 65536) break;                // (more parts of so many blocks: nothing but memory)
     }
   }
-  if (real_block_option / 256) parts = std::min(real_block_option / 256, pieces);
+  if (option / 256) parts = std::min(option / 256, pieces);
   const RealShape &s = shapes[plan.shape];
   const size_t blocks = real_blocks(s, batch, nx, ny, symmetric);
   plan.pieces_per_part = (unsigned)ceil_div(pieces, parts);

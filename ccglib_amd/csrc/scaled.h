@@ -70,6 +70,7 @@ struct OrthogonalizeParams {
   int type;
   int steps;
   float a, b, c, epsilon;
+  size_t block_option;                // REAL_BLOCK when the object was created
   void *workspace;
 };
 size_t orthogonalize_workspace_bytes(const OrthogonalizeParams &p);

@@ -48,7 +48,7 @@ const RealShape *shapes_of(const ScaledGemmParams &p) {
 }  // namespace
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
-  return plan_real_gemm(shapes_of(p), 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false);
+  return plan_real_gemm(shapes_of(p), 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {
