@@ -106,25 +106,44 @@ __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::typ
                                                  _Float16 *to_t, unsigned to_t_pitch, size_t to_t_batch, size_t to_t_plane,
                                                  const double *partial, unsigned count, float epsilon, float *factor) {
   using H = real::Halves<PAIRS>;
+  using V = typename Value<TYPE>::type;
+  typedef V eight_t __attribute__((ext_vector_type(8), aligned(sizeof(V))));
   __shared__ float tile[64][65];
   __shared__ double waves[4];
   const unsigned b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   float f;
   const int e = exponent_and_factor(sum_of(partial + (size_t)b * count, count, waves), epsilon, &f);
   if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) factor[b] = f;
-  const int c = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < 64; r += 4) {
-    if (r0 + r < m && c0 + c < n) {
-      const float v = __builtin_ldexpf((float)in[((size_t)b * m + r0 + r) * in_pitch + c0 + c], e);
-      tile[r][c] = v;
-      H::put(to + (size_t)b * to_batch + (size_t)(r0 + r) * to_pitch + c0 + c, to_plane, v);
+  // (eight neighbours at a time; what is behind a row's end is written as the zero that it is)
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const unsigned r = q * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+    const V *const from = in + ((size_t)b * m + r0 + r) * in_pitch + c0 + c;
+    float v[8] = {};
+    if (r0 + r < m) {
+      if (c0 + c + 8 <= n) {
+        const eight_t got = *reinterpret_cast<const eight_t *>(from);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_ldexpf((float)got[i], e);
+      } else {
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) {
+          if (c0 + c + i < n) v[i] = __builtin_ldexpf((float)from[i], e);
+        }
+      }
+      if (c0 + c < n) H::store(to + (size_t)b * to_batch + (size_t)(r0 + r) * to_pitch + c0 + c, to_plane, v);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tile[r][c + i] = v[i];
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 6; r < 64; r += 4) {
-    if (c0 + r < n && r0 + c < m) {
-      H::put(to_t + (size_t)b * to_t_batch + (size_t)(c0 + r) * to_t_pitch + r0 + c, to_t_plane, tile[c][r]);
-    }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const unsigned r = (threadIdx.x & 7) * 8, c = q * 32 + (threadIdx.x >> 3);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[r + i][c];
+    if (c0 + c < n && r0 + r < m) H::store(to_t + (size_t)b * to_t_batch + (size_t)(c0 + c) * to_t_pitch + r0 + r, to_t_plane, v);
   }
 }
 
