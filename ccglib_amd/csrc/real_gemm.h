@@ -144,8 +144,10 @@ template <int FORMAT> __device__ __forceinline__ WideFragment widened(const Frag
   for (int w = 0; w < 8; ++w) widen_word<FORMAT>(f, r, w);
   return r;
 }
-// 2^(byte - 127); infinity for 255, which stands for no number
-__device__ __forceinline__ float power_of_two(unsigned byte) { return __builtin_ldexpf(0x1p-127f, (int)byte); }
+// 2^(byte - 127); NaN for 255, which stands for no number
+__device__ __forceinline__ float power_of_two(unsigned byte) {
+  return byte == 255 ? __builtin_nanf("") : __builtin_ldexpf(0x1p-127f, (int)byte);
+}
 
 __device__ __forceinline__ float4_t mfma16(const Fragment &x, const Fragment &y, float4_t c, int q) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(half_of(x, q), half_of(y, q), c, 0, 0, 0);

@@ -9,18 +9,22 @@ namespace ccglib_amd {
 namespace {
 
 // (the shapes of scaled_gemm.h, in their order; see real_plan.h for the figures)
-constexpr RealShape kFloatShapes[] = {{256, 256, 1, 0.84f, 1.87f, 7.0f, 0.90f, "256x256"},
-                                      {128, 128, 2, 0.73f, 1.78f, 1.5f, 1.32f, "128x128"},
-                                      {64, 64, 2, 0.235f, 0.456f, 2.5f, 2.6f, "64x64"},
-                                      {64, 32, 2, 0.185f, 0.321f, 2.2f, 6.0f, "32x64"}};
-constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.76f, 1.71f, 6.9f, 0.81f, "256x256"},
-                                     {128, 128, 2, 0.70f, 1.67f, 1.4f, 1.32f, "128x128"},
-                                     {64, 64, 2, 0.20f, 0.44f, 2.4f, 2.7f, "64x64"},
-                                     {64, 32, 2, 0.18f, 0.31f, 2.1f, 6.4f, "32x64"}};
-constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.25f, 2.71f, 6.3f, 0.70f, "256x128"},
-                                     {128, 128, 2, 1.12f, 2.80f, 4.9f, 1.35f, "128x128"},
-                                     {64, 64, 2, 0.465f, 0.80f, 2.8f, 2.5f, "64x64"},
-                                     {64, 32, 2, 0.31f, 0.53f, 2.2f, 5.0f, "32x64"}};
+constexpr RealShape kFloatShapes[] = {{256, 256, 1, 1.02f, 1.86f, 6.8f, 0.93f, "256x256"},
+                                      {128, 128, 2, 0.72f, 1.38f, 3.4f, 1.20f, "128x128"},
+                                      {64, 64, 2, 0.234f, 0.431f, 2.8f, 2.5f, "64x64"},
+                                      {64, 32, 2, 0.187f, 0.325f, 2.1f, 6.2f, "32x64"},
+                                      {128, 128, 1, 0.35f, 0.63f, 3.9f, 1.00f, "128x128 8-wave"}};
+constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.93f, 1.64f, 7.0f, 0.89f, "256x256"},
+                                     {128, 128, 2, 0.69f, 1.30f, 3.2f, 1.20f, "128x128"},
+                                     {64, 64, 2, 0.20f, 0.417f, 2.6f, 2.6f, "64x64"},
+                                     {64, 32, 2, 0.186f, 0.31f, 2.0f, 6.4f, "32x64"},
+                                     {128, 128, 1, 0.29f, 0.56f, 4.0f, 1.00f, "128x128 8-wave"}};
+constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.14f, 2.43f, 7.8f, 0.75f, "256x128"},
+                                     {128, 128, 2, 1.06f, 2.26f, 7.3f, 1.22f, "128x128"},
+                                     {64, 64, 2, 0.44f, 0.745f, 3.4f, 2.3f, "64x64"},
+                                     {64, 32, 2, 0.304f, 0.49f, 2.35f, 5.2f, "32x64"},
+                                     {128, 128, 1, 0.79f, 1.31f, 5.6f, 0.93f, "128x128 8-wave"}};
+constexpr int kShapes = sizeof kFloatShapes / sizeof kFloatShapes[0];
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
   static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
 #define CCGLIB_TABLE kFloatShapes
@@ -48,7 +52,7 @@ const RealShape *shapes_of(const ScaledGemmParams &p) {
 }  // namespace
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
-  return plan_real_gemm(shapes_of(p), 4, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
+  return plan_real_gemm(shapes_of(p), kShapes, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {

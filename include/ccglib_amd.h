@@ -354,8 +354,8 @@ CCGLIB_API int ccglib_pipeline_run_static(
  * values along the row, then by the row (SCALE_ROWS) or by 128 rows
  * (SCALE_BLOCKS):
  *     scales[ceil(C / 128)][ccglib_scaled_pitch(R or ceil(R / 128))]
- * float, or one byte that holds a power of two (e8m0: 2^(byte - 127); what the
- * byte 255 scales is no finite number). A batch is such matrices one after the other. Values start
+ * float, or one byte that holds a power of two (e8m0: 2^(byte - 127), NaN for
+ * the byte 255). A batch is such matrices one after the other. Values start
  * at a multiple of 16 bytes.
  * ---------------------------------------------------------------------- */
 /* Groups of values that share a scale: 128 of a row, or 128 x 128 */

@@ -189,3 +189,21 @@ def test_empty_and_refusals_at_run():
         op.Run(t.data_ptr(), 0)
     with pytest.raises(RuntimeError, match="misaligned"):
         op.Run(t.data_ptr() + 2, t.data_ptr())
+
+
+@pytest.mark.parametrize("parts", [1, 3])
+def test_blocks_of_eight_waves(parts):
+    gen = torch.Generator().manual_seed(11)
+    t = VT.bfloat16
+    for B, M, N in [(2, 5, 9), (1, 70, 260), (2, 280, 130), (1, 400, 330)]:
+        g = update(B, M, N, t, gen)
+        with cc.option(cc.Option.real_block, 4 + 256 * parts):
+            got, _ = run(g, t)
+        assert near(got, orthogonalized(g), t), (B, M, N)
+
+
+def test_as_many_blocks_as_units():
+    t = VT.bfloat16
+    g = update(1, 1000, 4000, t, torch.Generator().manual_seed(12))
+    got, _ = run(g, t)
+    assert near(got, orthogonalized(g), t)

@@ -261,3 +261,41 @@ def test_refusals_at_run():
         op.Run(p, p + 2, p, p, p)
     with pytest.raises(RuntimeError, match="misaligned C"):
         op.Run(p, p, p, p, p + 1)
+
+
+@pytest.mark.parametrize("tc", list(WIDE))
+def test_the_e8m0_scale_that_is_no_number(tc):
+    """255 makes NaN of all that its group has a part in, and of nothing else."""
+    M, N, K = 70, 140, 300
+    gen = torch.Generator().manual_seed(8)
+    qa, sa, a = random_operand(gen, 1, M, K, VT.float8e4m3, SG.rows, ST.e8m0, 0.0)
+    qb, sb, b = random_operand(gen, 1, N, K, VT.float8e4m3, SG.rows, ST.e8m0, 0.0)
+    da, dsa = held(qa, sa, VT.float8e4m3, ST.e8m0)
+    db, dsb = held(qb, sb, VT.float8e4m3, ST.e8m0)
+    dsa[0, 1, 33] = 255
+    dsb[0, 2, 7] = 255
+    c = torch.zeros((M, N), dtype=WIDE[tc], device="cuda")
+    op = cc.ScaledGEMM(1, M, N, K, 0, stream(), c_type=tc, b_group=SG.rows, scale_type=ST.e8m0)
+    op.Run(da.data_ptr(), dsa.data_ptr(), db.data_ptr(), dsb.data_ptr(), c.data_ptr())
+    nan = torch.zeros((M, N), dtype=torch.bool, device="cuda")
+    nan[33, :] = True
+    nan[:, 7] = True
+    assert torch.equal(torch.isnan(c), nan)
+
+
+@pytest.mark.parametrize("tc", list(WIDE))
+@pytest.mark.parametrize("gb", list(SG))
+@pytest.mark.parametrize("st", list(ST))
+@pytest.mark.parametrize("parts", [1, 2, 3])
+def test_blocks_of_eight_waves(tc, gb, st, parts):
+    """The shape for as many blocks of 128 x 128 as there are units, at sizes that end inside blocks."""
+    with cc.option(cc.Option.real_block, 5 + 256 * parts):
+        for B, M, N, K in [(1, 1, 5, 16), (2, 70, 140, 130), (1, 270, 261, 384), (1, 33, 300, 515), (1, 140, 70, 640),
+                           (1, 129, 257, 1100)]:
+            product(B, M, N, K, tc=tc, gb=gb, st=st)
+
+
+def test_as_many_blocks_as_units():
+    for M, N, K in [(2048, 2048, 700), (2000, 2040, 1000)]:
+        op, c, want, _ = product(1, M, N, K, tc=VT.bfloat16, spread=0.0)
+        assert "8-wave" in op.KernelName()
