@@ -11,7 +11,10 @@ namespace real {
 // Matrices of the chain: fp16, or two fp16 for each value (v = first + second * 2^-11), a plane each. Rows are padded to a
 // whole 128 bytes, with zeros.
 template <bool PAIRS> struct Halves {
+  // (of two parts both see v rounded to 32 bits: made of the operations behind v in one instruction, the first part would
+  // now and then be the next one of fp16, and the second one what is left of another)
   static __device__ __forceinline__ _Float16 part(float v, int plane) {
+    if constexpr (PAIRS) asm("" : "+v"(v));
     const _Float16 h = (_Float16)v;
     return plane == 0 ? h : (_Float16)((v - (float)h) * 0x1p11f);
   }

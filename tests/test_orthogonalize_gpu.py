@@ -207,3 +207,15 @@ def test_as_many_blocks_as_units():
     g = update(1, 1000, 4000, t, torch.Generator().manual_seed(12))
     got, _ = run(g, t)
     assert near(got, orthogonalized(g), t)
+
+
+@pytest.mark.parametrize("M,N", [(64, 128), (600, 700), (1000, 1000)])
+@pytest.mark.parametrize("seed", [3, 4, 5])
+def test_no_row_of_a_32_bit_update_is_worse_than_its_roundings(M, N, seed):
+    """Every value of the chain has 22 bits, three matrices a step, five steps: 15 x 2^-22 = 3.6e-6 of a row. A value whose two
+    parts do not belong together is 2^-11 of itself off, 1.5e-5 and more of its row."""
+    g = torch.randn((2, M, N), generator=torch.Generator().manual_seed(seed)).cuda()
+    got, _ = run(g, VT.float32)
+    want = orthogonalized(g)
+    off = (got.double().cpu() - want).norm(dim=2) / want.norm(dim=2)
+    assert float(off.max()) < 4e-6
