@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::typ
 // A workgroup of 16 waves has one matrix, whose chain stays in LDS: X and X^T, A and P, rows 16 bytes longer than a multiple of
 // 64 bytes, so that the fragment reads of 16 rows fall on different banks. A wave computes 32 x 32 sums at a time; every
 // product is at most two rounds of them. What bounds it is latency: 15 products one after the other, three barriers a step.
-// 16 x 128 x 96 bf16: 80 us as 17 launches, 28 in one.
+// 16 x 128 x 96 bf16: 80 us as 17 launches, 28 in one (64 x 480: 78 and 36).
 constexpr unsigned kSmallWaves = 16, kSmallRounds = 2, kSmallPieces = 4, kSmallLds = 156 * 1024;
 struct SmallSizes {
   unsigned mp, np;                 // extents padded to 32
@@ -277,17 +277,29 @@ __global__ __launch_bounds__(64 * kSmallWaves) void orthogonalize_small(SmallArg
         lo[j][i] = 0.f;
       }
     }
-#pragma unroll PAIRS ? 2 : 4
-    for (unsigned at = 0; at < k; at += 32) {
-      real::half8_t fx[PLANES][2], fy[PLANES][2];
+    // (fragments are read one step of 32 ahead; behind the last one the last one's again)
+    real::half8_t fx[PLANES][2], fy[PLANES][2], next_x[PLANES][2], next_y[PLANES][2];
+    auto read = [&](unsigned at) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < PLANES; ++q) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          fx[q][i] = *reinterpret_cast<const real::half8_t *>(rx + q * planex + (i * 16 + fr) * px + at + g * 8);
-          fy[q][i] = *reinterpret_cast<const real::half8_t *>(ry + q * planey + (i * 16 + fr) * py + at + g * 8);
+          next_x[q][i] = *reinterpret_cast<const real::half8_t *>(rx + q * planex + (i * 16 + fr) * px + at + g * 8);
+          next_y[q][i] = *reinterpret_cast<const real::half8_t *>(ry + q * planey + (i * 16 + fr) * py + at + g * 8);
         }
       }
+    };
+    read(0);
+    for (unsigned at = 0; at < k; at += 32) {
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fx[q][i] = next_x[q][i];
+          fy[q][i] = next_y[q][i];
+        }
+      }
+      read(at + 32 < k ? at + 32 : at);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
