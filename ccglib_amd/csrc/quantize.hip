@@ -39,26 +39,40 @@ template <int TYPE> struct Eight {
   static constexpr int WORDS = TYPE == kFloat32 ? 8 : 4;
   unsigned w[WORDS];
 
+  __device__ __forceinline__ void load(const typename Loaded<TYPE>::type *p) {
+#pragma unroll
+    for (int h = 0; h < WORDS / 4; ++h) {
+      const uint4_unaligned_t got = reinterpret_cast<const uint4_unaligned_t *>(p)[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * h + e] = got[e];
+    }
+  }
+
   // From p on, of which `valid` are there; the others are zero.
-  __device__ __forceinline__ void load(const typename Loaded<TYPE>::type *p, int valid) {
-    if (valid >= 8) {
+  __device__ __forceinline__ void load_some(const typename Loaded<TYPE>::type *p, int valid) {
 #pragma unroll
-      for (int h = 0; h < WORDS / 4; ++h) {
-        const uint4_unaligned_t got = reinterpret_cast<const uint4_unaligned_t *>(p)[h];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * h + e] = got[e];
+    for (int e = 0; e < WORDS; ++e) {
+      if constexpr (TYPE == kFloat32) {
+        w[e] = e < valid ? reinterpret_cast<const unsigned *>(p)[e] : 0;
+      } else {
+        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+        const unsigned lo = 2 * e < valid ? q[2 * e] : 0, hi = 2 * e + 1 < valid ? q[2 * e + 1] : 0;
+        w[e] = lo | hi << 16;
       }
-    } else {
+    }
+  }
+
+  // Without the first n values (of 0 to 8), zeros behind the others.
+  __device__ __forceinline__ void drop(int n) {
+    constexpr int EACH = 8 / WORDS;
+    if constexpr (EACH == 2) {
 #pragma unroll
-      for (int e = 0; e < WORDS; ++e) {
-        if constexpr (TYPE == kFloat32) {
-          w[e] = e < valid ? reinterpret_cast<const unsigned *>(p)[e] : 0;
-        } else {
-          const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-          const unsigned lo = 2 * e < valid ? q[2 * e] : 0, hi = 2 * e + 1 < valid ? q[2 * e + 1] : 0;
-          w[e] = lo | hi << 16;
-        }
-      }
+      for (int e = 0; e < WORDS; ++e) w[e] = n & 1 ? w[e] >> 16 | (e + 1 < WORDS ? w[e + 1] << 16 : 0) : w[e];
+    }
+#pragma unroll
+    for (int by = 1; by <= WORDS; by *= 2) {
+#pragma unroll
+      for (int e = 0; e < WORDS; ++e) w[e] = n & by * EACH ? (e + by < WORDS ? w[e + by] : 0) : w[e];
     }
   }
 
@@ -79,6 +93,27 @@ template <int TYPE> struct Eight {
     for (int e = 0; e < WORDS; ++e) asm volatile("" : "+v"(w[e]));
   }
 };
+
+// Values n0 to n0 + 7 of R rows, of which `rows` are there (perhaps none) and have n values; `first`: the first one of them, behind
+// another row if there is none. Where a wave is not whole, its lanes read the row's last eight and the last row instead and
+// drop what they are not for: no lane waits for another's branch.
+template <int TYPE, int R>
+__device__ __forceinline__ void load_rows(const typename Loaded<TYPE>::type *first, size_t pitch, int rows, unsigned n0, unsigned n,
+                                          Eight<TYPE> (&v)[R]) {
+  if (__all(rows >= R && n0 + 8 <= n)) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i].load(first + (ptrdiff_t)i * (ptrdiff_t)pitch + n0);
+  } else if (n >= 8) {
+    const unsigned from = n0 < n - 8 ? n0 : n - 8, behind = n0 - from < 8 ? n0 - from : 8;
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i].load(first + (ptrdiff_t)(i < rows ? i : rows - 1) * (ptrdiff_t)pitch + from);
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i].drop(i < rows ? (int)behind : 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i].load_some(first + (ptrdiff_t)i * (ptrdiff_t)pitch + n0, i < rows && n0 < n ? (int)(n - n0) : 0);
+  }
+}
 
 // Magnitudes are compared as the integers that their bits are, in 16-bit types two at a time; infinity and NaN are the
 // largest ones.
@@ -229,8 +264,8 @@ __global__ __launch_bounds__(256) void quantize_rows(Args a) {
   if (row >= a.batch * a.m) return;
   const unsigned b = row / a.m, r = row - b * a.m;
   const unsigned n0 = g * kGroup + (threadIdx.x & 15) * 8;
-  Eight<TIN> v;
-  v.load(reinterpret_cast<const In *>(a.in) + (size_t)row * a.in_pitch + n0, n0 < a.n ? (int)(a.n - n0) : 0);
+  Eight<TIN> rows[1], &v = rows[0];
+  load_rows<TIN, 1>(reinterpret_cast<const In *>(a.in) + (size_t)row * a.in_pitch, a.in_pitch, 1, n0, a.n, rows);
   unsigned amax = 0;
 #pragma unroll
   for (int e = 0; e < v.WORDS; ++e) amax = larger_of_word<TIN>(amax, magnitudes<TIN, true>(v.w[e]));
@@ -260,11 +295,9 @@ __global__ __launch_bounds__(256) void quantize_tile(Args a) {
   const unsigned tiles = a.tiles_m * a.tiles_n, tile = id * part + (id < rest ? id : rest) + blockIdx.x / 8;
   const unsigned b = tile / tiles, t = tile - b * tiles, tm = t / a.tiles_n, tn = t - tm * a.tiles_n;
   const unsigned m0 = tm * kGroup + r8 * 8, n0 = tn * kGroup + c * 8;
-  const In *in = reinterpret_cast<const In *>(a.in) + ((size_t)b * a.m + m0) * a.in_pitch + n0;
-  const int valid = n0 < a.n ? (int)(a.n - n0) : 0;
+  const In *in = reinterpret_cast<const In *>(a.in) + ((size_t)b * a.m + m0) * a.in_pitch;
   Eight<TIN> v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i].load(in + (size_t)i * a.in_pitch, m0 + i < a.m ? valid : 0);
+  load_rows<TIN, 8>(in, a.in_pitch, (int)(a.m - m0), n0, a.n, v);
 
   unsigned rows[8], columns[8], all = 0;
   maxima_of<TIN, false>(v, rows, columns);
