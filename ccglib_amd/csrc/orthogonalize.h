@@ -188,11 +188,13 @@ template <bool PAIRS, int STEP> struct StoreChain {
 
 // Block shapes: BX x BY, waves, ring, waves a SIMD. 128 x 128 with eight waves is for products that have no more blocks than
 // units: P X of 1024 x 4096 takes 22.2 us with four waves a block and 15.6 with eight.
+// 192 x 192: A of 4096 x 8192 has 136 blocks of 256 x 256 for 256 units and takes 167 us, with 253 blocks 136.
 #define CCGLIB_HALF_SHAPES(DO) \
   DO(0, 256, 256, 2, 4, 2, 2)  \
   DO(1, 128, 128, 2, 2, 2, 2)  \
   DO(2, 64, 64, 2, 2, 4, 2)    \
-  DO(3, 128, 128, 4, 2, 4, 2)
+  DO(3, 128, 128, 4, 2, 4, 2)  \
+  DO(4, 192, 192, 4, 2, 3, 2)
 #define CCGLIB_HALF_PAIRS_SHAPES(DO) \
   DO(0, 128, 128, 2, 4, 2, 2)        \
   DO(1, 64, 64, 2, 2, 2, 2)

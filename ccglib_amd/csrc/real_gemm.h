@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_real(Args arg
   constexpr int WAVES = WX * WY, PLANES = T::kPlanes;
   constexpr int TX = BX / WX, TY = BY / WY, NX = TX / 16, NY = TY / 16;
   // (a lane's neighbours in D: 16 bytes of 16 or 32 bits each, so that a store instruction writes 64 bytes of a row at once)
-  constexpr int NT = T::kWide || NX < 2 ? 1 : 2, GROUP_ROWS = 16 * NT;
+  constexpr int NT = T::kWide || NX % 2 ? 1 : 2, GROUP_ROWS = 16 * NT;
   constexpr int X_COPIES = BX / 8 * PLANES, COPIES_ALL = X_COPIES + BY / 8 * PLANES;
   constexpr int OPERAND_COPIES = COPIES_ALL / WAVES;
   constexpr int SCALE_COPIES = T::kScaled ? (BX + BY + 63) / 64 : 0;

@@ -14,9 +14,9 @@ inline size_t real_blocks(const RealShape &s, size_t batch, size_t nx, size_t ny
 }
 
 // The time of a product as that of its busiest unit: rounds of blocks, all units full in all but the last one. The figures were
-// fitted to 30 problems from 1 x 8192 x 8192 to 4096 x 4096 x 4096 in every shape and 1 to 32 parts (8 bits: about 300 times of
-// each kind within 9 to 19 %, rms, near the fastest choice; fp16: the kernels of a trace). The choice is behind the fastest one
-// by 0.7 % (float scales), 1.1 % (e8m0) and 2 % (32-bit C) in the mean, and by 7, 15 and 9 % at most.
+// fitted to 38 problems from 1 x 8192 x 8192 to 8192 x 4096 x 4096 in every shape and 1 to 32 parts (those within 1.6 times the
+// fastest: 3 to 9 % off, rms; fp16: the kernels of a trace). The choice is behind the fastest one by 0.3 % (e8m0), 0.4 and 1.4 %
+// (float scales of blocks and rows) and 1.1 % (32-bit C) in the mean, and by 12 % at most.
 inline double real_gemm_us(const RealShape &s, size_t blocks, size_t pieces, size_t parts) {
   constexpr size_t kUnits = 256;
   const double per_part = (double)ceil_div(pieces, parts);

@@ -17,13 +17,16 @@ namespace real {
 
 // Block shapes: BX (columns of C) x BY (rows), waves, ring, waves a SIMD. 128 x 128 comes twice: with four waves, two blocks
 // to a unit, and with eight and twice the ring for problems that have no more blocks than units (2048 x 2048 x 4096, float
-// scales: 30.5 and 22.2 us; 4096 x 2048 x 2048, two blocks a unit: 22.1 and 25.3).
+// scales: 30.5 and 22.2 us; 4096 x 2048 x 2048, two blocks a unit: 22.1 and 25.3). 192 x 192 fills units that larger blocks
+// would leave idle and smaller ones would not feed (3000 x 3000 x 8192, e8m0: 256 x 256 78 us, 192 x 192 62, 128 x 128 101;
+// float scales of rows 111, 84, 127).
 #define CCGLIB_SCALED_SHAPES(DO) \
   DO(0, 256, 256, 2, 4, 2, 2)    \
   DO(1, 128, 128, 2, 2, 2, 2)    \
   DO(2, 64, 64, 2, 2, 4, 2)      \
   DO(3, 64, 32, 4, 1, 6, 2)      \
-  DO(4, 128, 128, 4, 2, 4, 2)
+  DO(4, 128, 128, 4, 2, 4, 2)    \
+  DO(5, 192, 192, 2, 4, 3, 2)
 // (fp16 operands take twice the registers)
 #define CCGLIB_WIDE_SHAPES(DO) \
   DO(0, 128, 256, 2, 4, 2, 2)  \
@@ -77,8 +80,10 @@ template <> hipError_t launch_scaled_mode<kWideE8m0>(const ScaledGemmParams &p, 
 template <int MODE, int FX, int FY>
 hipError_t launch_scaled(int shape, unsigned grid, const Args &a, const StoreC::Params &e, hipStream_t stream) {
 #define CCGLIB_CASE(ID, BX, BY, WX, WY, SLOTS, EU)                                                       \
-  case ID:                                                                                               \
-    gemm_real<MODE, FX, FY, BX, BY, WX, WY, SLOTS, EU, StoreC><<<grid, 64 * WX * WY, 0, stream>>>(a, e); \
+  case ID:                                                                                                 \
+    if constexpr (!ModeTraits<MODE>::kBlocks || BX % 128 == 0 || 128 % BX == 0) {                          \
+      gemm_real<MODE, FX, FY, BX, BY, WX, WY, SLOTS, EU, StoreC><<<grid, 64 * WX * WY, 0, stream>>>(a, e); \
+    }                                                                                                      \
     break;
   if constexpr (ModeTraits<MODE>::kWide) {
     switch (shape) { CCGLIB_WIDE_SHAPES(CCGLIB_CASE) }

@@ -9,25 +9,36 @@ namespace ccglib_amd {
 namespace {
 
 // (the shapes of scaled_gemm.h, in their order; see real_plan.h for the figures)
-constexpr RealShape kFloatShapes[] = {{256, 256, 1, 1.02f, 1.86f, 6.8f, 0.93f, "256x256"},
-                                      {128, 128, 2, 0.72f, 1.38f, 3.4f, 1.20f, "128x128"},
-                                      {64, 64, 2, 0.234f, 0.431f, 2.8f, 2.5f, "64x64"},
-                                      {64, 32, 2, 0.187f, 0.325f, 2.1f, 6.2f, "32x64"},
-                                      {128, 128, 1, 0.35f, 0.63f, 3.9f, 1.00f, "128x128 8-wave"}};
-constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.93f, 1.64f, 7.0f, 0.89f, "256x256"},
-                                     {128, 128, 2, 0.69f, 1.30f, 3.2f, 1.20f, "128x128"},
-                                     {64, 64, 2, 0.20f, 0.417f, 2.6f, 2.6f, "64x64"},
-                                     {64, 32, 2, 0.186f, 0.31f, 2.0f, 6.4f, "32x64"},
-                                     {128, 128, 1, 0.29f, 0.56f, 4.0f, 1.00f, "128x128 8-wave"}};
-constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.14f, 2.43f, 7.8f, 0.75f, "256x128"},
-                                     {128, 128, 2, 1.06f, 2.26f, 7.3f, 1.22f, "128x128"},
-                                     {64, 64, 2, 0.44f, 0.745f, 3.4f, 2.3f, "64x64"},
-                                     {64, 32, 2, 0.304f, 0.49f, 2.35f, 5.2f, "32x64"},
-                                     {128, 128, 1, 0.79f, 1.31f, 5.6f, 0.93f, "128x128 8-wave"}};
-constexpr int kShapes = sizeof kFloatShapes / sizeof kFloatShapes[0];
+constexpr RealShape kBlocksShapes[] = {{256, 256, 1, 0.92f, 1.79f, 8.0f, 0.69f, "256x256"},
+                                       {128, 128, 2, 0.81f, 1.07f, 4.2f, 1.06f, "128x128"},
+                                       {64, 64, 2, 0.243f, 0.442f, 2.5f, 2.4f, "64x64"},
+                                       {64, 32, 2, 0.181f, 0.33f, 2.7f, 4.5f, "32x64"},
+                                       {128, 128, 1, 0.45f, 0.62f, 3.4f, 0.92f, "128x128 8-wave"},
+                                       {192, 192, 1, 0.78f, 1.27f, 5.6f, 0.96f, "192x192"}};
+constexpr RealShape kRowsShapes[] = {{256, 256, 1, 1.16f, 2.17f, 8.6f, 0.82f, "256x256"},
+                                     {128, 128, 2, 0.88f, 1.25f, 4.3f, 1.15f, "128x128"},
+                                     {64, 64, 2, 0.278f, 0.481f, 2.6f, 2.4f, "64x64"},
+                                     {64, 32, 2, 0.206f, 0.356f, 2.5f, 4.6f, "32x64"},
+                                     {128, 128, 1, 0.55f, 0.69f, 3.9f, 0.88f, "128x128 8-wave"},
+                                     {192, 192, 1, 0.82f, 1.25f, 5.7f, 0.95f, "192x192"}};
+constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.84f, 1.56f, 7.8f, 0.74f, "256x256"},
+                                     {128, 128, 2, 0.76f, 0.95f, 4.8f, 1.23f, "128x128"},
+                                     {64, 64, 2, 0.213f, 0.433f, 2.3f, 2.5f, "64x64"},
+                                     {64, 32, 2, 0.164f, 0.306f, 3.2f, 5.4f, "32x64"},
+                                     {128, 128, 1, 0.38f, 0.53f, 3.6f, 1.05f, "128x128 8-wave"},
+                                     {192, 192, 1, 0.57f, 0.89f, 5.9f, 0.92f, "192x192"}};
+constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.34f, 1.97f, 8.5f, 0.98f, "256x128"},
+                                     {128, 128, 2, 1.13f, 1.97f, 7.1f, 1.73f, "128x128"},
+                                     {64, 64, 2, 0.459f, 0.758f, 2.9f, 2.4f, "64x64"},
+                                     {64, 32, 2, 0.304f, 0.505f, 2.6f, 4.1f, "32x64"},
+                                     {128, 128, 1, 0.87f, 1.24f, 5.4f, 1.08f, "128x128 8-wave"}};
+constexpr int kShapes = sizeof kBlocksShapes / sizeof kBlocksShapes[0], kWideCount = sizeof kWideShapes / sizeof kWideShapes[0];
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
   static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
-#define CCGLIB_TABLE kFloatShapes
+#define CCGLIB_TABLE kBlocksShapes
+CCGLIB_SCALED_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_TABLE
+#define CCGLIB_TABLE kRowsShapes
 CCGLIB_SCALED_SHAPES(CCGLIB_SAME)
 #undef CCGLIB_TABLE
 #define CCGLIB_TABLE kE8m0Shapes
@@ -46,13 +57,14 @@ int mode_of(const ScaledGemmParams &p) {
 }
 
 const RealShape *shapes_of(const ScaledGemmParams &p) {
-  return is_wide(p) ? kWideShapes : p.scale_type == kScaleE8m0 ? kE8m0Shapes : kFloatShapes;
+  if (is_wide(p)) return kWideShapes;
+  return p.scale_type == kScaleE8m0 ? kE8m0Shapes : p.group_b == kScaleBlocks ? kBlocksShapes : kRowsShapes;
 }
 
 }  // namespace
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
-  return plan_real_gemm(shapes_of(p), kShapes, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
+  return plan_real_gemm(shapes_of(p), is_wide(p) ? kWideCount : kShapes, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {
@@ -66,7 +78,9 @@ const char *describe_scaled_gemm(const ScaledGemmParams &p) {
 hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
   const RealShape &shape = shapes_of(p)[p.plan.shape];
-  const int mode = mode_of(p);
+  int mode = mode_of(p);
+  // (a wave of such a block has columns of two scales)
+  if (mode == real::kScaledBlocks && shape.bx % 128 != 0 && 128 % shape.bx != 0) mode = real::kScaledRows;
   real::Args a = {};
   a.x = static_cast<const char *>(p.b);
   a.y = static_cast<const char *>(p.a);

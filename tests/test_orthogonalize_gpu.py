@@ -219,3 +219,14 @@ def test_no_row_of_a_32_bit_update_is_worse_than_its_roundings(M, N, seed):
     want = orthogonalized(g)
     off = (got.double().cpu() - want).norm(dim=2) / want.norm(dim=2)
     assert float(off.max()) < 4e-6
+
+
+@pytest.mark.parametrize("parts", [1, 3])
+def test_blocks_of_192(parts):
+    gen = torch.Generator().manual_seed(13)
+    t = VT.bfloat16
+    for B, M, N in [(2, 5, 9), (1, 70, 260), (2, 280, 130), (1, 400, 330), (1, 390, 500)]:
+        g = update(B, M, N, t, gen)
+        with cc.option(cc.Option.real_block, 5 + 256 * parts):
+            got, _ = run(g, t)
+        assert near(got, orthogonalized(g), t), (B, M, N)

@@ -299,3 +299,19 @@ def test_as_many_blocks_as_units():
     for M, N, K in [(2048, 2048, 700), (2000, 2040, 1000)]:
         op, c, want, _ = product(1, M, N, K, tc=VT.bfloat16, spread=0.0)
         assert "8-wave" in op.KernelName()
+
+
+@pytest.mark.parametrize("tc", [VT.bfloat16, VT.float16])
+@pytest.mark.parametrize("ga,gb", list(itertools.product(SG, SG)))
+@pytest.mark.parametrize("st", list(ST))
+@pytest.mark.parametrize("parts", [1, 3])
+def test_blocks_of_192(tc, ga, gb, st, parts):
+    """Waves whose columns have two scales of 128 x 128; sizes that end inside blocks."""
+    with cc.option(cc.Option.real_block, 6 + 256 * parts):
+        for B, M, N, K in [(1, 1, 5, 16), (2, 70, 140, 130), (1, 270, 400, 384), (1, 193, 300, 515), (1, 385, 383, 1100)]:
+            product(B, M, N, K, tc=tc, ga=ga, gb=gb, st=st, ta=VT.float8e5m2)
+
+
+def test_192_is_chosen_where_larger_blocks_leave_units_idle():
+    op, c, want, _ = product(1, 3000, 3000, 600, tc=VT.bfloat16, st=ST.e8m0, spread=0.0)
+    assert "192x192" in op.KernelName()
