@@ -46,7 +46,8 @@ inline RealGemmPlan plan_real_gemm(const RealShape *shapes, int count, size_t ba
   size_t parts = 0;
   for (int s = first; s < end; ++s) {
     const size_t blocks = real_blocks(shapes[s], batch, nx, ny, symmetric);
-    for (size_t p = 1; p <= 32 && p <= pieces; p *= 2) {
+    for (size_t p : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (p > pieces) break;
       const double us = real_gemm_us(shapes[s], blocks, pieces, p);
       if (parts == 0 || us < best) {
         best = us;
