@@ -36,7 +36,7 @@ template <> struct Value<kFloat16> { using type = _Float16; };
 template <> struct Value<kBfloat16> { using type = __bf16; };
 
 // partial[b][block] = sum of the squares of a part of matrix b: a block has `rows` x kNormColumns values, a thread eight
-// neighbours at a time
+// neighbours at a time. Bound by memory: 4096 x 8192 bf16 15 us, 4.5 TB/s; 4096 x 1024 5 us, two round trips.
 constexpr unsigned kNormColumns = 2048;
 template <int TYPE>
 __global__ __launch_bounds__(256) void sum_of_squares(const typename Value<TYPE>::type *in, size_t pitch, unsigned m, unsigned n,
@@ -99,7 +99,8 @@ __device__ __forceinline__ int exponent_and_factor(double sum, float epsilon, fl
   return e;
 }
 
-// to[r][c] and to_t[c][r] = G[r][c] 2^e, 64 x 64 values a block
+// to[r][c] and to_t[c][r] = G[r][c] 2^e, 64 x 64 values a block, transposed through LDS. Bound by memory: 4096 x 8192 bf16
+// 43 us, 4.7 TB/s.
 template <int TYPE, bool PAIRS>
 __global__ __launch_bounds__(256) void to_halves(const typename Value<TYPE>::type *in, size_t in_pitch, unsigned m, unsigned n,
                                                  _Float16 *to, unsigned to_pitch, size_t to_batch, size_t to_plane,
@@ -533,8 +534,8 @@ Layout layout_of(const OrthogonalizeParams &p) {
   l.t_plane = l.n * l.mp;
   l.a_plane = l.m * l.mp;
   l.norm_x = (unsigned)ceil_div(p.n, (size_t)kNormColumns);
-  // (at least 16 rows, and at most about 2048 partial sums, which every block of to_halves adds up)
-  l.norm_rows = (unsigned)std::max<size_t>(16, ceil_div((size_t)p.m * l.norm_x, 2048));
+  // (at least 8 rows, and at most about 1024 partial sums, which every block of to_halves adds up)
+  l.norm_rows = (unsigned)std::max<size_t>(8, ceil_div((size_t)p.m * l.norm_x, 1024));
   l.norm_y = (unsigned)ceil_div(p.m, (size_t)l.norm_rows);
   size_t counters = 0, partial = 0;
   const Product products[] = {plan_product(p, l.m, l.m, l.n, true), plan_product(p, l.m, l.m, l.m, true),

