@@ -230,3 +230,18 @@ def test_blocks_of_192(parts):
         with cc.option(cc.Option.real_block, 5 + 256 * parts):
             got, _ = run(g, t)
         assert near(got, orthogonalized(g), t), (B, M, N)
+
+
+@pytest.mark.parametrize("t", list(WIDE))
+@pytest.mark.parametrize("M,N", [(333, 301), (150, 517), (60, 100)])
+def test_a_matrix_of_nan_leaves_nothing_behind(t, M, N):
+    """The object's next run, with an ordinary matrix, is that of a new object."""
+    gen = torch.Generator().manual_seed(14)
+    g = update(2, M, N, t, gen)
+    want, _ = run(g, t)
+    bad, out = torch.full_like(g, float("nan")), torch.empty_like(g)
+    op = cc.Orthogonalize(2, M, N, 0, stream(), t)
+    for x in (bad, g):
+        op.Run(x.data_ptr(), out.data_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
