@@ -6,7 +6,7 @@
 #include <new>
 
 #include "host_util.h"
-#include "scaled.h"
+#include "scaled_linear.h"
 
 using namespace ccglib_amd;
 
@@ -27,7 +27,6 @@ struct Buffer {
 
 bool is_group(int g) { return g == kScaleRows || g == kScaleBlocks; }
 bool is_scale(int s) { return s == kScaleFloat32 || s == kScaleE8m0; }
-size_t scale_size(int s) { return s == kScaleE8m0 ? 1 : 4; }
 bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
 
 // Allocates `bytes` and clears the first `zeroed`; the memory is cleared when the call returns.
@@ -100,11 +99,6 @@ int check_operand(const char *what, const void *values, const void *scales, int 
 
 size_t element(int type) { return (size_t)bits_of(type) / 8; }
 
-// Allocates what a planned product needs: counters (cleared), then partial sums.
-size_t gemm_workspace(const RealGemmPlan &plan) {
-  return plan.parts > 1 ? ceil_div(plan.counter_bytes, 256) * 256 + plan.partial_bytes : 0;
-}
-
 }  // namespace
 
 struct ccglib_quantize {
@@ -121,12 +115,10 @@ struct ccglib_scaled_gemm {
 };
 
 struct ccglib_scaled_linear {
-  size_t M, N, K;
-  int type, scale_type, device;
-  bool training, have_weights = false, have_forward = false;
+  ScaledLinearParams p;
+  int device;
   hipStream_t stream;
-  QuantizeParams x, w, dy;
-  ScaledGemmParams y, dx, dw;
+  bool have_weights = false, have_forward = false;
   Buffer memory;
 };
 
@@ -222,11 +214,14 @@ int ccglib_scaled_gemm_create(ccglib_scaled_gemm_t *gemm, size_t B, size_t M, si
   p.plan = plan_scaled_gemm(p);
   auto *g = new (std::nothrow) ccglib_scaled_gemm{p, device, static_cast<hipStream_t>(stream), {}};
   if (!g) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
-  if (int s = allocate(&g->workspace, gemm_workspace(p.plan), p.plan.counter_bytes)) {
+  // counters (cleared), then partial sums
+  const size_t counters = ceil_div(p.plan.counter_bytes, 256) * 256;
+  if (int s = allocate(&g->workspace, counters + p.plan.partial_bytes, p.plan.counter_bytes)) {
     delete g;
     return s;
   }
-  g->p.workspace = g->workspace.p;
+  g->p.arrived = reinterpret_cast<unsigned *>(g->workspace.at(0));
+  g->p.partial = reinterpret_cast<float *>(g->workspace.at(counters));
   *gemm = g;
   return CCGLIB_OK;
 }
@@ -273,132 +268,36 @@ int ccglib_scaled_linear_create(ccglib_scaled_linear_t *linear, size_t M, size_t
   if (!linear) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: linear");
   *linear = nullptr;
   if (M > kMostPitch || N > kMostPitch || K > kMostPitch) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
-  auto quantize = [&](size_t m, size_t n, int out, int group) {
-    QuantizeParams p = {};
-    p.batch = 1;
-    p.m = (unsigned)m;
-    p.n = (unsigned)n;
-    p.in_pitch = n;
-    p.type_in = type;
-    p.type_out = out;
-    p.group = group;
-    p.scale_type = scale_type;
-    return p;
-  };
-  auto gemm = [&](size_t m, size_t n, size_t k, int a, int c, int group_b) {
-    ScaledGemmParams p = {};
-    p.batch = 1;
-    p.m = (unsigned)m;
-    p.n = (unsigned)n;
-    p.k = (unsigned)k;
-    p.pitch_a = p.pitch_b = scaled_pitch(k);
-    p.pitch_c = n;
-    p.type_a = a;
-    p.type_b = kFloat8e4m3;
-    p.type_c = c;
-    p.group_a = kScaleRows;
-    p.group_b = group_b;
-    p.scale_type = scale_type;
-    return p;
-  };
-  const QuantizeParams qx = quantize(M, K, kFloat8e4m3, kScaleRows), qw = quantize(N, K, kFloat8e4m3, kScaleBlocks),
-                       qdy = quantize(M, N, gradient_type, kScaleRows);
-  ScaledGemmParams y = gemm(M, N, K, kFloat8e4m3, type, kScaleBlocks), dx = gemm(M, K, N, gradient_type, type, kScaleBlocks),
-                   dw = gemm(N, K, M, gradient_type, kFloat32, kScaleRows);
-  if (int s = check_quantize(qx, 1, M, K)) return s;
-  if (int s = check_quantize(qw, 1, N, K)) return s;
-  if (int s = check_quantize(qdy, 1, M, N)) return s;
-  if (int s = check_gemm(y, 1, M, N, K)) return s;
-  if (int s = check_gemm(dx, 1, M, K, N)) return s;
-  if (int s = check_gemm(dw, 1, N, K, M)) return s;
+  ScaledLinearParams p = scaled_linear_params(M, N, K, type, gradient_type, scale_type, training != 0);
+  if (int s = check_quantize(p.x, 1, M, K)) return s;
+  if (int s = check_quantize(p.w, 1, N, K)) return s;
+  if (int s = check_quantize(p.dy, 1, M, N)) return s;
+  if (int s = check_gemm(p.y, 1, M, N, K)) return s;
+  if (int s = check_gemm(p.dx, 1, M, K, N)) return s;
+  if (int s = check_gemm(p.dw, 1, N, K, M)) return s;
   if (int s = check_device(device)) return s;
   DeviceGuard guard(device);
   HIP_TRY(guard.status());
-  auto *l = new (std::nothrow) ccglib_scaled_linear;
+  auto *l = new (std::nothrow) ccglib_scaled_linear{p, device, static_cast<hipStream_t>(stream)};
   if (!l) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
-  l->M = M;
-  l->N = N;
-  l->K = K;
-  l->type = type;
-  l->scale_type = scale_type;
-  l->device = device;
-  l->training = training != 0;
-  l->stream = static_cast<hipStream_t>(stream);
-  // One allocation: counters and partial sums that the three products share (they run one after the other), then the
-  // 8-bit copies of x, w and dy in both orientations (without training: of x and w as they are).
-  size_t counters = 0, partial = 0, at = 0;
-  ScaledGemmParams *const products[] = {&y, &dx, &dw};
-  for (int i = 0; i < (l->training ? 3 : 1); ++i) {
-    ScaledGemmParams &p = *products[i];
-    p.plan = plan_scaled_gemm(p);
-    if (p.plan.counter_bytes > counters) counters = p.plan.counter_bytes;
-    if (p.plan.partial_bytes > partial) partial = p.plan.partial_bytes;
-  }
-  auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += ceil_div(bytes, 256) * 256;
-    return here;
-  };
-  take(counters);
-  // (a product's partial sums follow its own counters)
-  take(partial);
-  struct Copy {
-    size_t values, scales;
-  };
-  auto copy = [&](size_t rows, size_t k, int group) {
-    Copy c;
-    c.values = take(rows * scaled_pitch(k));
-    c.scales = take(ceil_div(k, kScaleGroup) * scaled_pitch(scale_rows(rows, group)) * scale_size(scale_type));
-    return c;
-  };
-  const Copy cx = copy(M, K, kScaleRows), cw = copy(N, K, kScaleBlocks);
-  Copy cxt{}, cwt{}, cdy{}, cdyt{};
-  if (l->training) {
-    cxt = copy(K, M, kScaleRows);
-    cwt = copy(K, N, kScaleBlocks);
-    cdy = copy(M, N, kScaleRows);
-    cdyt = copy(N, M, kScaleRows);
-  }
-  if (int s = allocate(&l->memory, at, counters)) {
+  plan_scaled_linear(&l->p);
+  place_scaled_linear(&l->p, nullptr);
+  if (int s = allocate(&l->memory, l->p.bytes, l->p.counter_bytes)) {
     delete l;
     return s;
   }
-  auto outputs = [&](QuantizeParams p, const Copy &direct, const Copy &transposed) {
-    p.out = l->memory.at(direct.values);
-    p.scales = l->memory.at(direct.scales);
-    if (l->training) {
-      p.out_t = l->memory.at(transposed.values);
-      p.scales_t = l->memory.at(transposed.scales);
-    }
-    return p;
-  };
-  l->x = outputs(qx, cx, cxt);
-  l->w = outputs(qw, cw, cwt);
-  if (l->training) l->dy = outputs(qdy, cdy, cdyt);
-  auto operands = [&](ScaledGemmParams p, const Copy &a, const Copy &b) {
-    p.a = l->memory.at(a.values);
-    p.scales_a = l->memory.at(a.scales);
-    p.b = l->memory.at(b.values);
-    p.scales_b = l->memory.at(b.scales);
-    p.workspace = l->memory.p;
-    return p;
-  };
-  l->y = operands(y, cx, cw);
-  if (l->training) {
-    l->dx = operands(dx, cdy, cwt);
-    l->dw = operands(dw, cdyt, cxt);
-  }
+  place_scaled_linear(&l->p, l->memory.at(0));
   *linear = l;
   return CCGLIB_OK;
 }
 
 int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t l, const void *d_w) {
   if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
-  if (!d_w && l->N && l->K) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: weights");
-  if (!aligned(d_w, element(l->type))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned weights");
+  if (!d_w && l->p.w.m && l->p.w.n) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: weights");
+  if (!aligned(d_w, element(l->p.x.type_in))) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned weights");
   DeviceGuard guard(l->device);
   HIP_TRY(guard.status());
-  QuantizeParams p = l->w;
+  QuantizeParams p = l->p.w;
   p.in = d_w;
   HIP_TRY(launch_quantize(p, l->stream));
   l->have_weights = true;
@@ -408,16 +307,16 @@ int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t l, const void *d_w) 
 int ccglib_scaled_linear_forward(ccglib_scaled_linear_t l, const void *d_x, void *d_y) {
   if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
   if (!l->have_weights) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: forward before the weights were set");
-  if ((!d_x && l->M && l->K) || (!d_y && l->M && l->N)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: x or y");
-  if (!aligned(d_x, element(l->type)) || !aligned(d_y, element(l->type))) {
+  if ((!d_x && l->p.x.m && l->p.x.n) || (!d_y && l->p.y.m && l->p.y.n)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: x or y");
+  if (!aligned(d_x, element(l->p.x.type_in)) || !aligned(d_y, element(l->p.x.type_in))) {
     return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned x or y");
   }
   DeviceGuard guard(l->device);
   HIP_TRY(guard.status());
-  QuantizeParams q = l->x;
+  QuantizeParams q = l->p.x;
   q.in = d_x;
   HIP_TRY(launch_quantize(q, l->stream));
-  ScaledGemmParams p = l->y;
+  ScaledGemmParams p = l->p.y;
   p.c = d_y;
   HIP_TRY(launch_scaled_gemm(p, l->stream));
   l->have_forward = true;
@@ -426,27 +325,27 @@ int ccglib_scaled_linear_forward(ccglib_scaled_linear_t l, const void *d_x, void
 
 int ccglib_scaled_linear_backward(ccglib_scaled_linear_t l, const void *d_dy, void *d_dx, void *d_dw, int accumulate_dw) {
   if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
-  if (!l->training) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward of a layer that was created without training");
+  if (!l->p.training) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward of a layer that was created without training");
   if (!l->have_forward) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward before forward");
   if (!d_dx && !d_dw) return CCGLIB_OK;
-  if (!d_dy && l->M && l->N) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: dy");
-  if (!aligned(d_dy, element(l->type)) || !aligned(d_dx, element(l->type)) || !aligned(d_dw, 4)) {
+  if (!d_dy && l->p.y.m && l->p.y.n) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: dy");
+  if (!aligned(d_dy, element(l->p.x.type_in)) || !aligned(d_dx, element(l->p.x.type_in)) || !aligned(d_dw, 4)) {
     return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: misaligned dy, dx or dw");
   }
   DeviceGuard guard(l->device);
   HIP_TRY(guard.status());
-  QuantizeParams q = l->dy;
+  QuantizeParams q = l->p.dy;
   q.in = d_dy;
   if (!d_dx) q.out = q.scales = nullptr;
   if (!d_dw) q.out_t = q.scales_t = nullptr;
   HIP_TRY(launch_quantize(q, l->stream));
   if (d_dx) {
-    ScaledGemmParams p = l->dx;
+    ScaledGemmParams p = l->p.dx;
     p.c = d_dx;
     HIP_TRY(launch_scaled_gemm(p, l->stream));
   }
   if (d_dw) {
-    ScaledGemmParams p = l->dw;
+    ScaledGemmParams p = l->p.dw;
     p.c = d_dw;
     p.accumulate = accumulate_dw != 0;
     HIP_TRY(launch_scaled_gemm(p, l->stream));

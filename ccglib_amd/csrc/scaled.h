@@ -29,7 +29,7 @@ struct QuantizeParams {
 };
 hipError_t launch_quantize(const QuantizeParams &p, hipStream_t stream);
 
-// What a product of given sizes runs as; the workspace is partial sums (floats), then a counter for each block of C.
+// What a product of given sizes runs as, and its workspace: partial sums (floats), and a counter for each block of C.
 struct RealGemmPlan {
   int shape = 0;
   unsigned parts = 1, pieces_per_part = 0;
@@ -55,7 +55,8 @@ struct ScaledGemmParams {
   int type_a, type_b, type_c, group_a, group_b, scale_type;
   int accumulate;
   RealGemmPlan plan;
-  void *workspace;
+  unsigned *arrived;                  // the plan's counters, zero when a product starts (it leaves them so)
+  float *partial;                     // the plan's partial sums
 };
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p);
 hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream);

@@ -103,8 +103,8 @@ hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream) {
   a.y_shift = p.group_a == kScaleBlocks ? 7 : 0;
   a.parts = p.plan.parts;
   a.pieces_per_part = p.plan.pieces_per_part;
-  a.arrived = static_cast<unsigned *>(p.workspace);
-  a.partial = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + ceil_div(p.plan.counter_bytes, 256) * 256);
+  a.arrived = p.arrived;
+  a.partial = p.partial;
   switch (mode) {
     case real::kScaledBlocks: return real::launch_scaled_mode<real::kScaledBlocks>(p, a, stream);
     case real::kScaledRows: return real::launch_scaled_mode<real::kScaledRows>(p, a, stream);
