@@ -9,18 +9,20 @@ import re
 import shutil
 import subprocess
 import sys
+import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB_PATH = os.path.join(HERE, "libccglib_amd.so")
-# (gemm_mfma.hip is compiled in parts, one per input type, so that they build in parallel)
-SOURCES = ["capi.hip", "gemm_mfma_f16.hip", "gemm_mfma_bf16.hip", "gemm_mfma_f32.hip",
-           "gemm_mfma_fp8.hip", "gemm_mfma_int1.hip", "gemm_mfma_dispatch.hip", "gemm_int1.hip",
-           "transpose.hip", "packing.hip", "host_copy.hip", "quantize.hip", "scaled_gemm.hip",
-           "scaled_gemm_blocks.hip", "scaled_gemm_rows.hip", "scaled_gemm_e8m0.hip",
-           "scaled_gemm_wide_blocks.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_e8m0.hip",
-           "orthogonalize.hip", "operators_capi.hip"]
+# (gemm_mfma.hip is compiled in parts, one per input type, and type of C for 16 bits, so that they build in parallel; those that
+# take longest come first)
+SOURCES = ["gemm_mfma_f16_f32.hip", "gemm_mfma_bf16_f32.hip", "gemm_mfma_f16_f16.hip", "gemm_mfma_bf16_bf16.hip",
+           "gemm_mfma_f32.hip", "gemm_mfma_fp8.hip", "scaled_gemm_rows.hip", "scaled_gemm_blocks.hip",
+           "scaled_gemm_e8m0.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_blocks.hip",
+           "scaled_gemm_wide_e8m0.hip", "orthogonalize.hip", "quantize.hip", "gemm_mfma_int1.hip", "transpose.hip",
+           "gemm_int1.hip", "packing.hip", "capi.hip", "operators_capi.hip", "scaled_gemm.hip",
+           "gemm_mfma_dispatch.hip", "host_copy.hip"]
 # Packed-fp32 instruction selection is switched off for all device code.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
@@ -58,8 +60,17 @@ def _with_includes(path, found=None):
     return found
 
 
+def _object(src):
+    return os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
+
+
+def _compiler_version():
+    r = subprocess.run([_hipcc(), "--version"], capture_output=True, text=True)
+    return "; ".join(r.stdout.splitlines()[:2])
+
+
 def _compile(src, force):
-    obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
+    obj = _object(src)
     path = os.path.join(CSRC, src)
     if not force and not _stale(obj, _with_includes(path)):
         return obj, ""
@@ -67,15 +78,17 @@ def _compile(src, force):
                                                    "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     lines = (r.stdout + r.stderr).splitlines()
-    kept, skip = [], 0
-    for l in lines:      # (the remarks, each with its source line and caret, stay out of the log)
-        if "kernel-resource-usage" in l:
-            skip = 2
+    kept, includes, skip = [], [], 0
+    for l in lines:      # (the remarks, each with its source line, caret and includes, stay out of the log)
+        if l.startswith("In file included from"):
+            includes.append(l)
+        elif "kernel-resource-usage" in l:
+            includes, skip = [], 2
         elif skip and (l.lstrip()[:1].isdigit() or l.strip().startswith("|")):
             skip -= 1
         elif "packed-fp32-ops" not in l:
-            kept.append(l)
-            skip = 0
+            kept += includes + [l]
+            includes, skip = [], 0
     log = "\n".join(kept)
     if r.returncode != 0:
         raise RuntimeError("hipcc failed for %s:\n%s" % (src, log))
@@ -102,21 +115,33 @@ def _no_scratch_in_gemm_kernels(src, remarks):
         elif "ScratchSize [bytes/lane]:" in l and name and ("complex_gemm_mfma" in name or "gemm_real" in name):
             size = int(l.split("ScratchSize [bytes/lane]:")[1].split("[")[0])
             if size > (0 if "complex_gemm_mfma_wide" in name or "gemm_real" in name else 32):
-                os.remove(os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o"))
+                os.remove(_object(src))
                 raise RuntimeError("%s: kernel %s spills %d bytes per lane to scratch memory; its "
                                    "explicit vmcnt counts would not hold" % (src, name, size))
 
 
 def build(force=False, verbose=False):
-    """Compile every HIP source for gfx950 and link the shared library."""
+    """Compile every HIP source for gfx950 and link the shared library.
+
+    A source's outcome is reported when it is known: its time (verbose), or what is wrong with it,
+    upon which nothing further is started."""
     os.makedirs(OBJ_DIR, exist_ok=True)
+    began = time.monotonic()
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        results = list(ex.map(lambda s: _compile(s, force), SOURCES))
-    objs = [o for o, _ in results]
-    if verbose:
-        for _, log in results:
-            if log.strip():
-                print(log)
+        sources = {ex.submit(_compile, s, force): s for s in SOURCES}
+        for done in concurrent.futures.as_completed(sources):
+            try:
+                _, log = done.result()
+            except Exception:
+                for other in sources:
+                    other.cancel()
+                print("%s: failed, %.0f s; compiler: %s" % (sources[done], time.monotonic() - began, _compiler_version()),
+                      file=sys.stderr, flush=True)
+                raise
+            if verbose:
+                print("%s%s: %.0f s" % (log.strip() + "\n" if log.strip() else "", sources[done], time.monotonic() - began),
+                      flush=True)
+    objs = [_object(s) for s in SOURCES]
     if force or _stale(LIB_PATH, objs):
         cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -3368,33 +3368,43 @@ hipError_t launch_typed(const GemmParams &p, hipStream_t stream) {
 
 // The instantiations are spread over several translation units so that they
 // compile in parallel: gemm_mfma_<part>.hip define CCGLIB_GEMM_MFMA_PART and
-// include this file (1 fp16, 2 bf16, 3 fp32, 4 fp8, 5 1-bit input; 0 the
-// dispatch below). Included without the macro (the tuning program), the file
-// holds everything.
+// include this file (1 fp16, 2 bf16, both with fp32 C; 6 fp16, 7 bf16, both with C of
+// the same type; 3 fp32, 4 fp8, 5 1-bit input; 0 the dispatch below). Included without the
+// macro, the file holds everything.
 #ifndef CCGLIB_GEMM_MFMA_PART
 #define CCGLIB_GEMM_MFMA_PART -1
 #endif
 #define CCGLIB_GEMM_MFMA_HAS(part) (CCGLIB_GEMM_MFMA_PART == -1 || CCGLIB_GEMM_MFMA_PART == (part))
 
-hipError_t launch_gemm_mfma_f16(const GemmParams &p, hipStream_t stream);
-hipError_t launch_gemm_mfma_bf16(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_f16_f32(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_f16_f16(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_bf16_f32(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_bf16_bf16(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_f32(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_fp8(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_int1(const GemmParams &p, hipStream_t stream);
 
 #if CCGLIB_GEMM_MFMA_HAS(1)
-hipError_t launch_gemm_mfma_f16(const GemmParams &p, hipStream_t stream) {
-  if (p.type_out == kFloat32) return launch_typed<kFloat16, kFloat32>(p, stream);
-  if (p.type_out == kFloat16) return launch_typed<kFloat16, kFloat16>(p, stream);
-  return hipErrorInvalidValue;
+hipError_t launch_gemm_mfma_f16_f32(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kFloat16, kFloat32>(p, stream);
+}
+#endif
+
+#if CCGLIB_GEMM_MFMA_HAS(6)
+hipError_t launch_gemm_mfma_f16_f16(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kFloat16, kFloat16>(p, stream);
 }
 #endif
 
 #if CCGLIB_GEMM_MFMA_HAS(2)
-hipError_t launch_gemm_mfma_bf16(const GemmParams &p, hipStream_t stream) {
-  if (p.type_out == kFloat32) return launch_typed<kBfloat16, kFloat32>(p, stream);
-  if (p.type_out == kBfloat16) return launch_typed<kBfloat16, kBfloat16>(p, stream);
-  return hipErrorInvalidValue;
+hipError_t launch_gemm_mfma_bf16_f32(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kBfloat16, kFloat32>(p, stream);
+}
+#endif
+
+#if CCGLIB_GEMM_MFMA_HAS(7)
+hipError_t launch_gemm_mfma_bf16_bf16(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kBfloat16, kBfloat16>(p, stream);
 }
 #endif
 
@@ -3517,8 +3527,12 @@ const char *describe_gemm_mfma(const GemmParams &p) {
 
 hipError_t launch_gemm_mfma(const GemmParams &p, hipStream_t stream) {
   switch (p.type_in) {
-    case kFloat16: return launch_gemm_mfma_f16(p, stream);
-    case kBfloat16: return launch_gemm_mfma_bf16(p, stream);
+    case kFloat16:
+      if (p.type_out == kFloat32) return launch_gemm_mfma_f16_f32(p, stream);
+      return p.type_out == kFloat16 ? launch_gemm_mfma_f16_f16(p, stream) : hipErrorInvalidValue;
+    case kBfloat16:
+      if (p.type_out == kFloat32) return launch_gemm_mfma_bf16_f32(p, stream);
+      return p.type_out == kBfloat16 ? launch_gemm_mfma_bf16_bf16(p, stream) : hipErrorInvalidValue;
     case kFloat32: return launch_gemm_mfma_f32(p, stream);
     case kFloat8e4m3:
     case kFloat8e5m2: return launch_gemm_mfma_fp8(p, stream);
