@@ -85,15 +85,21 @@ __device__ __forceinline__ double sum_of(const double *partial, unsigned count, 
 }
 
 // The exponent e of the power of two that X0 is G times, and the factor that is left: 2^-e / (|G| + epsilon).
-// (|G| 2^e is 128 to 256: far from what fp16 cannot hold at either end)
+// (|G| 2^e is 128 to 256: far from what fp16 cannot hold at either end; and the factor at most 2^-7, so that its square, by which
+// the first A is multiplied, is finite. Zeros have no such bound: they stay zeros by whatever they are multiplied, unless epsilon
+// is zero too, and the formula says 0 / 0.)
 __device__ __forceinline__ int exponent_and_factor(double sum, float epsilon, float *factor) {
   const double norm = __builtin_sqrt(sum);
   if (!(norm < __builtin_inf())) {   // an infinity or a NaN among the values: the result is NaN
     *factor = __builtin_nanf("");
     return 0;
   }
+  if (norm == 0.0) {
+    *factor = epsilon > 0.f ? 1.f : __builtin_nanf("");
+    return 0;
+  }
   int e = 0;
-  if (norm > 0.0) (void)__builtin_frexp(norm, &e);
+  (void)__builtin_frexp(norm, &e);
   e = 8 - e;
   *factor = (float)(__builtin_ldexp(1.0, -e) / (norm + (double)epsilon));
   return e;
