@@ -578,6 +578,10 @@ bool is_small(const OrthogonalizeParams &p) {
   return !p.block_option && fits_small(std::min(p.m, p.n), std::max(p.m, p.n), as_pairs(p.type) ? 2 : 1);
 }
 
+// Whether the one launch may not be used in place: its workgroups read and write a matrix each on their own, and a matrix of the
+// output then lies on another one of the input. (Several launches have read all of the input before the first writes.)
+bool meets_another_in_place(const OrthogonalizeParams &p) { return p.batch > 1 && p.in_pitch != p.out_pitch; }
+
 template <bool PAIRS, int STEP>
 hipError_t launch_product(const Product &r, const real::Args &a, const typename real::StoreChain<PAIRS, STEP>::Params &e,
                           hipStream_t stream) {
@@ -608,7 +612,7 @@ hipError_t launch_product(const Product &r, const real::Args &a, const typename 
 template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t stream) {
   constexpr bool PAIRS = TYPE != kBfloat16;
   using V = typename Value<TYPE>::type;
-  if (is_small(p)) {
+  if (is_small(p) && !(p.in == p.out && meets_another_in_place(p))) {
     SmallArgs a = {p.in, p.out, p.in_pitch, p.out_pitch, p.m, p.n, p.steps, p.a, p.b, p.c, p.epsilon};
     orthogonalize_small<TYPE><<<p.batch, 64 * kSmallWaves, 0, stream>>>(a);
     return hipGetLastError();
@@ -729,8 +733,12 @@ template <int TYPE> hipError_t launch(const OrthogonalizeParams &p, hipStream_t 
 
 }  // namespace
 
-size_t orthogonalize_workspace_bytes(const OrthogonalizeParams &p) { return is_small(p) ? 0 : layout_of(p).bytes; }
-size_t orthogonalize_zeroed_bytes(const OrthogonalizeParams &p) { return is_small(p) ? 0 : layout_of(p).zeroed; }
+size_t orthogonalize_workspace_bytes(const OrthogonalizeParams &p) {
+  return is_small(p) && !meets_another_in_place(p) ? 0 : layout_of(p).bytes;
+}
+size_t orthogonalize_zeroed_bytes(const OrthogonalizeParams &p) {
+  return is_small(p) && !meets_another_in_place(p) ? 0 : layout_of(p).zeroed;
+}
 
 hipError_t launch_orthogonalize(const OrthogonalizeParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
