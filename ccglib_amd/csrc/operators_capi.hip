@@ -83,14 +83,14 @@ int check_gemm(const ScaledGemmParams &p, size_t B, size_t M, size_t N, size_t K
                 least, kMostPitch, p.pitch_a, p.pitch_b);
   }
   if (p.pitch_c < N) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledGEMM: rows of C of %zu values at a distance of %zu", N, p.pitch_c);
-  // (blocks of C times pieces of K, each at least 16 x 64 values, are counted in 32 bits)
-  if (B && M && N && ceil_div(M, 16) > kMostBlocks / 64 / B / ceil_div(N, 64)) {
-    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
-  }
   // (a row's scale is found by a 32-bit offset in the scales of its group of K)
   if (scaled_pitch(scale_rows(M, p.group_a)) * scale_size(p.scale_type) > 0xffffffffu ||
       scaled_pitch(scale_rows(N, p.group_b)) * scale_size(p.scale_type) > 0xffffffffu) {
-    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledGEMM: scales of a group of K take 4 GiB or more");
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range: scales of a group of K take 4 GiB or more");
+  }
+  // (blocks of C times pieces of K, each at least 16 x 64 values, are counted in 32 bits)
+  if (B && M && N && ceil_div(M, 16) > kMostBlocks / 64 / B / ceil_div(N, 64)) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range");
   }
   return CCGLIB_OK;
 }
