@@ -95,6 +95,11 @@ int check_gemm(const ScaledGemmParams &p, size_t B, size_t M, size_t N, size_t K
   return CCGLIB_OK;
 }
 
+int check_launch(const ScaledGemmParams &p) {
+  if (scaled_gemm_launches(p)) return CCGLIB_OK;
+  return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "problem size out of range: more blocks of C than a launch takes");
+}
+
 int check_operand(const char *what, const void *values, const void *scales, int scale_type) {
   if (!values || !scales) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: %s", what);
   if (!aligned(values, 16)) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "%s: 8-bit values start at a multiple of 16 bytes", what);
@@ -213,10 +218,11 @@ int ccglib_scaled_gemm_create(ccglib_scaled_gemm_t *gemm, size_t B, size_t M, si
   p.scale_type = scale_type;
   p.accumulate = accumulate != 0;
   if (int s = check_gemm(p, B, M, N, K)) return s;
+  p.plan = plan_scaled_gemm(p);
+  if (int s = check_launch(p)) return s;
   if (int s = check_device(device)) return s;
   DeviceGuard guard(device);
   HIP_TRY(guard.status());
-  p.plan = plan_scaled_gemm(p);
   auto *g = new (std::nothrow) ccglib_scaled_gemm{p, device, static_cast<hipStream_t>(stream), {}};
   if (!g) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
   // counters (cleared), then partial sums
@@ -280,12 +286,15 @@ int ccglib_scaled_linear_create(ccglib_scaled_linear_t *linear, size_t M, size_t
   if (int s = check_gemm(p.y, 1, M, N, K)) return s;
   if (int s = check_gemm(p.dx, 1, M, K, N)) return s;
   if (int s = check_gemm(p.dw, 1, N, K, M)) return s;
+  plan_scaled_linear(&p);
+  for (const ScaledGemmParams *product : {&p.y, &p.dx, &p.dw}) {
+    if (int s = check_launch(*product)) return s;
+  }
   if (int s = check_device(device)) return s;
   DeviceGuard guard(device);
   HIP_TRY(guard.status());
   auto *l = new (std::nothrow) ccglib_scaled_linear{p, device, static_cast<hipStream_t>(stream)};
   if (!l) return fail(CCGLIB_ERROR_RUNTIME, "out of memory");
-  plan_scaled_linear(&l->p);
   place_scaled_linear(&l->p, nullptr);
   if (int s = allocate(&l->memory, l->p.bytes, l->p.counter_bytes)) {
     delete l;

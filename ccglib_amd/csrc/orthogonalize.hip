@@ -496,15 +496,16 @@ struct Product {
 };
 
 // (the shapes of orthogonalize.h, in their order; see real_plan.h for the figures)
-constexpr RealShape kHalfShapes[] = {{256, 256, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
-                                     {128, 128, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
-                                     {64, 64, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},
-                                     {128, 128, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"},
-                                     {192, 192, 1, 0.62f, 0.97f, 11.0f, 1.0f, "192x192"}};
-constexpr RealShape kPairsShapes[] = {{128, 128, 1, 1.15f, 1.40f, 7.0f, 1.3f, "128x128"},
-                                      {64, 64, 2, 0.50f, 0.80f, 6.0f, 2.6f, "64x64"}};
+constexpr RealShape kHalfShapes[] = {{256, 256, 512, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
+                                     {128, 128, 256, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
+                                     {64, 64, 256, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},
+                                     {128, 128, 512, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"},
+                                     {192, 192, 512, 1, 0.62f, 0.97f, 11.0f, 1.0f, "192x192"}};
+constexpr RealShape kPairsShapes[] = {{128, 128, 512, 1, 1.15f, 1.40f, 7.0f, 1.3f, "128x128"},
+                                      {64, 64, 256, 2, 0.50f, 0.80f, 6.0f, 2.6f, "64x64"}};
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
-  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
+  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY && CCGLIB_TABLE[ID].threads == 64 * WX * WY, \
+                "the table is in the order of the shapes");
 #define CCGLIB_TABLE kHalfShapes
 CCGLIB_HALF_SHAPES(CCGLIB_SAME)
 #undef CCGLIB_TABLE

@@ -13,6 +13,10 @@ inline size_t real_blocks(const RealShape &s, size_t batch, size_t nx, size_t ny
   return batch * (symmetric ? y * (y + 1) / 2 : ceil_div(nx, s.bx) * y);
 }
 
+// Whether a launch takes so many blocks: with 2^32 work-items or more it is no error to the runtime, but starts what is left
+// of their number modulo 2^32.
+inline bool real_launches(const RealShape &s, size_t blocks) { return blocks <= 0xffffffffu / s.threads; }
+
 // The time of a product as that of its busiest unit: rounds of blocks, all units full in all but the last one. The figures were
 // fitted to 38 problems from 1 x 8192 x 8192 to 8192 x 4096 x 4096 in every shape and 1 to 32 parts (those within 1.6 times the
 // fastest: 3 to 9 % off, rms; fp16: the kernels of a trace). The choice is behind the fastest one by 0.3 % (e8m0), 0.4 and 1.4 %
@@ -48,6 +52,7 @@ inline RealGemmPlan plan_real_gemm(const RealShape *shapes, int count, size_t ba
     const size_t blocks = real_blocks(shapes[s], batch, nx, ny, symmetric);
     for (size_t p : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       if (p > pieces) break;
+      if (!real_launches(shapes[s], blocks * p)) break;
       const double us = real_gemm_us(shapes[s], blocks, pieces, p);
       if (parts == 0 || us < best) {
         best = us;
@@ -57,6 +62,7 @@ inline RealGemmPlan plan_real_gemm(const RealShape *shapes, int count, size_t ba
       if (blocks * p > 65536) break;                // (more parts of so many blocks: nothing but memory)
     }
   }
+  if (parts == 0) parts = 1;                        // (no shape has few enough blocks: scaled_gemm_launches says so)
   if (option / 256) parts = std::min(option / 256, pieces);
   const RealShape &s = shapes[plan.shape];
   const size_t blocks = real_blocks(s, batch, nx, ny, symmetric);

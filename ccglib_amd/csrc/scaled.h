@@ -36,11 +36,11 @@ struct RealGemmPlan {
   size_t partial_bytes = 0, counter_bytes = 0;
 };
 
-// A block shape of the real products' kernel: columns and rows of a block, blocks that a compute unit holds, and what it costs
+// A block shape of the real products' kernel: columns and rows of a block, its threads, blocks that a compute unit holds, and what it costs
 // (us): a piece of K where a unit has one block, and where every unit has as many as it holds; a block's start and end;
 // joining parts of K, for each 64 x 64 sums.
 struct RealShape {
-  unsigned bx, by, per_unit;
+  unsigned bx, by, threads, per_unit;
   float alone_us, full_us, block_us, join_us;
   const char *name;
 };
@@ -60,6 +60,8 @@ struct ScaledGemmParams {
 };
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p);
 hipError_t launch_scaled_gemm(const ScaledGemmParams &p, hipStream_t stream);
+// Whether the plan is one that a launch takes.
+bool scaled_gemm_launches(const ScaledGemmParams &p);
 // Name of the kernel that the plan launches.
 const char *describe_scaled_gemm(const ScaledGemmParams &p);
 

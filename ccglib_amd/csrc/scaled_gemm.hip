@@ -9,32 +9,33 @@ namespace ccglib_amd {
 namespace {
 
 // (the shapes of scaled_gemm.h, in their order; see real_plan.h for the figures)
-constexpr RealShape kBlocksShapes[] = {{256, 256, 1, 0.92f, 1.79f, 8.0f, 0.69f, "256x256"},
-                                       {128, 128, 2, 0.81f, 1.07f, 4.2f, 1.06f, "128x128"},
-                                       {64, 64, 2, 0.243f, 0.442f, 2.5f, 2.4f, "64x64"},
-                                       {64, 32, 2, 0.181f, 0.33f, 2.7f, 4.5f, "32x64"},
-                                       {128, 128, 1, 0.45f, 0.62f, 3.4f, 0.92f, "128x128 8-wave"},
-                                       {192, 192, 1, 0.78f, 1.27f, 5.6f, 0.96f, "192x192"}};
-constexpr RealShape kRowsShapes[] = {{256, 256, 1, 1.16f, 2.17f, 8.6f, 0.82f, "256x256"},
-                                     {128, 128, 2, 0.88f, 1.25f, 4.3f, 1.15f, "128x128"},
-                                     {64, 64, 2, 0.278f, 0.481f, 2.6f, 2.4f, "64x64"},
-                                     {64, 32, 2, 0.206f, 0.356f, 2.5f, 4.6f, "32x64"},
-                                     {128, 128, 1, 0.55f, 0.69f, 3.9f, 0.88f, "128x128 8-wave"},
-                                     {192, 192, 1, 0.82f, 1.25f, 5.7f, 0.95f, "192x192"}};
-constexpr RealShape kE8m0Shapes[] = {{256, 256, 1, 0.84f, 1.56f, 7.8f, 0.74f, "256x256"},
-                                     {128, 128, 2, 0.76f, 0.95f, 4.8f, 1.23f, "128x128"},
-                                     {64, 64, 2, 0.213f, 0.433f, 2.3f, 2.5f, "64x64"},
-                                     {64, 32, 2, 0.164f, 0.306f, 3.2f, 5.4f, "32x64"},
-                                     {128, 128, 1, 0.38f, 0.53f, 3.6f, 1.05f, "128x128 8-wave"},
-                                     {192, 192, 1, 0.57f, 0.89f, 5.9f, 0.92f, "192x192"}};
-constexpr RealShape kWideShapes[] = {{128, 256, 1, 1.34f, 1.97f, 8.5f, 0.98f, "256x128"},
-                                     {128, 128, 2, 1.13f, 1.97f, 7.1f, 1.73f, "128x128"},
-                                     {64, 64, 2, 0.459f, 0.758f, 2.9f, 2.4f, "64x64"},
-                                     {64, 32, 2, 0.304f, 0.505f, 2.6f, 4.1f, "32x64"},
-                                     {128, 128, 1, 0.87f, 1.24f, 5.4f, 1.08f, "128x128 8-wave"}};
+constexpr RealShape kBlocksShapes[] = {{256, 256, 512, 1, 0.92f, 1.79f, 8.0f, 0.69f, "256x256"},
+                                       {128, 128, 256, 2, 0.81f, 1.07f, 4.2f, 1.06f, "128x128"},
+                                       {64, 64, 256, 2, 0.243f, 0.442f, 2.5f, 2.4f, "64x64"},
+                                       {64, 32, 256, 2, 0.181f, 0.33f, 2.7f, 4.5f, "32x64"},
+                                       {128, 128, 512, 1, 0.45f, 0.62f, 3.4f, 0.92f, "128x128 8-wave"},
+                                       {192, 192, 512, 1, 0.78f, 1.27f, 5.6f, 0.96f, "192x192"}};
+constexpr RealShape kRowsShapes[] = {{256, 256, 512, 1, 1.16f, 2.17f, 8.6f, 0.82f, "256x256"},
+                                     {128, 128, 256, 2, 0.88f, 1.25f, 4.3f, 1.15f, "128x128"},
+                                     {64, 64, 256, 2, 0.278f, 0.481f, 2.6f, 2.4f, "64x64"},
+                                     {64, 32, 256, 2, 0.206f, 0.356f, 2.5f, 4.6f, "32x64"},
+                                     {128, 128, 512, 1, 0.55f, 0.69f, 3.9f, 0.88f, "128x128 8-wave"},
+                                     {192, 192, 512, 1, 0.82f, 1.25f, 5.7f, 0.95f, "192x192"}};
+constexpr RealShape kE8m0Shapes[] = {{256, 256, 512, 1, 0.84f, 1.56f, 7.8f, 0.74f, "256x256"},
+                                     {128, 128, 256, 2, 0.76f, 0.95f, 4.8f, 1.23f, "128x128"},
+                                     {64, 64, 256, 2, 0.213f, 0.433f, 2.3f, 2.5f, "64x64"},
+                                     {64, 32, 256, 2, 0.164f, 0.306f, 3.2f, 5.4f, "32x64"},
+                                     {128, 128, 512, 1, 0.38f, 0.53f, 3.6f, 1.05f, "128x128 8-wave"},
+                                     {192, 192, 512, 1, 0.57f, 0.89f, 5.9f, 0.92f, "192x192"}};
+constexpr RealShape kWideShapes[] = {{128, 256, 512, 1, 1.34f, 1.97f, 8.5f, 0.98f, "256x128"},
+                                     {128, 128, 256, 2, 1.13f, 1.97f, 7.1f, 1.73f, "128x128"},
+                                     {64, 64, 256, 2, 0.459f, 0.758f, 2.9f, 2.4f, "64x64"},
+                                     {64, 32, 256, 2, 0.304f, 0.505f, 2.6f, 4.1f, "32x64"},
+                                     {128, 128, 512, 1, 0.87f, 1.24f, 5.4f, 1.08f, "128x128 8-wave"}};
 constexpr int kShapes = sizeof kBlocksShapes / sizeof kBlocksShapes[0], kWideCount = sizeof kWideShapes / sizeof kWideShapes[0];
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
-  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY, "the table is in the order of the shapes");
+  static_assert(CCGLIB_TABLE[ID].bx == BX && CCGLIB_TABLE[ID].by == BY && CCGLIB_TABLE[ID].threads == 64 * WX * WY, \
+                "the table is in the order of the shapes");
 #define CCGLIB_TABLE kBlocksShapes
 CCGLIB_SCALED_SHAPES(CCGLIB_SAME)
 #undef CCGLIB_TABLE
@@ -65,6 +66,11 @@ const RealShape *shapes_of(const ScaledGemmParams &p) {
 
 RealGemmPlan plan_scaled_gemm(const ScaledGemmParams &p) {
   return plan_real_gemm(shapes_of(p), is_wide(p) ? kWideCount : kShapes, p.batch, p.n, p.m, ceil_div(p.k, (size_t)real::kPieceBytes), false, real_block_option);
+}
+
+bool scaled_gemm_launches(const ScaledGemmParams &p) {
+  const RealShape &shape = shapes_of(p)[p.plan.shape];
+  return real_launches(shape, real_blocks(shape, p.batch, p.n, p.m, false) * p.plan.parts);
 }
 
 const char *describe_scaled_gemm(const ScaledGemmParams &p) {
