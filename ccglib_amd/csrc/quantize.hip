@@ -27,7 +27,12 @@ struct Args {
   size_t in_pitch;
   unsigned out_pitch, out_t_pitch, scales_pitch, scales_t_pitch;
   unsigned tiles_m, tiles_n;
+  unsigned blocks, grid_x;   // blocks in all; of a row of the grid
 };
+
+// (a launch of 2^32 work-items or more along one axis starts what is left of the number modulo 2^32)
+constexpr unsigned kThreads = 256, kGridRow = 1u << 23;
+__device__ __forceinline__ unsigned block_index(const Args &a) { return blockIdx.y * a.grid_x + blockIdx.x; }
 
 template <int TYPE> struct Loaded;
 template <> struct Loaded<kFloat32> { using type = float; };
@@ -257,9 +262,11 @@ template <int TOUT> __device__ __forceinline__ unsigned four(float a, float b, f
 // Groups along the rows, no transpose: sixteen lanes to a group, so that one row already spreads over the chip. One row of 4096
 // bf16: 2.0 us, a round trip.
 template <int TIN, int TOUT, bool E8M0>
-__global__ __launch_bounds__(256) void quantize_rows(Args a) {
+__global__ __launch_bounds__(kThreads) void quantize_rows(Args a) {
   using In = typename Loaded<TIN>::type;
-  const unsigned id = blockIdx.x * 16 + threadIdx.x / 16;   // group
+  const unsigned block = block_index(a);
+  if (block >= a.blocks) return;
+  const unsigned id = block * 16 + threadIdx.x / 16;   // group
   const unsigned groups = a.tiles_n;
   const unsigned row = id / groups, g = id - row * groups;   // (row: over all matrices)
   if (row >= a.batch * a.m) return;
@@ -285,15 +292,17 @@ __global__ __launch_bounds__(256) void quantize_rows(Args a) {
 // share lines of its L2. 8192 x 8192 bf16 rows, both ways: 64 us, 4.2 TB/s
 // where a copy reaches 4.9 (8191 x 8200, whose rows share lines: 71 us).
 template <int TIN, int TOUT, bool E8M0, bool BLOCKS, bool DIRECT, bool TRANSPOSED>
-__global__ __launch_bounds__(256) void quantize_tile(Args a) {
+__global__ __launch_bounds__(kThreads) void quantize_tile(Args a) {
   using In = typename Loaded<TIN>::type;
   constexpr int PITCH = kGroup + 16;
   __shared__ __attribute__((aligned(16))) unsigned char bytes[TRANSPOSED ? kGroup * PITCH : 16];
   __shared__ __attribute__((aligned(16))) unsigned maxima[TRANSPOSED || BLOCKS ? 4 * kGroup : 4];
   __shared__ __attribute__((aligned(16))) float factors[TRANSPOSED && !BLOCKS ? kGroup : 4];
   const int tid = threadIdx.x, c = tid & 15, r8 = tid >> 4, wave = tid >> 6;
-  const unsigned id = blockIdx.x & 7, part = gridDim.x / 8, rest = gridDim.x & 7;   // (block k runs on XCD k % 8)
-  const unsigned tiles = a.tiles_m * a.tiles_n, tile = id * part + (id < rest ? id : rest) + blockIdx.x / 8;
+  const unsigned block = block_index(a);
+  if (block >= a.blocks) return;
+  const unsigned id = block & 7, part = a.blocks / 8, rest = a.blocks & 7;   // (block k runs on XCD k % 8)
+  const unsigned tiles = a.tiles_m * a.tiles_n, tile = id * part + (id < rest ? id : rest) + block / 8;
   const unsigned b = tile / tiles, t = tile - b * tiles, tm = t / a.tiles_n, tn = t - tm * a.tiles_n;
   const unsigned m0 = tm * kGroup + r8 * 8, n0 = tn * kGroup + c * 8;
   const In *in = reinterpret_cast<const In *>(a.in) + ((size_t)b * a.m + m0) * a.in_pitch;
@@ -389,26 +398,26 @@ __global__ __launch_bounds__(256) void quantize_tile(Args a) {
 }
 
 template <int TIN, int TOUT, bool E8M0>
-hipError_t launch(const QuantizeParams &p, const Args &a, hipStream_t stream) {
+hipError_t launch(const QuantizeParams &p, Args a, hipStream_t stream) {
   const bool direct = p.out != nullptr, transposed = p.out_t != nullptr, blocks = p.group == kScaleBlocks;
-  if (direct && !transposed && !blocks) {
-    const size_t groups = (size_t)p.batch * p.m * a.tiles_n;
-    quantize_rows<TIN, TOUT, E8M0><<<(unsigned)ceil_div(groups, 16), 256, 0, stream>>>(a);
-    return hipGetLastError();
-  }
-  const unsigned grid = (unsigned)((size_t)p.batch * a.tiles_m * a.tiles_n);
-  if (blocks) {
+  const bool rows = direct && !transposed && !blocks;
+  a.blocks = (unsigned)(rows ? ceil_div((size_t)p.batch * p.m * a.tiles_n, 16) : (size_t)p.batch * a.tiles_m * a.tiles_n);
+  a.grid_x = a.blocks < kGridRow ? a.blocks : kGridRow;
+  const dim3 grid(a.grid_x, (unsigned)ceil_div(a.blocks, a.grid_x));
+  if (rows) {
+    quantize_rows<TIN, TOUT, E8M0><<<grid, kThreads, 0, stream>>>(a);
+  } else if (blocks) {
     if (direct && transposed) {
-      quantize_tile<TIN, TOUT, E8M0, true, true, true><<<grid, 256, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, true, true><<<grid, kThreads, 0, stream>>>(a);
     } else if (direct) {
-      quantize_tile<TIN, TOUT, E8M0, true, true, false><<<grid, 256, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, true, false><<<grid, kThreads, 0, stream>>>(a);
     } else {
-      quantize_tile<TIN, TOUT, E8M0, true, false, true><<<grid, 256, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, false, true><<<grid, kThreads, 0, stream>>>(a);
     }
   } else if (direct) {
-    quantize_tile<TIN, TOUT, E8M0, false, true, true><<<grid, 256, 0, stream>>>(a);
+    quantize_tile<TIN, TOUT, E8M0, false, true, true><<<grid, kThreads, 0, stream>>>(a);
   } else {
-    quantize_tile<TIN, TOUT, E8M0, false, false, true><<<grid, 256, 0, stream>>>(a);
+    quantize_tile<TIN, TOUT, E8M0, false, false, true><<<grid, kThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
@@ -425,7 +434,7 @@ template <int TIN> hipError_t launch_typed(const QuantizeParams &p, const Args &
 
 hipError_t launch_quantize(const QuantizeParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
-  Args a;
+  Args a = {};
   a.in = static_cast<const char *>(p.in);
   a.out = static_cast<unsigned char *>(p.out);
   a.out_t = static_cast<unsigned char *>(p.out_t);
