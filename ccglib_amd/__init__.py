@@ -364,7 +364,8 @@ class ScaledLinear(_Handle):
         _capi.check(_capi.load().ccglib_scaled_linear_forward(self._h, _ptr(d_x), _ptr(d_y)))
 
     def Backward(self, d_dy, d_dx, d_dw, accumulate_dw=False):
-        """dx = dy W, dW = dy^T x (or dW += ...), with the x and W of the last Forward; 0: not wanted."""
+        """dx = dy W, dW = dy^T x (or dW += ...), with the x and W of the last Forward; 0: not wanted.
+        After another SetWeights dx is refused until the next Forward."""
         _capi.check(_capi.load().ccglib_scaled_linear_backward(
             self._h, _ptr(d_dy), _ptr(d_dx), _ptr(d_dw), int(bool(accumulate_dw))))
 

@@ -128,7 +128,8 @@ struct ccglib_scaled_linear {
   ScaledLinearParams p;
   int device;
   hipStream_t stream;
-  bool have_weights = false, have_forward = false;
+  bool have_weights = false;
+  bool have_x = false, have_w = false;   // the copies of x and of W are those of the last forward
   Buffer memory;
 };
 
@@ -313,6 +314,7 @@ int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t l, const void *d_w) 
   HIP_TRY(guard.status());
   QuantizeParams p = l->p.w;
   p.in = d_w;
+  l->have_weights = l->have_w = false;
   HIP_TRY(launch_quantize(p, l->stream));
   l->have_weights = true;
   return CCGLIB_OK;
@@ -329,18 +331,22 @@ int ccglib_scaled_linear_forward(ccglib_scaled_linear_t l, const void *d_x, void
   HIP_TRY(guard.status());
   QuantizeParams q = l->p.x;
   q.in = d_x;
+  l->have_x = l->have_w = false;
   HIP_TRY(launch_quantize(q, l->stream));
   ScaledGemmParams p = l->p.y;
   p.c = d_y;
   HIP_TRY(launch_scaled_gemm(p, l->stream));
-  l->have_forward = true;
+  l->have_x = l->have_w = true;
   return CCGLIB_OK;
 }
 
 int ccglib_scaled_linear_backward(ccglib_scaled_linear_t l, const void *d_dy, void *d_dx, void *d_dw, int accumulate_dw) {
   if (!l) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null handle");
   if (!l->p.training) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward of a layer that was created without training");
-  if (!l->have_forward) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward before forward");
+  if (!l->have_x) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: backward before forward");
+  if (d_dx && !l->have_w) {
+    return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "ScaledLinear: dx with the W of the last forward, but the weights were set since then");
+  }
   if (!d_dx && !d_dw) return CCGLIB_OK;
   if (!d_dy && l->p.y.m && l->p.y.n) return fail(CCGLIB_ERROR_INVALID_ARGUMENT, "null pointer: dy");
   if (!aligned(d_dy, element(l->p.x.type_in)) || !aligned(d_dx, element(l->p.x.type_in)) || !aligned(d_dw, 4)) {

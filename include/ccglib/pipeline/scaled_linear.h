@@ -24,7 +24,7 @@ class ScaledLinear {
 
   void SetWeights(hipDeviceptr_t d_w) { detail::check(ccglib_scaled_linear_set_weights(handle_, d_w)); }
   void Forward(hipDeviceptr_t d_x, hipDeviceptr_t d_y) { detail::check(ccglib_scaled_linear_forward(handle_, d_x, d_y)); }
-  // d_dx or d_dw may be null.
+  // With the x and W of the last Forward (after another SetWeights d_dx is refused until the next one). d_dx or d_dw may be null.
   void Backward(hipDeviceptr_t d_dy, hipDeviceptr_t d_dx, hipDeviceptr_t d_dw, bool accumulate_dw = false) {
     detail::check(ccglib_scaled_linear_backward(handle_, d_dy, d_dx, d_dw, accumulate_dw));
   }

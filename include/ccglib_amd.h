@@ -406,10 +406,11 @@ CCGLIB_API int ccglib_scaled_gemm_destroy(ccglib_scaled_gemm_t gemm);
  * summed index, W (N x K) for 128 x 128; x and W in e4m3, dy in gradient_type.
  * x, y, W, dy and dx are of `type`, dw is float32. set_weights keeps 8-bit
  * copies of W until it is called again, forward those of x until the next one;
- * backward, with the x and W of then, computes
+ * backward, with the x and W of the last forward, computes
  *     dx = dy W,  dw = dy^T x  (accumulate_dw: dw += dy^T x);
- * d_dx or d_dw may be null. training = 0: forward only, half the work of
- * making the copies. */
+ * d_dx or d_dw may be null. Once set_weights has been called again that W is
+ * gone, and backward refuses to compute dx until the next forward.
+ * training = 0: forward only, half the work of making the copies. */
 CCGLIB_API int ccglib_scaled_linear_create(ccglib_scaled_linear_t *linear, size_t M, size_t N, size_t K, int device, void *stream,
                                            int type, int gradient_type, int scale_type, int training);
 CCGLIB_API int ccglib_scaled_linear_set_weights(ccglib_scaled_linear_t linear, const void *d_w);
