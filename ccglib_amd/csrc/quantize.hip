@@ -5,6 +5,7 @@
 //   e8m0 scales:     scale = 2^ceil(log2(amax / t)), factor = 1 / scale
 //   q = 8-bit value nearest to x * factor, ties to even; NaN stays NaN, infinity stays infinity or, in e4m3, is NaN
 // Values that are not finite leave the scale of their group alone. The bound is memory: 2 bytes in and 1 or 2 out a value.
+#include <algorithm>
 #include <type_traits>
 
 #include "scaled.h"
@@ -27,12 +28,7 @@ struct Args {
   size_t in_pitch;
   unsigned out_pitch, out_t_pitch, scales_pitch, scales_t_pitch;
   unsigned tiles_m, tiles_n;
-  unsigned blocks, grid_x;   // blocks in all; of a row of the grid
 };
-
-// (a launch of 2^32 work-items or more along one axis starts what is left of the number modulo 2^32)
-constexpr unsigned kThreads = 256, kGridRow = 1u << 23;
-__device__ __forceinline__ unsigned block_index(const Args &a) { return blockIdx.y * a.grid_x + blockIdx.x; }
 
 template <int TYPE> struct Loaded;
 template <> struct Loaded<kFloat32> { using type = float; };
@@ -262,11 +258,9 @@ template <int TOUT> __device__ __forceinline__ unsigned four(float a, float b, f
 // Groups along the rows, no transpose: sixteen lanes to a group, so that one row already spreads over the chip. One row of 4096
 // bf16: 2.0 us, a round trip.
 template <int TIN, int TOUT, bool E8M0>
-__global__ __launch_bounds__(kThreads) void quantize_rows(Args a) {
+__global__ __launch_bounds__(256) void quantize_rows(Args a) {
   using In = typename Loaded<TIN>::type;
-  const unsigned block = block_index(a);
-  if (block >= a.blocks) return;
-  const unsigned id = block * 16 + threadIdx.x / 16;   // group
+  const unsigned id = blockIdx.x * 16 + threadIdx.x / 16;   // group
   const unsigned groups = a.tiles_n;
   const unsigned row = id / groups, g = id - row * groups;   // (row: over all matrices)
   if (row >= a.batch * a.m) return;
@@ -292,17 +286,15 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(Args a) {
 // share lines of its L2. 8192 x 8192 bf16 rows, both ways: 64 us, 4.2 TB/s
 // where a copy reaches 4.9 (8191 x 8200, whose rows share lines: 71 us).
 template <int TIN, int TOUT, bool E8M0, bool BLOCKS, bool DIRECT, bool TRANSPOSED>
-__global__ __launch_bounds__(kThreads) void quantize_tile(Args a) {
+__global__ __launch_bounds__(256) void quantize_tile(Args a) {
   using In = typename Loaded<TIN>::type;
   constexpr int PITCH = kGroup + 16;
   __shared__ __attribute__((aligned(16))) unsigned char bytes[TRANSPOSED ? kGroup * PITCH : 16];
   __shared__ __attribute__((aligned(16))) unsigned maxima[TRANSPOSED || BLOCKS ? 4 * kGroup : 4];
   __shared__ __attribute__((aligned(16))) float factors[TRANSPOSED && !BLOCKS ? kGroup : 4];
   const int tid = threadIdx.x, c = tid & 15, r8 = tid >> 4, wave = tid >> 6;
-  const unsigned block = block_index(a);
-  if (block >= a.blocks) return;
-  const unsigned id = block & 7, part = a.blocks / 8, rest = a.blocks & 7;   // (block k runs on XCD k % 8)
-  const unsigned tiles = a.tiles_m * a.tiles_n, tile = id * part + (id < rest ? id : rest) + block / 8;
+  const unsigned id = blockIdx.x & 7, part = gridDim.x / 8, rest = gridDim.x & 7;   // (block k runs on XCD k % 8)
+  const unsigned tiles = a.tiles_m * a.tiles_n, tile = id * part + (id < rest ? id : rest) + blockIdx.x / 8;
   const unsigned b = tile / tiles, t = tile - b * tiles, tm = t / a.tiles_n, tn = t - tm * a.tiles_n;
   const unsigned m0 = tm * kGroup + r8 * 8, n0 = tn * kGroup + c * 8;
   const In *in = reinterpret_cast<const In *>(a.in) + ((size_t)b * a.m + m0) * a.in_pitch;
@@ -398,43 +390,47 @@ __global__ __launch_bounds__(kThreads) void quantize_tile(Args a) {
 }
 
 template <int TIN, int TOUT, bool E8M0>
-hipError_t launch(const QuantizeParams &p, Args a, hipStream_t stream) {
+hipError_t launch(const QuantizeParams &p, const Args &a, unsigned grid, hipStream_t stream) {
   const bool direct = p.out != nullptr, transposed = p.out_t != nullptr, blocks = p.group == kScaleBlocks;
-  const bool rows = direct && !transposed && !blocks;
-  a.blocks = (unsigned)(rows ? ceil_div((size_t)p.batch * p.m * a.tiles_n, 16) : (size_t)p.batch * a.tiles_m * a.tiles_n);
-  a.grid_x = a.blocks < kGridRow ? a.blocks : kGridRow;
-  const dim3 grid(a.grid_x, (unsigned)ceil_div(a.blocks, a.grid_x));
-  if (rows) {
-    quantize_rows<TIN, TOUT, E8M0><<<grid, kThreads, 0, stream>>>(a);
+  if (direct && !transposed && !blocks) {
+    quantize_rows<TIN, TOUT, E8M0><<<grid, 256, 0, stream>>>(a);
   } else if (blocks) {
     if (direct && transposed) {
-      quantize_tile<TIN, TOUT, E8M0, true, true, true><<<grid, kThreads, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, true, true><<<grid, 256, 0, stream>>>(a);
     } else if (direct) {
-      quantize_tile<TIN, TOUT, E8M0, true, true, false><<<grid, kThreads, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, true, false><<<grid, 256, 0, stream>>>(a);
     } else {
-      quantize_tile<TIN, TOUT, E8M0, true, false, true><<<grid, kThreads, 0, stream>>>(a);
+      quantize_tile<TIN, TOUT, E8M0, true, false, true><<<grid, 256, 0, stream>>>(a);
     }
   } else if (direct) {
-    quantize_tile<TIN, TOUT, E8M0, false, true, true><<<grid, kThreads, 0, stream>>>(a);
+    quantize_tile<TIN, TOUT, E8M0, false, true, true><<<grid, 256, 0, stream>>>(a);
   } else {
-    quantize_tile<TIN, TOUT, E8M0, false, false, true><<<grid, kThreads, 0, stream>>>(a);
+    quantize_tile<TIN, TOUT, E8M0, false, false, true><<<grid, 256, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
 
-template <int TIN> hipError_t launch_typed(const QuantizeParams &p, const Args &a, hipStream_t stream) {
+template <int TIN> hipError_t launch_typed(const QuantizeParams &p, const Args &a, unsigned grid, hipStream_t stream) {
   const bool e8m0 = p.scale_type == kScaleE8m0;
   if (p.type_out == kFloat8e4m3) {
-    return e8m0 ? launch<TIN, kFloat8e4m3, true>(p, a, stream) : launch<TIN, kFloat8e4m3, false>(p, a, stream);
+    return e8m0 ? launch<TIN, kFloat8e4m3, true>(p, a, grid, stream) : launch<TIN, kFloat8e4m3, false>(p, a, grid, stream);
   }
-  return e8m0 ? launch<TIN, kFloat8e5m2, true>(p, a, stream) : launch<TIN, kFloat8e5m2, false>(p, a, stream);
+  return e8m0 ? launch<TIN, kFloat8e5m2, true>(p, a, grid, stream) : launch<TIN, kFloat8e5m2, false>(p, a, grid, stream);
+}
+
+hipError_t launch_part(const QuantizeParams &p, const Args &a, size_t grid, hipStream_t stream) {
+  switch (p.type_in) {
+    case kFloat32: return launch_typed<kFloat32>(p, a, (unsigned)grid, stream);
+    case kFloat16: return launch_typed<kFloat16>(p, a, (unsigned)grid, stream);
+    default: return launch_typed<kBfloat16>(p, a, (unsigned)grid, stream);
+  }
 }
 
 }  // namespace
 
 hipError_t launch_quantize(const QuantizeParams &p, hipStream_t stream) {
   if (p.batch == 0 || p.m == 0 || p.n == 0) return hipSuccess;
-  Args a = {};
+  Args a;
   a.in = static_cast<const char *>(p.in);
   a.out = static_cast<unsigned char *>(p.out);
   a.out_t = static_cast<unsigned char *>(p.out_t);
@@ -450,11 +446,35 @@ hipError_t launch_quantize(const QuantizeParams &p, hipStream_t stream) {
   a.scales_t_pitch = (unsigned)scaled_pitch(scale_rows(p.n, p.group));
   a.tiles_m = (unsigned)ceil_div(p.m, kScaleGroup);
   a.tiles_n = (unsigned)ceil_div(p.n, kScaleGroup);
-  switch (p.type_in) {
-    case kFloat32: return launch_typed<kFloat32>(p, a, stream);
-    case kFloat16: return launch_typed<kFloat16>(p, a, stream);
-    default: return launch_typed<kBfloat16>(p, a, stream);
+
+  // A launch of 2^32 work-items or more is no error to the runtime, but starts what is left of the number modulo 2^32: as many
+  // matrices at a time as one takes, or as many rows of a matrix.
+  constexpr size_t kMost = 0xffffffffu / 256;
+  const bool rows_only = p.out && !p.out_t && p.group == kScaleRows;
+  const size_t each = rows_only ? (size_t)p.m * a.tiles_n : (size_t)a.tiles_m * a.tiles_n;   // groups, or tiles, of a matrix
+  const size_t most = rows_only ? kMost * 16 : kMost;
+  if (!rows_only && each > most) return hipErrorInvalidValue;                                // (no card holds that many values)
+  const size_t matrices = std::max<size_t>(1, most / each), rows = each <= most ? p.m : most / a.tiles_n;
+  const size_t in_size = (size_t)p.in_pitch * bits_of(p.type_in) / 8, scale = p.scale_type == kScaleE8m0 ? 1 : 4;
+  for (size_t b = 0; b < p.batch; b += matrices) {
+    for (size_t r = 0; r < p.m; r += rows) {
+      Args part = a;
+      part.batch = (unsigned)std::min<size_t>(matrices, p.batch - b);
+      part.m = (unsigned)std::min<size_t>(rows, p.m - r);
+      part.in += (b * p.m + r) * in_size;
+      if (a.out) {
+        part.out += (b * p.m + r) * a.out_pitch;
+        part.scales += (b * a.tiles_n * a.scales_pitch + r) * scale;
+      }
+      if (a.out_t) {
+        part.out_t += b * p.n * a.out_t_pitch;
+        part.scales_t += b * a.tiles_m * a.scales_t_pitch * scale;
+      }
+      const size_t grid = rows_only ? ceil_div((size_t)part.batch * part.m * a.tiles_n, 16) : part.batch * each;
+      if (const hipError_t e = launch_part(p, part, grid, stream)) return e;
+    }
   }
+  return hipSuccess;
 }
 
 }  // namespace ccglib_amd

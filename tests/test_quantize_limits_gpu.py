@@ -52,3 +52,12 @@ def test_matrices(group, direct):
     check(x, qt, st[:, 0])
     if direct:
         check(x, q, s[:, 0])
+
+
+def test_matrices_of_16_rows():
+    B, M = 2 ** 24 + 8, 16                    # (16 rows a block, as many matrices as a launch takes and nine more)
+    x = values(B * M)
+    q, s = torch.full((B * M, 16), 0x55, dtype=torch.uint8, device="cuda"), torch.zeros((B, 1, M), device="cuda")
+    cc.Quantize(B, M, 1, 0, stream(), VT.bfloat16).Run(x.data_ptr(), q.data_ptr(), s.data_ptr())
+    torch.cuda.synchronize()
+    check(x, q, s.view(-1))
