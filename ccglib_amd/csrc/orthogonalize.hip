@@ -7,7 +7,8 @@
 // P X needs X with its columns contiguous, so X is kept in both orientations, and the epilogue of P X writes both.
 //
 // bf16 updates: the chain is fp16 (11 bits where the update has 8), sums are 32 bits. X0 is G times a power of two, which
-// loses nothing; the rest of 1 / (|G| + epsilon) is a factor of the first step's epilogues. fp16 and fp32 updates: every
+// loses nothing of values above 2^-24 |G|, and 2^-32 |G| at most of those below, which have fewer bits in fp16; the rest of
+// 1 / (|G| + epsilon) is a factor of the first step's epilogues. fp16 and fp32 updates: every
 // value of the chain is two fp16, 22 bits, and three of the four products are added up (the fourth is 2^-22 of the first).
 // |G| is summed in 64 bits, so that no G overflows it.
 #include <algorithm>
@@ -495,7 +496,7 @@ struct Product {
   size_t blocks;                           // in all
 };
 
-// (the shapes of orthogonalize.h, in their order; see real_plan.h for the figures)
+// (the shapes of orthogonalize.h, in their order; the figures are estimates from a trace of a few sizes, see real_plan.h)
 constexpr RealShape kHalfShapes[] = {{256, 256, 512, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
                                      {128, 128, 256, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
                                      {64, 64, 256, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},

@@ -16,9 +16,12 @@
 // Sums: X supplies the instruction's rows, Y its columns, and the rows of X are permuted inside groups of 16 NT
 // (by the copies), so that a lane's registers hold 4 NT consecutive x at one y: wide stores.
 //
-// What bounds it: large products the power limit (matrix instructions busy 51 to 72 %, clock 1.8 to 2.1 GHz): 8192^3 with float
-// scales 470 us, 2340 TFLOP/s, with e8m0 scales 404 to 446 us, 8 bits as fp16 1050 TFLOP/s, fp16 1230 TFLOP/s. A single row the memory:
-// 8192 x 8192 bytes in 13.9 us. Blocks that are alone on a unit one round trip a piece, which is what the deeper rings are for.
+// What bounds it: in large products the matrix instructions are busy 40 to 60 % of the cycles, at a clock that the power limit
+// has down to 2.0 to 2.2 GHz of 2.4, next to LDS reads, copies, barriers and, with float scales, the vector additions. 8192^3: float
+// scales for 128 x 128 458 us, 2400 TFLOP/s; for rows 541, 2030; e8m0 440, 2500 (a library product of the same values without block
+// scales 329, 3340); 8 bits as fp16 901 to 1031, 1070 to 1220; fp16 P X of 4096 x 8192 219, 1250 (library 1570). Other cards
+// are up to 6 % slower in all of them. A single row: 8192 x 8192 bytes in 14 us out of the last-level cache, in 19.5 (3.4 TB/s) where
+// they come from memory. Blocks that are alone on a unit: one round trip a piece, which is what the deeper rings are for.
 #ifndef CCGLIB_AMD_REAL_GEMM_H_
 #define CCGLIB_AMD_REAL_GEMM_H_
 

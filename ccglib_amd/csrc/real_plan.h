@@ -17,10 +17,12 @@ inline size_t real_blocks(const RealShape &s, size_t batch, size_t nx, size_t ny
 // of their number modulo 2^32.
 inline bool real_launches(const RealShape &s, size_t blocks) { return blocks <= 0xffffffffu / s.threads; }
 
-// The time of a product as that of its busiest unit: rounds of blocks, all units full in all but the last one. The figures were
-// fitted to 38 problems from 1 x 8192 x 8192 to 8192 x 4096 x 4096 in every shape and 1 to 32 parts (those within 1.6 times the
-// fastest: 3 to 9 % off, rms; fp16: the kernels of a trace). The choice is behind the fastest one by 0.3 % (e8m0), 0.4 and 1.4 %
-// (float scales of blocks and rows) and 1.1 % (32-bit C) in the mean, and by 12 % at most.
+// The time of a product as that of its busiest unit: rounds of blocks, all units full in all but the last one. The figures of the
+// 8-bit products were fitted to 38 problems from 1 x 8192 x 8192 to 8192 x 4096 x 4096 in every shape and 1 to 32 parts. On 30 other
+// problems, most of them small, the choice is behind the fastest shape and number of parts by 2.1 and 1.5 % (float scales of blocks and
+// rows), 3.2 % (e8m0) and 1.5 % (32-bit C) in the mean, and by 5 to 11 % where it is wrong (3000 x 3000 x 8192 with 32-bit C: 22 %). The
+// figures of the updates are estimates from a trace: whole updates of 12 sizes are 0.3 % (bf16) and 1.5 % (float32) in the mean, 8 % at
+// most, behind the fastest single shape for all of their products.
 inline double real_gemm_us(const RealShape &s, size_t blocks, size_t pieces, size_t parts) {
   constexpr size_t kUnits = 256;
   const double per_part = (double)ceil_div(pieces, parts);

@@ -4,8 +4,8 @@
 // sums one group from zero, and the vector ALU adds it to C's sum with the product of the two scales: one fused operation
 // for each element and group where B has a scale for 128 x 128 values (a lane's scale of A times a uniform one), two where
 // each row of B has its own. Powers of two (e8m0) are what the matrix instruction takes as its own scales.
-// Sums are held in 32 bits throughout, and rounded once, to the type of C; a 32-bit C is multiplied by the fp16
-// instruction, since the 8-bit one does not sum to 32 bits (kWide* in real_gemm.h).
+// Sums of groups are held in 32 bits and rounded once, to the type of C. Inside a group the 8-bit instruction sums to fewer
+// bits, which is enough for a C of 16; a 32-bit C is multiplied by the fp16 instruction (kWide* in real_gemm.h).
 #ifndef CCGLIB_AMD_SCALED_GEMM_H_
 #define CCGLIB_AMD_SCALED_GEMM_H_
 

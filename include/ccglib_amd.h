@@ -389,10 +389,15 @@ CCGLIB_API int ccglib_quantize_destroy(ccglib_quantize_t quantize);
 /* C[m][n] (+)= sum over groups g of 128 of K of
  *     scale_a[g][m] scale_b[g][n] sum over k in g of A[m][k] B[n][k]
  * for B matrices each of M x K and N x K, C M x N row-major (float32, float16,
- * bfloat16). Sums are held in 32 bits and rounded once. accumulate: C, which is
- * float32 then, is added to. pitch_a, pitch_b: bytes between rows where they
- * are not ccglib_scaled_pitch(K) (0; multiples of 16); pitch_c: elements
- * between rows of C (0: N). K may be 0 (a sum of nothing). */
+ * bfloat16). Sums of groups are held in 32 bits and rounded once; inside a
+ * group those of a float32 C are too, those of a 16-bit C are the 8-bit matrix
+ * instruction's, which drops what lies 2^-13 below the largest of eight
+ * neighbouring products (1e-5 to 9e-5 of the sum). Where B has a scale for
+ * 128 x 128, scale_a scale_b is formed first, a float that may neither
+ * overflow nor become denormal. accumulate: C, which is float32 then, is added
+ * to. pitch_a, pitch_b: bytes between rows where they are not
+ * ccglib_scaled_pitch(K) (0; multiples of 16); pitch_c: elements between rows of
+ * C (0: N). K may be 0 (a sum of nothing). Scales of less than 4 GiB a group of K. */
 CCGLIB_API int ccglib_scaled_gemm_create(ccglib_scaled_gemm_t *gemm, size_t B, size_t M, size_t N, size_t K, int device,
                                          void *stream, int type_a, int type_b, int type_c, int group_a, int group_b,
                                          int scale_type, int accumulate, size_t pitch_a, size_t pitch_b, size_t pitch_c);
