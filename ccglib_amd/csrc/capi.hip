@@ -39,7 +39,9 @@ int fail(int code, const char *fmt, ...) {
   return code;
 }
 
+// (the runtime keeps a failed call's error until it is asked for: the next launch, of whatever object, would report it as its own)
 int fail_hip(hipError_t e, const char *what) {
+  (void)hipGetLastError();
   return fail(CCGLIB_ERROR_RUNTIME, "%s: %s", what, hipGetErrorString(e));
 }
 
