@@ -16,6 +16,14 @@ block scales and orthogonalised updates:
     ccglib::pipeline::ScaledLinear        -> ScaledLinear
     ccglib::orthogonalize::Orthogonalize  -> Orthogonalize
 
+linear layers of 16-bit values, also grouped by expert, and what brings rows to
+experts and back:
+
+    ccglib::pipeline::FusedLinear         -> FusedLinear
+    ccglib::pipeline::GroupedLinear       -> GroupedLinear
+    ccglib::route::Route                  -> Route
+    ccglib::route::Combine                -> Combine
+
 Device buffers are passed as integer device addresses (e.g. ``tensor.data_ptr()``),
 streams as integer ``hipStream_t`` handles (0 = default stream). Every ``Run``
 only enqueues work on the stream. Errors raise ``RuntimeError`` with the
@@ -29,8 +37,8 @@ from . import _capi
 
 __all__ = ["ValueType", "ComplexAxisLocation", "Direction", "MemOrder", "Variant",
            "Precision", "GEMM", "Transpose", "Packing", "Pipeline", "ScaleGroup", "ScaleType",
-           "Quantize", "ScaledGEMM", "ScaledLinear", "Orthogonalize", "scaled_pitch", "ceildiv",
-           "version"]
+           "Quantize", "ScaledGEMM", "ScaledLinear", "Orthogonalize", "Activation", "FusedLinear",
+           "GroupedLinear", "Route", "Combine", "scaled_pitch", "ceildiv", "version"]
 
 
 class ValueType(enum.IntEnum):          # include/ccglib/common/value_type.h:14-22
@@ -73,6 +81,14 @@ class ScaleType(enum.IntEnum):
     """A scale is a float32 number, or a power of two in one byte: 2^(byte - 127)."""
     float32 = 0
     e8m0 = 1
+
+
+class Activation(enum.IntEnum):
+    """What a linear layer does to its sums (formulas: include/ccglib_amd.h)."""
+    none = 0
+    relu = 1
+    gelu = 2
+    silu = 3
 
 
 _BITS = {ValueType.int1: 1, ValueType.float8e4m3: 8, ValueType.float8e5m2: 8,
@@ -385,3 +401,114 @@ class Orthogonalize(_Handle):
 
     def Run(self, d_input, d_output):
         _capi.check(_capi.load().ccglib_orthogonalize_run(self._h, _ptr(d_input), _ptr(d_output)))
+
+
+class FusedLinear(_Handle):
+    """A linear layer of 16-bit values: z = x W^T + bias, y = act(z) + residual, and its backward
+    pass. x [M][x_pitch], W [N][w_pitch], y, z and residual [M][y_pitch]; pitches of 0: K, K, N."""
+    _destroy = "ccglib_fused_linear_destroy"
+
+    def __init__(self, M, N, K, device, stream, type=ValueType.bfloat16, activation=Activation.none,
+                 gradient_type=ValueType.float32, training=True, x_pitch=0, w_pitch=0, y_pitch=0):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_fused_linear_create(
+            ctypes.byref(self._h), M, N, K, int(device), _ptr(stream), int(type), int(activation),
+            int(gradient_type), int(bool(training)), int(x_pitch), int(w_pitch), int(y_pitch)))
+
+    def Forward(self, d_x, d_w, d_bias, d_residual, d_y, d_z=0):
+        """0 for no bias, no residual, a z that is not wanted (Backward wants it where there is an
+        activation). d_y may be d_residual."""
+        _capi.check(_capi.load().ccglib_fused_linear_forward(
+            self._h, _ptr(d_x), _ptr(d_w), _ptr(d_bias), _ptr(d_residual), _ptr(d_y), _ptr(d_z)))
+
+    def Backward(self, d_dy, d_z, d_x, d_w, d_dx, d_dw, d_dbias=0, accumulate=False):
+        """dz = dy act'(z), dx = dz W, dW (+)= dz^T x, dbias (+)= column sums of dz; 0 for a gradient
+        that is not wanted. dW and dbias are of gradient_type; accumulate: of float32 only."""
+        _capi.check(_capi.load().ccglib_fused_linear_backward(
+            self._h, _ptr(d_dy), _ptr(d_z), _ptr(d_x), _ptr(d_w), _ptr(d_dx), _ptr(d_dw), _ptr(d_dbias),
+            int(bool(accumulate))))
+
+    def KernelName(self, product=0):
+        """Which kernel computes y (0), dx (1), dW (2)."""
+        buf = ctypes.create_string_buffer(160)
+        _capi.check(_capi.load().ccglib_fused_linear_kernel_name(self._h, product, buf, len(buf)))
+        return buf.value.decode()
+
+
+class GroupedLinear(_Handle):
+    """FusedLinear with a W and a bias for each of E experts, W [E][N][w_pitch], bias [E][N], and M
+    rows that are sorted by expert: rows offsets[e] to offsets[e + 1] - 1 (int32, device memory) go
+    through expert e's; other rows are left alone."""
+    _destroy = "ccglib_grouped_linear_destroy"
+
+    def __init__(self, E, M, N, K, device, stream, type=ValueType.bfloat16, activation=Activation.none,
+                 gradient_type=ValueType.float32, training=True, x_pitch=0, w_pitch=0, y_pitch=0):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_grouped_linear_create(
+            ctypes.byref(self._h), E, M, N, K, int(device), _ptr(stream), int(type), int(activation),
+            int(gradient_type), int(bool(training)), int(x_pitch), int(w_pitch), int(y_pitch)))
+
+    def Forward(self, d_x, d_offsets, d_w, d_bias, d_residual, d_y, d_z=0):
+        _capi.check(_capi.load().ccglib_grouped_linear_forward(
+            self._h, _ptr(d_x), _ptr(d_offsets), _ptr(d_w), _ptr(d_bias), _ptr(d_residual), _ptr(d_y),
+            _ptr(d_z)))
+
+    def Backward(self, d_dy, d_z, d_x, d_offsets, d_w, d_dx, d_dw, d_dbias=0, accumulate=False):
+        """As FusedLinear's; dW [E][N][w_pitch] and dbias [E][N] of all experts."""
+        _capi.check(_capi.load().ccglib_grouped_linear_backward(
+            self._h, _ptr(d_dy), _ptr(d_z), _ptr(d_x), _ptr(d_offsets), _ptr(d_w), _ptr(d_dx), _ptr(d_dw),
+            _ptr(d_dbias), int(bool(accumulate))))
+
+    def KernelName(self, product=0):
+        """Which kernel computes y (0), dx (1), dW (2)."""
+        buf = ctypes.create_string_buffer(160)
+        _capi.check(_capi.load().ccglib_grouped_linear_kernel_name(self._h, product, buf, len(buf)))
+        return buf.value.decode()
+
+
+class Route(_Handle):
+    """Which k of E experts each of T tokens goes to: the largest of its logits [T][E], their weights
+    by a softmax (normalize: of the k, else of all E), and where its rows lie when all are sorted by
+    expert."""
+    _destroy = "ccglib_route_destroy"
+
+    def __init__(self, T, E, k, device, stream, type=ValueType.float32, normalize=True):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_route_create(
+            ctypes.byref(self._h), T, E, k, int(device), _ptr(stream), int(type), int(bool(normalize))))
+
+    def Run(self, d_logits, d_experts, d_weights, d_offsets, d_slots):
+        """experts, slots [T][k] int32, weights [T][k] float32, offsets [E + 1] int32."""
+        _capi.check(_capi.load().ccglib_route_run(
+            self._h, _ptr(d_logits), _ptr(d_experts), _ptr(d_weights), _ptr(d_offsets), _ptr(d_slots)))
+
+    def Backward(self, d_logits, d_experts, d_weights, d_dweights, d_dlogits):
+        """dlogits [T][E], of the logits' type, from dweights [T][k] float32 and what Run wrote."""
+        _capi.check(_capi.load().ccglib_route_backward(
+            self._h, _ptr(d_logits), _ptr(d_experts), _ptr(d_weights), _ptr(d_dweights), _ptr(d_dlogits)))
+
+
+class Combine(_Handle):
+    """Rows of N 16-bit values between T tokens and the places of their k rows each: slots [T][k]
+    int32, weights [T][k] float32 (0: all 1). A slot outside 0 to rows - 1 is passed over."""
+    _destroy = "ccglib_combine_destroy"
+
+    def __init__(self, T, k, N, device, stream, type=ValueType.bfloat16, rows=0, y_pitch=0, out_pitch=0):
+        super().__init__()
+        _capi.check(_capi.load().ccglib_combine_create(
+            ctypes.byref(self._h), T, k, N, int(device), _ptr(stream), int(type), int(rows), int(y_pitch),
+            int(out_pitch)))
+
+    def Run(self, d_y, d_slots, d_weights, d_out):
+        """out[t] = sum over j of weights[t][j] y[slots[t][j]]"""
+        _capi.check(_capi.load().ccglib_combine_run(self._h, _ptr(d_y), _ptr(d_slots), _ptr(d_weights), _ptr(d_out)))
+
+    def Spread(self, d_x, d_slots, d_weights, d_y):
+        """y[slots[t][j]] = weights[t][j] x[t]"""
+        _capi.check(_capi.load().ccglib_combine_spread(self._h, _ptr(d_x), _ptr(d_slots), _ptr(d_weights), _ptr(d_y)))
+
+    def Backward(self, d_dout, d_y, d_slots, d_weights, d_dy, d_dweights=0):
+        """Of Run: dy[slots[t][j]] = weights[t][j] dout[t], dweights[t][j] = <dout[t], y[slots[t][j]]>; 0 for
+        one that is not wanted."""
+        _capi.check(_capi.load().ccglib_combine_backward(
+            self._h, _ptr(d_dout), _ptr(d_y), _ptr(d_slots), _ptr(d_weights), _ptr(d_dy), _ptr(d_dweights)))

@@ -57,6 +57,25 @@ SIGNATURES = {
     "ccglib_orthogonalize_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i, _f, _f, _f, _f, _sz, _sz]),
     "ccglib_orthogonalize_run": (_i, [_vp, _vp, _vp]),
     "ccglib_orthogonalize_destroy": (_i, [_vp]),
+    "ccglib_fused_linear_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i, _sz, _sz, _sz]),
+    "ccglib_fused_linear_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_fused_linear_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i]),
+    "ccglib_fused_linear_kernel_name": (_i, [_vp, _i, ctypes.c_char_p, _sz]),
+    "ccglib_fused_linear_destroy": (_i, [_vp]),
+    "ccglib_grouped_linear_create": (_i, [_pvp, _sz, _sz, _sz, _sz, _i, _vp, _i, _i, _i, _i, _sz, _sz, _sz]),
+    "ccglib_grouped_linear_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_grouped_linear_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i]),
+    "ccglib_grouped_linear_kernel_name": (_i, [_vp, _i, ctypes.c_char_p, _sz]),
+    "ccglib_grouped_linear_destroy": (_i, [_vp]),
+    "ccglib_route_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _i]),
+    "ccglib_route_run": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_route_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_route_destroy": (_i, [_vp]),
+    "ccglib_combine_create": (_i, [_pvp, _sz, _sz, _sz, _i, _vp, _i, _sz, _sz, _sz]),
+    "ccglib_combine_run": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "ccglib_combine_spread": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "ccglib_combine_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ccglib_combine_destroy": (_i, [_vp]),
 }
 
 _lib = None

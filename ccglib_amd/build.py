@@ -20,8 +20,10 @@ LIB_PATH = os.path.join(HERE, "libccglib_amd.so")
 SOURCES = ["gemm_mfma_f16_f32.hip", "gemm_mfma_bf16_f32.hip", "gemm_mfma_f16_f16.hip", "gemm_mfma_bf16_bf16.hip",
            "gemm_mfma_f32.hip", "gemm_mfma_fp8.hip", "scaled_gemm_rows.hip", "scaled_gemm_blocks.hip",
            "scaled_gemm_e8m0.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_blocks.hip",
-           "scaled_gemm_wide_e8m0.hip", "orthogonalize.hip", "quantize.hip", "gemm_mfma_int1.hip", "transpose.hip",
-           "gemm_int1.hip", "packing.hip", "capi.hip", "operators_capi.hip", "scaled_gemm.hip",
+           "scaled_gemm_wide_e8m0.hip", "orthogonalize.hip", "quantize.hip", "linear_f16_output.hip",
+           "linear_bf16_output.hip", "linear_f16_input.hip", "linear_bf16_input.hip", "linear_f16_weights.hip",
+           "linear_bf16_weights.hip", "gemm_mfma_int1.hip", "transpose.hip", "combine.hip", "route.hip", "linear.hip",
+           "gemm_int1.hip", "packing.hip", "capi.hip", "operators_capi.hip", "linear_capi.hip", "scaled_gemm.hip",
            "gemm_mfma_dispatch.hip", "host_copy.hip"]
 # Packed-fp32 instruction selection is switched off for all device code.
 HIPCC_FLAGS = [
@@ -106,15 +108,15 @@ def _no_scratch_in_gemm_kernels(src, remarks):
     ones of ragged 16-bit pairs two or three, and reload them where a block moves
     to its next C tile (the compiler waits for all memory operations there), and those of 32-bit pairs
     to 16-bit C one address while they look for NaN behind the K loop; anything beyond
-    those few bytes stops the build as well. The real products (gemm_real) count their copies too
-    and must not spill."""
+    those few bytes stops the build as well. The real products (gemm_real, gemm_linear) count their
+    copies too and must not spill."""
     name = None
     for l in remarks:
         if "Function Name:" in l:
             name = l.split("Function Name:")[1].split("[")[0].strip()
-        elif "ScratchSize [bytes/lane]:" in l and name and ("complex_gemm_mfma" in name or "gemm_real" in name):
+        elif "ScratchSize [bytes/lane]:" in l and name and any(n in name for n in ("complex_gemm_mfma", "gemm_real", "gemm_linear")):
             size = int(l.split("ScratchSize [bytes/lane]:")[1].split("[")[0])
-            if size > (0 if "complex_gemm_mfma_wide" in name or "gemm_real" in name else 32):
+            if size > (0 if any(n in name for n in ("complex_gemm_mfma_wide", "gemm_real", "gemm_linear")) else 32):
                 os.remove(_object(src))
                 raise RuntimeError("%s: kernel %s spills %d bytes per lane to scratch memory; its "
                                    "explicit vmcnt counts would not hold" % (src, name, size))

@@ -4,6 +4,7 @@
 #define CCGLIB_AMD_HOST_UTIL_H_
 
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 #include "../../include/ccglib_amd.h"
 
@@ -42,6 +43,28 @@ class DeviceGuard {
 
 // Whether the ordinal names a gfx950 device.
 int check_device(int device);
+
+// Device memory of an object.
+struct Buffer {
+  void *p = nullptr;
+  ~Buffer() {
+    if (p) (void)hipFree(p);
+  }
+  char *at(size_t offset) const { return static_cast<char *>(p) + offset; }
+};
+
+// Allocates `bytes` and clears the first `zeroed`; the memory is cleared when the call returns.
+inline int allocate(Buffer *b, size_t bytes, size_t zeroed) {
+  if (bytes == 0) return CCGLIB_OK;
+  HIP_TRY(hipMalloc(&b->p, bytes));
+  if (zeroed) {
+    HIP_TRY(hipMemset(b->p, 0, zeroed));
+    HIP_TRY(hipStreamSynchronize(nullptr));
+  }
+  return CCGLIB_OK;
+}
+
+inline bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
 
 }  // namespace ccglib_amd
 #endif  // CCGLIB_AMD_HOST_UTIL_H_

@@ -1,0 +1,427 @@
+// 16-bit linear layers: which kernel each of their products runs as, their launches, and what the backward pass does
+// before its products: dz = dy act'(z), rounded to the 16 bits that the matrix cores multiply, and the bias' gradient from the same
+// values in 32.
+#include <algorithm>
+#include <cstdio>
+
+#include "linear_gemm.h"
+#include "real_plan.h"
+
+namespace ccglib_amd {
+namespace {
+
+using namespace linear;
+
+// (the shapes of linear_gemm.h, in their order; see real_plan.h for the figures)
+constexpr RealShape kShapes[] = {{256, 256, 512, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
+                                 {128, 128, 256, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
+                                 {64, 64, 256, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},
+                                 {64, 32, 256, 2, 0.14f, 0.2f, 4.0f, 4.5f, "32x64"},
+                                 {128, 128, 512, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"}};
+constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
+#define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
+  static_assert(kShapes[ID].bx == BX && kShapes[ID].by == BY && kShapes[ID].threads == 64 * WX * WY, \
+                "the table is in the order of the shapes");
+CCGLIB_LINEAR_SHAPES(CCGLIB_SAME)
+#undef CCGLIB_SAME
+
+#define HIP_PASS(expr)                         \
+  do {                                         \
+    const hipError_t e_ = (expr);              \
+    if (e_ != hipSuccess) return e_;           \
+  } while (0)
+
+// x, y and k of a product
+struct Extents {
+  size_t nx, ny, k;
+};
+Extents extents(const LinearParams &p, int kind) {
+  if (kind == kOutput) return {p.n, p.m, p.k};
+  if (kind == kInput) return {p.k, p.m, p.n};
+  return {p.k, p.n, p.m};
+}
+
+// Blocks that a product is launched with: where rows are grouped, as many as there can be however they are (a group's
+// last block may hold one row).
+size_t launched_blocks(const LinearParams &p, int kind, const RealShape &s) {
+  const Extents e = extents(p, kind);
+  const size_t x = ceil_div(e.nx, s.bx);
+  if (!p.grouped) return x * ceil_div(e.ny, s.by);
+  if (kind == kWeights) return p.groups * x * ceil_div(e.ny, s.by);
+  const size_t some = std::min<size_t>(p.groups, p.m);      // (groups that have rows)
+  return x * (some + (p.m - some) / s.by);
+}
+
+RealGemmPlan plan_product(const LinearParams &p, int kind) {
+  const Extents e = extents(p, kind);
+  if (!p.grouped) return plan_real_gemm(kShapes, kShapeCount, 1, e.nx, e.ny, ceil_div(e.k, (size_t)kPiece), false, real_block_option);
+  // K is not cut: that of kWeights has as many lengths as there are groups, and the other products have blocks of many groups
+  RealGemmPlan plan;
+  double best = 0.0;
+  for (int s = 0; s < kShapeCount; ++s) {
+    const RealShape &shape = kShapes[s];
+    if (real_block_option && s != (int)std::min<size_t>(real_block_option % 256 - 1, kShapeCount - 1)) continue;
+    double blocks = (double)ceil_div(e.nx, shape.bx);
+    size_t pieces = ceil_div(e.k, (size_t)kPiece);
+    if (kind == kWeights) {
+      blocks *= (double)p.groups * (double)ceil_div(e.ny, shape.by);
+      pieces = ceil_div((size_t)p.m, (size_t)p.groups * kPiece);
+    } else {   // (groups of about the same size: half a block more than their rows fill)
+      blocks *= std::max((double)std::min(p.groups, p.m), (double)p.m / shape.by + 0.5 * std::min(p.groups, p.m));
+    }
+    const double us = real_gemm_us(shape, (size_t)blocks, std::max<size_t>(1, pieces), 1);
+    if (best == 0.0 || us < best) {
+      best = us;
+      plan.shape = s;
+    }
+  }
+  return plan;
+}
+
+// ---- before the products of the backward pass ----
+
+constexpr unsigned kGradientRows = 64, kGradientColumns = 512;   // of a block
+
+template <int TYPE> __device__ __forceinline__ void activation_gradient(int activation, const float (&z)[8], float (&g)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (activation == kRelu) {
+      g[e] = z[e] > 0.f ? g[e] : 0.f;
+    } else {
+      // act(z) = z s(a(z)): act' = s + z a' s (1 - s), whose second part is nothing where s (1 - s) is (a' may be infinite there)
+      const float a = activation == kGelu ? gelu_argument(z[e]) : z[e];
+      const float slope = activation == kGelu ? __builtin_fmaf(3.f * kGelu3 * z[e], z[e], kGelu1) : 1.f;
+      const float s = sigmoid(a), curve = s * (1.f - s);
+      g[e] *= curve == 0.f ? s : __builtin_fmaf(z[e] * slope, curve, s);
+    }
+  }
+}
+
+struct GradientArgs {
+  const char *dy, *z;
+  size_t pitch;                  // elements, of dy and z
+  char *dz;                      // null: not wanted
+  size_t dz_pitch;
+  float *sums;                   // [row block][n]; null: not wanted
+  unsigned n, rows;
+  int activation;
+  // as linear::Args
+  const int *offsets;
+  unsigned groups;
+};
+
+// dz = dy act'(z) and, for each block of kGradientRows rows of a group, the sums of its columns. Bound by memory.
+template <int TYPE> __global__ __launch_bounds__(256) void linear_gradient(GradientArgs a) {
+  using T = typename Value<TYPE>::type;
+  __shared__ float joined[3][kGradientColumns];
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned x = blockIdx.x * kGradientColumns + lane * 8, left = x < a.n ? a.n - x : 0;
+  unsigned first = blockIdx.y * kGradientRows, until = first + kGradientRows < a.rows ? first + kGradientRows : a.rows;
+  if (a.offsets) {
+    Args find = {};
+    find.offsets = a.offsets;
+    find.groups = a.groups;
+    find.rows = a.rows;
+    if (blockIdx.y >= all_row_blocks<kGradientRows>(find)) return;
+    const RowBlock r = find_row_block<kGradientRows>(find, blockIdx.y);
+    const Span s = span_of(a.offsets, r.group, a.rows);
+    first = s.first + r.block * kGradientRows;
+    until = s.first + s.count < first + kGradientRows ? s.first + s.count : first + kGradientRows;
+  }
+  float sum[8] = {};
+#pragma unroll 4
+  for (unsigned row = first + wave; row < until; row += 4) {
+    if (left == 0) break;
+    float g[8], z[8];
+    load_row(reinterpret_cast<const T *>(a.dy) + (size_t)row * a.pitch + x, left, g);
+    if (a.activation != kNone) {
+      load_row(reinterpret_cast<const T *>(a.z) + (size_t)row * a.pitch + x, left, z);
+      activation_gradient<TYPE>(a.activation, z, g);
+    }
+    if (a.dz) real::store_row(reinterpret_cast<T *>(a.dz) + (size_t)row * a.dz_pitch + x, left, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += g[e];
+  }
+  if (!a.sums) return;
+  if (wave > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) joined[wave - 1][e * 64 + lane] = sum[e];
+  }
+  __syncthreads();
+  if (wave == 0 && left) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = (sum[e] + joined[0][e * 64 + lane]) + (joined[1][e * 64 + lane] + joined[2][e * 64 + lane]);
+    real::store_row(a.sums + (size_t)blockIdx.y * a.n + x, left, sum);
+  }
+}
+
+// db (+)= the sums of a group's row blocks, in their order.
+struct JoinArgs {
+  const float *sums;
+  char *db;
+  unsigned n, rows, blocks;      // row blocks that there can be
+  int type, accumulate;
+  const int *offsets;
+  unsigned groups;
+};
+__global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
+  const unsigned x = blockIdx.x * 256 + threadIdx.x, group = blockIdx.y;
+  unsigned from = 0, count = (a.rows + kGradientRows - 1) / kGradientRows;
+  if (a.offsets) {
+    Args before = {};
+    before.offsets = a.offsets;
+    before.groups = group;
+    before.rows = a.rows;
+    from = all_row_blocks<kGradientRows>(before);
+    count = (span_of(a.offsets, group, a.rows).count + kGradientRows - 1) / kGradientRows;
+  }
+  if (x >= a.n) return;
+  if (from > a.blocks) from = a.blocks;      // (offsets that fall: no sums are read that nobody can have written)
+  if (count > a.blocks - from) count = a.blocks - from;
+  float sum = 0.f;
+#pragma unroll 8
+  for (unsigned b = 0; b < count; ++b) sum += a.sums[(size_t)(from + b) * a.n + x];
+  const size_t at = (size_t)group * a.n + x;
+  if (a.type == kFloat32) {
+    float *const db = reinterpret_cast<float *>(a.db) + at;
+    *db = a.accumulate ? *db + sum : sum;
+  } else if (a.type == kFloat16) {
+    reinterpret_cast<_Float16 *>(a.db)[at] = (_Float16)sum;
+  } else {
+    reinterpret_cast<__bf16 *>(a.db)[at] = (__bf16)sum;
+  }
+}
+
+// Copies of the last 16 values of up to three arrays of 16-bit values, 8 zeros behind them (linear_gemm.h: Tail).
+constexpr size_t kTailBytes = 64;
+struct TailArgs {
+  const unsigned short *end[3];
+  unsigned short *to[3];
+  unsigned have[3];              // values in front of `end`, 16 at most
+};
+__global__ __launch_bounds__(64) void copy_tails(TailArgs a) {
+  const unsigned i = threadIdx.x;
+  for (int t = 0; t < 3; ++t) {
+    if (!a.to[t] || i >= 32) continue;
+    a.to[t][i] = i < 16 && 16 - i <= a.have[t] ? *(a.end[t] - (16 - i)) : (unsigned short)0;
+  }
+}
+
+// An operand of a product: an array of 16-bit values.
+struct Operand {
+  const void *p;
+  size_t rows, columns, pitch;   // elements
+};
+
+// Collects the copies of ends that products need, and makes them.
+class Tails {
+ public:
+  explicit Tails(char *memory) : memory_(memory) {}
+  // k: the length of the sum, strided: whether the operand's rows are along it
+  Tail of(const Operand &o, size_t k, bool strided) {
+    const bool loose = o.pitch % 8 != 0 || (uintptr_t)o.p % 16 != 0;
+    if (!loose || (!strided && k >= 8) || o.rows == 0 || o.columns == 0) return {};
+    const size_t values = (o.rows - 1) * o.pitch + o.columns;
+    const char *const end = static_cast<const char *>(o.p) + 2 * values;
+    char *to = nullptr;
+    for (int i = 0; i < count_; ++i) {
+      if (reinterpret_cast<const char *>(args_.end[i]) == end) to = reinterpret_cast<char *>(args_.to[i]);
+    }
+    if (!to) {
+      to = memory_ + count_ * kTailBytes;
+      args_.end[count_] = reinterpret_cast<const unsigned short *>(end);
+      args_.to[count_] = reinterpret_cast<unsigned short *>(to);
+      args_.have[count_] = (unsigned)std::min<size_t>(16, values);
+      ++count_;
+    }
+    return {to, end};
+  }
+  hipError_t launch(hipStream_t stream) const {
+    if (count_ == 0) return hipSuccess;
+    copy_tails<<<1, 64, 0, stream>>>(args_);
+    return hipGetLastError();
+  }
+
+ private:
+  char *memory_;
+  TailArgs args_ = {};
+  int count_ = 0;
+};
+
+Args product_args(const LinearParams &p, int kind, const Operand &x, const Operand &y, const int *offsets, Tails *tails) {
+  const Extents e = extents(p, kind);
+  const RealGemmPlan &plan = p.plan[kind];
+  const RealShape &s = kShapes[plan.shape];
+  Args a = {};
+  a.x = static_cast<const char *>(x.p);
+  a.y = static_cast<const char *>(y.p);
+  a.nx = (unsigned)e.nx;
+  a.ny = (unsigned)e.ny;
+  a.k = (unsigned)e.k;
+  a.x_pitch = (unsigned)(2 * x.pitch);
+  a.y_pitch = (unsigned)(2 * y.pitch);
+  a.x_tail = tails->of(x, kind == kWeights && p.grouped ? 8 : e.k, kind != kOutput);
+  a.y_tail = tails->of(y, kind == kWeights && p.grouped ? 8 : e.k, kind == kWeights);
+  a.offsets = p.grouped ? offsets : nullptr;
+  a.groups = p.groups;
+  a.rows = p.m;
+  a.x_group = 2 * (size_t)p.n * p.w_pitch;
+  a.blocks_x = (unsigned)ceil_div(e.nx, s.bx);
+  a.blocks_y = (unsigned)ceil_div(e.ny, s.by);
+  a.parts = plan.parts;
+  a.pieces_per_part = plan.pieces_per_part;
+  a.arrived = reinterpret_cast<unsigned *>(p.workspace);
+  a.partial = reinterpret_cast<float *>(p.workspace + p.partial);
+  return a;
+}
+
+hipError_t launch_product(const LinearParams &p, int kind, const Args &a, const StoreParams &s, hipStream_t stream) {
+  const RealGemmPlan &plan = p.plan[kind];
+  const unsigned grid = (unsigned)(launched_blocks(p, kind, kShapes[plan.shape]) * plan.parts);
+  if (grid == 0) return hipSuccess;
+  if (p.type == kFloat16) {
+    if (kind == kOutput) return launch_gemm<kFloat16, kOutput>(plan.shape, grid, a, s, stream);
+    if (kind == kInput) return launch_gemm<kFloat16, kInput>(plan.shape, grid, a, s, stream);
+    return launch_gemm<kFloat16, kWeights>(plan.shape, grid, a, s, stream);
+  }
+  if (kind == kOutput) return launch_gemm<kBfloat16, kOutput>(plan.shape, grid, a, s, stream);
+  if (kind == kInput) return launch_gemm<kBfloat16, kInput>(plan.shape, grid, a, s, stream);
+  return launch_gemm<kBfloat16, kWeights>(plan.shape, grid, a, s, stream);
+}
+
+size_t dz_pitch(const LinearParams &p) { return ceil_div(p.n, (size_t)8) * 8; }
+
+// Blocks of rows whose columns are summed: as many as there can be.
+size_t gradient_blocks(const LinearParams &p) {
+  if (!p.grouped) return ceil_div(p.m, (size_t)kGradientRows);
+  const size_t some = std::min<size_t>(p.groups, p.m);
+  return some + (p.m - some) / kGradientRows;
+}
+
+}  // namespace
+
+void plan_linear(LinearParams *p) {
+  const int kinds = p->training ? 3 : 1;
+  size_t counters = 0, partial = 0;
+  for (int kind = 0; kind < kinds; ++kind) {
+    p->plan[kind] = plan_product(*p, kind);
+    counters = std::max(counters, p->plan[kind].counter_bytes);
+    partial = std::max(partial, p->plan[kind].partial_bytes);
+  }
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += ceil_div(bytes, 256) * 256;
+    return here;
+  };
+  p->zeroed = counters;
+  take(counters);
+  p->partial = take(partial);
+  p->dz = take(p->training && p->activation != kNone ? 2 * (size_t)p->m * dz_pitch(*p) : 0);
+  p->sums = take(p->training ? 4 * gradient_blocks(*p) * p->n : 0);
+  p->tails = take(3 * kTailBytes);
+  p->bytes = at;
+}
+
+bool linear_launches(const LinearParams &p) {
+  for (int kind = 0; kind < (p.training ? 3 : 1); ++kind) {
+    const RealShape &s = kShapes[p.plan[kind].shape];
+    if (!real_launches(s, launched_blocks(p, kind, s) * p.plan[kind].parts)) return false;
+  }
+  if (!p.training) return true;
+  // (blocks of rows are a grid's second axis, groups too)
+  const size_t columns = ceil_div(p.n, (size_t)kGradientColumns);
+  return gradient_blocks(p) <= 65535 && gradient_blocks(p) * columns <= 0xffffffu && ceil_div(p.n, (size_t)256) * p.groups <= 0xffffffu;
+}
+
+const char *describe_linear(const LinearParams &p, int kind) {
+  static thread_local char name[96];
+  static const char *const kinds[] = {"forward", "input's gradient", "weights' gradient"};
+  snprintf(name, sizeof name, "gemm_linear<%s, %s> %s block, K in %u", p.type == kFloat16 ? "float16" : "bfloat16", kinds[kind],
+           kShapes[p.plan[kind].shape].name, p.plan[kind].parts);
+  return name;
+}
+
+hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, hipStream_t stream) {
+  if (p.m == 0 || p.n == 0) return hipSuccess;
+  Tails tails(p.workspace + p.tails);
+  const Operand x = {f.x, p.m, p.k, p.x_pitch}, w = {f.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
+  const Args a = product_args(p, kOutput, w, x, f.offsets, &tails);
+  HIP_PASS(tails.launch(stream));
+  StoreParams s = {};
+  s.out = static_cast<char *>(f.y);
+  s.z = static_cast<char *>(f.z);
+  s.bias = static_cast<const char *>(f.bias);
+  s.residual = static_cast<const char *>(f.residual);
+  s.pitch = p.y_pitch;
+  s.activation = p.activation;
+  return launch_product(p, kOutput, a, s, stream);
+}
+
+hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b, hipStream_t stream) {
+  if (p.n == 0) {
+    // (sums of nothing)
+    if (!b.dx || p.m == 0 || p.k == 0) return hipSuccess;
+  }
+  const bool activated = p.activation != kNone;
+  Operand dz = {b.dy, p.m, p.n, p.y_pitch};
+  if (p.m && p.n && (b.dbias || (activated && (b.dx || b.dw)))) {
+    GradientArgs g = {};
+    g.dy = static_cast<const char *>(b.dy);
+    g.z = static_cast<const char *>(b.z);
+    g.pitch = p.y_pitch;
+    g.dz = activated && (b.dx || b.dw) ? p.workspace + p.dz : nullptr;
+    g.dz_pitch = dz_pitch(p);
+    g.sums = b.dbias ? reinterpret_cast<float *>(p.workspace + p.sums) : nullptr;
+    g.n = p.n;
+    g.rows = p.m;
+    g.activation = p.activation;
+    g.offsets = p.grouped ? b.offsets : nullptr;
+    g.groups = p.groups;
+    const dim3 grid((unsigned)ceil_div(p.n, (size_t)kGradientColumns), (unsigned)gradient_blocks(p));
+    if (p.type == kFloat16) {
+      linear_gradient<kFloat16><<<grid, 256, 0, stream>>>(g);
+    } else {
+      linear_gradient<kBfloat16><<<grid, 256, 0, stream>>>(g);
+    }
+    HIP_PASS(hipGetLastError());
+  }
+  if (activated) dz = {p.workspace + p.dz, p.m, p.n, dz_pitch(p)};
+  if (b.dbias && p.n) {
+    JoinArgs j = {};
+    j.sums = reinterpret_cast<const float *>(p.workspace + p.sums);
+    j.db = static_cast<char *>(b.dbias);
+    j.n = p.n;
+    j.rows = p.m;
+    j.blocks = (unsigned)gradient_blocks(p);
+    j.type = p.gradient_type;
+    j.accumulate = b.accumulate;
+    j.offsets = p.grouped ? b.offsets : nullptr;
+    j.groups = p.groups;
+    join_sums<<<dim3((unsigned)ceil_div(p.n, (size_t)256), p.groups), 256, 0, stream>>>(j);
+    HIP_PASS(hipGetLastError());
+  }
+  Tails tails(p.workspace + p.tails);
+  const Operand x = {b.x, p.m, p.k, p.x_pitch}, w = {b.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
+  Args input = {}, weights = {};
+  if (b.dx) input = product_args(p, kInput, w, dz, b.offsets, &tails);
+  if (b.dw) weights = product_args(p, kWeights, x, dz, b.offsets, &tails);
+  HIP_PASS(tails.launch(stream));
+  StoreParams s = {};
+  if (b.dx && p.m && p.k) {
+    s.out = static_cast<char *>(b.dx);
+    s.pitch = p.x_pitch;
+    HIP_PASS(launch_product(p, kInput, input, s, stream));
+  }
+  if (b.dw && p.n && p.k) {
+    s.out = static_cast<char *>(b.dw);
+    s.pitch = p.w_pitch;
+    s.group = (size_t)p.n * p.w_pitch;
+    s.wide = p.gradient_type == kFloat32;
+    s.accumulate = b.accumulate;
+    HIP_PASS(launch_product(p, kWeights, weights, s, stream));
+  }
+  return hipSuccess;
+}
+
+}  // namespace ccglib_amd

@@ -1,0 +1,4 @@
+// 16-bit linear layers: the kernels of one type and product (see linear_gemm.h)
+#define CCGLIB_LINEAR_TYPE kBfloat16
+#define CCGLIB_LINEAR_KIND kWeights
+#include "linear_gemm.h"

@@ -16,30 +16,8 @@ constexpr size_t kMostRows = 0x7fffffffu;     // rows, and values of a row, of a
 constexpr size_t kMostPitch = (size_t)1 << 23;  // bytes: 256 rows are addressed with 32-bit offsets
 constexpr size_t kMostBlocks = 0x7fffffffu;
 
-// Device memory of an object.
-struct Buffer {
-  void *p = nullptr;
-  ~Buffer() {
-    if (p) (void)hipFree(p);
-  }
-  char *at(size_t offset) const { return static_cast<char *>(p) + offset; }
-};
-
 bool is_group(int g) { return g == kScaleRows || g == kScaleBlocks; }
 bool is_scale(int s) { return s == kScaleFloat32 || s == kScaleE8m0; }
-bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
-
-// Allocates `bytes` and clears the first `zeroed`; the memory is cleared when the call returns.
-int allocate(Buffer *b, size_t bytes, size_t zeroed) {
-  if (bytes == 0) return CCGLIB_OK;
-  HIP_TRY(hipMalloc(&b->p, bytes));
-  if (zeroed) {
-    HIP_TRY(hipMemset(b->p, 0, zeroed));
-    HIP_TRY(hipStreamSynchronize(nullptr));
-  }
-  return CCGLIB_OK;
-}
-
 int check_quantize(const QuantizeParams &p, size_t B, size_t M, size_t N) {
   if (!is_wide_float(p.type_in)) {
     return fail(CCGLIB_ERROR_UNSUPPORTED, "Quantize: input is float32, float16 or bfloat16 (type %d)", p.type_in);

@@ -1,0 +1,340 @@
+// Route: for each of T rows of E logits the k largest (ties: the lower number first), their weights by a softmax, and where the T k
+// rows lie when they are sorted by expert, those of an expert in their order: an expert's first place plus the number of earlier
+// rows that chose it. Two launches: the first chooses, and counts for each tile of rows how many chose which expert; in the second every
+// block adds up the tiles before its own and numbers its rows. One tile: one launch. Counts are sums of whole numbers, so that places do not depend
+// on the order of blocks.
+//
+// A row is held by 16 lanes (64 from 257 experts on), PER neighbouring logits a lane, as whole numbers of the same order; each
+// round takes the maximum of all lanes by DPP and removes it.
+#include <algorithm>
+
+#include "linear_gemm.h"
+#include "route.h"
+
+namespace ccglib_amd {
+namespace {
+
+using linear::Value;
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+
+// Whole numbers in the order of the floats: the two zeros alike, NaN above all, 0 below all.
+__device__ __forceinline__ unsigned key_of(float v) {
+  const unsigned u = v == 0.f ? 0u : __builtin_bit_cast(unsigned, v);
+  return v != v ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+  if (key == 0xffffffffu) return __builtin_nanf("");
+  return __builtin_bit_cast(float, key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
+// What `join` makes of the values of all LANES (16, a DPP row, or 64) that hold a row, in each of them.
+template <int LANES, typename T, typename Join> __device__ __forceinline__ T over_lanes(T v, Join join) {
+  auto rotated = [&](auto control) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(control)::value, 0xf, 0xf, false));
+  };
+  v = join(v, rotated(std::integral_constant<int, 0x121>{}));   // row_ror by 1, 2, 4 and 8
+  v = join(v, rotated(std::integral_constant<int, 0x122>{}));
+  v = join(v, rotated(std::integral_constant<int, 0x124>{}));
+  v = join(v, rotated(std::integral_constant<int, 0x128>{}));
+  if constexpr (LANES == 64) {
+    v = join(v, __shfl_xor(v, 16));
+    v = join(v, __shfl_xor(v, 32));
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ float sum(float a, float b) { return a + b; }
+
+// PER neighbouring logits of a row from `first` on, as floats; `e` logits in all.
+template <typename T, int PER> __device__ __forceinline__ void load_logits(const T *row, unsigned first, unsigned e, float (&v)[PER]) {
+  linear::load_row(row + first, first < e ? e - first : 0, v);
+}
+
+struct ChooseArgs {
+  const char *logits;
+  int *experts;
+  float *weights;
+  int *offsets, *slots;
+  unsigned *counts;
+  unsigned tokens, e, k, tile, tiles;
+  int normalize;
+};
+
+// How many rows of a tile chose an expert, as numbers of the whole array: sums over the tiles before it.
+struct Shared {
+  unsigned base[kMostExperts];              // an expert's next place
+  unsigned below[kMostExperts];
+  unsigned short waves[kWaves][kMostExperts];
+  unsigned totals[kWaves];
+};
+
+// First places of all experts from their totals in s.base: sums of what lies in front. All kThreads threads.
+__device__ __forceinline__ void first_places(Shared &s, unsigned e) {
+  const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const unsigned mine = t < e ? s.base[t] : 0;
+  unsigned n = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const unsigned other = (unsigned)__shfl_up((int)n, d);
+    if (lane >= (unsigned)d) n += other;
+  }
+  if (lane == 63) s.totals[wave] = n;
+  __syncthreads();
+  unsigned before = 0;
+  for (unsigned w = 0; w < wave; ++w) before += s.totals[w];
+  if (t < e) s.base[t] = before + n - mine;
+  __syncthreads();
+}
+
+// Places of the rows of one tile, from the experts' next places in s.base. `count` rows (of tokens times k).
+__device__ __forceinline__ void place_rows(Shared &s, const int *experts, int *slots, unsigned count, unsigned e) {
+  const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  for (unsigned at = 0; at < count; at += kThreads) {
+    for (unsigned i = t; i < e; i += kThreads) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s.waves[w][i] = 0;
+    }
+    __syncthreads();
+    const bool have = at + t < count;
+    const unsigned mine = have ? (unsigned)experts[at + t] : 0;
+    // lanes with the same expert
+    unsigned long long same = __ballot(have);
+    for (unsigned bit = 1; bit < e; bit <<= 1) {
+      const unsigned long long set = __ballot((mine & bit) != 0);
+      same &= mine & bit ? set : ~set;
+    }
+    const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1));
+    if (have && rank == 0) s.waves[wave][mine] = (unsigned short)__popcll(same);
+    __syncthreads();
+    for (unsigned i = t; i < e; i += kThreads) {     // (the places of each wave's first)
+      unsigned all = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const unsigned n = s.waves[w][i];
+        s.waves[w][i] = (unsigned short)all;
+        all += n;
+      }
+      s.below[i] = all;
+    }
+    __syncthreads();
+    if (have) slots[at + t] = (int)(s.base[mine] + s.waves[wave][mine] + rank);
+    __syncthreads();
+    for (unsigned i = t; i < e; i += kThreads) s.base[i] += s.below[i];
+  }
+}
+
+template <int TYPE, int LANES, int PER> __global__ __launch_bounds__(kThreads) void route_choose(ChooseArgs a) {
+  using T = typename Value<TYPE>::type;
+  __shared__ Shared s;
+  for (unsigned i = threadIdx.x; i < a.e; i += kThreads) s.base[i] = 0;
+  __syncthreads();
+  const unsigned group = threadIdx.x / LANES, l = threadIdx.x % LANES;
+  const unsigned begin = blockIdx.x * a.tile, end = a.tokens - begin < a.tile ? a.tokens : begin + a.tile;
+  for (unsigned t = begin + group; t < end; t += kThreads / LANES) {
+    float v[PER];
+    load_logits(reinterpret_cast<const T *>(a.logits) + (size_t)t * a.e, l * PER, a.e, v);
+    unsigned keys[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) keys[i] = l * PER + i < a.e ? key_of(v[i]) : 0u;
+    unsigned my_expert = 0;
+    float my_value = 0.f, top = 0.f;
+    for (unsigned j = 0; j < a.k; ++j) {
+      unsigned best = keys[0];
+#pragma unroll
+      for (int i = 1; i < PER; ++i) best = larger(best, keys[i]);
+      const unsigned most = over_lanes<LANES>(best, larger);
+      // the lowest of those that hold it: as the largest of numbers that fall
+      unsigned number = 0;
+      if (best == most) {
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) number = keys[i] == most ? ~(l * PER + i) : number;
+      }
+      const unsigned chosen = ~over_lanes<LANES>(number, larger);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) keys[i] = l * PER + i == chosen ? 0u : keys[i];
+      const float value = value_of(most);
+      if (j == 0) top = value;
+      if (l == j) {
+        my_expert = chosen;
+        my_value = value;
+      }
+    }
+    // (a row of nothing but -inf has weights of zero)
+    const float over = top == -__builtin_inff() ? 0.f : top;
+    const float mine = l < a.k ? __expf(my_value - over) : 0.f;
+    float all;
+    if (a.normalize) {
+      all = over_lanes<LANES>(mine, sum);
+    } else {
+      float some = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) some += l * PER + i < a.e ? __expf(v[i] - over) : 0.f;
+      all = over_lanes<LANES>(some, sum);
+    }
+    if (l < a.k) {
+      const size_t at = (size_t)t * a.k + l;
+      a.experts[at] = (int)my_expert;
+      a.weights[at] = all == 0.f ? 0.f : mine / all;
+      atomicAdd(&s.base[my_expert], 1u);
+    }
+  }
+  __syncthreads();
+  if (a.tiles > 1) {
+    for (unsigned i = threadIdx.x; i < a.e; i += kThreads) a.counts[(size_t)blockIdx.x * a.e + i] = s.base[i];
+    return;
+  }
+  first_places(s, a.e);
+  for (unsigned i = threadIdx.x; i < a.e; i += kThreads) a.offsets[i] = (int)s.base[i];
+  if (threadIdx.x == 0) a.offsets[a.e] = (int)(a.tokens * a.k);
+  __syncthreads();       // (the block's own stores of a.experts are behind the barrier before)
+  place_rows(s, a.experts, a.slots, a.tokens * a.k, a.e);
+}
+
+__global__ __launch_bounds__(kThreads) void route_place(ChooseArgs a) {
+  __shared__ Shared s;
+  const unsigned t = threadIdx.x;
+  for (unsigned i = t; i < a.e; i += kThreads) s.base[i] = s.below[i] = 0;
+  __syncthreads();
+  // several threads an expert, each every so many tiles: their loads are on their way together
+  const unsigned ways = kThreads / a.e, e = t % a.e, way = t / a.e;
+  if (way < ways) {
+    unsigned all = 0, below = 0;
+#pragma unroll 8
+    for (unsigned b = way; b < a.tiles; b += ways) {
+      const unsigned n = a.counts[(size_t)b * a.e + e];
+      all += n;
+      below += b < blockIdx.x ? n : 0;
+    }
+    atomicAdd(&s.base[e], all);
+    atomicAdd(&s.below[e], below);
+  }
+  __syncthreads();
+  first_places(s, a.e);
+  if (blockIdx.x == 0) {
+    for (unsigned i = t; i < a.e; i += kThreads) a.offsets[i] = (int)s.base[i];
+    if (t == 0) a.offsets[a.e] = (int)(a.tokens * a.k);
+  }
+  for (unsigned i = t; i < a.e; i += kThreads) s.base[i] += s.below[i];
+  __syncthreads();
+  const unsigned begin = blockIdx.x * a.tile, end = a.tokens - begin < a.tile ? a.tokens : begin + a.tile;
+  place_rows(s, a.experts + (size_t)begin * a.k, a.slots + (size_t)begin * a.k, (end - begin) * a.k, a.e);
+}
+
+struct BackwardArgs {
+  const char *logits;
+  const int *experts;
+  const float *weights, *dweights;
+  char *dlogits;
+  unsigned tokens, e, k;
+  int normalize;
+};
+
+// inner = sum_j w_j dw_j;  normalized: dl_e = w_j (dw_j - inner) at the chosen, 0 elsewhere (the softmax is one of the chosen);
+// else dl_e = p_e ((dw_j at the chosen, 0 elsewhere) - inner). Bound by memory.
+template <int TYPE, int LANES, int PER> __global__ __launch_bounds__(256) void route_backward(BackwardArgs a) {
+  using T = typename Value<TYPE>::type;
+  const unsigned l = threadIdx.x % LANES, t = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (t >= a.tokens) return;      // (all lanes of a row together)
+  const size_t at = (size_t)t * a.k + l;
+  const unsigned expert = l < a.k ? (unsigned)a.experts[at] : 0xffffffffu;
+  const float w = l < a.k ? a.weights[at] : 0.f, dw = l < a.k ? a.dweights[at] : 0.f;
+  const float inner = over_lanes<LANES>(w * dw, sum);
+  float d[PER] = {}, p[PER];
+  if (!a.normalize) {
+    load_logits(reinterpret_cast<const T *>(a.logits) + (size_t)t * a.e, l * PER, a.e, p);
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (l * PER + i >= a.e) p[i] = -__builtin_inff();
+      top = p[i] > top || p[i] != p[i] ? p[i] : top;
+    }
+    top = over_lanes<LANES>(top, [](float x, float y) { return x != x || x > y ? x : y; });
+    const float over = top == -__builtin_inff() ? 0.f : top;
+    float some = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      p[i] = __expf(p[i] - over);
+      some += p[i];
+    }
+    const float all = over_lanes<LANES>(some, sum), scale = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      p[i] *= scale;
+      d[i] = -inner;
+    }
+  }
+  const float mine = a.normalize ? w * (dw - inner) : dw;
+  for (unsigned j = 0; j < a.k; ++j) {
+    const int from = (int)((threadIdx.x & 63) / LANES * LANES + j);
+    const unsigned chosen = (unsigned)__shfl((int)expert, from);
+    const float add = __shfl(mine, from);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) d[i] += l * PER + i == chosen ? add : 0.f;
+  }
+  if (!a.normalize) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) d[i] *= p[i];
+  }
+  if (l * PER < a.e) real::store_row(reinterpret_cast<T *>(a.dlogits) + (size_t)t * a.e + l * PER, a.e - l * PER, d);
+}
+
+// Calls `f` with the lanes of a row and the logits of a lane.
+template <typename F> void by_experts(unsigned e, F &&f) {
+  using std::integral_constant;
+  if (e <= 16) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  if (e <= 32) return f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  if (e <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  if (e <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  if (e <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  if (e <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+}
+template <typename F> void by_type(int type, F &&f) {
+  using std::integral_constant;
+  if (type == kFloat32) return f(integral_constant<int, kFloat32>{});
+  if (type == kFloat16) return f(integral_constant<int, kFloat16>{});
+  return f(integral_constant<int, kBfloat16>{});
+}
+
+}  // namespace
+
+void plan_route(RouteParams *p) {
+  // 256 tiles at most: each block adds up the counts of all
+  const size_t least = 64;
+  p->tile = (unsigned)std::max(least, ceil_div(ceil_div(p->tokens, (size_t)256), least) * least);
+  p->tiles = (unsigned)std::max<size_t>(1, ceil_div(p->tokens, (size_t)p->tile));
+}
+
+size_t route_workspace_bytes(const RouteParams &p) { return p.tiles > 1 ? sizeof(unsigned) * p.tiles * p.experts : 0; }
+
+hipError_t launch_route(const RouteParams &p, const void *logits, int *experts, float *weights, int *offsets, int *slots,
+                        hipStream_t stream) {
+  const ChooseArgs a = {static_cast<const char *>(logits), experts, weights, offsets, slots, p.counts, p.tokens, p.experts,
+                        p.chosen, p.tile, p.tiles, p.normalize};
+  by_type(p.type, [&](auto type) {
+    by_experts(p.experts, [&](auto lanes, auto per) {
+      route_choose<decltype(type)::value, decltype(lanes)::value, decltype(per)::value><<<p.tiles, kThreads, 0, stream>>>(a);
+    });
+  });
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.tiles == 1) return e;
+  route_place<<<p.tiles, kThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_route_backward(const RouteParams &p, const void *logits, const int *experts, const float *weights,
+                                 const float *dweights, void *dlogits, hipStream_t stream) {
+  if (p.tokens == 0) return hipSuccess;
+  const BackwardArgs a = {static_cast<const char *>(logits), experts, weights, dweights, static_cast<char *>(dlogits), p.tokens,
+                          p.experts, p.chosen, p.normalize};
+  by_type(p.type, [&](auto type) {
+    by_experts(p.experts, [&](auto lanes, auto per) {
+      const unsigned grid = (unsigned)ceil_div(p.tokens, (size_t)(256 / decltype(lanes)::value));
+      route_backward<decltype(type)::value, decltype(lanes)::value, decltype(per)::value><<<grid, 256, 0, stream>>>(a);
+    });
+  });
+  return hipGetLastError();
+}
+
+}  // namespace ccglib_amd

@@ -24,6 +24,8 @@ enum Direction { forward = 0, backward = 1 };
 // 128 x 128 - and what a scale is, a float or a power of two in a byte.
 enum ScaleGroup { scale_rows = 0, scale_blocks = 1 };
 enum ScaleType { scale_float32 = 0, scale_e8m0 = 1 };
+// What a linear layer does to its sums (no counterpart in the reference).
+enum Activation { activation_none = 0, activation_relu = 1, activation_gelu = 2, activation_silu = 3 };
 
 namespace mma {
 enum MemOrder { row_major = 0, col_major = 1 };

@@ -121,7 +121,8 @@ CCGLIB_API const char *ccglib_version(void);
  *                    ccglib_pipeline_reads_in_place tells which one an object
  *                    took.
  *   REAL_BLOCK       0 (default): the block shape of a real product (ScaledGEMM,
- *                    ScaledLinear, Orthogonalize) and the parts that its K is
+ *                    ScaledLinear, Orthogonalize, FusedLinear, GroupedLinear,
+ *                    whose K is not cut) and the parts that its K is
  *                    cut into are chosen by its sizes; otherwise 1 plus the
  *                    shape's number (the last one where there are fewer), plus
  *                    256 times the number of parts (0: chosen).
@@ -436,6 +437,96 @@ CCGLIB_API int ccglib_orthogonalize_create(ccglib_orthogonalize_t *orthogonalize
                                            size_t in_pitch, size_t out_pitch);
 CCGLIB_API int ccglib_orthogonalize_run(ccglib_orthogonalize_t orthogonalize, const void *d_in, void *d_out);
 CCGLIB_API int ccglib_orthogonalize_destroy(ccglib_orthogonalize_t orthogonalize);
+
+/* ------------------------------------------------------------------------
+ * Linear layers of 16-bit values with what stands around the product, the same
+ * grouped by expert, and what brings rows to experts and back. No counterpart
+ * in the reference. Values are float16 or bfloat16, sums 32 bits, rounded once.
+ * Buffers start at a multiple of their element; rows whose distance and start
+ * are multiples of 16 bytes are the fast ones. Outputs lie apart from all inputs,
+ * but y may be the residual.
+ * ---------------------------------------------------------------------- */
+/* act(z): z; max(z, 0); z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); z / (1 + e^-z) */
+enum { CCGLIB_ACTIVATION_NONE = 0, CCGLIB_ACTIVATION_RELU = 1, CCGLIB_ACTIVATION_GELU = 2, CCGLIB_ACTIVATION_SILU = 3 };
+
+typedef struct ccglib_fused_linear *ccglib_fused_linear_t;
+typedef struct ccglib_grouped_linear *ccglib_grouped_linear_t;
+typedef struct ccglib_route *ccglib_route_t;
+typedef struct ccglib_combine *ccglib_combine_t;
+
+/* A linear layer of K inputs and N outputs on M rows, x [M][K], W [N][K]:
+ *     forward:   z = x W^T + bias,  y = act(z) + residual
+ *     backward:  dz = dy act'(z),  dx = dz W,
+ *                dW (+)= dz^T x,  dbias (+)= sum over rows of dz
+ * (the residual's gradient is dy). bias, residual and z may be null: z is
+ * stored where the backward pass is to have it; without an activation that
+ * needs none. act is taken of the sum before z is rounded, act' of the z that
+ * was stored. dz is rounded to 16 bits, as the matrix instructions want it,
+ * dbias is summed without that. dx, dw, dbias: null if not wanted. dw and dbias are of
+ * gradient_type, the values' type or float32; float32 ones may be added to
+ * (accumulate). training = 0: forward only. x_pitch, w_pitch, y_pitch:
+ * elements between rows of x and dx, of W and dW, of y, z, residual and dy (0: K, K, N).
+ * kernel_name, product 0 to 2: that of y, of dx, of dW. */
+CCGLIB_API int ccglib_fused_linear_create(ccglib_fused_linear_t *linear, size_t M, size_t N, size_t K, int device, void *stream,
+                                          int type, int activation, int gradient_type, int training, size_t x_pitch,
+                                          size_t w_pitch, size_t y_pitch);
+CCGLIB_API int ccglib_fused_linear_forward(ccglib_fused_linear_t linear, const void *d_x, const void *d_w, const void *d_bias,
+                                           const void *d_residual, void *d_y, void *d_z);
+CCGLIB_API int ccglib_fused_linear_backward(ccglib_fused_linear_t linear, const void *d_dy, const void *d_z, const void *d_x,
+                                            const void *d_w, void *d_dx, void *d_dw, void *d_dbias, int accumulate);
+CCGLIB_API int ccglib_fused_linear_kernel_name(ccglib_fused_linear_t linear, int product, char *buffer, size_t size);
+CCGLIB_API int ccglib_fused_linear_destroy(ccglib_fused_linear_t linear);
+
+/* The same with E weight matrices, W [E][N][K] and bias [E][N], for M rows that
+ * are sorted by expert: rows offsets[e] to offsets[e + 1] - 1 are multiplied
+ * with W[e]. offsets is device memory, E + 1 int32 that do not fall (what lies outside 0 to M counts
+ * as the nearer end); an expert may have no rows, whose dW and dbias are zero then.
+ * Rows in front of offsets[0] and from offsets[E] on are neither read nor written. 1 to 1024 experts. */
+CCGLIB_API int ccglib_grouped_linear_create(ccglib_grouped_linear_t *linear, size_t E, size_t M, size_t N, size_t K, int device,
+                                            void *stream, int type, int activation, int gradient_type, int training,
+                                            size_t x_pitch, size_t w_pitch, size_t y_pitch);
+CCGLIB_API int ccglib_grouped_linear_forward(ccglib_grouped_linear_t linear, const void *d_x, const void *d_offsets,
+                                             const void *d_w, const void *d_bias, const void *d_residual, void *d_y, void *d_z);
+CCGLIB_API int ccglib_grouped_linear_backward(ccglib_grouped_linear_t linear, const void *d_dy, const void *d_z, const void *d_x,
+                                              const void *d_offsets, const void *d_w, void *d_dx, void *d_dw, void *d_dbias,
+                                              int accumulate);
+CCGLIB_API int ccglib_grouped_linear_kernel_name(ccglib_grouped_linear_t linear, int product, char *buffer, size_t size);
+CCGLIB_API int ccglib_grouped_linear_destroy(ccglib_grouped_linear_t linear);
+
+/* Which k of E experts each of T tokens goes to. logits [T][E] (float32, float16,
+ * bfloat16). run writes, for each token, largest first and of equal ones the
+ * lower number first:
+ *     experts [T][k]  int32
+ *     weights [T][k]  float32: softmax of the k logits (normalize), or of all E
+ *     offsets [E + 1] int32, slots [T][k] int32: where the token's rows lie when
+ *                     all T k rows are sorted by expert, those of an expert in the order of tokens
+ * NaN counts as the largest; a token whose logits are all -inf has weights of 0.
+ * backward: dlogits [T][E] from dweights [T][k], with what run wrote; logits may
+ * be null with normalize. 1 <= k <= 16, k <= E <= 1024, T < 2^24. */
+CCGLIB_API int ccglib_route_create(ccglib_route_t *route, size_t T, size_t E, size_t k, int device, void *stream, int type,
+                                   int normalize);
+CCGLIB_API int ccglib_route_run(ccglib_route_t route, const void *d_logits, void *d_experts, void *d_weights, void *d_offsets,
+                                void *d_slots);
+CCGLIB_API int ccglib_route_backward(ccglib_route_t route, const void *d_logits, const void *d_experts, const void *d_weights,
+                                     const void *d_dweights, void *d_dlogits);
+CCGLIB_API int ccglib_route_destroy(ccglib_route_t route);
+
+/* Rows of N values between T tokens and `rows` places (0: T k), slots [T][k] int32,
+ * weights [T][k] float32 or null (1):
+ *     run:       out[t] = sum over j of weights[t][j] y[slots[t][j]]
+ *     spread:    y[slots[t][j]] = weights[t][j] x[t]
+ *     backward:  dy[slots[t][j]] = weights[t][j] dout[t],  dweights[t][j] = <dout[t], y[slots[t][j]]>
+ * (of run; dy or dweights may be null, y too without dweights. The gradient of spread's x is run of dy.)
+ * A slot outside 0 to rows - 1 is passed over: it adds nothing, nothing is written for it, and
+ * its dweights is 0. Slots that are written differ from each other; places that no slot names are left
+ * as they are. y_pitch, out_pitch: elements between rows of y and dy, of x, out and dout (0: N). k <= 16, T < 2^24. */
+CCGLIB_API int ccglib_combine_create(ccglib_combine_t *combine, size_t T, size_t k, size_t N, int device, void *stream, int type,
+                                     size_t rows, size_t y_pitch, size_t out_pitch);
+CCGLIB_API int ccglib_combine_run(ccglib_combine_t combine, const void *d_y, const void *d_slots, const void *d_weights, void *d_out);
+CCGLIB_API int ccglib_combine_spread(ccglib_combine_t combine, const void *d_x, const void *d_slots, const void *d_weights, void *d_y);
+CCGLIB_API int ccglib_combine_backward(ccglib_combine_t combine, const void *d_dout, const void *d_y, const void *d_slots,
+                                       const void *d_weights, void *d_dy, void *d_dweights);
+CCGLIB_API int ccglib_combine_destroy(ccglib_combine_t combine);
 
 #ifdef __cplusplus
 }
