@@ -17,7 +17,7 @@ constexpr RealShape kShapes[] = {{256, 256, 512, 1, 1.0f, 1.55f, 14.0f, 0.8f, "2
                                  {128, 128, 256, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
                                  {64, 64, 256, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},
                                  {64, 32, 256, 2, 0.14f, 0.2f, 4.0f, 4.5f, "32x64"},
-                                 {128, 128, 512, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"}};
+                                 {128, 128, 512, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"},{192, 192, 512, 1, 0.62f, 0.97f, 11.0f, 1.0f, "192x192"},{128, 256, 512, 1, 0.62f, 0.87f, 9.0f, 1.0f, "256x128"}};
 constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
   static_assert(kShapes[ID].bx == BX && kShapes[ID].by == BY && kShapes[ID].threads == 64 * WX * WY, \

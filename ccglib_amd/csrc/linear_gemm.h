@@ -440,11 +440,14 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
   // A step is the products of one X tile with JJ Y tiles. What a step needs is read while the ones before it run: the
   // fragment of X tile i + 1 behind the first products of tile i; the fragments of Y and the first X fragment of the
   // next piece behind the products of the last tile, at whose start the wave waits for its copies of that piece and passes the
-  // barrier. The order is written out, as in real_gemm.h.
+  // barrier. Behind it nobody reads this piece's slot any more: the copies of the piece that is to lie there go out at once, BEHIND of
+  // them behind the last tile's products, the others behind the next piece's first ones, so that they have a whole piece's time
+  // (8192^3 with all of them in the next piece: 845 us). The order is written out, as in real_gemm.h.
   constexpr int JJ = NY % 2 ? 1 : 2, SPT = NY / JJ, STEPS = NX * SPT;
-  // Copies go out behind the products before the last tile's, a few at a time: all of them lie in front of the wait there,
-  // which counts on it
-  constexpr int COPY_STEPS = STEPS - SPT, PER_STEP = COPY_STEPS > 0 ? (COPIES + COPY_STEPS - 1) / COPY_STEPS : 0;
+  constexpr int COPY_STEPS = STEPS - SPT, PER_STEP = 1;
+  constexpr int BEHIND = COPY_STEPS == 0 || SPT * PER_STEP > COPIES ? COPIES : SPT * PER_STEP;
+  constexpr int PER_BEHIND = (BEHIND + SPT - 1) / SPT, REST = COPIES - BEHIND;
+  constexpr int PER_REST = REST == 0 ? 0 : REST <= COPY_STEPS * PER_STEP ? PER_STEP : (REST + COPY_STEPS - 1) / (COPY_STEPS ? COPY_STEPS : 1);
   const unsigned n = last > first ? last - first : 0;
   if (n > 0) {
 #pragma unroll
@@ -455,21 +458,24 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
       }
     }
     Fragment y[NY], x[2];
-    unsigned slot = 0, refill = SLOTS - 1;
-    if (n >= (unsigned)SLOTS - 1) {   // (SLOTS - 2 later pieces are on their way)
-      real::wait_copies_then_barrier<COPIES *(SLOTS - 2)>();
+    if (n >= (unsigned)SLOTS) {   // (what piece -1 would have begun)
+      static_for<BEHIND>([&](auto c) { copy_one(SLOTS - 1, c, may_end); });
+      real::wait_copies_then_barrier<COPIES *(SLOTS - 2) + BEHIND>();
     } else {
       real::wait_copies_then_barrier<0>();
     }
+    unsigned slot = 0, before = SLOTS - 1;      // of this piece, of the one before
     x[0] = read_x(0, 0);
 #pragma unroll
     for (int j = 0; j < NY; ++j) y[j] = read_y(0, j);
-    // One piece. REFILL: 0 no further piece is copied; 1 one is; 2 one is, perhaps one of the last; 3 this is the last piece
-    auto piece = [&](auto refill_kind) {
-      constexpr int REFILL = decltype(refill_kind)::value;
-      constexpr bool LAST = REFILL == 3, COPY = REFILL == 1 || REFILL == 2;
+    // Piece t. What is copied: kAll the rest of piece t + SLOTS - 1 and the first of piece t + SLOTS; kEnds the same, where these may
+    // be the last ones of K; kRest the rest only; kNothing; kLast nothing, and no piece follows.
+    enum { kAll, kEnds, kRest, kNothing, kLast };
+    auto piece = [&](auto what) {
+      constexpr int WHAT = decltype(what)::value;
+      constexpr bool LAST = WHAT == kLast, COPY_REST = WHAT <= kRest, COPY_BEHIND = WHAT <= kEnds;
       const unsigned next = slot + 1 == SLOTS ? 0 : slot + 1;
-      const typename std::conditional<REFILL == 2, std::true_type, std::false_type>::type end{};
+      const std::integral_constant<bool, WHAT != kAll> end{};
       // Values of the last chunk along k that have been multiplied already, or lie beyond a row of less than 8
       Fragment keep;
       auto clear = [&](Fragment &f) {
@@ -492,10 +498,10 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
         constexpr int m = step, i = m / SPT, js = m % SPT, to = (i + 1) % 2;
         constexpr bool at_end = i == NX - 1;
         CCGLIB_PIN;
-        if constexpr (COPY_STEPS == 0 && m == 0 && COPY) static_for<COPIES>([&](auto c) { copy_one(refill, c, end); });
-        if constexpr (at_end && js == 0 && !LAST) {
+        if constexpr (at_end && js == 0) {
+          if constexpr (COPY_REST) advance();
           // (as many later pieces are on their way; behind the last copies all of them have to have arrived)
-          real::wait_copies_then_barrier<COPY ? COPIES *(SLOTS - 2) : 0>();
+          if constexpr (!LAST) real::wait_copies_then_barrier<COPY_REST ? COPIES *(SLOTS - 2) : 0>();
         }
         if constexpr (js == 0) {
           if constexpr (!at_end) {
@@ -506,44 +512,52 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
         }
 #pragma unroll
         for (int h = 0; h < JJ; ++h) pin(y[js * JJ + h]);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        auto products = [&](int q) {
 #pragma unroll
           for (int h = 0; h < JJ; ++h) {
             const int j = js * JJ + h;
             acc[j][i] = mfma<TYPE>(x[i % 2], y[j], acc[j][i], q);
           }
-        }
 #pragma unroll
-        for (int h = 0; h < JJ; ++h) pin(acc[js * JJ + h][i]);
+          for (int h = 0; h < JJ; ++h) pin(acc[js * JJ + h][i]);
+          CCGLIB_PIN;
+        };
+        products(0);
+        if constexpr (!at_end && COPY_REST) {
+          constexpr int c0 = m * PER_REST < REST ? m * PER_REST : REST, c1 = (m + 1) * PER_REST < REST ? (m + 1) * PER_REST : REST;
+          static_for<c1 - c0>([&](auto c) { copy_one(before, std::integral_constant<int, BEHIND + c0 + decltype(c)::value>{}, end); });
+        }
+        if constexpr (at_end && COPY_BEHIND) {
+          constexpr int c0 = js * PER_BEHIND < BEHIND ? js * PER_BEHIND : BEHIND;
+          constexpr int c1 = (js + 1) * PER_BEHIND < BEHIND ? (js + 1) * PER_BEHIND : BEHIND;
+          static_for<c1 - c0>([&](auto c) { copy_one(slot, std::integral_constant<int, c0 + decltype(c)::value>{}, end); });
+        }
         CCGLIB_PIN;
+        products(1);
         if constexpr (at_end && !LAST) {
 #pragma unroll
           for (int h = 0; h < JJ; ++h) y[js * JJ + h] = read_y(next, js * JJ + h);
         }
-        constexpr int c0 = m * PER_STEP < COPIES ? m * PER_STEP : COPIES;
-        constexpr int c1 = (m + 1) * PER_STEP < COPIES ? (m + 1) * PER_STEP : COPIES;
-        static_assert(c0 == c1 || m < COPY_STEPS, "copies lie in front of the wait");
-        if constexpr (c0 < c1 && COPY) {
-          static_for<c1 - c0>([&](auto c) { copy_one(refill, std::integral_constant<int, c0 + decltype(c)::value>{}, end); });
-        }
         if constexpr (js == SPT - 1 && !at_end) clear(x[to]);
       });
       if constexpr (NX % 2 == 1) x[0] = x[1];   // (the next piece's first tile, where its predecessor was in use)
-      if constexpr (COPY) advance();
-      refill = slot;
+      before = slot;
       slot = next;
     };
     // (pieces of K's end, or of an operand's, are among the last two)
     const unsigned plain = n > 2 ? n - 2 : 0;
     unsigned t = 0;
 #pragma unroll 1
-    for (; t + SLOTS - 1 < plain; ++t) piece(std::integral_constant<int, 1>{});
+    for (; t + SLOTS < plain; ++t) piece(std::integral_constant<int, kAll>{});
 #pragma unroll 1
-    for (; t + SLOTS - 1 < n; ++t) piece(std::integral_constant<int, 2>{});
+    for (; t + SLOTS < n; ++t) piece(std::integral_constant<int, kEnds>{});
+    if (t + SLOTS == n) {
+      piece(std::integral_constant<int, kRest>{});
+      ++t;
+    }
 #pragma unroll 1
-    for (; t + 1 < n; ++t) piece(std::integral_constant<int, 0>{});
-    piece(std::integral_constant<int, 3>{});
+    for (; t + 1 < n; ++t) piece(std::integral_constant<int, kNothing>{});
+    piece(std::integral_constant<int, kLast>{});
   }
 
   // ---- parts of K joined: in the order of the parts, whichever block arrives last (as in real_gemm.h) ----
@@ -630,7 +644,9 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
   DO(1, 128, 128, 2, 2, 2, 2)    \
   DO(2, 64, 64, 2, 2, 4, 2)      \
   DO(3, 64, 32, 4, 1, 6, 2)      \
-  DO(4, 128, 128, 4, 2, 4, 2)
+  DO(4, 128, 128, 4, 2, 4, 2)    \
+  DO(5, 192, 192, 4, 2, 3, 2)    \
+  DO(6, 128, 256, 2, 4, 3, 2)
 
 template <int TYPE, int KIND> hipError_t launch_gemm(int shape, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream);
 #define CCGLIB_DECLARE(TYPE, KIND) \
