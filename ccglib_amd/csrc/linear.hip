@@ -80,7 +80,9 @@ RealGemmPlan plan_product(const LinearParams &p, int kind) {
 
 // ---- before the products of the backward pass ----
 
-constexpr unsigned kGradientRows = 64, kGradientColumns = 512;   // of a block
+// Columns and rows of a block. Few rows a block where 64 would leave units idle: a wave's loads are on their way together then (300 x 255:
+// 12.8 us with 64 rows, FIGURE with 16).
+constexpr unsigned kGradientColumns = 512, kFewRows = 16, kManyRows = 64;
 
 template <int TYPE> __device__ __forceinline__ void activation_gradient(int activation, const float (&z)[8], float (&g)[8]) {
 #pragma unroll
@@ -97,6 +99,19 @@ template <int TYPE> __device__ __forceinline__ void activation_gradient(int acti
   }
 }
 
+// Copies of the last 16 values of up to three arrays of 16-bit values, 8 zeros behind them (linear_gemm.h: Tail).
+constexpr size_t kTailBytes = 64;
+struct TailArgs {
+  const unsigned short *end[3];
+  unsigned short *to[3];
+  unsigned have[3];              // values in front of `end`, 16 at most
+};
+__device__ __forceinline__ void make_tails(const TailArgs &a) {
+  const unsigned i = threadIdx.x % 32, t = threadIdx.x / 32;
+  if (t < 3 && a.to[t]) a.to[t][i] = i < 16 && 16 - i <= a.have[t] ? *(a.end[t] - (16 - i)) : (unsigned short)0;
+}
+__global__ __launch_bounds__(128) void copy_tails(TailArgs a) { make_tails(a); }
+
 struct GradientArgs {
   const char *dy, *z;
   size_t pitch;                  // elements, of dy and z
@@ -110,23 +125,20 @@ struct GradientArgs {
   unsigned groups;
 };
 
-// dz = dy act'(z) and, for each block of kGradientRows rows of a group, the sums of its columns. Bound by memory.
-template <int TYPE> __global__ __launch_bounds__(256) void linear_gradient(GradientArgs a) {
+// dz = dy act'(z) and, for each block of ROWS rows of a group, the sums of its columns. Bound by memory.
+template <int TYPE, unsigned ROWS> __global__ __launch_bounds__(256) void linear_gradient(GradientArgs a, TailArgs tails) {
   using T = typename Value<TYPE>::type;
   __shared__ float joined[3][kGradientColumns];
+  if (blockIdx.x == 0 && blockIdx.y == 0) make_tails(tails);
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned x = blockIdx.x * kGradientColumns + lane * 8, left = x < a.n ? a.n - x : 0;
-  unsigned first = blockIdx.y * kGradientRows, until = first + kGradientRows < a.rows ? first + kGradientRows : a.rows;
+  unsigned first = blockIdx.y * ROWS, until = first + ROWS < a.rows ? first + ROWS : a.rows;
   if (a.offsets) {
-    Args find = {};
-    find.offsets = a.offsets;
-    find.groups = a.groups;
-    find.rows = a.rows;
-    if (blockIdx.y >= all_row_blocks<kGradientRows>(find)) return;
-    const RowBlock r = find_row_block<kGradientRows>(find, blockIdx.y);
-    const Span s = span_of(a.offsets, r.group, a.rows);
-    first = s.first + r.block * kGradientRows;
-    until = s.first + s.count < first + kGradientRows ? s.first + s.count : first + kGradientRows;
+    RowBlocks<ROWS> blocks(a.offsets, a.groups, a.rows);
+    if (blockIdx.y >= blocks.all()) return;
+    const RowBlock r = blocks.find(blockIdx.y);
+    first = r.rows.first + r.block * ROWS;
+    until = r.rows.first + r.rows.count < first + ROWS ? r.rows.first + r.rows.count : first + ROWS;
   }
   float sum[8] = {};
 #pragma unroll 4
@@ -164,16 +176,12 @@ struct JoinArgs {
   const int *offsets;
   unsigned groups;
 };
-__global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
+template <unsigned ROWS> __global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
   const unsigned x = blockIdx.x * 256 + threadIdx.x, group = blockIdx.y;
-  unsigned from = 0, count = (a.rows + kGradientRows - 1) / kGradientRows;
+  unsigned from = 0, count = (a.rows + ROWS - 1) / ROWS;
   if (a.offsets) {
-    Args before = {};
-    before.offsets = a.offsets;
-    before.groups = group;
-    before.rows = a.rows;
-    from = all_row_blocks<kGradientRows>(before);
-    count = (span_of(a.offsets, group, a.rows).count + kGradientRows - 1) / kGradientRows;
+    if (group > 0) from = RowBlocks<ROWS>(a.offsets, group, a.rows).all();
+    count = (span_of(a.offsets, group, a.rows).count + ROWS - 1) / ROWS;
   }
   if (x >= a.n) return;
   if (from > a.blocks) from = a.blocks;      // (offsets that fall: no sums are read that nobody can have written)
@@ -189,21 +197,6 @@ __global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
     reinterpret_cast<_Float16 *>(a.db)[at] = (_Float16)sum;
   } else {
     reinterpret_cast<__bf16 *>(a.db)[at] = (__bf16)sum;
-  }
-}
-
-// Copies of the last 16 values of up to three arrays of 16-bit values, 8 zeros behind them (linear_gemm.h: Tail).
-constexpr size_t kTailBytes = 64;
-struct TailArgs {
-  const unsigned short *end[3];
-  unsigned short *to[3];
-  unsigned have[3];              // values in front of `end`, 16 at most
-};
-__global__ __launch_bounds__(64) void copy_tails(TailArgs a) {
-  const unsigned i = threadIdx.x;
-  for (int t = 0; t < 3; ++t) {
-    if (!a.to[t] || i >= 32) continue;
-    a.to[t][i] = i < 16 && 16 - i <= a.have[t] ? *(a.end[t] - (16 - i)) : (unsigned short)0;
   }
 }
 
@@ -236,9 +229,10 @@ class Tails {
     }
     return {to, end};
   }
+  const TailArgs &args() const { return args_; }
   hipError_t launch(hipStream_t stream) const {
     if (count_ == 0) return hipSuccess;
-    copy_tails<<<1, 64, 0, stream>>>(args_);
+    copy_tails<<<1, 128, 0, stream>>>(args_);
     return hipGetLastError();
   }
 
@@ -291,11 +285,29 @@ hipError_t launch_product(const LinearParams &p, int kind, const Args &a, const 
 
 size_t dz_pitch(const LinearParams &p) { return ceil_div(p.n, (size_t)8) * 8; }
 
-// Blocks of rows whose columns are summed: as many as there can be.
-size_t gradient_blocks(const LinearParams &p) {
-  if (!p.grouped) return ceil_div(p.m, (size_t)kGradientRows);
+// Blocks of `rows` rows of a group: as many as there can be.
+size_t row_blocks(const LinearParams &p, size_t rows) {
+  if (!p.grouped) return ceil_div(p.m, rows);
   const size_t some = std::min<size_t>(p.groups, p.m);
-  return some + (p.m - some) / kGradientRows;
+  return some + (p.m - some) / rows;
+}
+unsigned gradient_rows(const LinearParams &p) {
+  return row_blocks(p, kManyRows) * ceil_div(p.n, (size_t)kGradientColumns) < 512 ? kFewRows : kManyRows;
+}
+size_t gradient_blocks(const LinearParams &p) { return row_blocks(p, gradient_rows(p)); }
+
+template <unsigned ROWS> hipError_t launch_gradient(const LinearParams &p, const GradientArgs &g, const TailArgs &t, hipStream_t stream) {
+  const dim3 grid((unsigned)ceil_div(p.n, (size_t)kGradientColumns), (unsigned)gradient_blocks(p));
+  if (p.type == kFloat16) {
+    linear_gradient<kFloat16, ROWS><<<grid, 256, 0, stream>>>(g, t);
+  } else {
+    linear_gradient<kBfloat16, ROWS><<<grid, 256, 0, stream>>>(g, t);
+  }
+  return hipGetLastError();
+}
+template <unsigned ROWS> hipError_t launch_join(const LinearParams &p, const JoinArgs &j, hipStream_t stream) {
+  join_sums<ROWS><<<dim3((unsigned)ceil_div(p.n, (size_t)256), p.groups), 256, 0, stream>>>(j);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -355,6 +367,7 @@ hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, 
   s.residual = static_cast<const char *>(f.residual);
   s.pitch = p.y_pitch;
   s.activation = p.activation;
+  s.past = 2 * (size_t)p.m * p.n * (f.z ? 2 : 1) >= kPastCachesBytes;
   return launch_product(p, kOutput, a, s, stream);
 }
 
@@ -363,8 +376,14 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
     // (sums of nothing)
     if (!b.dx || p.m == 0 || p.k == 0) return hipSuccess;
   }
-  const bool activated = p.activation != kNone;
+  const bool activated = p.activation != kNone, few = gradient_rows(p) == kFewRows;
   Operand dz = {b.dy, p.m, p.n, p.y_pitch};
+  if (activated) dz = {p.workspace + p.dz, p.m, p.n, dz_pitch(p)};
+  Tails tails(p.workspace + p.tails);
+  const Operand x = {b.x, p.m, p.k, p.x_pitch}, w = {b.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
+  Args input = {}, weights = {};
+  if (b.dx) input = product_args(p, kInput, w, dz, b.offsets, &tails);
+  if (b.dw) weights = product_args(p, kWeights, x, dz, b.offsets, &tails);
   if (p.m && p.n && (b.dbias || (activated && (b.dx || b.dw)))) {
     GradientArgs g = {};
     g.dy = static_cast<const char *>(b.dy);
@@ -378,15 +397,10 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
     g.activation = p.activation;
     g.offsets = p.grouped ? b.offsets : nullptr;
     g.groups = p.groups;
-    const dim3 grid((unsigned)ceil_div(p.n, (size_t)kGradientColumns), (unsigned)gradient_blocks(p));
-    if (p.type == kFloat16) {
-      linear_gradient<kFloat16><<<grid, 256, 0, stream>>>(g);
-    } else {
-      linear_gradient<kBfloat16><<<grid, 256, 0, stream>>>(g);
-    }
-    HIP_PASS(hipGetLastError());
+    HIP_PASS(few ? launch_gradient<kFewRows>(p, g, tails.args(), stream) : launch_gradient<kManyRows>(p, g, tails.args(), stream));
+  } else {
+    HIP_PASS(tails.launch(stream));
   }
-  if (activated) dz = {p.workspace + p.dz, p.m, p.n, dz_pitch(p)};
   if (b.dbias && p.n) {
     JoinArgs j = {};
     j.sums = reinterpret_cast<const float *>(p.workspace + p.sums);
@@ -398,19 +412,13 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
     j.accumulate = b.accumulate;
     j.offsets = p.grouped ? b.offsets : nullptr;
     j.groups = p.groups;
-    join_sums<<<dim3((unsigned)ceil_div(p.n, (size_t)256), p.groups), 256, 0, stream>>>(j);
-    HIP_PASS(hipGetLastError());
+    HIP_PASS(few ? launch_join<kFewRows>(p, j, stream) : launch_join<kManyRows>(p, j, stream));
   }
-  Tails tails(p.workspace + p.tails);
-  const Operand x = {b.x, p.m, p.k, p.x_pitch}, w = {b.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
-  Args input = {}, weights = {};
-  if (b.dx) input = product_args(p, kInput, w, dz, b.offsets, &tails);
-  if (b.dw) weights = product_args(p, kWeights, x, dz, b.offsets, &tails);
-  HIP_PASS(tails.launch(stream));
   StoreParams s = {};
   if (b.dx && p.m && p.k) {
     s.out = static_cast<char *>(b.dx);
     s.pitch = p.x_pitch;
+    s.past = 2 * (size_t)p.m * p.k >= kPastCachesBytes;
     HIP_PASS(launch_product(p, kInput, input, s, stream));
   }
   if (b.dw && p.n && p.k) {
@@ -418,6 +426,7 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
     s.pitch = p.w_pitch;
     s.group = (size_t)p.n * p.w_pitch;
     s.wide = p.gradient_type == kFloat32;
+    s.past = (s.wide ? 4 : 2) * (size_t)p.groups * p.n * p.k >= kPastCachesBytes;
     s.accumulate = b.accumulate;
     HIP_PASS(launch_product(p, kWeights, weights, s, stream));
   }

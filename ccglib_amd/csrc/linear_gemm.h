@@ -73,43 +73,64 @@ __device__ __forceinline__ Span span_of(const int *offsets, unsigned g, unsigned
   return s;
 }
 
-// The group that row block `target` belongs to when the groups' blocks of BY rows are numbered one after the other, and
-// its number inside the group; *all: how many there are. Each wave looks for itself, 64 groups at a time.
+// Groups' blocks of BY rows, numbered one after the other. Each wave looks for itself, 64 groups at a time, a lane each.
 struct RowBlock {
-  unsigned group, block;
+  unsigned group, block;    // which group, and which of its blocks
+  Span rows;                // the group's
 };
-template <int BY> __device__ __forceinline__ unsigned blocks_of_groups(const Args &a, unsigned from, unsigned *mine) {
-  const unsigned lane = threadIdx.x & 63, g = from + lane;
-  unsigned n = g < a.groups ? (span_of(a.offsets, g, a.rows).count + BY - 1) / BY : 0u;
-  *mine = n;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const unsigned other = (unsigned)__shfl_up((int)n, d);
-    if (lane >= (unsigned)d) n += other;
-  }
-  return n;      // (of this lane and those below)
-}
-template <int BY> __device__ __forceinline__ unsigned all_row_blocks(const Args &a) {
-  unsigned all = 0, mine;
-  for (unsigned g = 0; g < a.groups; g += 64) all += (unsigned)__builtin_amdgcn_readlane((int)blocks_of_groups<BY>(a, g, &mine), 63);
-  return all;
-}
-template <int BY> __device__ __forceinline__ RowBlock find_row_block(const Args &a, unsigned target) {
-  for (unsigned g = 0; g < a.groups; g += 64) {
-    unsigned mine;
-    const unsigned until = blocks_of_groups<BY>(a, g, &mine);
-    const unsigned long long behind = __ballot(until > target);
-    if (behind) {
-      const int lane = __builtin_ctzll(behind);
-      RowBlock r;
-      r.group = g + lane;
-      r.block = target - (unsigned)__builtin_amdgcn_readlane((int)(until - mine), lane);
-      return r;
+template <int BY> class RowBlocks {
+ public:
+  __device__ __forceinline__ RowBlocks(const int *offsets, unsigned groups, unsigned rows)
+      : offsets_(offsets), groups_(groups), rows_(rows) {
+    load(0);
+    all_ = last_lane(until_);
+    if (groups > 64) {
+      for (unsigned g = 64; g < groups; g += 64) {
+        load(g);
+        all_ += last_lane(until_);
+      }
     }
-    target -= (unsigned)__builtin_amdgcn_readlane((int)until, 63);
   }
-  return {0, 0xffffffffu};   // (not reached: target is one of all)
-}
+  __device__ __forceinline__ unsigned all() const { return all_; }
+  // Block `target` of all() (which is less).
+  __device__ __forceinline__ RowBlock find(unsigned target) {
+    unsigned from = 0;
+    if (groups_ > 64) {
+      for (;; from += 64) {
+        load(from);
+        const unsigned here = last_lane(until_);
+        if (target < here || from + 64 >= groups_) break;
+        target -= here;
+      }
+    }
+    const unsigned long long behind = __ballot(until_ > target);
+    const int lane = behind ? __builtin_ctzll(behind) : 63;
+    RowBlock r;
+    r.group = uniform(from + lane);
+    r.rows.first = (unsigned)__builtin_amdgcn_readlane((int)mine_.first, lane);
+    r.rows.count = (unsigned)__builtin_amdgcn_readlane((int)mine_.count, lane);
+    r.block = target - ((unsigned)__builtin_amdgcn_readlane((int)until_, lane) - (r.rows.count + BY - 1) / BY);
+    return r;
+  }
+
+ private:
+  static __device__ __forceinline__ unsigned last_lane(unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)v, 63); }
+  // until_: blocks of this lane's group and those of lower lanes
+  __device__ __forceinline__ void load(unsigned from) {
+    const unsigned lane = threadIdx.x & 63, g = from + lane;
+    mine_ = {0, 0};
+    if (g < groups_) mine_ = span_of(offsets_, g, rows_);
+    until_ = (mine_.count + BY - 1) / BY;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const unsigned other = (unsigned)__shfl_up((int)until_, d);
+      if (lane >= (unsigned)d) until_ += other;
+    }
+  }
+  const int *offsets_;
+  unsigned groups_, rows_, all_, until_;
+  Span mine_;
+};
 
 // Which part of D a workgroup has.
 struct Place {
@@ -120,44 +141,43 @@ struct Place {
 template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a) {
   Place p;
   p.none = false;
-  p.group = 0;
-  p.part = 0;
-  unsigned t, blocks_y = a.blocks_y, first = 0;
+  p.group = p.part = 0;
+  p.rows = {0, a.rows};
+  // groups of four block rows, y fastest: the blocks that an XCD works on at one time share rows of X and of Y
+  auto spread = [&](unsigned t, unsigned blocks_y) {
+    constexpr unsigned GROUP = 4;
+    const unsigned g = t / (GROUP * a.blocks_x), in = t - g * GROUP * a.blocks_x;
+    const unsigned rows = blocks_y - g * GROUP < GROUP ? blocks_y - g * GROUP : GROUP;
+    p.by = uniform(g * GROUP + in % rows);
+    p.bx = uniform(in / rows);
+    p.tile = uniform(t);
+  };
   if (a.offsets && KIND != kWeights) {
-    blocks_y = all_row_blocks<BY>(a);
-    const unsigned all = blocks_y * a.blocks_x;
+    RowBlocks<BY> blocks(a.offsets, a.groups, a.rows);
+    const unsigned all = blocks.all() * a.blocks_x;
     if (blockIdx.x >= all) {
       p.none = true;
       return p;
     }
-    t = xcd_remap(blockIdx.x, all);
-  } else {
-    const unsigned per_matrix = a.blocks_x * a.blocks_y, id = xcd_remap(blockIdx.x, gridDim.x), rest = id / per_matrix;
-    t = id - rest * per_matrix;
-    if (a.offsets) {
-      p.group = uniform(rest);
-    } else {
-      p.part = uniform(rest);
-    }
-    first = rest * per_matrix;
+    spread(xcd_remap(blockIdx.x, all), blocks.all());
+    const RowBlock r = blocks.find(p.by);
+    p.group = r.group;
+    p.by = r.block;
+    p.rows = r.rows;
+    return p;
   }
-  p.tile = uniform(a.offsets ? first + t : t);
-  // groups of four block rows, y fastest: the blocks that an XCD works on at one time share rows of X and of Y
-  constexpr unsigned GROUP = 4;
-  const unsigned g = t / (GROUP * a.blocks_x), in = t - g * GROUP * a.blocks_x;
-  const unsigned rows = blocks_y - g * GROUP < GROUP ? blocks_y - g * GROUP : GROUP;
-  p.by = uniform(g * GROUP + in % rows);
-  p.bx = uniform(in / rows);
-  p.rows = {0, a.rows};
+  const unsigned per_matrix = a.blocks_x * a.blocks_y;
   if (a.offsets) {
-    if (KIND != kWeights) {
-      const RowBlock r = find_row_block<BY>(a, p.by);
-      p.group = uniform(r.group);
-      p.by = uniform(r.block);
-    }
+    // (each XCD has an eighth of every group's blocks: groups differ in their rows)
+    p.group = uniform(blockIdx.x / per_matrix);
+    spread(xcd_remap(blockIdx.x - p.group * per_matrix, per_matrix), a.blocks_y);
     p.rows = span_of(a.offsets, p.group, a.rows);
     p.rows.first = uniform(p.rows.first);
     p.rows.count = uniform(p.rows.count);
+  } else {
+    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
+    p.part = uniform(id / per_matrix);
+    spread(id - p.part * per_matrix, a.blocks_y);
   }
   return p;
 }
@@ -223,6 +243,25 @@ template <typename T, int N> __device__ __forceinline__ void load_row(const T *f
   }
 }
 
+// real::store_row, past the caches: what is more than the last-level cache holds is not in it when it is read next, and only
+// displaces operands (8192^3 with residual and z, 256 MiB of y and z: 874 us in the ordinary way, 827 past; 128 MiB: 79 and 80).
+template <typename T, int N> __device__ __forceinline__ void store_row(int past, T *to, unsigned left, const float (&v)[N]) {
+  constexpr int E = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
+  typedef T piece_t __attribute__((ext_vector_type(E)));
+  typedef piece_t piece_unaligned_t __attribute__((aligned(sizeof(T))));
+  if (past && left >= (unsigned)N) {
+#pragma unroll
+    for (int i = 0; i < N; i += E) {
+      piece_unaligned_t w;
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = (T)v[i + e];
+      __builtin_nontemporal_store(w, reinterpret_cast<piece_unaligned_t *>(to + i));
+    }
+  } else {
+    real::store_row(to, left, v);
+  }
+}
+
 // What becomes of the sums of D.
 struct StoreParams {
   char *out, *z;                  // z: may be null (kOutput)
@@ -231,6 +270,7 @@ struct StoreParams {
   size_t group;                   // elements from one group's out to the next (kWeights)
   int activation;
   int wide, accumulate;           // kWeights: out is float32, and added to
+  int past;                       // out and z are stored past the caches
 };
 
 // `v`: N neighbours from x on (`left` of them inside the row) in row y of D, or of all groups' rows.
@@ -244,7 +284,7 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] += bias[e];
     }
-    if (p.z) real::store_row(reinterpret_cast<T *>(p.z) + at, left, v);
+    if (p.z) store_row(p.past, reinterpret_cast<T *>(p.z) + at, left, v);
     activate(p.activation, v);
     if (p.residual) {
       float r[N];
@@ -252,13 +292,13 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] += r[e];
     }
-    real::store_row(reinterpret_cast<T *>(p.out) + at, left, v);
+    store_row(p.past, reinterpret_cast<T *>(p.out) + at, left, v);
   } else if constexpr (KIND == kInput) {
-    real::store_row(reinterpret_cast<T *>(p.out) + at, left, v);
+    store_row(p.past, reinterpret_cast<T *>(p.out) + at, left, v);
   } else {
     const size_t here = (size_t)group * p.group + at;
     if (!p.wide) {
-      real::store_row(reinterpret_cast<T *>(p.out) + here, left, v);
+      store_row(p.past, reinterpret_cast<T *>(p.out) + here, left, v);
     } else {
       float *const out = reinterpret_cast<float *>(p.out) + here;
       if (p.accumulate) {
@@ -267,7 +307,7 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] += old[e];
       }
-      real::store_row(out, left, v);
+      store_row(p.past, out, left, v);
     }
   }
 }

@@ -5,7 +5,7 @@
 // on the order of blocks.
 //
 // A row is held by 16 lanes (64 from 257 experts on), PER neighbouring logits a lane, as whole numbers of the same order; each
-// round takes the maximum of all lanes by DPP and removes it.
+// round takes the maximum of all lanes by DPP, and the lane that holds it removes it, stores its number and counts it.
 #include <algorithm>
 
 #include "linear_gemm.h"
@@ -65,7 +65,7 @@ struct ChooseArgs {
 struct Shared {
   unsigned base[kMostExperts];              // an expert's next place
   unsigned below[kMostExperts];
-  unsigned short waves[kWaves][kMostExperts];
+  unsigned waves[kWaves][kMostExperts];
   unsigned totals[kWaves];
 };
 
@@ -87,40 +87,50 @@ __device__ __forceinline__ void first_places(Shared &s, unsigned e) {
   __syncthreads();
 }
 
-// Places of the rows of one tile, from the experts' next places in s.base. `count` rows (of tokens times k).
+// How many lanes below this one have the same expert as it (rank), and how many have it in all; lanes with `have` count.
+struct Alike {
+  unsigned rank, all;
+};
+__device__ __forceinline__ Alike alike(bool have, unsigned expert, unsigned e) {
+  unsigned long long same = __ballot(have);
+  for (unsigned bit = 1; bit < e; bit <<= 1) {
+    const unsigned long long set = __ballot((expert & bit) != 0);
+    same &= expert & bit ? set : ~set;
+  }
+  return {(unsigned)__popcll(same & ((1ull << (threadIdx.x & 63)) - 1)), (unsigned)__popcll(same)};
+}
+
+// Places of the rows of one tile, `count` of them, from the experts' next places in s.base. Each wave has a piece of them: it counts them,
+// learns from the counts of the waves before it where its own begin, and numbers them, 64 at a time.
 __device__ __forceinline__ void place_rows(Shared &s, const int *experts, int *slots, unsigned count, unsigned e) {
   const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (unsigned at = 0; at < count; at += kThreads) {
-    for (unsigned i = t; i < e; i += kThreads) {
+  const unsigned piece = (count + kThreads - 1) / kThreads * 64, from = wave * piece, until = from + piece < count ? from + piece : count;
+  for (unsigned i = t; i < e; i += kThreads) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) s.waves[w][i] = 0;
-    }
-    __syncthreads();
-    const bool have = at + t < count;
-    const unsigned mine = have ? (unsigned)experts[at + t] : 0;
-    // lanes with the same expert
-    unsigned long long same = __ballot(have);
-    for (unsigned bit = 1; bit < e; bit <<= 1) {
-      const unsigned long long set = __ballot((mine & bit) != 0);
-      same &= mine & bit ? set : ~set;
-    }
-    const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1));
-    if (have && rank == 0) s.waves[wave][mine] = (unsigned short)__popcll(same);
-    __syncthreads();
-    for (unsigned i = t; i < e; i += kThreads) {     // (the places of each wave's first)
-      unsigned all = 0;
+    for (int w = 0; w < kWaves; ++w) s.waves[w][i] = 0;
+  }
+  __syncthreads();
+  for (unsigned at = from + lane; at < until; at += 64) atomicAdd(&s.waves[wave][experts[at]], 1u);
+  __syncthreads();
+  for (unsigned i = t; i < e; i += kThreads) {
+    unsigned next = s.base[i];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const unsigned n = s.waves[w][i];
-        s.waves[w][i] = (unsigned short)all;
-        all += n;
-      }
-      s.below[i] = all;
+    for (int w = 0; w < kWaves; ++w) {
+      const unsigned n = s.waves[w][i];
+      s.waves[w][i] = next;
+      next += n;
     }
-    __syncthreads();
-    if (have) slots[at + t] = (int)(s.base[mine] + s.waves[wave][mine] + rank);
-    __syncthreads();
-    for (unsigned i = t; i < e; i += kThreads) s.base[i] += s.below[i];
+  }
+  __syncthreads();
+  for (unsigned at = from; at < until; at += 64) {
+    const bool have = at + lane < until;
+    const unsigned mine = have ? (unsigned)experts[at + lane] : 0;
+    const Alike a = alike(have, mine, e);
+    const unsigned place = s.waves[wave][mine] + a.rank;
+    if (have) slots[at + lane] = (int)place;
+    __builtin_amdgcn_wave_barrier();       // (all lanes have read, before the first of each expert writes)
+    if (have && a.rank == 0) s.waves[wave][mine] = place + a.all;
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -137,29 +147,34 @@ template <int TYPE, int LANES, int PER> __global__ __launch_bounds__(kThreads) v
     unsigned keys[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) keys[i] = l * PER + i < a.e ? key_of(v[i]) : 0u;
-    unsigned my_expert = 0;
-    float my_value = 0.f, top = 0.f;
+    unsigned my_key = 0, top_key = 0;
+    const size_t at = (size_t)t * a.k;
     for (unsigned j = 0; j < a.k; ++j) {
       unsigned best = keys[0];
 #pragma unroll
       for (int i = 1; i < PER; ++i) best = larger(best, keys[i]);
       const unsigned most = over_lanes<LANES>(best, larger);
-      // the lowest of those that hold it: as the largest of numbers that fall
+      // the lowest lane of the row that holds it, and its lowest logit that does
+      const unsigned long long holders = __ballot(best == most) >> (threadIdx.x & 63 & ~(LANES - 1));
+      const bool winner = l == (unsigned)__builtin_ctzll(holders);
+      bool open = winner;
       unsigned number = 0;
-      if (best == most) {
 #pragma unroll
-        for (int i = PER - 1; i >= 0; --i) number = keys[i] == most ? ~(l * PER + i) : number;
+      for (int i = 0; i < PER; ++i) {
+        const bool hit = open && keys[i] == most;
+        open = open && !hit;
+        keys[i] = hit ? 0u : keys[i];
+        number = hit ? i : number;
       }
-      const unsigned chosen = ~over_lanes<LANES>(number, larger);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) keys[i] = l * PER + i == chosen ? 0u : keys[i];
-      const float value = value_of(most);
-      if (j == 0) top = value;
-      if (l == j) {
-        my_expert = chosen;
-        my_value = value;
+      if (winner) {
+        number += l * PER;
+        a.experts[at + j] = (int)number;
+        atomicAdd(&s.base[number], 1u);
       }
+      if (j == 0) top_key = most;
+      my_key = l == j ? most : my_key;
     }
+    const float top = value_of(top_key), my_value = value_of(my_key);
     // (a row of nothing but -inf has weights of zero)
     const float over = top == -__builtin_inff() ? 0.f : top;
     const float mine = l < a.k ? __expf(my_value - over) : 0.f;
@@ -173,10 +188,7 @@ template <int TYPE, int LANES, int PER> __global__ __launch_bounds__(kThreads) v
       all = over_lanes<LANES>(some, sum);
     }
     if (l < a.k) {
-      const size_t at = (size_t)t * a.k + l;
-      a.experts[at] = (int)my_expert;
-      a.weights[at] = all == 0.f ? 0.f : mine / all;
-      atomicAdd(&s.base[my_expert], 1u);
+      a.weights[at + l] = all == 0.f ? 0.f : mine / all;
     }
   }
   __syncthreads();
@@ -200,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void route_place(ChooseArgs a) {
   const unsigned ways = kThreads / a.e, e = t % a.e, way = t / a.e;
   if (way < ways) {
     unsigned all = 0, below = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (unsigned b = way; b < a.tiles; b += ways) {
       const unsigned n = a.counts[(size_t)b * a.e + e];
       all += n;
