@@ -78,6 +78,17 @@ RealGemmPlan plan_product(const LinearParams &p, int kind) {
   return plan;
 }
 
+// Rows of x that a block has where y is linear_rows.hip's, 0 where it is not: every block reads x from the caches, which costs more
+// than it saves where x is long (us, linear_rows and gemm_linear: 16 rows of 4096 x 2048 6.0 and 9.1, 32 rows of 577 x 1000 4.5 and
+// 7.2, 16 rows of 8192 x 8192 33 and 30), and each expert's W once for 16 rows (64 experts of 2048 x 2048: 16 rows 18 and 22, 128
+// rows 75 to 84 and 84, 256 rows 93 to 98 and 92).
+int plan_few_rows(const LinearParams &p) {
+  if (real_block_option) return 0;
+  if (p.grouped) return p.m <= 2 * p.groups ? 16 : 0;
+  if (p.m > 32 || (size_t)p.m * p.k > 65536) return 0;
+  return p.m <= 16 ? 16 : 32;
+}
+
 // ---- before the products of the backward pass ----
 
 // Columns and rows of a block. Few rows a block where 64 would leave units idle: a wave's loads are on their way together then (300 x 255:
@@ -242,6 +253,9 @@ class Tails {
   int count_ = 0;
 };
 
+// Half of an XCD's L2.
+constexpr size_t kStaysInCaches = (size_t)2 << 20;
+
 Args product_args(const LinearParams &p, int kind, const Operand &x, const Operand &y, const int *offsets, Tails *tails) {
   const Extents e = extents(p, kind);
   const RealGemmPlan &plan = p.plan[kind];
@@ -264,6 +278,7 @@ Args product_args(const LinearParams &p, int kind, const Operand &x, const Opera
   a.blocks_y = (unsigned)ceil_div(e.ny, s.by);
   a.parts = plan.parts;
   a.pieces_per_part = plan.pieces_per_part;
+  a.rotate = kind != kWeights && 2 * e.ny * e.k <= kStaysInCaches;
   a.arrived = reinterpret_cast<unsigned *>(p.workspace);
   a.partial = reinterpret_cast<float *>(p.workspace + p.partial);
   return a;
@@ -310,12 +325,16 @@ template <unsigned ROWS> hipError_t launch_join(const LinearParams &p, const Joi
   return hipGetLastError();
 }
 
+// Blocks of linear_rows.hip: as many as there can be.
+size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, p.few_rows); }
+
 }  // namespace
 
 void plan_linear(LinearParams *p) {
   const int kinds = p->training ? 3 : 1;
   size_t counters = 0, partial = 0;
-  for (int kind = 0; kind < kinds; ++kind) {
+  p->few_rows = plan_few_rows(*p);
+  for (int kind = p->few_rows ? 1 : 0; kind < kinds; ++kind) {
     p->plan[kind] = plan_product(*p, kind);
     counters = std::max(counters, p->plan[kind].counter_bytes);
     partial = std::max(partial, p->plan[kind].partial_bytes);
@@ -336,7 +355,8 @@ void plan_linear(LinearParams *p) {
 }
 
 bool linear_launches(const LinearParams &p) {
-  for (int kind = 0; kind < (p.training ? 3 : 1); ++kind) {
+  if (p.few_rows && few_rows_blocks(p) > 0xffffffffu / 512) return false;
+  for (int kind = p.few_rows ? 1 : 0; kind < (p.training ? 3 : 1); ++kind) {
     const RealShape &s = kShapes[p.plan[kind].shape];
     if (!real_launches(s, launched_blocks(p, kind, s) * p.plan[kind].parts)) return false;
   }
@@ -348,6 +368,10 @@ bool linear_launches(const LinearParams &p) {
 
 const char *describe_linear(const LinearParams &p, int kind) {
   static thread_local char name[96];
+  if (kind == kOutput && p.few_rows) {
+    snprintf(name, sizeof name, "linear_rows<%s> %d rows a block", p.type == kFloat16 ? "float16" : "bfloat16", p.few_rows);
+    return name;
+  }
   static const char *const kinds[] = {"forward", "input's gradient", "weights' gradient"};
   snprintf(name, sizeof name, "gemm_linear<%s, %s> %s block, K in %u", p.type == kFloat16 ? "float16" : "bfloat16", kinds[kind],
            kShapes[p.plan[kind].shape].name, p.plan[kind].parts);
@@ -356,10 +380,6 @@ const char *describe_linear(const LinearParams &p, int kind) {
 
 hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, hipStream_t stream) {
   if (p.m == 0 || p.n == 0) return hipSuccess;
-  Tails tails(p.workspace + p.tails);
-  const Operand x = {f.x, p.m, p.k, p.x_pitch}, w = {f.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
-  const Args a = product_args(p, kOutput, w, x, f.offsets, &tails);
-  HIP_PASS(tails.launch(stream));
   StoreParams s = {};
   s.out = static_cast<char *>(f.y);
   s.z = static_cast<char *>(f.z);
@@ -368,6 +388,14 @@ hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, 
   s.pitch = p.y_pitch;
   s.activation = p.activation;
   s.past = 2 * (size_t)p.m * p.n * (f.z ? 2 : 1) >= kPastCachesBytes;
+  Tails tails(p.workspace + p.tails);
+  const Operand x = {f.x, p.m, p.k, p.x_pitch}, w = {f.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
+  Args a = product_args(p, kOutput, w, x, f.offsets, &tails);
+  if (p.few_rows) {      // (which reads no more than the rows)
+    a.blocks_x = (unsigned)linear_rows_blocks(p.n);
+    return launch_linear_rows(p.type, p.few_rows, (unsigned)few_rows_blocks(p), a, s, stream);
+  }
+  HIP_PASS(tails.launch(stream));
   return launch_product(p, kOutput, a, s, stream);
 }
 

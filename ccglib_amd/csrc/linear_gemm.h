@@ -56,6 +56,7 @@ struct Args {
   size_t x_group;                  // bytes from one group's X to the next (kOutput, kInput)
   unsigned blocks_x, blocks_y;     // (of a group: kWeights)
   unsigned parts, pieces_per_part; // as in real_gemm.h
+  unsigned rotate;                 // blocks begin at different pieces of K (see below)
   float *partial;
   unsigned *arrived;
 };
@@ -382,7 +383,14 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
   // (kept in registers: its address is a scalar load, behind which the LDS reads would be waited for all together)
   const char *zeros = real::g_zeros;
   real::pin_scalar(zeros);
-  unsigned piece_next = first;
+  // Blocks whose Y stays in the caches whatever they ask for begin at different pieces of K: rows lie a multiple of the memory
+  // channels' stride apart as often as not, and all blocks at one k ask the same few channels (linear_rows.hip has figures). The last two
+  // pieces stay the last.
+  const unsigned count = last > first ? last - first : 0, plain = count > 2 ? count - 2 : 0;
+  const unsigned begin = args.rotate && plain > 0 ? at.bx % plain : 0;
+  x_next += (size_t)begin * x_step;
+  y_next += (size_t)begin * y_step;
+  unsigned piece_next = first + begin, copied = 0;
   // Copy n of the wave's COPIES of the next piece. `end`: it may be one of the last two pieces of K.
   auto copy_one = [&](unsigned slot, auto copy, auto end) {
     constexpr int n = decltype(copy)::value;
@@ -422,6 +430,14 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
     x_next += x_step;
     y_next += y_step;
     ++piece_next;
+    ++copied;
+    auto jump = [&](int pieces) {
+      x_next += (long long)pieces * (long long)x_step;
+      y_next += (long long)pieces * (long long)y_step;
+      piece_next += pieces;
+    };
+    if (copied == plain - begin) jump(-(int)plain);
+    if (copied == plain) jump((int)(plain - begin));
   };
   const std::true_type may_end{};
 
@@ -488,7 +504,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
   constexpr int BEHIND = COPY_STEPS == 0 || SPT * PER_STEP > COPIES ? COPIES : SPT * PER_STEP;
   constexpr int PER_BEHIND = (BEHIND + SPT - 1) / SPT, REST = COPIES - BEHIND;
   constexpr int PER_REST = REST == 0 ? 0 : REST <= COPY_STEPS * PER_STEP ? PER_STEP : (REST + COPY_STEPS - 1) / (COPY_STEPS ? COPY_STEPS : 1);
-  const unsigned n = last > first ? last - first : 0;
+  const unsigned n = count;
   if (n > 0) {
 #pragma unroll
     for (int t = 0; t < SLOTS - 1; ++t) {
@@ -585,7 +601,6 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
       slot = next;
     };
     // (pieces of K's end, or of an operand's, are among the last two)
-    const unsigned plain = n > 2 ? n - 2 : 0;
     unsigned t = 0;
 #pragma unroll 1
     for (; t + SLOTS < plain; ++t) piece(std::integral_constant<int, kAll>{});
@@ -698,6 +713,10 @@ CCGLIB_DECLARE(kBfloat16, kOutput)
 CCGLIB_DECLARE(kBfloat16, kInput)
 CCGLIB_DECLARE(kBfloat16, kWeights)
 #undef CCGLIB_DECLARE
+
+// y of few rows (linear_rows.hip): blocks of 16 columns and `by` rows, 16 or 32
+size_t linear_rows_blocks(size_t n);
+hipError_t launch_linear_rows(int type, int by, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream);
 
 #ifdef CCGLIB_LINEAR_KIND
 template <>

@@ -99,6 +99,14 @@ def test_every_length_of_an_experts_rows(rows):
             run_layer(3, M, 40, 24, VT.bfloat16, ACT.none, [0, rows, rows + 3, M])
 
 
+@pytest.mark.parametrize("spans", list(SPANS))
+@pytest.mark.parametrize("E,M,N,K", [(1, 2, 33, 1031), (40, 60, 17, 1030), (66, 100, 40, 24), (100, 3, 50, 2048)])
+def test_few_rows(spans, E, M, N, K):
+    """What the kernel for a few rows takes: an expert may have more than 16 of them."""
+    layer = run_layer(E, M, N, K, VT.bfloat16, ACT.silu, SPANS[spans](M, E), pitches=(K + 1, K, N), shift=E % 2)
+    assert "linear_rows" in layer.KernelName()
+
+
 def test_offsets_outside_the_rows_count_as_the_nearer_end():
     run_layer(4, 50, 24, 40, VT.bfloat16, ACT.none, [0, 10, 50, 50, 50], held=[-7, 10, 51, 2 ** 31 - 1, 60])
 
