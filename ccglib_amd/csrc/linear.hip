@@ -2,6 +2,7 @@
 // before its products: dz = dy act'(z), rounded to the 16 bits that the matrix cores multiply, and the bias' gradient from the same
 // values in 32.
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 
 #include "linear_gemm.h"
@@ -12,12 +13,15 @@ namespace {
 
 using namespace linear;
 
-// (the shapes of linear_gemm.h, in their order; see real_plan.h for the figures)
-constexpr RealShape kShapes[] = {{256, 256, 512, 1, 1.0f, 1.55f, 14.0f, 0.8f, "256x256"},
-                                 {128, 128, 256, 2, 0.62f, 0.87f, 9.0f, 1.3f, "128x128"},
-                                 {64, 64, 256, 2, 0.18f, 0.27f, 5.0f, 2.6f, "64x64"},
-                                 {64, 32, 256, 2, 0.14f, 0.2f, 4.0f, 4.5f, "32x64"},
-                                 {128, 128, 512, 1, 0.35f, 0.54f, 7.0f, 1.3f, "128x128 8-wave"},{192, 192, 512, 1, 0.62f, 0.97f, 11.0f, 1.0f, "192x192"},{128, 256, 512, 1, 0.62f, 0.87f, 9.0f, 1.0f, "256x128"}};
+// (the shapes of linear_gemm.h, in their order; see real_plan.h for the figures. These were fitted to y, dx and dW of 34 problems from
+// 1 x 8192 x 8192 to 8192 x 8192 x 2048, some of odd sizes, in every shape and 1 to 16 parts: there the choice is 1.2 % behind the
+// fastest shape and number of parts in the mean, 13 % at most.)
+constexpr RealShape kShapes[] = {{256, 256, 512, 1, 0.99f, 1.82f, 8.2f, 0.97f, "256x256"},
+                                 {64, 64, 256, 2, 0.30f, 0.55f, 4.8f, 2.6f, "64x64"},
+                                 {64, 32, 256, 2, 0.26f, 0.49f, 4.7f, 4.1f, "32x64"},
+                                 {128, 128, 512, 1, 0.395f, 0.57f, 6.4f, 1.33f, "128x128"},
+                                 {192, 192, 512, 1, 0.615f, 1.01f, 8.7f, 0.83f, "192x192"},
+                                 {128, 256, 512, 1, 0.55f, 0.97f, 7.5f, 0.82f, "256x128"}};
 constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
   static_assert(kShapes[ID].bx == BX && kShapes[ID].by == BY && kShapes[ID].threads == 64 * WX * WY, \
@@ -55,21 +59,32 @@ size_t launched_blocks(const LinearParams &p, int kind, const RealShape &s) {
 RealGemmPlan plan_product(const LinearParams &p, int kind) {
   const Extents e = extents(p, kind);
   if (!p.grouped) return plan_real_gemm(kShapes, kShapeCount, 1, e.nx, e.ny, ceil_div(e.k, (size_t)kPiece), false, real_block_option);
-  // K is not cut: that of kWeights has as many lengths as there are groups, and the other products have blocks of many groups
+  // K is not cut: that of kWeights has as many lengths as there are groups, and the other products have blocks of many groups. How
+  // many rows each group has is not known here: the mean of what even and uneven groups would take, and of a few blocks more or less, so
+  // that no choice hangs on a round of blocks that is just full.
   RealGemmPlan plan;
   double best = 0.0;
   for (int s = 0; s < kShapeCount; ++s) {
     const RealShape &shape = kShapes[s];
     if (real_block_option && s != (int)std::min<size_t>(real_block_option % 256 - 1, kShapeCount - 1)) continue;
-    double blocks = (double)ceil_div(e.nx, shape.bx);
-    size_t pieces = ceil_div(e.k, (size_t)kPiece);
-    if (kind == kWeights) {
-      blocks *= (double)p.groups * (double)ceil_div(e.ny, shape.by);
-      pieces = ceil_div((size_t)p.m, (size_t)p.groups * kPiece);
-    } else {   // (groups of about the same size: half a block more than their rows fill)
-      blocks *= std::max((double)std::min(p.groups, p.m), (double)p.m / shape.by + 0.5 * std::min(p.groups, p.m));
+    double us = 0.0;
+    for (const bool uneven : {false, true}) {
+      double weights = 0.0, blocks = 0.0;
+      auto weight = [&](unsigned g) {      // (rows of a group: the logarithm of their number is about normal)
+        const double q = (g + 0.5) / p.groups;
+        return uneven ? std::pow(q / (1.0 - q), 0.4) : 1.0;
+      };
+      for (unsigned g = 0; g < p.groups; ++g) weights += weight(g);
+      for (unsigned g = 0; g < p.groups; ++g) {
+        const double rows = weight(g) / weights * p.m;
+        blocks += kind == kWeights ? (double)ceil_div(e.ny, shape.by) : rows < 1.0 ? rows : std::ceil(rows / shape.by);
+      }
+      blocks *= (double)ceil_div(e.nx, shape.bx);
+      const size_t pieces = kind == kWeights ? ceil_div((size_t)p.m, (size_t)p.groups * kPiece) : ceil_div(e.k, (size_t)kPiece);
+      for (const double more : {0.95, 1.0, 1.05, 1.1}) {      // (those of kWeights are known)
+        us += real_gemm_us(shape, std::max<size_t>(1, (size_t)(kind == kWeights ? blocks : blocks * more)), std::max<size_t>(1, pieces), 1);
+      }
     }
-    const double us = real_gemm_us(shape, (size_t)blocks, std::max<size_t>(1, pieces), 1);
     if (best == 0.0 || us < best) {
       best = us;
       plan.shape = s;

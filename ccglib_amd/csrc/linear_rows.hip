@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows(Args args, StoreParams
   if (left == 0 || row >= rows.count) return;
   float bias[4] = {};
   if (params.bias) load_row(reinterpret_cast<const typename Value<TYPE>::type *>(params.bias) + (size_t)group * args.nx + out_x, left, bias);
-  store_sums<TYPE, kOutput>(params, bias, group, rows.first + row, out_x, left, v);
+  store_sums<TYPE, kOutput, false>(params, bias, group, rows.first + row, out_x, left, v);
 }
 
 template <int TYPE, int NY> hipError_t launch(unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream) {

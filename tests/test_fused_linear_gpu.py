@@ -71,7 +71,7 @@ def test_forward_and_backward(t, activation, M, N, K):
 
 
 @pytest.mark.parametrize("t", list(HALF))
-@pytest.mark.parametrize("shape,parts", [(s, p) for s in range(1, 6) for p in (1, 3)])
+@pytest.mark.parametrize("shape,parts", [(s, p) for s in range(1, 7) for p in (1, 3)])
 @pytest.mark.parametrize("M,N,K", [(300, 261, 713), (33, 600, 64), (512, 256, 1000)])
 def test_every_shape(t, shape, parts, M, N, K):
     with cc.option(cc.Option.real_block, shape + 256 * parts):
@@ -79,7 +79,7 @@ def test_every_shape(t, shape, parts, M, N, K):
     assert "K in" in layer.KernelName(2)
 
 
-@pytest.mark.parametrize("shape", range(1, 6))
+@pytest.mark.parametrize("shape", range(1, 7))
 @pytest.mark.parametrize("K", [1, 2, 7, 8, 9, 15, 63, 64, 65, 71, 72, 120, 127, 128, 129, 191, 193, 256, 449])
 def test_every_length_of_the_sum(shape, K):
     """K is the sum's length of y, N of dx, M of dW."""
@@ -89,7 +89,7 @@ def test_every_length_of_the_sum(shape, K):
         run_layer(K, 40, 24, VT.bfloat16, ACT.none)
 
 
-@pytest.mark.parametrize("shape", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("shape", range(0, 7))
 @pytest.mark.parametrize("pitches,shift", [((584, 584, 264), 0), ((584, 584, 264), 1), ((577, 577, 255), 3), ((579, 581, 257), 0),
                                            ((1000, 600, 400), 5)])
 def test_distances_and_addresses(shape, pitches, shift):

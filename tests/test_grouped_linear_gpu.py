@@ -69,7 +69,7 @@ def test_forward_and_backward(t, activation, spans, E, M, N, K):
     run_layer(E, M, N, K, t, activation, SPANS[spans](M, E))
 
 
-@pytest.mark.parametrize("shape", range(1, 6))
+@pytest.mark.parametrize("shape", range(1, 7))
 @pytest.mark.parametrize("spans", ["even", "rows before and behind", "one each"])
 def test_every_shape(shape, spans):
     with cc.option(cc.Option.real_block, shape):
@@ -77,7 +77,7 @@ def test_every_shape(shape, spans):
         run_layer(9, 100, 24, 136, VT.float16, ACT.relu, SPANS[spans](100, 9))
 
 
-@pytest.mark.parametrize("shape", range(0, 6))
+@pytest.mark.parametrize("shape", range(0, 7))
 @pytest.mark.parametrize("pitches,shift", [((584, 584, 264), 0), ((577, 577, 255), 3), ((579, 581, 257), 1)])
 def test_distances_and_addresses(shape, pitches, shift):
     with cc.option(cc.Option.real_block, shape):
@@ -94,7 +94,7 @@ def test_gradients_of_weights_in_either_type(gradient_type, accumulate):
 @pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 127, 128, 129, 191, 200, 255, 257])
 def test_every_length_of_an_experts_rows(rows):
     M = 2 * rows + 3
-    for shape in range(1, 6):
+    for shape in range(1, 7):
         with cc.option(cc.Option.real_block, shape):
             run_layer(3, M, 40, 24, VT.bfloat16, ACT.none, [0, rows, rows + 3, M])
 
