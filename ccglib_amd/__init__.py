@@ -411,27 +411,31 @@ class FusedLinear(_Handle):
     def __init__(self, M, N, K, device, stream, type=ValueType.bfloat16, activation=Activation.none,
                  gradient_type=ValueType.float32, training=True, x_pitch=0, w_pitch=0, y_pitch=0):
         super().__init__()
-        _capi.check(_capi.load().ccglib_fused_linear_create(
+        self._lib = _capi.load()
+        _capi.check(self._lib.ccglib_fused_linear_create(
             ctypes.byref(self._h), M, N, K, int(device), _ptr(stream), int(type), int(activation),
             int(gradient_type), int(bool(training)), int(x_pitch), int(w_pitch), int(y_pitch)))
 
     def Forward(self, d_x, d_w, d_bias, d_residual, d_y, d_z=0):
         """0 for no bias, no residual, a z that is not wanted (Backward wants it where there is an
         activation). d_y may be d_residual."""
-        _capi.check(_capi.load().ccglib_fused_linear_forward(
-            self._h, _ptr(d_x), _ptr(d_w), _ptr(d_bias), _ptr(d_residual), _ptr(d_y), _ptr(d_z)))
+        status = self._lib.ccglib_fused_linear_forward(self._h, int(d_x), int(d_w), int(d_bias),
+            int(d_residual), int(d_y), int(d_z))
+        if status:
+            _capi.check(status)
 
     def Backward(self, d_dy, d_z, d_x, d_w, d_dx, d_dw, d_dbias=0, accumulate=False):
         """dz = dy act'(z), dx = dz W, dW (+)= dz^T x, dbias (+)= column sums of dz; 0 for a gradient
         that is not wanted. dW and dbias are of gradient_type; accumulate: of float32 only."""
-        _capi.check(_capi.load().ccglib_fused_linear_backward(
-            self._h, _ptr(d_dy), _ptr(d_z), _ptr(d_x), _ptr(d_w), _ptr(d_dx), _ptr(d_dw), _ptr(d_dbias),
-            int(bool(accumulate))))
+        status = self._lib.ccglib_fused_linear_backward(self._h, int(d_dy), int(d_z), int(d_x), int(d_w),
+            int(d_dx), int(d_dw), int(d_dbias), int(bool(accumulate)))
+        if status:
+            _capi.check(status)
 
     def KernelName(self, product=0):
         """Which kernel computes y (0), dx (1), dW (2)."""
         buf = ctypes.create_string_buffer(160)
-        _capi.check(_capi.load().ccglib_fused_linear_kernel_name(self._h, product, buf, len(buf)))
+        _capi.check(self._lib.ccglib_fused_linear_kernel_name(self._h, product, buf, len(buf)))
         return buf.value.decode()
 
 
@@ -444,25 +448,28 @@ class GroupedLinear(_Handle):
     def __init__(self, E, M, N, K, device, stream, type=ValueType.bfloat16, activation=Activation.none,
                  gradient_type=ValueType.float32, training=True, x_pitch=0, w_pitch=0, y_pitch=0):
         super().__init__()
-        _capi.check(_capi.load().ccglib_grouped_linear_create(
+        self._lib = _capi.load()
+        _capi.check(self._lib.ccglib_grouped_linear_create(
             ctypes.byref(self._h), E, M, N, K, int(device), _ptr(stream), int(type), int(activation),
             int(gradient_type), int(bool(training)), int(x_pitch), int(w_pitch), int(y_pitch)))
 
     def Forward(self, d_x, d_offsets, d_w, d_bias, d_residual, d_y, d_z=0):
-        _capi.check(_capi.load().ccglib_grouped_linear_forward(
-            self._h, _ptr(d_x), _ptr(d_offsets), _ptr(d_w), _ptr(d_bias), _ptr(d_residual), _ptr(d_y),
-            _ptr(d_z)))
+        status = self._lib.ccglib_grouped_linear_forward(self._h, int(d_x), int(d_offsets), int(d_w),
+            int(d_bias), int(d_residual), int(d_y), int(d_z))
+        if status:
+            _capi.check(status)
 
     def Backward(self, d_dy, d_z, d_x, d_offsets, d_w, d_dx, d_dw, d_dbias=0, accumulate=False):
         """As FusedLinear's; dW [E][N][w_pitch] and dbias [E][N] of all experts."""
-        _capi.check(_capi.load().ccglib_grouped_linear_backward(
-            self._h, _ptr(d_dy), _ptr(d_z), _ptr(d_x), _ptr(d_offsets), _ptr(d_w), _ptr(d_dx), _ptr(d_dw),
-            _ptr(d_dbias), int(bool(accumulate))))
+        status = self._lib.ccglib_grouped_linear_backward(self._h, int(d_dy), int(d_z), int(d_x),
+            int(d_offsets), int(d_w), int(d_dx), int(d_dw), int(d_dbias), int(bool(accumulate)))
+        if status:
+            _capi.check(status)
 
     def KernelName(self, product=0):
         """Which kernel computes y (0), dx (1), dW (2)."""
         buf = ctypes.create_string_buffer(160)
-        _capi.check(_capi.load().ccglib_grouped_linear_kernel_name(self._h, product, buf, len(buf)))
+        _capi.check(self._lib.ccglib_grouped_linear_kernel_name(self._h, product, buf, len(buf)))
         return buf.value.decode()
 
 
@@ -474,18 +481,23 @@ class Route(_Handle):
 
     def __init__(self, T, E, k, device, stream, type=ValueType.float32, normalize=True):
         super().__init__()
-        _capi.check(_capi.load().ccglib_route_create(
+        self._lib = _capi.load()
+        _capi.check(self._lib.ccglib_route_create(
             ctypes.byref(self._h), T, E, k, int(device), _ptr(stream), int(type), int(bool(normalize))))
 
     def Run(self, d_logits, d_experts, d_weights, d_offsets, d_slots):
         """experts, slots [T][k] int32, weights [T][k] float32, offsets [E + 1] int32."""
-        _capi.check(_capi.load().ccglib_route_run(
-            self._h, _ptr(d_logits), _ptr(d_experts), _ptr(d_weights), _ptr(d_offsets), _ptr(d_slots)))
+        status = self._lib.ccglib_route_run(self._h, int(d_logits), int(d_experts), int(d_weights),
+            int(d_offsets), int(d_slots))
+        if status:
+            _capi.check(status)
 
     def Backward(self, d_logits, d_experts, d_weights, d_dweights, d_dlogits):
         """dlogits [T][E], of the logits' type, from dweights [T][k] float32 and what Run wrote."""
-        _capi.check(_capi.load().ccglib_route_backward(
-            self._h, _ptr(d_logits), _ptr(d_experts), _ptr(d_weights), _ptr(d_dweights), _ptr(d_dlogits)))
+        status = self._lib.ccglib_route_backward(self._h, int(d_logits), int(d_experts), int(d_weights),
+            int(d_dweights), int(d_dlogits))
+        if status:
+            _capi.check(status)
 
 
 class Combine(_Handle):
@@ -495,20 +507,27 @@ class Combine(_Handle):
 
     def __init__(self, T, k, N, device, stream, type=ValueType.bfloat16, rows=0, y_pitch=0, out_pitch=0):
         super().__init__()
-        _capi.check(_capi.load().ccglib_combine_create(
+        self._lib = _capi.load()
+        _capi.check(self._lib.ccglib_combine_create(
             ctypes.byref(self._h), T, k, N, int(device), _ptr(stream), int(type), int(rows), int(y_pitch),
             int(out_pitch)))
 
     def Run(self, d_y, d_slots, d_weights, d_out):
         """out[t] = sum over j of weights[t][j] y[slots[t][j]]"""
-        _capi.check(_capi.load().ccglib_combine_run(self._h, _ptr(d_y), _ptr(d_slots), _ptr(d_weights), _ptr(d_out)))
+        status = self._lib.ccglib_combine_run(self._h, int(d_y), int(d_slots), int(d_weights), int(d_out))
+        if status:
+            _capi.check(status)
 
     def Spread(self, d_x, d_slots, d_weights, d_y):
         """y[slots[t][j]] = weights[t][j] x[t]"""
-        _capi.check(_capi.load().ccglib_combine_spread(self._h, _ptr(d_x), _ptr(d_slots), _ptr(d_weights), _ptr(d_y)))
+        status = self._lib.ccglib_combine_spread(self._h, int(d_x), int(d_slots), int(d_weights), int(d_y))
+        if status:
+            _capi.check(status)
 
     def Backward(self, d_dout, d_y, d_slots, d_weights, d_dy, d_dweights=0):
         """Of Run: dy[slots[t][j]] = weights[t][j] dout[t], dweights[t][j] = <dout[t], y[slots[t][j]]>; 0 for
         one that is not wanted."""
-        _capi.check(_capi.load().ccglib_combine_backward(
-            self._h, _ptr(d_dout), _ptr(d_y), _ptr(d_slots), _ptr(d_weights), _ptr(d_dy), _ptr(d_dweights)))
+        status = self._lib.ccglib_combine_backward(self._h, int(d_dout), int(d_y), int(d_slots),
+            int(d_weights), int(d_dy), int(d_dweights))
+        if status:
+            _capi.check(status)
