@@ -23,7 +23,7 @@ struct LinearParams {
   int type, gradient_type, activation;
   size_t x_pitch, w_pitch, y_pitch;    // elements from row to row: of x and dx; W and dW; y, z, residual, dy
   RealGemmPlan plan[3];                // by Kind
-  int few_rows;                        // y: rows of x a block of linear_rows.hip has; 0: y is gemm_linear's
+  bool few_rows;                       // y is linear_rows.hip's, else gemm_linear's
   // the workspace, and where in it (bytes): counters first, which are zero whenever a product starts
   char *workspace;
   size_t zeroed, partial, dz, sums, tails, bytes;

@@ -93,15 +93,18 @@ RealGemmPlan plan_product(const LinearParams &p, int kind) {
   return plan;
 }
 
-// Rows of x that a block has where y is linear_rows.hip's, 0 where it is not: every block reads x from the caches, which costs more
-// than it saves where x is long (us, linear_rows and gemm_linear: 16 rows of 4096 x 2048 6.0 and 9.1, 32 rows of 577 x 1000 4.5 and
-// 7.2, 16 rows of 8192 x 8192 33 and 30), and each expert's W once for 16 rows (64 experts of 2048 x 2048: 16 rows 18 and 22, 128
-// rows 75 to 84 and 84, 256 rows 93 to 98 and 92).
-int plan_few_rows(const LinearParams &p) {
-  if (real_block_option) return 0;
-  if (p.grouped) return p.m <= 2 * p.groups ? 16 : 0;
-  if (p.m > 32 || (size_t)p.m * p.k > 65536) return 0;
-  return p.m <= 16 ? 16 : 32;
+// Whether y is linear_rows.hip's. Its blocks of 16 x 16 read their operands from the caches again and again, but wait for no ring. us,
+// linear_rows and gemm_linear: single rows of x, bound by W's bytes, 24.8 and 30.1 (8192 x 8192 out of memory; 12 rows of 8192 x 4096
+// 17.1 and 15.6); small products, bound by their launch, 4.3 and 7.7 (64 x 255 x 1000), 6.6 and 7.9 (300 x 577 x 1000), then 12.1 and 8.1
+// (128 x 4096 x 1000); many blocks with little K 6.4 and 5.0 (128 x 4096 x 256). Rows that are not whole chunks are read in halves:
+// 59 and 33 (1 x 8191 x 8191), 5.0 and 6.7 (1 x 1000 x 577). Each expert's W is read for every 16 of its rows: 16 rows over 64 experts of
+// 2048 x 2048 18 and 22, 128 rows 75 to 84 and 84, 256 rows 93 to 98 and 92.
+bool plan_few_rows(const LinearParams &p) {
+  if (real_block_option) return false;
+  const double rows = p.m, outputs = rows * p.n, products = outputs * p.k;
+  if (p.x_pitch % 8 || p.w_pitch % 8) return products <= 10e6;
+  if (p.grouped ? p.m <= 2 * p.groups : p.m <= 4 && rows * p.k <= 32768) return true;
+  return outputs <= 262144 && products <= (p.grouped ? 100e6 : 175e6);
 }
 
 // ---- before the products of the backward pass ----
@@ -341,7 +344,7 @@ template <unsigned ROWS> hipError_t launch_join(const LinearParams &p, const Joi
 }
 
 // Blocks of linear_rows.hip: as many as there can be.
-size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, p.few_rows); }
+size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, kRowsOfX); }
 
 }  // namespace
 
@@ -370,7 +373,7 @@ void plan_linear(LinearParams *p) {
 }
 
 bool linear_launches(const LinearParams &p) {
-  if (p.few_rows && few_rows_blocks(p) > 0xffffffffu / 512) return false;
+  if (p.few_rows && few_rows_blocks(p) > 0xffffffffu / 256) return false;
   for (int kind = p.few_rows ? 1 : 0; kind < (p.training ? 3 : 1); ++kind) {
     const RealShape &s = kShapes[p.plan[kind].shape];
     if (!real_launches(s, launched_blocks(p, kind, s) * p.plan[kind].parts)) return false;
@@ -384,7 +387,7 @@ bool linear_launches(const LinearParams &p) {
 const char *describe_linear(const LinearParams &p, int kind) {
   static thread_local char name[96];
   if (kind == kOutput && p.few_rows) {
-    snprintf(name, sizeof name, "linear_rows<%s> %d rows a block", p.type == kFloat16 ? "float16" : "bfloat16", p.few_rows);
+    snprintf(name, sizeof name, "linear_rows<%s>", p.type == kFloat16 ? "float16" : "bfloat16");
     return name;
   }
   static const char *const kinds[] = {"forward", "input's gradient", "weights' gradient"};
@@ -408,7 +411,7 @@ hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, 
   Args a = product_args(p, kOutput, w, x, f.offsets, &tails);
   if (p.few_rows) {      // (which reads no more than the rows)
     a.blocks_x = (unsigned)linear_rows_blocks(p.n);
-    return launch_linear_rows(p.type, p.few_rows, (unsigned)few_rows_blocks(p), a, s, stream);
+    return launch_linear_rows(p.type, (unsigned)few_rows_blocks(p), a, s, stream);
   }
   HIP_PASS(tails.launch(stream));
   return launch_product(p, kOutput, a, s, stream);

@@ -715,9 +715,10 @@ CCGLIB_DECLARE(kBfloat16, kInput)
 CCGLIB_DECLARE(kBfloat16, kWeights)
 #undef CCGLIB_DECLARE
 
-// y of few rows (linear_rows.hip): blocks of 16 columns and `by` rows, 16 or 32
+// y of few rows (linear_rows.hip): blocks of 16 columns and kRowsOfX rows
+constexpr int kRowsOfX = 16;
 size_t linear_rows_blocks(size_t n);
-hipError_t launch_linear_rows(int type, int by, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream);
+hipError_t launch_linear_rows(int type, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream);
 
 #ifdef CCGLIB_LINEAR_KIND
 template <>

@@ -1,6 +1,6 @@
 // y = act(x W^T + bias) + residual for a few rows of x: single tokens, and experts that have a row or two each.
 //
-// Bound by memory: W is read once. A block has 16 rows of W and 16 NY of x; its waves share K out among themselves, CHUNKS x 32
+// Bound by memory: W is read once. A block has 16 rows of W and 16 of x; its waves share K out among themselves, CHUNKS x 32
 // values at a time each, and are added up at the end, in their order, through LDS. Values go from memory to the registers of the
 // 16x16x32 instruction as they are (lane l: 8 values along k of row l % 16), the next ones on their way while the last ones are multiplied:
 // no LDS and no barrier in the loop, where gemm_linear's ring waits a round trip a piece. One row of 4096 x 2048: 4.6 us, 9.0 there; of
@@ -38,11 +38,11 @@ template <int TYPE> __device__ __forceinline__ float4_t mfma_one(const int4_t &x
   }
 }
 
-template <int TYPE, int WAVES, int NY, int CHUNKS>
+template <int TYPE, int WAVES, int CHUNKS>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows(Args args, StoreParams params) {
-  constexpr int BY = 16 * NY;
+  constexpr int BY = kRowsOfX;
   constexpr unsigned STEP = 32 * CHUNKS;
-  __shared__ float4_t sums[WAVES][NY][64];
+  __shared__ float4_t sums[WAVES][64];
   const int lane = threadIdx.x & 63;
   const unsigned wave = uniform(threadIdx.x >> 6);
   const unsigned fr = lane & 15, g = lane >> 4;
@@ -60,33 +60,23 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows(Args args, StoreParams
   const unsigned x0 = bx * kRowsOfW, y0 = by * BY;
   const unsigned x_row = x0 + fr < args.nx ? x0 + fr : args.nx - 1;      // (rows past the end: never stored)
   const char *const x = args.x + (size_t)group * args.x_group + (size_t)x_row * args.x_pitch;
-  const char *y[NY];
-#pragma unroll
-  for (int j = 0; j < NY; ++j) {
-    const unsigned row = y0 + j * 16 + fr;
-    y[j] = args.y + (size_t)(rows.first + (row < rows.count ? row : rows.count - 1)) * args.y_pitch;
-  }
+  const unsigned y_row = y0 + fr < rows.count ? y0 + fr : rows.count - 1;
+  const char *const y = args.y + (size_t)(rows.first + y_row) * args.y_pitch;
 
-  float4_t acc[NY];
-#pragma unroll
-  for (int j = 0; j < NY; ++j) acc[j] = 0.f;
+  float4_t acc = {0.f, 0.f, 0.f, 0.f};
   struct Values {
-    int4_t x[CHUNKS], y[CHUNKS][NY];
+    int4_t x[CHUNKS], y[CHUNKS];
   };
   auto load = [&](Values &v, unsigned k) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       v.x[c] = load_8<false>(x, k + c * 32 + g * 8, args.k);
-#pragma unroll
-      for (int j = 0; j < NY; ++j) v.y[c][j] = load_8<false>(y[j], k + c * 32 + g * 8, args.k);
+      v.y[c] = load_8<false>(y, k + c * 32 + g * 8, args.k);
     }
   };
   auto multiply = [&](const Values &v) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-      for (int j = 0; j < NY; ++j) acc[j] = mfma_one<TYPE>(v.x[c], v.y[c][j], acc[j]);
-    }
+    for (int c = 0; c < CHUNKS; ++c) acc = mfma_one<TYPE>(v.x[c], v.y[c], acc);
   };
   // Whole steps of all waves, then what is left. Blocks begin at different ones: rows lie a multiple of the memory channels' stride
   // apart as often as not, and all blocks at one k ask the same few channels (one row, 8192 x 8192 out of memory: 30.7 us all from the first
@@ -117,41 +107,36 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows(Args args, StoreParams
     }
   }
   for (unsigned k = whole + wave * 32; k < args.k; k += WAVES * 32) {
-    const int4_t left = load_8<true>(x, k + g * 8, args.k);
-#pragma unroll
-    for (int j = 0; j < NY; ++j) acc[j] = mfma_one<TYPE>(left, load_8<true>(y[j], k + g * 8, args.k), acc[j]);
+    acc = mfma_one<TYPE>(load_8<true>(x, k + g * 8, args.k), load_8<true>(y, k + g * 8, args.k), acc);
   }
 
-#pragma unroll
-  for (int j = 0; j < NY; ++j) sums[wave][j][lane] = acc[j];
+  sums[wave][lane] = acc;
   __syncthreads();
-  // (a wave for each 16 rows of x)
-  if (wave >= (unsigned)NY) return;
+  if (wave > 0) return;
   float v[4] = {};
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += sums[w][wave][lane][e];
+    for (int e = 0; e < 4; ++e) v[e] += sums[w][lane][e];
   }
-  const unsigned out_x = x0 + g * 4, left = out_x < args.nx ? args.nx - out_x : 0, row = y0 + wave * 16 + fr;
+  const unsigned out_x = x0 + g * 4, left = out_x < args.nx ? args.nx - out_x : 0, row = y0 + fr;
   if (left == 0 || row >= rows.count) return;
   float bias[4] = {};
   if (params.bias) load_row(reinterpret_cast<const typename Value<TYPE>::type *>(params.bias) + (size_t)group * args.nx + out_x, left, bias);
   store_sums<TYPE, kOutput, false>(params, bias, group, rows.first + row, out_x, left, v);
 }
 
-template <int TYPE, int NY> hipError_t launch(unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream) {
-  linear_rows<TYPE, kRowsWaves, NY, kRowsChunks><<<grid, 64 * kRowsWaves, 0, stream>>>(a, s);
-  return hipGetLastError();
-}
-
 }  // namespace
 
 size_t linear_rows_blocks(size_t n) { return ceil_div(n, (size_t)kRowsOfW); }
 
-hipError_t launch_linear_rows(int type, int by, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream) {
-  if (type == kFloat16) return by == 16 ? launch<kFloat16, 1>(grid, a, s, stream) : launch<kFloat16, 2>(grid, a, s, stream);
-  return by == 16 ? launch<kBfloat16, 1>(grid, a, s, stream) : launch<kBfloat16, 2>(grid, a, s, stream);
+hipError_t launch_linear_rows(int type, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream) {
+  if (type == kFloat16) {
+    linear_rows<kFloat16, kRowsWaves, kRowsChunks><<<grid, 64 * kRowsWaves, 0, stream>>>(a, s);
+  } else {
+    linear_rows<kBfloat16, kRowsWaves, kRowsChunks><<<grid, 64 * kRowsWaves, 0, stream>>>(a, s);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace linear

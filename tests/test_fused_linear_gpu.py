@@ -247,10 +247,10 @@ def test_refusals_of_a_run():
         layer.KernelName(3)
 
 
-@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 32])
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33])
 @pytest.mark.parametrize("N,K", [(1, 1), (15, 31), (16, 32), (17, 33), (40, 255), (33, 1024), (50, 1031), (64, 1800), (100, 2048)])
 def test_few_rows(M, N, K):
-    """What the kernel for a few rows takes: whole steps of K or none, and what is left of it, at even and odd distances."""
+    """The kernel for a few rows: whole steps of K or none, and what is left of it, at even and odd distances."""
     layer = run_layer(M, N, K, VT.bfloat16, ACT.gelu, pitches=(K + M % 3, K + M % 2, N + M % 5), shift=M % 2)
     run_layer(M, N, K, VT.float16, ACT.none, bias=False, residual=False)
-    assert ("linear_rows" in layer.KernelName()) == (M * K <= 65536)
+    assert "linear_rows" in layer.KernelName()
