@@ -22,7 +22,8 @@ SOURCES = ["gemm_mfma_f16_f32.hip", "gemm_mfma_bf16_f32.hip", "gemm_mfma_f16_f16
            "scaled_gemm_e8m0.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_blocks.hip",
            "scaled_gemm_wide_e8m0.hip", "orthogonalize.hip", "quantize.hip", "linear_f16_output.hip",
            "linear_bf16_output.hip", "linear_f16_input.hip", "linear_bf16_input.hip", "linear_f16_weights.hip",
-           "linear_bf16_weights.hip", "linear_rows.hip", "gemm_mfma_int1.hip", "transpose.hip", "combine.hip", "route.hip", "linear.hip",
+           "linear_bf16_weights.hip", "linear_f16_backward.hip",
+           "linear_bf16_backward.hip", "linear_rows.hip", "gemm_mfma_int1.hip", "transpose.hip", "combine.hip", "route.hip", "linear.hip",
            "gemm_int1.hip", "packing.hip", "capi.hip", "operators_capi.hip", "linear_capi.hip", "scaled_gemm.hip",
            "gemm_mfma_dispatch.hip", "host_copy.hip"]
 # Packed-fp32 instruction selection is switched off for all device code.

@@ -24,9 +24,11 @@ struct LinearParams {
   size_t x_pitch, w_pitch, y_pitch;    // elements from row to row: of x and dx; W and dW; y, z, residual, dy
   RealGemmPlan plan[3];                // by Kind
   bool few_rows;                       // y is linear_rows.hip's, else gemm_linear's
-  // the workspace, and where in it (bytes): counters first, which are zero whenever a product starts
+  bool together;                       // dx and dW in one launch, where both are wanted
+  // the workspace, and where in it (bytes): counters first, which are zero whenever a product starts; products that run one after the other
+  // share theirs
   char *workspace;
-  size_t zeroed, partial, dz, sums, tails, bytes;
+  size_t zeroed, counters[3], partial[3], dz, sums, tails, bytes;
 };
 
 // Fills in the plans and the workspace's layout.

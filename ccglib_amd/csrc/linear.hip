@@ -5,7 +5,7 @@
 #include <cmath>
 #include <cstdio>
 
-#include "linear_gemm.h"
+#include "linear_backward.h"
 #include "real_plan.h"
 
 namespace ccglib_amd {
@@ -56,9 +56,16 @@ size_t launched_blocks(const LinearParams &p, int kind, const RealShape &s) {
   return x * (some + (p.m - some) / s.by);
 }
 
-RealGemmPlan plan_product(const LinearParams &p, int kind) {
+// option: REAL_BLOCK. *expected: what it takes, where the shape is given.
+RealGemmPlan plan_product(const LinearParams &p, int kind, size_t option, double *expected = nullptr) {
   const Extents e = extents(p, kind);
-  if (!p.grouped) return plan_real_gemm(kShapes, kShapeCount, 1, e.nx, e.ny, ceil_div(e.k, (size_t)kPiece), false, real_block_option);
+  if (!p.grouped) {
+    const size_t pieces = std::max<size_t>(1, ceil_div(e.k, (size_t)kPiece));
+    const RealGemmPlan plan = plan_real_gemm(kShapes, kShapeCount, 1, e.nx, e.ny, pieces, false, option);
+    const RealShape &shape = kShapes[plan.shape];
+    if (expected) *expected = real_gemm_us(shape, real_blocks(shape, 1, e.nx, e.ny, false), pieces, plan.parts);
+    return plan;
+  }
   // K is not cut: that of kWeights has as many lengths as there are groups, and the other products have blocks of many groups. How
   // many rows each group has is not known here: the mean of what even and uneven groups would take, and of a few blocks more or less, so
   // that no choice hangs on a round of blocks that is just full.
@@ -66,7 +73,7 @@ RealGemmPlan plan_product(const LinearParams &p, int kind) {
   double best = 0.0;
   for (int s = 0; s < kShapeCount; ++s) {
     const RealShape &shape = kShapes[s];
-    if (real_block_option && s != (int)std::min<size_t>(real_block_option % 256 - 1, kShapeCount - 1)) continue;
+    if (option && s != (int)std::min<size_t>(option % 256 - 1, kShapeCount - 1)) continue;
     double us = 0.0;
     for (const bool uneven : {false, true}) {
       double weights = 0.0, blocks = 0.0;
@@ -90,7 +97,32 @@ RealGemmPlan plan_product(const LinearParams &p, int kind) {
       plan.shape = s;
     }
   }
+  if (expected) *expected = best / 8;
   return plan;
+}
+
+// dx and dW in one launch (linear_backward.h): in a shape in which the units hold all blocks of both at once.
+bool plan_together(LinearParams *p) {
+  double best = 0.0;
+  for (int s = 0; s < kShapeCount; ++s) {
+    const RealShape &shape = kShapes[s];
+    const size_t forced = real_block_option ? std::min<size_t>(real_block_option % 256 - 1, kShapeCount - 1) : (size_t)s;
+    if (!backward_in_one(s) || (size_t)s != forced) continue;
+    double us[2];
+    RealGemmPlan plan[2];
+    size_t blocks = 0;
+    for (int i = 0; i < 2; ++i) {
+      plan[i] = plan_product(*p, i ? kWeights : kInput, real_block_option ? real_block_option : (size_t)s + 1, us + i);
+      blocks += launched_blocks(*p, i ? kWeights : kInput, shape) * plan[i].parts;
+    }
+    if (blocks > (size_t)256 * shape.per_unit) continue;
+    const double longer = std::max(us[0], us[1]);
+    if (best > 0.0 && longer >= best) continue;
+    best = longer;
+    p->plan[kInput] = plan[0];
+    p->plan[kWeights] = plan[1];
+  }
+  return best > 0.0;
 }
 
 // Whether y is linear_rows.hip's. Its blocks of 16 x 16 read their operands from the caches again and again, but wait for no ring. us,
@@ -108,10 +140,6 @@ bool plan_few_rows(const LinearParams &p) {
 }
 
 // ---- before the products of the backward pass ----
-
-// Columns and rows of a block. Few rows a block where 64 would leave units idle: a wave's loads are on their way together then (300 x 255:
-// 12.8 us with 64 rows, FIGURE with 16).
-constexpr unsigned kGradientColumns = 512, kFewRows = 16, kManyRows = 64;
 
 template <int TYPE> __device__ __forceinline__ void activation_gradient(int activation, const float (&z)[8], float (&g)[8]) {
 #pragma unroll
@@ -196,38 +224,7 @@ template <int TYPE, unsigned ROWS> __global__ __launch_bounds__(256) void linear
   }
 }
 
-// db (+)= the sums of a group's row blocks, in their order.
-struct JoinArgs {
-  const float *sums;
-  char *db;
-  unsigned n, rows, blocks;      // row blocks that there can be
-  int type, accumulate;
-  const int *offsets;
-  unsigned groups;
-};
-template <unsigned ROWS> __global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
-  const unsigned x = blockIdx.x * 256 + threadIdx.x, group = blockIdx.y;
-  unsigned from = 0, count = (a.rows + ROWS - 1) / ROWS;
-  if (a.offsets) {
-    if (group > 0) from = RowBlocks<ROWS>(a.offsets, group, a.rows).all();
-    count = (span_of(a.offsets, group, a.rows).count + ROWS - 1) / ROWS;
-  }
-  if (x >= a.n) return;
-  if (from > a.blocks) from = a.blocks;      // (offsets that fall: no sums are read that nobody can have written)
-  if (count > a.blocks - from) count = a.blocks - from;
-  float sum = 0.f;
-#pragma unroll 8
-  for (unsigned b = 0; b < count; ++b) sum += a.sums[(size_t)(from + b) * a.n + x];
-  const size_t at = (size_t)group * a.n + x;
-  if (a.type == kFloat32) {
-    float *const db = reinterpret_cast<float *>(a.db) + at;
-    *db = a.accumulate ? *db + sum : sum;
-  } else if (a.type == kFloat16) {
-    reinterpret_cast<_Float16 *>(a.db)[at] = (_Float16)sum;
-  } else {
-    reinterpret_cast<__bf16 *>(a.db)[at] = (__bf16)sum;
-  }
-}
+__global__ __launch_bounds__(256) void join_sums(JoinArgs a) { join(a, blockIdx.x); }
 
 // An operand of a product: an array of 16-bit values.
 struct Operand {
@@ -297,8 +294,8 @@ Args product_args(const LinearParams &p, int kind, const Operand &x, const Opera
   a.parts = plan.parts;
   a.pieces_per_part = plan.pieces_per_part;
   a.rotate = kind != kWeights && 2 * e.ny * e.k <= kStaysInCaches;
-  a.arrived = reinterpret_cast<unsigned *>(p.workspace);
-  a.partial = reinterpret_cast<float *>(p.workspace + p.partial);
+  a.arrived = reinterpret_cast<unsigned *>(p.workspace + p.counters[kind]);
+  a.partial = reinterpret_cast<float *>(p.workspace + p.partial[kind]);
   return a;
 }
 
@@ -338,11 +335,6 @@ template <unsigned ROWS> hipError_t launch_gradient(const LinearParams &p, const
   }
   return hipGetLastError();
 }
-template <unsigned ROWS> hipError_t launch_join(const LinearParams &p, const JoinArgs &j, hipStream_t stream) {
-  join_sums<ROWS><<<dim3((unsigned)ceil_div(p.n, (size_t)256), p.groups), 256, 0, stream>>>(j);
-  return hipGetLastError();
-}
-
 // Blocks of linear_rows.hip: as many as there can be.
 size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, kRowsOfX); }
 
@@ -353,9 +345,22 @@ void plan_linear(LinearParams *p) {
   size_t counters = 0, partial = 0;
   p->few_rows = plan_few_rows(*p);
   for (int kind = p->few_rows ? 1 : 0; kind < kinds; ++kind) {
-    p->plan[kind] = plan_product(*p, kind);
-    counters = std::max(counters, p->plan[kind].counter_bytes);
-    partial = std::max(partial, p->plan[kind].partial_bytes);
+    p->plan[kind] = plan_product(*p, kind, real_block_option);
+  }
+  p->together = p->training && plan_together(p);
+  // (where dW runs beside dx it has counters and sums of its own)
+  size_t apart = 0, apart_partial = 0;
+  for (int kind = 0; kind < kinds; ++kind) {
+    const RealGemmPlan &plan = p->plan[kind];
+    if (kind == kWeights && p->together) {
+      apart = ceil_div(counters, 256) * 256;
+      apart_partial = ceil_div(partial, 256) * 256;
+      counters = apart + plan.counter_bytes;
+      partial = apart_partial + plan.partial_bytes;
+    } else {
+      counters = std::max(counters, plan.counter_bytes);
+      partial = std::max(partial, plan.partial_bytes);
+    }
   }
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -365,7 +370,11 @@ void plan_linear(LinearParams *p) {
   };
   p->zeroed = counters;
   take(counters);
-  p->partial = take(partial);
+  const size_t sums = take(partial);
+  for (int kind = 0; kind < 3; ++kind) {
+    p->counters[kind] = kind == kWeights ? apart : 0;
+    p->partial[kind] = sums + (kind == kWeights ? apart_partial : 0);
+  }
   p->dz = take(p->training && p->activation != kNone ? 2 * (size_t)p->m * dz_pitch(*p) : 0);
   p->sums = take(p->training ? 4 * gradient_blocks(*p) * p->n : 0);
   p->tails = take(3 * kTailBytes);
@@ -447,35 +456,47 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
   } else {
     HIP_PASS(tails.launch(stream));
   }
+  JoinArgs j = {};
+  unsigned joins = 0;
   if (b.dbias && p.n) {
-    JoinArgs j = {};
     j.sums = reinterpret_cast<const float *>(p.workspace + p.sums);
     j.db = static_cast<char *>(b.dbias);
     j.n = p.n;
     j.rows = p.m;
     j.blocks = (unsigned)gradient_blocks(p);
+    j.few = few;
     j.type = p.gradient_type;
     j.accumulate = b.accumulate;
     j.offsets = p.grouped ? b.offsets : nullptr;
     j.groups = p.groups;
-    HIP_PASS(few ? launch_join<kFewRows>(p, j, stream) : launch_join<kManyRows>(p, j, stream));
+    joins = (unsigned)join_workgroups(p.n, p.groups);
   }
-  StoreParams s = {};
-  if (b.dx && p.m && p.k) {
-    s.out = static_cast<char *>(b.dx);
-    s.pitch = p.x_pitch;
-    s.past = 2 * (size_t)p.m * p.k >= kPastCachesBytes;
-    HIP_PASS(launch_product(p, kInput, input, s, stream));
+  StoreParams si = {}, sw = {};
+  si.out = static_cast<char *>(b.dx);
+  si.pitch = p.x_pitch;
+  si.past = 2 * (size_t)p.m * p.k >= kPastCachesBytes;
+  sw.out = static_cast<char *>(b.dw);
+  sw.pitch = p.w_pitch;
+  sw.group = (size_t)p.n * p.w_pitch;
+  sw.wide = p.gradient_type == kFloat32;
+  sw.past = (sw.wide ? 4 : 2) * (size_t)p.groups * p.n * p.k >= kPastCachesBytes;
+  sw.accumulate = b.accumulate;
+  const bool have_dx = b.dx && p.m && p.k, have_dw = b.dw && p.n && p.k;
+  if (p.together && have_dx && have_dw) {
+    BackwardArgs a = {input, weights, si, sw, j, 0, 0};
+    const RealShape &shape = kShapes[p.plan[kInput].shape];
+    a.input_blocks = (unsigned)(launched_blocks(p, kInput, shape) * p.plan[kInput].parts);
+    a.weights_blocks = (unsigned)(launched_blocks(p, kWeights, shape) * p.plan[kWeights].parts);
+    const unsigned grid = a.input_blocks + a.weights_blocks + joins;
+    if (p.type == kFloat16) return launch_backward<kFloat16>(p.plan[kInput].shape, grid, a, stream);
+    return launch_backward<kBfloat16>(p.plan[kInput].shape, grid, a, stream);
   }
-  if (b.dw && p.n && p.k) {
-    s.out = static_cast<char *>(b.dw);
-    s.pitch = p.w_pitch;
-    s.group = (size_t)p.n * p.w_pitch;
-    s.wide = p.gradient_type == kFloat32;
-    s.past = (s.wide ? 4 : 2) * (size_t)p.groups * p.n * p.k >= kPastCachesBytes;
-    s.accumulate = b.accumulate;
-    HIP_PASS(launch_product(p, kWeights, weights, s, stream));
+  if (joins) {
+    join_sums<<<joins, 256, 0, stream>>>(j);
+    HIP_PASS(hipGetLastError());
   }
+  if (have_dx) HIP_PASS(launch_product(p, kInput, input, si, stream));
+  if (have_dw) HIP_PASS(launch_product(p, kWeights, weights, sw, stream));
   return hipSuccess;
 }
 

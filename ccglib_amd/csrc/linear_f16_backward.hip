@@ -1,0 +1,3 @@
+// 16-bit linear layers: the kernels of small backward passes of one type (see linear_backward.h)
+#define CCGLIB_LINEAR_TYPE kFloat16
+#include "linear_backward.h"

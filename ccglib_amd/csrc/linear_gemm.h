@@ -139,7 +139,8 @@ struct Place {
   unsigned group, bx, by, part, tile;
   Span rows;                // the group's
 };
-template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a) {
+// Block `id` of `count` that a launch has for the product.
+template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a, unsigned id, unsigned count) {
   Place p;
   p.none = false;
   p.group = p.part = 0;
@@ -156,11 +157,11 @@ template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a
   if (a.offsets && KIND != kWeights) {
     RowBlocks<BY> blocks(a.offsets, a.groups, a.rows);
     const unsigned all = blocks.all() * a.blocks_x;
-    if (blockIdx.x >= all) {
+    if (id >= all) {
       p.none = true;
       return p;
     }
-    spread(xcd_remap(blockIdx.x, all), blocks.all());
+    spread(xcd_remap(id, all), blocks.all());
     const RowBlock r = blocks.find(p.by);
     p.group = r.group;
     p.by = r.block;
@@ -170,15 +171,15 @@ template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a
   const unsigned per_matrix = a.blocks_x * a.blocks_y;
   if (a.offsets) {
     // (each XCD has an eighth of every group's blocks: groups differ in their rows)
-    p.group = uniform(blockIdx.x / per_matrix);
-    spread(xcd_remap(blockIdx.x - p.group * per_matrix, per_matrix), a.blocks_y);
+    p.group = uniform(id / per_matrix);
+    spread(xcd_remap(id - p.group * per_matrix, per_matrix), a.blocks_y);
     p.rows = span_of(a.offsets, p.group, a.rows);
     p.rows.first = uniform(p.rows.first);
     p.rows.count = uniform(p.rows.count);
   } else {
-    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
-    p.part = uniform(id / per_matrix);
-    spread(id - p.part * per_matrix, a.blocks_y);
+    const unsigned t = xcd_remap(id, count);
+    p.part = uniform(t / per_matrix);
+    spread(t - p.part * per_matrix, a.blocks_y);
   }
   return p;
 }
@@ -314,20 +315,22 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
   }
 }
 
-template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS, int WAVES_PER_EU>
-__global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args args, StoreParams params) {
+template <int BX, int BY, int SLOTS> constexpr int kLdsBytes = SLOTS *(BX + BY) * kPiece * 2;
+
+// Block `id` of `blocks` of a product. lds: kLdsBytes, at a multiple of 256.
+template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS>
+__device__ __forceinline__ void product(const Args &args, const StoreParams &params, char *lds, unsigned id, unsigned blocks) {
   constexpr bool X_ROWS = KIND == kOutput, Y_ROWS = KIND != kWeights;     // k is contiguous
   constexpr int WAVES = WX * WY, TX = BX / WX, TY = BY / WY, NX = TX / 16, NY = TY / 16;
   constexpr int NT = NX % 2 ? 1 : 2, UNIT_X = 32 * NT;
   constexpr int X_BYTES = BX * kPiece * 2, Y_BYTES = BY * kPiece * 2, SLOT_BYTES = X_BYTES + Y_BYTES;
   constexpr int X_COPIES = BX / 8 / WAVES, Y_COPIES = BY / 8 / WAVES, COPIES = X_COPIES + Y_COPIES;
   static_assert(BX / 8 % WAVES == 0 && BY / 8 % WAVES == 0, "a wave's copies are of one operand each");
-  __shared__ __attribute__((aligned(256))) char lds[SLOTS * SLOT_BYTES];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wx = wave % WX, wy = wave / WX;
-  const Place at = place<KIND, BY>(args);
+  const Place at = place<KIND, BY>(args, id, blocks);
   if (at.none) return;
   const unsigned x0 = at.bx * BX, y0 = at.by * BY;
   // rows of Y and length of K that this block's group has
@@ -692,6 +695,12 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
       store_sums<TYPE, KIND, TX % 64 == 0>(params, bias, at.group, Y_ROWS ? at.rows.first + row : row, x, left, v);
     }
   }
+}
+
+template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS, int WAVES_PER_EU>
+__global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args args, StoreParams params) {
+  __shared__ __attribute__((aligned(256))) char lds[kLdsBytes<BX, BY, SLOTS>];
+  product<TYPE, KIND, BX, BY, WX, WY, SLOTS>(args, params, lds, blockIdx.x, gridDim.x);
 }
 
 // Block shapes: BX x BY, waves, ring, waves a SIMD. (128 x 128 with four waves, two blocks to a unit, was nowhere the fastest of 34 problems
