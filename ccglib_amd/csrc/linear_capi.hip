@@ -245,7 +245,7 @@ int ccglib_route_create(ccglib_route_t *route, size_t T, size_t E, size_t k, int
     delete r;
     return s;
   }
-  r->p.counts = static_cast<unsigned *>(r->workspace.p);
+  r->p.counts = static_cast<unsigned short *>(r->workspace.p);
   *route = r;
   return CCGLIB_OK;
 }

@@ -14,7 +14,7 @@ struct RouteParams {
   int type;
   bool normalize;
   unsigned tile, tiles;          // tokens that a block counts, how many such blocks there are (1 at least)
-  unsigned *counts;              // [tiles][experts]; null where there is one tile
+  unsigned short *counts;        // [tiles][experts, in whole quads]; null where there is one tile
 };
 void plan_route(RouteParams *p);
 size_t route_workspace_bytes(const RouteParams &p);

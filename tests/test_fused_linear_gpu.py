@@ -254,3 +254,9 @@ def test_few_rows(M, N, K):
     layer = run_layer(M, N, K, VT.bfloat16, ACT.gelu, pitches=(K + M % 3, K + M % 2, N + M % 5), shift=M % 2)
     run_layer(M, N, K, VT.float16, ACT.none, bias=False, residual=False)
     assert "linear_rows" in layer.KernelName()
+
+
+@pytest.mark.parametrize("M,N,K", [(600, 600, 72), (8, 600, 1030)])
+def test_operands_beyond_32_bits(M, N, K):
+    """Rows 8 MiB apart: 5 GB of W, and of x, y, z and their gradients where there are 600 rows."""
+    run_layer(M, N, K, VT.bfloat16, ACT.gelu, pitches=(1 << 22,) * 3)

@@ -151,3 +151,9 @@ def test_refusals_of_a_run():
         layer.Backward(p, p, p, p, p, p, p, accumulate=True)
     with pytest.raises(RuntimeError, match="without training"):
         cc.GroupedLinear(2, 4, 4, 4, 0, stream(), training=False).Backward(p, p, p, p, p, p, p)
+
+
+@pytest.mark.parametrize("M,K", [(600, 72), (11, 1030)])
+def test_operands_beyond_32_bits(M, K):
+    """Rows 8 MiB apart: 5 GB of W, which experts lie all over."""
+    run_layer(4, M, 150, K, VT.float16, ACT.silu, [0, 3, 5, 9, M], pitches=(1 << 22,) * 3)

@@ -325,3 +325,38 @@ def test_a_captured_fused_layer():
             run()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, (y, dx, dw, db)))
+
+
+def test_the_most_tokens():
+    """2^24 - 1 rows of 300 logits, more of them than 32 bits count, in more tiles than otherwise, since 16 bits count a tile's rows of an
+    expert. Logits are a row's permutation of 0 to 299, so that all answers are known: 37 e + t = 299 or 298 modulo 300, 37 * 73 = 1."""
+    T, E, k = (1 << 24) - 1, 300, 2
+    logits = torch.empty((T, E), dtype=torch.float16, device="cuda")
+    rows, step = torch.arange(T, device="cuda"), 1 << 20
+    for at in range(0, T, step):
+        logits[at:at + step] = (rows[at:at + step, None].int() + 37 * torch.arange(E, device="cuda", dtype=torch.int32)) % E
+    experts, slots = (torch.full((T, k), -1, dtype=torch.int32, device="cuda") for _ in range(2))
+    weights, offsets = torch.full((T, k), math.nan, device="cuda"), torch.full((E + 1,), -1, dtype=torch.int32, device="cuda")
+    route = cc.Route(T, E, k, 0, stream(), VT.float16)
+    route.Run(logits.data_ptr(), experts.data_ptr(), weights.data_ptr(), offsets.data_ptr(), slots.data_ptr())
+    want = torch.stack([(E - 1 - rows) * 73 % E, (E - 2 - rows) * 73 % E], dim=1)
+    assert torch.equal(experts.long(), want)
+    assert torch.equal(offsets[1:].long(), torch.bincount(want.flatten(), minlength=E).cumsum(0)) and int(offsets[0]) == 0
+    order = torch.sort(want.flatten(), stable=True).indices
+    assert torch.equal(slots.flatten()[order].long(), torch.arange(T * k, device="cuda"))
+    p = 1 / (1 + math.exp(-1.0))
+    error = (88 + 8 + E) * 2.0 ** -23                       # (as check_route's)
+    assert float((weights.double() - torch.tensor([p, 1 - p], dtype=torch.float64, device="cuda")).abs().max()) <= error
+    dweights = torch.tensor([3.0, -1.0], device="cuda").repeat(T, 1)
+    dlogits = logits.fill_(math.nan)                        # (logits are not read where the weights are of the chosen alone)
+    route.Backward(0, experts.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
+    size = p * (1 - p) * 4.0                                # w_0 (dw_0 - (w_0 dw_0 + w_1 dw_1)), and the second is its opposite
+    for at in range(0, T, step):
+        full = torch.zeros((min(step, T - at), E), dtype=torch.float64, device="cuda")
+        full.scatter_(1, want[at:at + step], torch.tensor([size, -size], dtype=torch.float64, device="cuda").repeat(len(full), 1))
+        assert float((dlogits[at:at + step].double() - full).abs().max()) <= 8 * error + 2.0 ** -11 * size
+
+
+def test_combine_beyond_32_bits():
+    """Rows 8 MiB apart, 5 GB of each operand."""
+    run_combine(600, 1, 40, VT.bfloat16, 610, True, 1 << 22, 1 << 22, holes=True)
