@@ -117,7 +117,7 @@ def main():
     parser.add_argument("--experts", type=int, default=16)
     parser.add_argument("--chosen", type=int, default=2)
     parser.add_argument("--batch", type=int, default=4096)
-    parser.add_argument("--steps", type=int, default=1.0)
+    parser.add_argument("--steps", type=int, default=200)
     parser.add_argument("--rate", type=float, default=1.0)
     parser.add_argument("--report", type=int, default=40)
     args = parser.parse_args()
