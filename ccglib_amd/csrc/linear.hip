@@ -242,17 +242,16 @@ class Tails {
     if (!loose || (!strided && k >= 8) || o.rows == 0 || o.columns == 0) return {};
     const size_t values = (o.rows - 1) * o.pitch + o.columns;
     const char *const end = static_cast<const char *>(o.p) + 2 * values;
-    char *to = nullptr;
-    for (int i = 0; i < count_; ++i) {
-      if (reinterpret_cast<const char *>(args_.end[i]) == end) to = reinterpret_cast<char *>(args_.to[i]);
-    }
-    if (!to) {
-      to = memory_ + count_ * kTailBytes;
-      args_.end[count_] = reinterpret_cast<const unsigned short *>(end);
-      args_.to[count_] = reinterpret_cast<unsigned short *>(to);
-      args_.have[count_] = (unsigned)std::min<size_t>(16, values);
+    int i = 0;
+    while (i < count_ && reinterpret_cast<const char *>(args_.end[i]) != end) ++i;
+    char *const to = memory_ + i * kTailBytes;
+    if (i == count_) {
+      args_.end[i] = reinterpret_cast<const unsigned short *>(end);
+      args_.to[i] = reinterpret_cast<unsigned short *>(to);
       ++count_;
     }
+    // (operands may end together and start apart: W may be a row of x)
+    args_.have[i] = std::max(args_.have[i], (unsigned)std::min<size_t>(16, values));
     return {to, end};
   }
   const TailArgs &args() const { return args_; }

@@ -445,6 +445,8 @@ CCGLIB_API int ccglib_orthogonalize_destroy(ccglib_orthogonalize_t orthogonalize
  * Buffers start at a multiple of their element; rows whose distance and start
  * are multiples of 16 bytes are the fast ones. Outputs lie apart from all inputs,
  * but y may be the residual.
+ * FusedLinear, GroupedLinear and Route hold scratch memory, so that the calls of
+ * one object, and graphs captured of them, run one after the other.
  * ---------------------------------------------------------------------- */
 /* act(z): z; max(z, 0); z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); z / (1 + e^-z) */
 enum { CCGLIB_ACTIVATION_NONE = 0, CCGLIB_ACTIVATION_RELU = 1, CCGLIB_ACTIVATION_GELU = 2, CCGLIB_ACTIVATION_SILU = 3 };
@@ -481,7 +483,8 @@ CCGLIB_API int ccglib_fused_linear_destroy(ccglib_fused_linear_t linear);
  * are sorted by expert: rows offsets[e] to offsets[e + 1] - 1 are multiplied
  * with W[e]. offsets is device memory, E + 1 int32 that do not fall (what lies outside 0 to M counts
  * as the nearer end); an expert may have no rows, whose dW and dbias are zero then.
- * Rows in front of offsets[0] and from offsets[E] on are neither read nor written. 1 to 1024 experts. */
+ * Rows in front of offsets[0] and from offsets[E] on are neither read nor written. (Offsets that fall leave
+ * results unspecified, of these M rows and E experts only.) 1 to 1024 experts. */
 CCGLIB_API int ccglib_grouped_linear_create(ccglib_grouped_linear_t *linear, size_t E, size_t M, size_t N, size_t K, int device,
                                             void *stream, int type, int activation, int gradient_type, int training,
                                             size_t x_pitch, size_t w_pitch, size_t y_pitch);

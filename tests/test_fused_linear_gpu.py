@@ -260,3 +260,18 @@ def test_few_rows(M, N, K):
 def test_operands_beyond_32_bits(M, N, K):
     """Rows 8 MiB apart: 5 GB of W, and of x, y, z and their gradients where there are 600 rows."""
     run_layer(M, N, K, VT.bfloat16, ACT.gelu, pitches=(1 << 22,) * 3)
+
+
+def test_weights_that_are_the_last_row_of_x():
+    """The two end together and are of different lengths. Small whole numbers: sums are exact."""
+    M, N, K = 3, 1, 2
+    x = torch.tensor([[1, 2], [3, 4], [5, 6]], dtype=torch.bfloat16, device="cuda")
+    dy = torch.tensor([[1], [10], [100]], dtype=torch.bfloat16, device="cuda")
+    y, dx, dw = torch.empty_like(dy), torch.empty_like(x), torch.empty((N, K), device="cuda")
+    layer = cc.FusedLinear(M, N, K, 0, stream())
+    w = x.data_ptr() + 2 * (M - 1) * K
+    layer.Forward(x.data_ptr(), w, 0, 0, y.data_ptr())
+    layer.Backward(dy.data_ptr(), 0, x.data_ptr(), w, dx.data_ptr(), dw.data_ptr())
+    torch.cuda.synchronize()
+    assert y.flatten().tolist() == [17, 39, 61]
+    assert dx.tolist() == [[5, 6], [50, 60], [500, 600]] and dw.tolist() == [[531, 642]]
