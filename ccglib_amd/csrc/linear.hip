@@ -21,8 +21,10 @@ constexpr RealShape kShapes[] = {{256, 256, 512, 1, 0.99f, 1.82f, 8.2f, 0.97f, "
                                  {64, 32, 256, 2, 0.26f, 0.49f, 4.7f, 4.1f, "32x64"},
                                  {128, 128, 512, 1, 0.395f, 0.57f, 6.4f, 1.33f, "128x128"},
                                  {192, 192, 512, 1, 0.615f, 1.01f, 8.7f, 0.83f, "192x192"},
-                                 {128, 256, 512, 1, 0.55f, 0.97f, 7.5f, 0.82f, "256x128"}};
-constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
+                                 {128, 256, 512, 1, 0.55f, 0.97f, 7.5f, 0.82f, "256x128"},
+                                 {256, 256, 512, 1, 0.99f, 1.82f, 8.2f, 0.97f, "256x256 (the last ones cut)"}};
+constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0], kWholeShapes = kShapeCount - 1;
+static_assert(kWholeShapes == kCutShape, "the last of them");
 #define CCGLIB_SAME(ID, BX, BY, WX, WY, SLOTS, EU) \
   static_assert(kShapes[ID].bx == BX && kShapes[ID].by == BY && kShapes[ID].threads == 64 * WX * WY, \
                 "the table is in the order of the shapes");
@@ -47,23 +49,51 @@ Extents extents(const LinearParams &p, int kind) {
 
 // Blocks that a product is launched with: where rows are grouped, as many as there can be however they are (a group's
 // last block may hold one row).
-size_t launched_blocks(const LinearParams &p, int kind, const RealShape &s) {
+size_t launched_blocks(const LinearParams &p, int kind, int shape) {
+  const RealShape &s = kShapes[shape];
   const Extents e = extents(p, kind);
   const size_t x = ceil_div(e.nx, s.bx);
-  if (!p.grouped) return x * ceil_div(e.ny, s.by);
+  if (!p.grouped) {
+    const size_t blocks = x * ceil_div(e.ny, s.by);
+    if (shape != kCutShape) return blocks;
+    const LastRound last = last_round((unsigned)(blocks % kUnits));
+    return blocks + (size_t)last.blocks * (last.cut - 1);
+  }
   if (kind == kWeights) return p.groups * x * ceil_div(e.ny, s.by);
   const size_t some = std::min<size_t>(p.groups, p.m);      // (groups that have rows)
-  return x * (some + (p.m - some) / s.by);
+  return x * (some + (p.m - some) / s.by) + (shape == kCutShape ? kMostCut : 0);
 }
+
+// Microseconds of a product with K in one part.
+double product_us(int shape, size_t blocks, size_t pieces) {
+  blocks = std::max<size_t>(1, blocks);
+  pieces = std::max<size_t>(1, pieces);
+  if (shape != kCutShape) return real_gemm_us(kShapes[shape], blocks, pieces, 1);
+  const LastRound last = last_round((unsigned)(blocks % kUnits));
+  if (last.cut == 1) return real_gemm_us(kShapes[shape], blocks, pieces, 1);
+  return real_gemm_us(kShapes[shape], blocks - last.blocks, pieces, 1) +
+         real_gemm_us(kShapes[last.cut == 2 ? 5 : 3], (size_t)last.blocks * last.cut, pieces, 1);
+}
+// The shape that REAL_BLOCK asks for
+int shape_of(size_t option) { return (int)std::min<size_t>(option % 256 - 1, kShapeCount - 1); }
 
 // option: REAL_BLOCK. *expected: what it takes, where the shape is given.
 RealGemmPlan plan_product(const LinearParams &p, int kind, size_t option, double *expected = nullptr) {
   const Extents e = extents(p, kind);
   if (!p.grouped) {
     const size_t pieces = std::max<size_t>(1, ceil_div(e.k, (size_t)kPiece));
-    const RealGemmPlan plan = plan_real_gemm(kShapes, kShapeCount, 1, e.nx, e.ny, pieces, false, option);
+    RealGemmPlan plan = plan_real_gemm(kShapes, kWholeShapes, 1, e.nx, e.ny, pieces, false, option);
     const RealShape &shape = kShapes[plan.shape];
-    if (expected) *expected = real_gemm_us(shape, real_blocks(shape, 1, e.nx, e.ny, false), pieces, plan.parts);
+    const double us = real_gemm_us(shape, real_blocks(shape, 1, e.nx, e.ny, false), pieces, plan.parts);
+    if (expected) *expected = us;
+    const RealShape &cut = kShapes[kCutShape];
+    const size_t blocks = real_blocks(cut, 1, e.nx, e.ny, false);
+    if (option ? shape_of(option) == kCutShape : product_us(kCutShape, blocks, pieces) < us && real_launches(cut, blocks + kMostCut)) {
+      plan = {};
+      plan.shape = kCutShape;
+      plan.parts = 1;
+      plan.pieces_per_part = (unsigned)pieces;
+    }
     return plan;
   }
   // K is not cut: that of kWeights has as many lengths as there are groups, and the other products have blocks of many groups. How
@@ -73,7 +103,8 @@ RealGemmPlan plan_product(const LinearParams &p, int kind, size_t option, double
   double best = 0.0;
   for (int s = 0; s < kShapeCount; ++s) {
     const RealShape &shape = kShapes[s];
-    if (option && s != (int)std::min<size_t>(option % 256 - 1, kShapeCount - 1)) continue;
+    if (s == kCutShape && kind == kWeights) continue;      // (whose blocks take as long as their group's rows are many)
+    if (option && s != (kind == kWeights && shape_of(option) == kCutShape ? 0 : shape_of(option))) continue;
     double us = 0.0;
     for (const bool uneven : {false, true}) {
       double weights = 0.0, blocks = 0.0;
@@ -89,7 +120,7 @@ RealGemmPlan plan_product(const LinearParams &p, int kind, size_t option, double
       blocks *= (double)ceil_div(e.nx, shape.bx);
       const size_t pieces = kind == kWeights ? ceil_div((size_t)p.m, (size_t)p.groups * kPiece) : ceil_div(e.k, (size_t)kPiece);
       for (const double more : {0.95, 1.0, 1.05, 1.1}) {      // (those of kWeights are known)
-        us += real_gemm_us(shape, std::max<size_t>(1, (size_t)(kind == kWeights ? blocks : blocks * more)), std::max<size_t>(1, pieces), 1);
+        us += product_us(s, (size_t)(kind == kWeights ? blocks : blocks * more), pieces);
       }
     }
     if (best == 0.0 || us < best) {
@@ -105,17 +136,15 @@ RealGemmPlan plan_product(const LinearParams &p, int kind, size_t option, double
 bool plan_together(LinearParams *p) {
   double best = 0.0;
   for (int s = 0; s < kShapeCount; ++s) {
-    const RealShape &shape = kShapes[s];
-    const size_t forced = real_block_option ? std::min<size_t>(real_block_option % 256 - 1, kShapeCount - 1) : (size_t)s;
-    if (!backward_in_one(s) || (size_t)s != forced) continue;
+    if (!backward_in_one(s) || (real_block_option && s != shape_of(real_block_option))) continue;
     double us[2];
     RealGemmPlan plan[2];
     size_t blocks = 0;
     for (int i = 0; i < 2; ++i) {
       plan[i] = plan_product(*p, i ? kWeights : kInput, real_block_option ? real_block_option : (size_t)s + 1, us + i);
-      blocks += launched_blocks(*p, i ? kWeights : kInput, shape) * plan[i].parts;
+      blocks += launched_blocks(*p, i ? kWeights : kInput, s) * plan[i].parts;
     }
-    if (blocks > (size_t)256 * shape.per_unit) continue;
+    if (blocks > (size_t)kUnits * kShapes[s].per_unit) continue;
     const double longer = std::max(us[0], us[1]);
     if (best > 0.0 && longer >= best) continue;
     best = longer;
@@ -300,7 +329,7 @@ Args product_args(const LinearParams &p, int kind, const Operand &x, const Opera
 
 hipError_t launch_product(const LinearParams &p, int kind, const Args &a, const StoreParams &s, hipStream_t stream) {
   const RealGemmPlan &plan = p.plan[kind];
-  const unsigned grid = (unsigned)(launched_blocks(p, kind, kShapes[plan.shape]) * plan.parts);
+  const unsigned grid = (unsigned)(launched_blocks(p, kind, plan.shape) * plan.parts);
   if (grid == 0) return hipSuccess;
   if (p.type == kFloat16) {
     if (kind == kOutput) return launch_gemm<kFloat16, kOutput>(plan.shape, grid, a, s, stream);
@@ -383,8 +412,8 @@ void plan_linear(LinearParams *p) {
 bool linear_launches(const LinearParams &p) {
   if (p.few_rows && few_rows_blocks(p) > 0xffffffffu / 256) return false;
   for (int kind = p.few_rows ? 1 : 0; kind < (p.training ? 3 : 1); ++kind) {
-    const RealShape &s = kShapes[p.plan[kind].shape];
-    if (!real_launches(s, launched_blocks(p, kind, s) * p.plan[kind].parts)) return false;
+    const int shape = p.plan[kind].shape;
+    if (!real_launches(kShapes[shape], launched_blocks(p, kind, shape) * p.plan[kind].parts)) return false;
   }
   if (!p.training) return true;
   // (blocks of rows are a grid's second axis, groups too)
@@ -483,12 +512,12 @@ hipError_t launch_linear_backward(const LinearParams &p, const LinearBackward &b
   const bool have_dx = b.dx && p.m && p.k, have_dw = b.dw && p.n && p.k;
   if (p.together && have_dx && have_dw) {
     BackwardArgs a = {input, weights, si, sw, j, 0, 0};
-    const RealShape &shape = kShapes[p.plan[kInput].shape];
+    const int shape = p.plan[kInput].shape;
     a.input_blocks = (unsigned)(launched_blocks(p, kInput, shape) * p.plan[kInput].parts);
     a.weights_blocks = (unsigned)(launched_blocks(p, kWeights, shape) * p.plan[kWeights].parts);
     const unsigned grid = a.input_blocks + a.weights_blocks + joins;
-    if (p.type == kFloat16) return launch_backward<kFloat16>(p.plan[kInput].shape, grid, a, stream);
-    return launch_backward<kBfloat16>(p.plan[kInput].shape, grid, a, stream);
+    if (p.type == kFloat16) return launch_backward<kFloat16>(shape, grid, a, stream);
+    return launch_backward<kBfloat16>(shape, grid, a, stream);
   }
   if (joins) {
     join_sums<<<joins, 256, 0, stream>>>(j);

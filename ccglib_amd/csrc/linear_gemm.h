@@ -138,12 +138,28 @@ struct Place {
   bool none;
   unsigned group, bx, by, part, tile;
   Span rows;                // the group's
+  unsigned cut, piece;      // the workgroup has one of `cut` pieces of the block
 };
-// Block `id` of `count` that a launch has for the product.
-template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a, unsigned id, unsigned count) {
+
+// Blocks of the last round, where they are so few that the units hold two or four pieces of each of them: how many, and what they are
+// cut into (gemm_linear_cut).
+constexpr unsigned kUnits = 256;
+struct LastRound {
+  unsigned blocks, cut;
+};
+__host__ __device__ __forceinline__ LastRound last_round(unsigned blocks) {
+  const unsigned rest = blocks % kUnits;
+  return {rest, rest > kUnits / 2 ? 1u : rest > kUnits / 4 ? 2u : 4u};
+}
+// More workgroups than blocks, at most
+constexpr unsigned kMostCut = 3 * kUnits / 4;
+
+// Block `id` of `count` that a launch has for the product. CUT: the last round's blocks are cut.
+template <int KIND, int BY, bool CUT> __device__ __forceinline__ Place place(const Args &a, unsigned id, unsigned count) {
   Place p;
   p.none = false;
-  p.group = p.part = 0;
+  p.group = p.part = p.piece = 0;
+  p.cut = 1;
   p.rows = {0, a.rows};
   // groups of four block rows, y fastest: the blocks that an XCD works on at one time share rows of X and of Y
   auto spread = [&](unsigned t, unsigned blocks_y) {
@@ -154,14 +170,31 @@ template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a
     p.bx = uniform(in / rows);
     p.tile = uniform(t);
   };
+  // Which of all blocks, in the order of the XCDs
+  auto order = [&](unsigned all) {
+    if constexpr (CUT) {
+      const LastRound last = last_round(all);
+      const unsigned whole = all - last.blocks;
+      if (id >= whole) {
+        if (id - whole >= last.blocks * last.cut) return all;
+        const unsigned n = xcd_remap(id - whole, last.blocks * last.cut);
+        p.cut = uniform(last.cut);
+        p.piece = uniform(n % last.cut);
+        return whole + n / last.cut;
+      }
+      return xcd_remap(id, whole);
+    }
+    return id < all ? xcd_remap(id, all) : all;
+  };
   if (a.offsets && KIND != kWeights) {
     RowBlocks<BY> blocks(a.offsets, a.groups, a.rows);
     const unsigned all = blocks.all() * a.blocks_x;
-    if (id >= all) {
+    const unsigned t = order(all);
+    if (t >= all) {
       p.none = true;
       return p;
     }
-    spread(xcd_remap(id, all), blocks.all());
+    spread(t, blocks.all());
     const RowBlock r = blocks.find(p.by);
     p.group = r.group;
     p.by = r.block;
@@ -177,7 +210,7 @@ template <int KIND, int BY> __device__ __forceinline__ Place place(const Args &a
     p.rows.first = uniform(p.rows.first);
     p.rows.count = uniform(p.rows.count);
   } else {
-    const unsigned t = xcd_remap(id, count);
+    const unsigned t = order(CUT ? per_matrix : count);
     p.part = uniform(t / per_matrix);
     spread(t - p.part * per_matrix, a.blocks_y);
   }
@@ -317,9 +350,10 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
 
 template <int BX, int BY, int SLOTS> constexpr int kLdsBytes = SLOTS *(BX + BY) * kPiece * 2;
 
-// Block `id` of `blocks` of a product. lds: kLdsBytes, at a multiple of 256.
+// The block of D from x0, y0 on. lds: kLdsBytes, at a multiple of 256.
 template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS>
-__device__ __forceinline__ void product(const Args &args, const StoreParams &params, char *lds, unsigned id, unsigned blocks) {
+__device__ __forceinline__ void product_at(const Args &args, const StoreParams &params, char *lds, const Place &at, unsigned x0,
+                                           unsigned y0) {
   constexpr bool X_ROWS = KIND == kOutput, Y_ROWS = KIND != kWeights;     // k is contiguous
   constexpr int WAVES = WX * WY, TX = BX / WX, TY = BY / WY, NX = TX / 16, NY = TY / 16;
   constexpr int NT = NX % 2 ? 1 : 2, UNIT_X = 32 * NT;
@@ -330,9 +364,6 @@ __device__ __forceinline__ void product(const Args &args, const StoreParams &par
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wx = wave % WX, wy = wave / WX;
-  const Place at = place<KIND, BY>(args, id, blocks);
-  if (at.none) return;
-  const unsigned x0 = at.bx * BX, y0 = at.by * BY;
   // rows of Y and length of K that this block's group has
   const unsigned ny = Y_ROWS && args.offsets ? at.rows.count : args.ny;
   const unsigned k_all = !Y_ROWS && args.offsets ? at.rows.count : args.k;
@@ -697,10 +728,39 @@ __device__ __forceinline__ void product(const Args &args, const StoreParams &par
   }
 }
 
+// Block `id` of `blocks` of a product.
+template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS>
+__device__ __forceinline__ void product(const Args &args, const StoreParams &params, char *lds, unsigned id, unsigned blocks) {
+  const Place at = place<KIND, BY, false>(args, id, blocks);
+  if (!at.none) product_at<TYPE, KIND, BX, BY, WX, WY, SLOTS>(args, params, lds, at, at.bx * BX, at.by * BY);
+}
+
 template <int TYPE, int KIND, int BX, int BY, int WX, int WY, int SLOTS, int WAVES_PER_EU>
 __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args args, StoreParams params) {
   __shared__ __attribute__((aligned(256))) char lds[kLdsBytes<BX, BY, SLOTS>];
   product<TYPE, KIND, BX, BY, WX, WY, SLOTS>(args, params, lds, blockIdx.x, gridDim.x);
+}
+
+// 256 x 256 blocks whose last round, if it leaves half of the units idle, is one of 128 x 256 or 128 x 128 pieces. K is not cut, and rows
+// of groups are not its length.
+template <int TYPE, int KIND> __global__ __launch_bounds__(512, 2) void gemm_linear_cut(Args args, StoreParams params) {
+  __shared__ __attribute__((aligned(256))) char lds[kLdsBytes<128, 256, 3>];
+  static_assert(kLdsBytes<256, 256, 2> <= sizeof lds && kLdsBytes<128, 128, 4> <= sizeof lds, "one after the other");
+  const Place at = place<KIND, 256, true>(args, blockIdx.x, gridDim.x);
+  if (at.none) return;
+  unsigned x0 = at.bx * 256, y0 = at.by * 256;
+  if (at.cut == 1) {
+    product_at<TYPE, KIND, 256, 256, 2, 4, 2>(args, params, lds, at, x0, y0);
+    return;
+  }
+  x0 += at.piece % 2 * 128;
+  y0 += at.piece / 2 * 128;
+  if (x0 >= args.nx || y0 >= (KIND != kWeights && args.offsets ? at.rows.count : args.ny)) return;
+  if (at.cut == 2) {
+    product_at<TYPE, KIND, 128, 256, 2, 4, 3>(args, params, lds, at, x0, y0);
+  } else {
+    product_at<TYPE, KIND, 128, 128, 4, 2, 4>(args, params, lds, at, x0, y0);
+  }
 }
 
 // Block shapes: BX x BY, waves, ring, waves a SIMD. (128 x 128 with four waves, two blocks to a unit, was nowhere the fastest of 34 problems
@@ -712,6 +772,7 @@ __global__ __launch_bounds__(64 * WX * WY, WAVES_PER_EU) void gemm_linear(Args a
   DO(3, 128, 128, 4, 2, 4, 2)    \
   DO(4, 192, 192, 4, 2, 3, 2)    \
   DO(5, 128, 256, 2, 4, 3, 2)
+constexpr int kCutShape = 6;   // gemm_linear_cut
 
 template <int TYPE, int KIND> hipError_t launch_gemm(int shape, unsigned grid, const Args &a, const StoreParams &s, hipStream_t stream);
 #define CCGLIB_DECLARE(TYPE, KIND) \
@@ -740,6 +801,9 @@ hipError_t launch_gemm<CCGLIB_LINEAR_TYPE, CCGLIB_LINEAR_KIND>(int shape, unsign
     break;
     CCGLIB_LINEAR_SHAPES(CCGLIB_CASE)
 #undef CCGLIB_CASE
+  case kCutShape:
+    gemm_linear_cut<CCGLIB_LINEAR_TYPE, CCGLIB_LINEAR_KIND><<<grid, 512, 0, stream>>>(a, s);
+    break;
   }
   return hipGetLastError();
 }

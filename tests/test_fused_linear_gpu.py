@@ -275,3 +275,22 @@ def test_weights_that_are_the_last_row_of_x():
     torch.cuda.synchronize()
     assert y.flatten().tolist() == [17, 39, 61]
     assert dx.tolist() == [[5, 6], [50, 60], [500, 600]] and dw.tolist() == [[531, 642]]
+
+
+@pytest.mark.parametrize("t", list(HALF))
+@pytest.mark.parametrize("rows,columns,rest", [(4000, 5100, 64), (3900, 6100, 128), (5000, 6100, 224), (200, 1500, 6)])
+def test_a_last_round_of_cut_blocks(t, rows, columns, rest):
+    """Blocks of 256 x 256 in rounds of 256, those of the last one whole, in halves or in quarters; of all three products in turn."""
+    assert -(-rows // 256) * -(-columns // 256) % 256 == rest
+    with cc.option(cc.Option.real_block, 7):
+        for M, N, K in ((rows, columns, 72), (rows, 37, columns), (100, rows, columns)):
+            layer = run_layer(M, N, K, t, ACT.silu)
+            assert all("cut" in layer.KernelName(product) for product in range(3))
+        run_layer(70, 255, 577, t, ACT.gelu, pitches=(579, 581, 257), shift=1)
+
+
+@pytest.mark.parametrize("K", [1, 7, 8, 9, 63, 64, 65, 127, 128, 129, 191, 200, 320, 333])
+def test_every_length_of_the_sum_in_cut_blocks(K):
+    with cc.option(cc.Option.real_block, 7):
+        run_layer(260, 300, K, VT.bfloat16, ACT.none)
+        run_layer(130, K, 520, VT.float16, ACT.none)

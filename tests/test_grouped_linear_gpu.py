@@ -157,3 +157,13 @@ def test_refusals_of_a_run():
 def test_operands_beyond_32_bits(M, K):
     """Rows 8 MiB apart: 5 GB of W, which experts lie all over."""
     run_layer(4, M, 150, K, VT.float16, ACT.silu, [0, 3, 5, 9, M], pitches=(1 << 22,) * 3)
+
+
+@pytest.mark.parametrize("spans", list(SPANS))
+@pytest.mark.parametrize("M,N,K", [(4000, 5100, 72), (3900, 40, 6100), (300, 520, 200)])
+def test_a_last_round_of_cut_blocks(spans, M, N, K):
+    """How many blocks there are is known to the kernel alone."""
+    with cc.option(cc.Option.real_block, 7):
+        layer = run_layer(3, M, N, K, VT.bfloat16, ACT.silu, SPANS[spans](M, 3))
+        assert ["cut" in layer.KernelName(product) for product in range(3)] == [True, True, False]
+        run_layer(3, 70, 255, 577, VT.float16, ACT.gelu, [0, 30, 31, 70], pitches=(579, 581, 257), shift=1)
