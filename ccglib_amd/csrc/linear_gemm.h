@@ -133,6 +133,27 @@ template <int BY> class RowBlocks {
   Span mine_;
 };
 
+// The group that is `nth` if those with many rows go first, in five classes of their number: dW's blocks take as long as their group's rows are many, and
+// a long one that begins last keeps the others waiting (us, as they come and like this: 16384 rows, up to 3224 of a group, over 8 of 2048 x 2048
+// 149 and 133; 4096, up to 395, over 32 of 1024 x 2048 73 and 68; 8192, up to 585, over 64 of 2048 x 1024 163 and 151; of 15 such cases the
+// mean is 0.97, the worst 1.02). Beyond 64 groups each of them is a small part of the whole: as they come.
+__device__ __forceinline__ unsigned by_length(const Args &a, unsigned nth) {
+  if (a.groups > 64) return nth;
+  const unsigned lane = threadIdx.x & 63;
+  const bool have = lane < a.groups;
+  const float times = have ? (float)span_of(a.offsets, lane, a.rows).count * (float)a.groups / (float)a.rows : 0.f;   // the mean's
+  const int mine = times >= 4.f ? 0 : times >= 2.f ? 1 : times >= 1.f ? 2 : times >= 0.5f ? 3 : 4;
+  unsigned long long these = 0;
+  for (int c = 0; c < 5; ++c) {
+    these = __ballot(have && mine == c);
+    const unsigned n = (unsigned)__popcll(these);
+    if (nth < n) break;
+    nth -= n;
+  }
+  for (; nth > 0; --nth) these &= these - 1;
+  return uniform((unsigned)__builtin_ctzll(these));
+}
+
 // Which part of D a workgroup has.
 struct Place {
   bool none;
@@ -204,8 +225,9 @@ template <int KIND, int BY, bool CUT> __device__ __forceinline__ Place place(con
   const unsigned per_matrix = a.blocks_x * a.blocks_y;
   if (a.offsets) {
     // (each XCD has an eighth of every group's blocks: groups differ in their rows)
-    p.group = uniform(id / per_matrix);
-    spread(xcd_remap(id - p.group * per_matrix, per_matrix), a.blocks_y);
+    const unsigned nth = uniform(id / per_matrix);
+    p.group = by_length(a, nth);
+    spread(xcd_remap(id - nth * per_matrix, per_matrix), a.blocks_y);
     p.rows = span_of(a.offsets, p.group, a.rows);
     p.rows.first = uniform(p.rows.first);
     p.rows.count = uniform(p.rows.count);
@@ -345,6 +367,33 @@ __device__ __forceinline__ void store_sums(const StoreParams &p, const float (&b
       }
       store_row(LINES && p.past, out, left, v);
     }
+  }
+}
+
+// The same for 32 bits of dW in 32 columns that are all inside, x the first of the lane's first four: lanes 16 apart hold 8 neighbours each, and
+// exchange them so that a store writes 64 bytes of a row in one piece, not 16 of each 32. 256 x 256 blocks, us: 512 rows over 16
+// experts of 4096 x 4096 472 and 222 (1 GiB), 8192 rows over 64 of 2048 x 1024 213 and 158, 2048 x 8192 x 8192 262 and 235. (Waves
+// of 64 columns lose as often as they gain: 32 of 1024 x 2048 78 and 97, 16 of 4096 x 4096 429 and 243, 2048 x 8192 x 8192 272 and 289. Whole lines by one store
+// more: nothing gained, and 10 to 20 % lost where old values are added to.)
+template <bool LINES>
+__device__ __forceinline__ void store_wide(const StoreParams &p, unsigned group, unsigned y, unsigned x, float4_t a, float4_t b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float lower = a[e], upper = b[e];
+    const auto rows = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, lower), __builtin_bit_cast(unsigned, upper), false, false);
+    const auto halves = __builtin_amdgcn_permlane32_swap(rows[0], rows[1], false, false);
+    const unsigned first = halves[0], second = halves[1];
+    a[e] = __builtin_bit_cast(float, first);
+    b[e] = __builtin_bit_cast(float, second);
+  }
+  float *const out = reinterpret_cast<float *>(p.out) + (size_t)group * p.group + (size_t)y * p.pitch + x;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[4], old[4] = {};
+    if (p.accumulate) load_row(out + h * 16, 4, old);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (h ? b : a)[e] + old[e];
+    store_row(LINES && p.past, out + h * 16, 4, v);
   }
 }
 
@@ -706,6 +755,18 @@ __device__ __forceinline__ void product_at(const Args &args, const StoreParams &
   constexpr int N = 4 * NT;
 #pragma unroll
   for (int i = 0; i < NX; i += NT) {
+    if constexpr (KIND == kWeights && NT == 2 && TX != 64) {
+      const unsigned x = x0 + wx * TX + i * 16;
+      if (params.wide && x + 32 <= args.nx) {
+        CCGLIB_PIN;
+#pragma unroll
+        for (int j = 0; j < NY; ++j) {
+          const unsigned row = y0 + wy * TY + j * 16 + fr;
+          if (row < ny) store_wide<TX % 64 == 0>(params, at.group, row, x + g * 4, acc[j][i], acc[j][i + 1]);
+        }
+        continue;
+      }
+    }
     const unsigned x = x0 + wx * TX + i * 16 + g * N, left = x < args.nx ? args.nx - x : 0;
     CCGLIB_PIN;      // (one tile's loads at a time: all of them at once take more registers than there are)
     if (left == 0) continue;

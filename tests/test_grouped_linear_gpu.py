@@ -167,3 +167,14 @@ def test_a_last_round_of_cut_blocks(spans, M, N, K):
         layer = run_layer(3, M, N, K, VT.bfloat16, ACT.silu, SPANS[spans](M, 3))
         assert ["cut" in layer.KernelName(product) for product in range(3)] == [True, True, False]
         run_layer(3, 70, 255, 577, VT.float16, ACT.gelu, [0, 30, 31, 70], pitches=(579, 581, 257), shift=1)
+
+
+@pytest.mark.parametrize("gradient_type", [VT.float32, VT.bfloat16])
+@pytest.mark.parametrize("E", [1, 7, 64, 65])
+def test_experts_of_very_different_loads(E, gradient_type):
+    """dW's experts take turns in classes of their rows' number: each of them once, whatever the numbers are."""
+    counts = [(700 if e % 9 == 4 else 130 if e % 5 == 2 else e % 3 * 20) for e in range(E)]
+    offsets = [3 + sum(counts[:e]) for e in range(E + 1)]
+    for shape in (1, 2, 4):
+        with cc.option(cc.Option.real_block, shape):
+            run_layer(E, offsets[-1] + 5, 70, 330, VT.bfloat16, ACT.none, offsets, gradient_type, accumulate=gradient_type == VT.float32)
