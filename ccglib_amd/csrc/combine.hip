@@ -1,8 +1,9 @@
 // Combine: out[t] = sum over j of w[t][j] y[slot[t][j]], and the way back: dy[slot] = w dout[t], dw[t][j] = <dout[t], y[slot]>.
 // Sums are 32 bits, in the order of j. A slot that is no row of y counts as a row of zeros.
 //
-// Bound by memory: a row of y is read once and used once. 64 or 256 threads have a token, 8 neighbouring columns a thread at
-// a time, and all its rows' loads are on their way together.
+// Bound by memory: a row of y is read once and used once. 64 or 256 threads have a token (up to 512 columns, and from there on), 8 neighbouring columns a
+// thread at a time, and all its rows' loads are on their way together. 4099 tokens, 2 rows of 4104 each: 17.0 us, 5.9 TB/s (part of y
+// is still in the last-level cache); the way back of 16384 tokens, 4 rows of 4096 each, with dw: 241 us, 5.0 TB/s.
 #include "linear_gemm.h"
 #include "route.h"
 
