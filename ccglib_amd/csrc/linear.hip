@@ -253,7 +253,10 @@ template <int TYPE, unsigned ROWS> __global__ __launch_bounds__(256) void linear
   }
 }
 
-__global__ __launch_bounds__(256) void join_sums(JoinArgs a) { join(a, blockIdx.x); }
+__global__ __launch_bounds__(256) void join_sums(JoinArgs a) {
+  __shared__ float lds[256];
+  join(a, lds, blockIdx.x);
+}
 
 // An operand of a product: an array of 16-bit values.
 struct Operand {
@@ -418,7 +421,7 @@ bool linear_launches(const LinearParams &p) {
   if (!p.training) return true;
   // (blocks of rows are a grid's second axis, groups too)
   const size_t columns = ceil_div(p.n, (size_t)kGradientColumns);
-  return gradient_blocks(p) <= 65535 && gradient_blocks(p) * columns <= 0xffffffu && ceil_div(p.n, (size_t)256) * p.groups <= 0xffffffu;
+  return gradient_blocks(p) <= 65535 && gradient_blocks(p) * columns <= 0xffffffu && join_workgroups(p.n, p.groups) <= 0xffffffu;
 }
 
 const char *describe_linear(const LinearParams &p, int kind) {
