@@ -178,3 +178,73 @@ def test_experts_of_very_different_loads(E, gradient_type):
     for shape in (1, 2, 4):
         with cc.option(cc.Option.real_block, shape):
             run_layer(E, offsets[-1] + 5, 70, 330, VT.bfloat16, ACT.none, offsets, gradient_type, accumulate=gradient_type == VT.float32)
+
+
+@pytest.mark.parametrize("shape", [2, 7])
+def test_two_graphs_of_one_layer_with_changing_loads(shape):
+    """They share its scratch memory and are replayed in turn; each replay takes the offsets that it finds, and gives the bits of an eager
+    run of another object."""
+    E, M, N, K, t = 5, 700, 264, 330, VT.bfloat16
+    gen = torch.Generator().manual_seed(shape)
+    side = torch.cuda.Stream()
+    with cc.option(cc.Option.real_block, shape):
+        shared = cc.GroupedLinear(E, M, N, K, 0, side.cuda_stream, t, ACT.gelu)
+        other = cc.GroupedLinear(E, M, N, K, 0, stream(), t, ACT.gelu)
+
+    def buffers():
+        ins = [torch.randn(s, generator=gen).to(HALF[t]).cuda() for s in ((M, K), (E * N, K), (M, N))]
+        outs = [torch.zeros(s, dtype=d, device="cuda") for s, d in (((M, N), HALF[t]), ((M, N), HALF[t]), ((M, K), HALF[t]),
+                                                                    ((E * N, K), torch.float32), ((E, N), torch.float32))]
+        return ins, outs, torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+
+    def run(layer, held):
+        (x, w, dy), (y, z, dx, dw, db), o = held
+        layer.Forward(x.data_ptr(), o.data_ptr(), w.data_ptr(), 0, 0, y.data_ptr(), z.data_ptr())
+        layer.Backward(dy.data_ptr(), z.data_ptr(), x.data_ptr(), o.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+
+    sets, graphs = [buffers(), buffers()], []
+    torch.cuda.synchronize()
+    for held in sets:
+        with torch.cuda.stream(side):
+            run(shared, held)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run(shared, held)
+        graphs.append(graph)
+    for spans in list(SPANS.values())[:4]:
+        for held, graph in zip(sets, graphs):
+            held[2].copy_(torch.tensor(spans(M, E), dtype=torch.int32))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            again = (held[0], [torch.zeros_like(v) for v in held[1]], held[2])
+            run(other, again)
+            torch.cuda.synchronize()
+            first, until = int(held[2][0]), int(held[2][-1])
+            for got, want in zip(held[1][:3], again[1][:3]):
+                assert torch.equal(got[first:until], want[first:until])
+            assert all(torch.equal(got, want) for got, want in zip(held[1][3:], again[1][3:]))
+
+
+@pytest.mark.parametrize("shape", [0, 1, 2, 7])
+def test_offsets_that_fall_harm_nothing_else(shape):
+    """Results are unspecified; what lies around the outputs is left alone."""
+    E, M, N, K, t = 4, 300, 70, 90, VT.bfloat16
+    gen = torch.Generator().manual_seed(4)
+    x, w, dy = (among_nan(torch.randn(s, generator=gen).to(HALF[t])) for s in ((M, K), (E * N, K), (M, N)))
+    outs = [among_nan(torch.zeros(s, dtype=d)) for s, d in (((M, N), HALF[t]), ((M, N), HALF[t]), ((M, K), HALF[t]),
+                                                            ((E * N, K), torch.float32), ((E, N), torch.float32))]
+    with cc.option(cc.Option.real_block, shape):
+        layer = cc.GroupedLinear(E, M, N, K, 0, stream(), t, ACT.silu)
+    y, z, dx, dw, db = outs
+    for offsets in ([0, 300, 0, 300, 0], [300, 200, 100, 50, 0], [-5, 2 ** 31 - 1, -2 ** 31, 299, 3]):
+        o = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        layer.Forward(x.data_ptr(), o.data_ptr(), w.data_ptr(), 0, 0, y.data_ptr(), z.data_ptr())
+        layer.Backward(dy.data_ptr(), z.data_ptr(), x.data_ptr(), o.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+        torch.cuda.synchronize()
+    for out in outs:
+        size = out.numel()
+        whole = torch.empty(0, dtype=out.dtype, device="cuda").set_(out.untyped_storage())
+        at = out.storage_offset()
+        assert bool(whole[:at].isnan().all()) and bool(whole[at + size:].isnan().all())
