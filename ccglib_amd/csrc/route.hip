@@ -5,10 +5,11 @@
 // on the order of blocks.
 //
 // A row is held by 16 lanes (64 from 257 experts on), PER neighbouring logits a lane, as whole numbers of the same order; each
-// round takes the maximum of all lanes by DPP, and the lane that holds it removes it, stores its number and counts it.
+// round takes the maximum of all lanes by DPP, and the lane that holds it removes it, stores its number and counts it. 16-bit logits have room for their
+// number beside them: nothing is removed, a round looks for the largest below the last one.
 //
 // 65536 rows of 128 float32 logits, 8 chosen of each: 19.7 us to choose (8 rounds of 47 vector instructions for 4 rows a wave, 1.8 us
-// each; 6 us would be reading the logits), 7.5 to place (13 while every block read the tiles' counts as 32 bits and in the same order,
+// each; 6 us would be reading the logits; of bfloat16 12.6, 19 instructions a round for 19.4 us with the other way), 7.5 to place (13 while every block read the tiles' counts as 32 bits and in the same order,
 // lines of one channel at a time), 14.6 for the backward pass, which is bound by memory (67 MB, 4.6 TB/s).
 #include <algorithm>
 
@@ -30,6 +31,19 @@ __device__ __forceinline__ unsigned key_of(float v) {
 __device__ __forceinline__ float value_of(unsigned key) {
   if (key == 0xffffffffu) return __builtin_nanf("");
   return __builtin_bit_cast(float, key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
+// A 16-bit value's order and, below it, its place among the logits, the first ones highest: no two are alike, so that one maximum says which logit
+// it is. 0 is below all.
+template <typename T> __device__ __forceinline__ unsigned placed_key_of(float v, unsigned place) {
+  const T narrow = (T)v;      // (exact: it was one)
+  const unsigned u = v == 0.f ? 0u : __builtin_bit_cast(unsigned short, narrow);
+  const unsigned key = v != v ? 0xffffu : u >> 15 ? ~u & 0xffffu : u | 0x8000u;
+  return key << 16 | (0xffffu - place);
+}
+template <typename T> __device__ __forceinline__ float placed_value_of(unsigned key) {
+  const unsigned u = key >> 31 ? key >> 16 & 0x7fffu : ~key >> 16;
+  return (float)__builtin_bit_cast(T, (unsigned short)u);
 }
 
 // What `join` makes of the values of all LANES (16, a DPP row, or 64) that hold a row, in each of them.
@@ -181,36 +195,60 @@ template <int TYPE, int LANES, int PER> __global__ __launch_bounds__(kThreads) v
     const unsigned next = t + kThreads / LANES;
     if (next < end) load_logits(reinterpret_cast<const T *>(a.logits) + (size_t)next * a.e, l * PER, a.e, ahead);
     unsigned keys[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) keys[i] = l * PER + i < a.e ? key_of(v[i]) : 0u;
-    unsigned my_key = 0, top_key = 0;
     const size_t at = (size_t)t * a.k;
-    for (unsigned j = 0; j < a.k; ++j) {
-      unsigned best = keys[0];
+    float top, my_value;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int i = 1; i < PER; ++i) best = larger(best, keys[i]);
-      const unsigned most = over_lanes<LANES>(best, larger);
-      // the lowest lane of the row that holds it, and its lowest logit that does
-      const unsigned long long holders = __ballot(best == most) >> (threadIdx.x & 63 & ~(LANES - 1));
-      const bool winner = l == (unsigned)__builtin_ctzll(holders);
-      bool open = winner;
-      unsigned number = 0;
+      for (int i = 0; i < PER; ++i) keys[i] = l * PER + i < a.e ? placed_key_of<T>(v[i], l * PER + i) : 0u;
+      unsigned my_key = 0, top_key = 0, last = 0;
+      for (unsigned j = 0; j < a.k; ++j) {
+        // the largest below the last one: of the differences from it, modulo 2^32, those of the keys that have been taken are the smallest
+        unsigned best = keys[0] - last;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const bool hit = open && keys[i] == most;
-        open = open && !hit;
-        keys[i] = hit ? 0u : keys[i];
-        number = hit ? i : number;
+        for (int i = 1; i < PER; ++i) best = larger(best, keys[i] - last);
+        last += over_lanes<LANES>(best, larger);
+        if (j == 0) top_key = last;
+        my_key = l == j ? last : my_key;
       }
-      if (winner) {
-        number += l * PER;
-        a.experts[at + j] = (int)number;
+      top = placed_value_of<T>(top_key);
+      my_value = placed_value_of<T>(my_key);
+      if (l < a.k) {
+        const unsigned number = 0xffffu - (my_key & 0xffffu);
+        a.experts[at + l] = (int)number;
         atomicAdd(&s.base[number], 1u);
       }
-      if (j == 0) top_key = most;
-      my_key = l == j ? most : my_key;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) keys[i] = l * PER + i < a.e ? key_of(v[i]) : 0u;
+      unsigned my_key = 0, top_key = 0;
+      for (unsigned j = 0; j < a.k; ++j) {
+        unsigned best = keys[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) best = larger(best, keys[i]);
+        const unsigned most = over_lanes<LANES>(best, larger);
+        // the lowest lane of the row that holds it, and its lowest logit that does
+        const unsigned long long holders = __ballot(best == most) >> (threadIdx.x & 63 & ~(LANES - 1));
+        const bool winner = l == (unsigned)__builtin_ctzll(holders);
+        bool open = winner;
+        unsigned number = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const bool hit = open && keys[i] == most;
+          open = open && !hit;
+          keys[i] = hit ? 0u : keys[i];
+          number = hit ? i : number;
+        }
+        if (winner) {
+          number += l * PER;
+          a.experts[at + j] = (int)number;
+          atomicAdd(&s.base[number], 1u);
+        }
+        if (j == 0) top_key = most;
+        my_key = l == j ? most : my_key;
+      }
+      top = value_of(top_key);
+      my_value = value_of(my_key);
     }
-    const float top = value_of(top_key), my_value = value_of(my_key);
     // (a row of nothing but -inf has weights of zero)
     const float over = top == -__builtin_inff() ? 0.f : top;
     const float mine = l < a.k ? __expf(my_value - over) : 0.f;

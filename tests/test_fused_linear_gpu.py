@@ -294,3 +294,11 @@ def test_every_length_of_the_sum_in_cut_blocks(K):
     with cc.option(cc.Option.real_block, 7):
         run_layer(260, 300, K, VT.bfloat16, ACT.none)
         run_layer(130, K, 520, VT.float16, ACT.none)
+
+
+@pytest.mark.parametrize("K", [1, 8, 31, 32, 33, 64, 127, 128, 129, 160, 1000, 1023, 1024, 1025, 1056, 1152, 1999, 2048, 2080, 3100])
+def test_every_length_of_the_sum_of_few_rows(K):
+    """Whole steps of all waves, the whole 32 values behind them, and the end."""
+    layer = run_layer(3, 20, K, VT.bfloat16, ACT.none)
+    assert "linear_rows" in layer.KernelName()
+    run_layer(3, 20, K, VT.float16, ACT.none, pitches=(K + 3, K + 1, 20), shift=1)

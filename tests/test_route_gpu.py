@@ -360,3 +360,36 @@ def test_the_most_tokens():
 def test_combine_beyond_32_bits():
     """Rows 8 MiB apart, 5 GB of each operand."""
     run_combine(600, 1, 40, VT.bfloat16, 610, True, 1 << 22, 1 << 22, holes=True)
+
+
+@pytest.mark.parametrize("t", list(TORCH))
+def test_the_smallest_differences(t):
+    """Neighbouring values, among them the smallest above and below zero, and both infinities: bits decide."""
+    info = torch.finfo(TORCH[t])
+    step = {VT.float16: 2.0 ** -24, VT.bfloat16: 2.0 ** -133, VT.float32: 2.0 ** -149}[t]
+    values = [0.0, -0.0, step, -step, 2 * step, -2 * step, info.tiny, -info.tiny, info.max, -info.max, math.inf, -math.inf, 1.0,
+              1.0 + info.eps, 1.0 - info.eps / 2, -1.0]
+    assert len(set(torch.tensor(values, dtype=TORCH[t]).tolist())) == len(values) - 1          # (the zeros)
+    gen = torch.Generator().manual_seed(3)
+    logits = torch.stack([torch.tensor(values, dtype=TORCH[t])[torch.randperm(len(values), generator=gen)] for _ in range(200)])
+    for k in (3, 16):
+        experts, _, offsets, slots, _, _ = run_route(logits, k, True)
+        e, _, o, s = routed(logits, k, True)
+        assert torch.equal(experts.long(), e) and offsets.tolist() == o and torch.equal(slots.long(), s)
+
+
+@pytest.mark.parametrize("t", list(HALF))
+def test_masks_and_values_that_are_not_finite_of_16_bits(t):
+    gen = torch.Generator().manual_seed(1)
+    logits = torch.randn((40, 300), generator=gen)
+    logits[:, 5:280] = -math.inf
+    logits[3] = -math.inf
+    logits[6] = torch.finfo(HALF[t]).min
+    for normalize in (True, False):
+        check_route(logits.to(HALF[t]), 16, normalize)
+        check_route(logits[:, :30].to(HALF[t]), 12, normalize)
+    logits = torch.zeros((4, 20))
+    logits[0, 7], logits[0, 3], logits[1], logits[2, 11] = math.nan, math.inf, math.nan, math.inf
+    experts, weights, _, _, _, _ = run_route(logits.to(HALF[t]), 3, True)
+    assert experts.tolist() == [[7, 3, 0], [0, 1, 2], [11, 0, 1], [0, 1, 2]]
+    assert bool(weights[:3].isnan().any(dim=1).all()) and not bool(weights[3].isnan().any())
