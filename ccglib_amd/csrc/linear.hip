@@ -344,6 +344,16 @@ hipError_t launch_product(const LinearParams &p, int kind, const Args &a, const 
   return launch_gemm<kBfloat16, kWeights>(plan.shape, grid, a, s, stream);
 }
 
+// Whether y and z are stored past the caches: where these do not hold what the product reads and writes, so that what is stored would
+// push out operands and residual that are still to be read (us, kept and past, with residual and z: 8192 x 4096 x 4096, 288 MiB, 251 and 217; 16384 x
+// 2048 x 2048, 264 MiB, 163 and 128; 8192 x 8192 x 1024 with the residual alone, 288 MiB, 191 and 155; below 256 MiB 0 to 7 % either way, and the
+// next layer finds y there). y alone, dx and dW gain nothing up to 256 MiB of their own (16383 rows over 16 experts of 4096 x 2048: 298 and 311).
+bool past_caches(const LinearParams &p, const LinearForward &f) {
+  const size_t x = (size_t)p.m * p.k, y = (size_t)p.m * p.n, w = (size_t)p.groups * p.n * p.k;
+  if (!f.z && !f.residual) return 2 * y >= kPastCachesBytes;
+  return 2 * (x + w + y * (1 + (f.z ? 1 : 0) + (f.residual ? 1 : 0))) >= kPastCachesBytes;
+}
+
 size_t dz_pitch(const LinearParams &p) { return ceil_div(p.n, (size_t)8) * 8; }
 
 // Blocks of `rows` rows of a group: as many as there can be.
@@ -445,7 +455,7 @@ hipError_t launch_linear_forward(const LinearParams &p, const LinearForward &f, 
   s.residual = static_cast<const char *>(f.residual);
   s.pitch = p.y_pitch;
   s.activation = p.activation;
-  s.past = 2 * (size_t)p.m * p.n * (f.z ? 2 : 1) >= kPastCachesBytes;
+  s.past = past_caches(p, f);
   Tails tails(p.workspace + p.tails);
   const Operand x = {f.x, p.m, p.k, p.x_pitch}, w = {f.w, (size_t)p.groups * p.n, p.k, p.w_pitch};
   Args a = product_args(p, kOutput, w, x, f.offsets, &tails);

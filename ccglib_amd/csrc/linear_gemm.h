@@ -308,7 +308,7 @@ template <typename T, int N> __device__ __forceinline__ void load_row(const T *f
 }
 
 // real::store_row, past the caches: what is more than the last-level cache holds is not in it when it is read next, and only
-// displaces operands (8192^3 with residual and z, 256 MiB of y and z: 874 us in the ordinary way, 827 past; 128 MiB: 79 and 80).
+// displaces operands (8192^3 with residual and z: 874 us in the ordinary way, 827 past).
 template <typename T, int N> __device__ __forceinline__ void store_row(bool past, T *to, unsigned left, const float (&v)[N]) {
   constexpr int E = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
   typedef T piece_t __attribute__((ext_vector_type(E)));

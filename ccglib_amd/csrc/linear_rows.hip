@@ -106,27 +106,27 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows(Args args, StoreParams
       multiply(a);
     }
   }
-  // What is left, less than a step of all waves: its whole 32 values in turn, and those of the end to the next wave. All on their way
-  // together too (one row, 4096 x 1000: 4.4 us one after the other, 3.7 like this; 8192 x 8000: 23.1 and 22.4).
+  // What is left, less than a step of all waves: its whole 32 values, two neighbours (a line of the cache) to a wave in turn, and those of the end. All on
+  // their way together too (one row, 4096 x 1000: 4.4 us one after the other, 3.7 like this; 8192 x 8000: 23.1 and 22.4).
   const unsigned left_chunks = (args.k - whole) / 32, end = whole + left_chunks * 32;
-  const bool has_end = end < args.k && wave == left_chunks % WAVES;
+  const bool has_end = end < args.k && wave == left_chunks / 2 % WAVES;
   int4_t x_end = {0, 0, 0, 0}, y_end = {0, 0, 0, 0};
   if (has_end) {
     x_end = load_8<true>(x, end + g * 8, args.k);
     y_end = load_8<true>(y, end + g * 8, args.k);
   }
-  if (wave < left_chunks) {
+  if (wave * 2 < left_chunks) {
     Values v;
 #pragma unroll
     for (unsigned c = 0; c < (unsigned)CHUNKS; ++c) {
-      const unsigned n = c * WAVES + wave;
+      const unsigned n = (c / 2 * WAVES + wave) * 2 + c % 2;
       if (n >= left_chunks) break;
       v.x[c] = load_8<false>(x, whole + n * 32 + g * 8, args.k);
       v.y[c] = load_8<false>(y, whole + n * 32 + g * 8, args.k);
     }
 #pragma unroll
     for (unsigned c = 0; c < (unsigned)CHUNKS; ++c) {
-      if (c * WAVES + wave < left_chunks) acc = mfma_one<TYPE>(v.x[c], v.y[c], acc);
+      if ((c / 2 * WAVES + wave) * 2 + c % 2 < left_chunks) acc = mfma_one<TYPE>(v.x[c], v.y[c], acc);
     }
   }
   if (has_end) acc = mfma_one<TYPE>(x_end, y_end, acc);
