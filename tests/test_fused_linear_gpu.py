@@ -302,3 +302,36 @@ def test_every_length_of_the_sum_of_few_rows(K):
     layer = run_layer(3, 20, K, VT.bfloat16, ACT.none)
     assert "linear_rows" in layer.KernelName()
     run_layer(3, 20, K, VT.float16, ACT.none, pitches=(K + 3, K + 1, 20), shift=1)
+
+
+def test_two_layers_at_once():
+    """On two streams, with parts of K joined and ends of rows copied in scratch memory of their own: the bits of one after the other."""
+    M, N, K, t = 70, 129, 4099, VT.bfloat16
+    gen = torch.Generator().manual_seed(8)
+    layers, held = [], []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        with cc.option(cc.Option.real_block, 3 + 256 * 4):
+            layers.append((cc.FusedLinear(M, N, K, 0, side.cuda_stream, t, ACT.gelu), side))
+        ins = [made(gen, r, c, t).to(HALF[t]).cuda() for r, c in ((M, K), (N, K), (M, N))]
+        outs = [torch.zeros(s, dtype=d, device="cuda") for s, d in (((M, N), HALF[t]), ((M, N), HALF[t]), ((M, K), HALF[t]),
+                                                                    ((N, K), torch.float32), ((N,), torch.float32))]
+        held.append((ins, outs))
+
+    def run(layer, both):
+        (x, w, dy), (y, z, dx, dw, db) = both
+        layer.Forward(x.data_ptr(), w.data_ptr(), 0, 0, y.data_ptr(), z.data_ptr())
+        layer.Backward(dy.data_ptr(), z.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+
+    torch.cuda.synchronize()
+    alone = []
+    for (layer, _), both in zip(layers, held):
+        run(layer, both)
+        torch.cuda.synchronize()
+        alone.append([v.clone() for v in both[1]])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (layer, _), both in zip(layers, held):
+            run(layer, both)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for want, both in zip(alone, held) for a, b in zip(want, both[1]))
