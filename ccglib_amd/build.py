@@ -15,15 +15,16 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB_PATH = os.path.join(HERE, "libccglib_amd.so")
-# (gemm_mfma.hip is compiled in parts, one per input type, and type of C for 16 bits, so that they build in parallel; those that
-# take longest come first)
-SOURCES = ["gemm_mfma_f16_f32.hip", "gemm_mfma_bf16_f32.hip", "gemm_mfma_f16_f16.hip", "gemm_mfma_bf16_bf16.hip",
-           "gemm_mfma_f32.hip", "gemm_mfma_fp8.hip", "scaled_gemm_rows.hip", "scaled_gemm_blocks.hip",
-           "scaled_gemm_e8m0.hip", "scaled_gemm_wide_rows.hip", "scaled_gemm_wide_blocks.hip",
-           "scaled_gemm_wide_e8m0.hip", "orthogonalize.hip", "quantize.hip", "linear_f16_output.hip",
-           "linear_bf16_output.hip", "linear_f16_input.hip", "linear_bf16_input.hip", "linear_f16_weights.hip",
-           "linear_bf16_weights.hip", "linear_f16_backward.hip",
-           "linear_bf16_backward.hip", "linear_rows.hip", "gemm_mfma_int1.hip", "transpose.hip", "combine.hip", "route.hip", "linear.hip",
+# (gemm_mfma.hip is compiled in parts, one per input type, and type of C and kind of rows for 16 bits, so that they build in
+# parallel; those that take longest come first)
+SOURCES = ["gemm_mfma_f16_f32.hip", "gemm_mfma_bf16_f32.hip", "gemm_mfma_f32.hip", "gemm_mfma_f16_f16.hip",
+           "gemm_mfma_bf16_bf16.hip", "gemm_mfma_fp8.hip", "gemm_mfma_f16_f32_pairs.hip", "gemm_mfma_bf16_f32_pairs.hip",
+           "gemm_mfma_f16_f16_pairs.hip", "gemm_mfma_bf16_bf16_pairs.hip", "scaled_gemm_e8m0.hip", "scaled_gemm_wide_rows.hip",
+           "scaled_gemm_wide_blocks.hip", "scaled_gemm_wide_e8m0.hip", "quantize.hip", "scaled_gemm_rows.hip",
+           "scaled_gemm_blocks.hip", "orthogonalize.hip", "linear_f16_output.hip",
+           "linear_bf16_output.hip", "linear_f16_weights.hip", "linear_bf16_weights.hip", "linear_f16_input.hip",
+           "linear_bf16_input.hip", "gemm_mfma_int1.hip", "linear_f16_backward.hip",
+           "linear_bf16_backward.hip", "linear_rows.hip", "transpose.hip", "combine.hip", "route.hip", "linear.hip",
            "gemm_int1.hip", "packing.hip", "capi.hip", "operators_capi.hip", "linear_capi.hip", "scaled_gemm.hip",
            "gemm_mfma_dispatch.hip", "host_copy.hip"]
 # Packed-fp32 instruction selection is switched off for all device code.
@@ -43,6 +44,22 @@ def _defines():
 
 def _hipcc():
     return shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+
+
+def _jobs():
+    """How many sources are compiled at a time: a processor each, and not more than 16 (one takes up to 0.6 GB)."""
+    return max(1, min(16, len(os.sched_getaffinity(0)), len(SOURCES)))
+
+
+def _run(cmd):
+    """Runs the compiler or the linker. One that ends without an error in the source to report (it was killed, or ran out of
+    something) is run once more; what it said the first time stays in the output."""
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0 and not re.search(r"^\S+:\d+(:\d+)?: (fatal )?error:|undefined symbol|undefined reference", r.stdout + r.stderr, re.M):
+        again = subprocess.run(cmd, capture_output=True, text=True)
+        again.stderr = "%s\nended with status %d and was run again\n%s" % ((r.stdout + r.stderr).rstrip(), r.returncode, again.stderr)
+        return again
+    return r
 
 
 def _stale(target, deps):
@@ -79,7 +96,7 @@ def _compile(src, force):
         return obj, ""
     cmd = [_hipcc()] + HIPCC_FLAGS + _defines() + ["-Rpass-analysis=kernel-resource-usage", "-c", path,
                                                    "-o", obj]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    r = _run(cmd)
     lines = (r.stdout + r.stderr).splitlines()
     kept, includes, skip = [], [], 0
     for l in lines:      # (the remarks, each with its source line, caret and includes, stay out of the log)
@@ -130,7 +147,7 @@ def build(force=False, verbose=False):
     upon which nothing further is started."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     began = time.monotonic()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=_jobs()) as ex:
         sources = {ex.submit(_compile, s, force): s for s in SOURCES}
         for done in concurrent.futures.as_completed(sources):
             try:
@@ -147,7 +164,7 @@ def build(force=False, verbose=False):
     objs = [_object(s) for s in SOURCES]
     if force or _stale(LIB_PATH, objs):
         cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
-        r = subprocess.run(cmd, capture_output=True, text=True)
+        r = _run(cmd)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     return LIB_PATH

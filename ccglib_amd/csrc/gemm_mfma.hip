@@ -3209,7 +3209,10 @@ inline bool waves_share_k(const GemmParams &p) {
   const size_t tiles = (size_t)p.batch * ceil_div(p.nx, 32) * ceil_div(p.ny, 32);
   return p.type_in == kInt1 && p.k_tiles > 1 && tiles <= 3 * (size_t)compute_units();
 }
-template <int DT, int TOUT>
+// Which input a translation unit has the kernels for (see the end of this file): rows of (re, im) pairs, what is not such, or both.
+enum Rows { kAnyRows, kPairRows, kOtherRows };
+
+template <int DT, int TOUT, Rows ROWS = kAnyRows>
 hipError_t launch_waves(const GemmParams &p, WaveShape shape, hipStream_t stream) {
   auto launch = [&](auto loader) {
     constexpr int L = decltype(loader)::value;
@@ -3222,11 +3225,14 @@ hipError_t launch_waves(const GemmParams &p, WaveShape shape, hipStream_t stream
     }
     return launch_wave<DT, TOUT, L, 2, 2>(p, stream);
   };
-  if constexpr (DT != kInt1) {
+  if constexpr (DT != kInt1 && ROWS != kOtherRows) {
     if (p.input_interleaved) return launch(std::integral_constant<int, kLoadInterleavedRagged>{});
   }
-  if (p.variant == kOpt) return launch(std::integral_constant<int, kLoadTiled>{});
-  return launch(std::integral_constant<int, kLoadPlanarRagged>{});
+  if constexpr (ROWS != kPairRows) {
+    if (p.variant == kOpt) return launch(std::integral_constant<int, kLoadTiled>{});
+    return launch(std::integral_constant<int, kLoadPlanarRagged>{});
+  }
+  return hipErrorInvalidValue;
 }
 
 // 128 x 128 blocks (16-bit input: of eight or four waves, see block_choice).
@@ -3244,11 +3250,11 @@ hipError_t launch_128x128(const GemmParams &p, hipStream_t stream) {
   }
 }
 
-template <int DT, int TOUT>
+template <int DT, int TOUT, Rows ROWS = kAnyRows>
 hipError_t launch_typed(const GemmParams &p, hipStream_t stream) {
   if constexpr (DT != kFloat32) {
     const WaveShape waves = wave_choice(p);
-    if (waves != kNoWaves) return launch_waves<DT, TOUT>(p, waves, stream);
+    if (waves != kNoWaves) return launch_waves<DT, TOUT, ROWS>(p, waves, stream);
   }
   constexpr int KPM = DtypeTraits<DT>::kTilesPerMfma;
   const size_t k_bytes = (size_t)p.k * bits_of(p.type_in) / 8;
@@ -3281,87 +3287,96 @@ hipError_t launch_typed(const GemmParams &p, hipStream_t stream) {
     if (k_bytes >= 16) return launch(std::integral_constant<int, kLoadPlanarRagged>{});
   }
   else if (p.input_interleaved) {
-    // raw (re, im) rows straight from the caller: the host side only takes this
-    // path for rows of at least 16 bytes
-    const bool ragged = 2 * k_bytes % 16 != 0 || (uintptr_t)p.x % 16 != 0 || (uintptr_t)p.y % 16 != 0;
-    if (ragged && 2 * k_bytes < 16) return hipErrorInvalidValue;
-    if (ragged) {
-      if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedRagged, MS>(p, stream);
-      if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedRagged>(p, stream);
-      return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedRagged, MS>(p, stream);
-    } else if constexpr (BITS16) {
-      if (wide_tiles_apply(p) && wide_tiles_pay(p)) return launch_wide<DT, TOUT, true>(p, stream);
-      if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedVec>(p, stream);
-      if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedVec>(p, stream);
-      return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedVec>(p, stream);
-    } else {
-      if (shape == k64x64) {
-        return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedVec, 32>(p, stream);
-      }
-      if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedVec>(p, stream);
-      return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedVec, 32>(p, stream);
-    }
-  }
-  else if (p.variant == kOpt || planar_direct) {
-    if constexpr (BITS16) {
-      // 16-bit input, tiled operands, planar C without beta: 192 x 256 block, 4 waves
-      // of 192 x 64 (one per SIMD), where that pays
-      if (wide_tiles_apply(p) && wide_tiles_pay(p)) return launch_wide<DT, TOUT>(p, stream);
-    }
-    if constexpr (BITS16) {
-      // 16-bit input: 256 x 128 block, 8 waves of 64 x 64 (two per SIMD), 3-slot ring.
-      // Interleaved fp32 C: in the exchanged-roles layout a lane's (re, im) pairs of
-      // a row lie 32 bytes apart, so every store instruction would write half
-      // cache lines; the other layout regroups the tile through LDS into whole
-      // rows of pairs (measured 5 % faster at B=64 512x4096x576).
-      if constexpr (TOUT == kFloat32) {
-        if (p.variant == kOpt && p.c_interleaved && shape == k256x128) {
-          return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 16, false>(p, stream);
+    if constexpr (ROWS != kOtherRows) {
+      // raw (re, im) rows straight from the caller: the host side only takes this
+      // path for rows of at least 16 bytes
+      const bool ragged = 2 * k_bytes % 16 != 0 || (uintptr_t)p.x % 16 != 0 || (uintptr_t)p.y % 16 != 0;
+      if (ragged && 2 * k_bytes < 16) return hipErrorInvalidValue;
+      if (ragged) {
+        if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedRagged, MS>(p, stream);
+        if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedRagged>(p, stream);
+        return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedRagged, MS>(p, stream);
+      } else if constexpr (BITS16) {
+        if (wide_tiles_apply(p) && wide_tiles_pay(p)) return launch_wide<DT, TOUT, true>(p, stream);
+        if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedVec>(p, stream);
+        if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedVec>(p, stream);
+        return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedVec>(p, stream);
+      } else {
+        if (shape == k64x64) {
+          return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadInterleavedVec, 32>(p, stream);
         }
+        if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadInterleavedVec>(p, stream);
+        return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadInterleavedVec, 32>(p, stream);
       }
-      // problems too small to give every compute unit a 256 x 128 tile: 128 x 128
-      // blocks (launch_128x128), or 64 x 64 blocks, 4 waves of 32 x 32,
-      // 5-slot ring, two blocks a unit
-      if (shape == k64x64) {
+    }
+    return hipErrorInvalidValue;
+  }
+  else if constexpr (ROWS != kPairRows) {
+    if (p.variant == kOpt || planar_direct) {
+      if constexpr (BITS16) {
+        // 16-bit input, tiled operands, planar C without beta: 192 x 256 block, 4 waves
+        // of 192 x 64 (one per SIMD), where that pays
+        if (wide_tiles_apply(p) && wide_tiles_pay(p)) return launch_wide<DT, TOUT>(p, stream);
+      }
+      if constexpr (BITS16) {
+        // 16-bit input: 256 x 128 block, 8 waves of 64 x 64 (two per SIMD), 3-slot ring.
+        // Interleaved fp32 C: in the exchanged-roles layout a lane's (re, im) pairs of
+        // a row lie 32 bytes apart, so every store instruction would write half
+        // cache lines; the other layout regroups the tile through LDS into whole
+        // rows of pairs (measured 5 % faster at B=64 512x4096x576).
+        if constexpr (TOUT == kFloat32) {
+          if (p.variant == kOpt && p.c_interleaved && shape == k256x128) {
+            return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 16, false>(p, stream);
+          }
+        }
+        // problems too small to give every compute unit a 256 x 128 tile: 128 x 128
+        // blocks (launch_128x128), or 64 x 64 blocks, 4 waves of 32 x 32,
+        // 5-slot ring, two blocks a unit
+        if (shape == k64x64) {
+          return p.variant == kOpt
+                     ? launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadTiled, 16>(p, stream)
+                     : launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarVec, 16>(p, stream);
+        }
+        if (shape == k128x128) {
+          return p.variant == kOpt ? launch_128x128<DT, TOUT, kLoadTiled>(p, stream)
+                                   : launch_128x128<DT, TOUT, kLoadPlanarVec>(p, stream);
+        }
         return p.variant == kOpt
-                   ? launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadTiled, 16>(p, stream)
-                   : launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarVec, 16>(p, stream);
-      }
-      if (shape == k128x128) {
-        return p.variant == kOpt ? launch_128x128<DT, TOUT, kLoadTiled>(p, stream)
-                                 : launch_128x128<DT, TOUT, kLoadPlanarVec>(p, stream);
-      }
-      return p.variant == kOpt
-                 ? launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 16, true>(p, stream)
-                 : launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarVec, 16, true>(p, stream);
-    } else {
-      // fp8: the 32x32x64 MFMA takes one K tile per instruction, which lets the
-      // same block shape and ring as for 16-bit input fit into LDS
-      // (small problems: 128 x 128 blocks, 4 waves of 64 x 64, or 64 x 64 blocks, 4 waves
-      // of 32 x 32; two blocks a unit)
-      if (shape == k64x64) {
+                   ? launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 16, true>(p, stream)
+                   : launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarVec, 16, true>(p, stream);
+      } else {
+        // fp8: the 32x32x64 MFMA takes one K tile per instruction, which lets the
+        // same block shape and ring as for 16-bit input fit into LDS
+        // (small problems: 128 x 128 blocks, 4 waves of 64 x 64, or 64 x 64 blocks, 4 waves
+        // of 32 x 32; two blocks a unit)
+        if (shape == k64x64) {
+          return p.variant == kOpt
+                     ? launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadTiled, 32>(p, stream)
+                     : launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarVec, 32>(p, stream);
+        }
+        if (shape == k128x128) {
+          return p.variant == kOpt ? launch_128x128<DT, TOUT, kLoadTiled>(p, stream)
+                                   : launch_128x128<DT, TOUT, kLoadPlanarVec>(p, stream);
+        }
         return p.variant == kOpt
-                   ? launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadTiled, 32>(p, stream)
-                   : launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarVec, 32>(p, stream);
+                   ? launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 32>(p, stream)
+                   : launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarVec, 32>(p, stream);
       }
-      if (shape == k128x128) {
-        return p.variant == kOpt ? launch_128x128<DT, TOUT, kLoadTiled>(p, stream)
-                                 : launch_128x128<DT, TOUT, kLoadPlanarVec>(p, stream);
-      }
-      return p.variant == kOpt
-                 ? launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadTiled, 32>(p, stream)
-                 : launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarVec, 32>(p, stream);
+    }
+    else if (k_bytes >= 16) {
+      if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarRagged, MS>(p, stream);
+      if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadPlanarRagged>(p, stream);
+      return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarRagged, MS, BITS16>(p, stream);
     }
   }
-  else if (k_bytes >= 16) {
-    if (shape == k64x64) return launch_dtl<DT, TOUT, 64, 64, 32, 32, 5, 2, kLoadPlanarRagged, MS>(p, stream);
-    if (shape == k128x128) return launch_128x128<DT, TOUT, kLoadPlanarRagged>(p, stream);
-    return launch_block<DT, TOUT, 256, 128, 64, 64, 3, 2, kLoadPlanarRagged, MS, BITS16>(p, stream);
+  if constexpr (ROWS == kPairRows) {
+    return hipErrorInvalidValue;
+  } else {
+    // fp8 stages are twice as large (two K tiles per MFMA): one wave per SIMD
+    // with the full register file
+    constexpr int WPE = (KPM == 2) ? 1 : 2;
+    return launch_config<DT, TOUT, 128, 128, 64, 64, KPM, kLoadPlanarElem, WPE>(p, stream);
   }
-  // fp8 stages are twice as large (two K tiles per MFMA): one wave per SIMD
-  // with the full register file
-  constexpr int WPE = (KPM == 2) ? 1 : 2;
-  return launch_config<DT, TOUT, 128, 128, 64, 64, KPM, kLoadPlanarElem, WPE>(p, stream);
 }
 
 }  // namespace
@@ -3369,42 +3384,66 @@ hipError_t launch_typed(const GemmParams &p, hipStream_t stream) {
 // The instantiations are spread over several translation units so that they
 // compile in parallel: gemm_mfma_<part>.hip define CCGLIB_GEMM_MFMA_PART and
 // include this file (1 fp16, 2 bf16, both with fp32 C; 6 fp16, 7 bf16, both with C of
-// the same type; 3 fp32, 4 fp8, 5 1-bit input; 0 the dispatch below). Included without the
-// macro, the file holds everything.
+// the same type; 8 to 11 the same four for rows of pairs; 3 fp32, 4 fp8, 5 1-bit input;
+// 0 the dispatch below). Included without the macro, the file holds everything.
 #ifndef CCGLIB_GEMM_MFMA_PART
 #define CCGLIB_GEMM_MFMA_PART -1
 #endif
 #define CCGLIB_GEMM_MFMA_HAS(part) (CCGLIB_GEMM_MFMA_PART == -1 || CCGLIB_GEMM_MFMA_PART == (part))
 
 hipError_t launch_gemm_mfma_f16_f32(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_f16_f32_pairs(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_f16_f16(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_f16_f16_pairs(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_bf16_f32(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_bf16_f32_pairs(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_bf16_bf16(const GemmParams &p, hipStream_t stream);
+hipError_t launch_gemm_mfma_bf16_bf16_pairs(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_f32(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_fp8(const GemmParams &p, hipStream_t stream);
 hipError_t launch_gemm_mfma_int1(const GemmParams &p, hipStream_t stream);
 
 #if CCGLIB_GEMM_MFMA_HAS(1)
 hipError_t launch_gemm_mfma_f16_f32(const GemmParams &p, hipStream_t stream) {
-  return launch_typed<kFloat16, kFloat32>(p, stream);
+  return launch_typed<kFloat16, kFloat32, kOtherRows>(p, stream);
+}
+#endif
+#if CCGLIB_GEMM_MFMA_HAS(8)
+hipError_t launch_gemm_mfma_f16_f32_pairs(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kFloat16, kFloat32, kPairRows>(p, stream);
 }
 #endif
 
 #if CCGLIB_GEMM_MFMA_HAS(6)
 hipError_t launch_gemm_mfma_f16_f16(const GemmParams &p, hipStream_t stream) {
-  return launch_typed<kFloat16, kFloat16>(p, stream);
+  return launch_typed<kFloat16, kFloat16, kOtherRows>(p, stream);
+}
+#endif
+#if CCGLIB_GEMM_MFMA_HAS(10)
+hipError_t launch_gemm_mfma_f16_f16_pairs(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kFloat16, kFloat16, kPairRows>(p, stream);
 }
 #endif
 
 #if CCGLIB_GEMM_MFMA_HAS(2)
 hipError_t launch_gemm_mfma_bf16_f32(const GemmParams &p, hipStream_t stream) {
-  return launch_typed<kBfloat16, kFloat32>(p, stream);
+  return launch_typed<kBfloat16, kFloat32, kOtherRows>(p, stream);
+}
+#endif
+#if CCGLIB_GEMM_MFMA_HAS(9)
+hipError_t launch_gemm_mfma_bf16_f32_pairs(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kBfloat16, kFloat32, kPairRows>(p, stream);
 }
 #endif
 
 #if CCGLIB_GEMM_MFMA_HAS(7)
 hipError_t launch_gemm_mfma_bf16_bf16(const GemmParams &p, hipStream_t stream) {
-  return launch_typed<kBfloat16, kBfloat16>(p, stream);
+  return launch_typed<kBfloat16, kBfloat16, kOtherRows>(p, stream);
+}
+#endif
+#if CCGLIB_GEMM_MFMA_HAS(11)
+hipError_t launch_gemm_mfma_bf16_bf16_pairs(const GemmParams &p, hipStream_t stream) {
+  return launch_typed<kBfloat16, kBfloat16, kPairRows>(p, stream);
 }
 #endif
 
@@ -3526,13 +3565,16 @@ const char *describe_gemm_mfma(const GemmParams &p) {
 }
 
 hipError_t launch_gemm_mfma(const GemmParams &p, hipStream_t stream) {
+  const bool pairs = p.input_interleaved;
   switch (p.type_in) {
     case kFloat16:
-      if (p.type_out == kFloat32) return launch_gemm_mfma_f16_f32(p, stream);
-      return p.type_out == kFloat16 ? launch_gemm_mfma_f16_f16(p, stream) : hipErrorInvalidValue;
+      if (p.type_out == kFloat32) return pairs ? launch_gemm_mfma_f16_f32_pairs(p, stream) : launch_gemm_mfma_f16_f32(p, stream);
+      if (p.type_out != kFloat16) return hipErrorInvalidValue;
+      return pairs ? launch_gemm_mfma_f16_f16_pairs(p, stream) : launch_gemm_mfma_f16_f16(p, stream);
     case kBfloat16:
-      if (p.type_out == kFloat32) return launch_gemm_mfma_bf16_f32(p, stream);
-      return p.type_out == kBfloat16 ? launch_gemm_mfma_bf16_bf16(p, stream) : hipErrorInvalidValue;
+      if (p.type_out == kFloat32) return pairs ? launch_gemm_mfma_bf16_f32_pairs(p, stream) : launch_gemm_mfma_bf16_f32(p, stream);
+      if (p.type_out != kBfloat16) return hipErrorInvalidValue;
+      return pairs ? launch_gemm_mfma_bf16_bf16_pairs(p, stream) : launch_gemm_mfma_bf16_bf16(p, stream);
     case kFloat32: return launch_gemm_mfma_f32(p, stream);
     case kFloat8e4m3:
     case kFloat8e5m2: return launch_gemm_mfma_fp8(p, stream);
