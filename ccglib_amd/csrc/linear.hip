@@ -154,18 +154,36 @@ bool plan_together(LinearParams *p) {
   return best > 0.0;
 }
 
-// Whether y is linear_rows.hip's. Its blocks of 16 x 16 read their operands from the caches again and again, but wait for no ring. us,
-// linear_rows and gemm_linear: single rows of x, bound by W's bytes, 24.8 and 30.1 (8192 x 8192 out of memory; 12 rows of 8192 x 4096
-// 17.1 and 15.6); small products, bound by their launch, 4.3 and 7.7 (64 x 255 x 1000), 6.6 and 7.9 (300 x 577 x 1000), then 12.1 and 8.1
-// (128 x 4096 x 1000); many blocks with little K 6.4 and 5.0 (128 x 4096 x 256). Rows that are not whole chunks are read in halves:
-// 59 and 33 (1 x 8191 x 8191), 5.0 and 6.7 (1 x 1000 x 577). Each expert's W is read for every 16 of its rows: 16 rows over 64 experts of
-// 2048 x 2048 18 and 22, 128 rows 75 to 84 and 84, 256 rows 93 to 98 and 92.
+// Blocks of `rows` rows of a group: as many as there can be.
+size_t row_blocks(const LinearParams &p, size_t rows) {
+  if (!p.grouped) return ceil_div(p.m, rows);
+  const size_t some = std::min<size_t>(p.groups, p.m);
+  return some + (p.m - some) / rows;
+}
+// Blocks of linear_rows.hip: as many as there can be.
+size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, kRowsOfX); }
+
+// Whether y is linear_rows.hip's. Its blocks of 16 x 16 read their operands from the caches again and again, but wait for no ring: about 2.6 us and
+// 1.7 for each 1024 of K and 256 blocks, where gemm_linear takes 3.9 and 3.4 for 1024 of K whatever the blocks. us, linear_rows and gemm_linear, W
+// in the caches (W out of memory):
+//   up to 256 blocks    16 x 4096 x 4096 10.1 and 12.3 (12.6 and 13.4); K = 6144 14.0 and 14.5 (18.4 and 16.4)
+//   512                 16 x 8192 x 2048 10.0 and 10.8 (11.8 and 11.8); 128 x 1000 x 3000 13.0 and 11.4 (14.0 and 11.7)
+//   768                 128 x 1280 x 768 6.5 and 6.8 (6.7 and 6.8); x 1000 5.8 and 7.5; x 1024 7.8 and 7.5; x 1536 10.4 and 9.8
+//   1024                256 x 1024 x 256 4.4 and 4.6; x 512 6.2 and 6.1 (6.3 and 6.0); x 768 8.0 and 6.9
+//   1280                128 x 2560 x 256 (5.2 and 4.9); of experts, whose rows fill fewer blocks as a rule: 256 rows over 64 of 256 x 256 (5.2 and 5.3)
+// Up to four rows with long sums are bound by W's bytes: 8192 x 8192 24.8 and 30.1 (27.4 and 27.7). Rows that are not whole chunks are read in halves:
+// 59 and 33 (1 x 8191 x 8191), 5.0 and 6.7 (1 x 1000 x 577).
+// An expert's W is read for every 16 of its rows, and how many it has is not known here. Up to 16 rows in all read it once: 16 over 64 experts of 2048 x 2048
+// 24.5 and 22.0 where each has its own, 7.4 and 11.2 where one has all; over 16 of 4096 x 4096 90 and 102, 12.2 and 17.3. More rows of large W would be 5 % faster with
+// usual loads and as many times slower as an expert has 16 of them: 256 over 128 of 4096 x 4096 634 and 656, all to one 142 and 40 (8192 x 8192 507 and 65);
+// over 1024 of 512 x 512 100 and 71, all to one 57 and 31.
 bool plan_few_rows(const LinearParams &p) {
   if (real_block_option) return false;
-  const double rows = p.m, outputs = rows * p.n, products = outputs * p.k;
+  const double rows = p.m, products = rows * p.n * p.k;
   if (p.x_pitch % 8 || p.w_pitch % 8) return products <= 10e6;
-  if (p.grouped ? p.m <= 2 * p.groups : p.m <= 4 && rows * p.k <= 32768) return true;
-  return outputs <= 262144 && products <= (p.grouped ? 100e6 : 175e6);
+  if (p.grouped ? p.m <= (unsigned)kRowsOfX : p.m <= 4 && rows * p.k <= 32768) return true;
+  const size_t rounds = ceil_div(few_rows_blocks(p), (size_t)kUnits);
+  return rounds <= (p.grouped ? 5 : 4) && rounds * rounds * p.k <= 10000 && p.k <= 5000;
 }
 
 // ---- before the products of the backward pass ----
@@ -356,12 +374,6 @@ bool past_caches(const LinearParams &p, const LinearForward &f) {
 
 size_t dz_pitch(const LinearParams &p) { return ceil_div(p.n, (size_t)8) * 8; }
 
-// Blocks of `rows` rows of a group: as many as there can be.
-size_t row_blocks(const LinearParams &p, size_t rows) {
-  if (!p.grouped) return ceil_div(p.m, rows);
-  const size_t some = std::min<size_t>(p.groups, p.m);
-  return some + (p.m - some) / rows;
-}
 unsigned gradient_rows(const LinearParams &p) {
   return row_blocks(p, kManyRows) * ceil_div(p.n, (size_t)kGradientColumns) < 512 ? kFewRows : kManyRows;
 }
@@ -376,9 +388,6 @@ template <unsigned ROWS> hipError_t launch_gradient(const LinearParams &p, const
   }
   return hipGetLastError();
 }
-// Blocks of linear_rows.hip: as many as there can be.
-size_t few_rows_blocks(const LinearParams &p) { return linear_rows_blocks(p.n) * row_blocks(p, kRowsOfX); }
-
 }  // namespace
 
 void plan_linear(LinearParams *p) {
