@@ -444,14 +444,16 @@ bool linear_launches(const LinearParams &p) {
 }
 
 const char *describe_linear(const LinearParams &p, int kind) {
-  static thread_local char name[96];
+  static thread_local char name[128];
   if (kind == kOutput && p.few_rows) {
     snprintf(name, sizeof name, "linear_rows<%s>", p.type == kFloat16 ? "float16" : "bfloat16");
     return name;
   }
   static const char *const kinds[] = {"forward", "input's gradient", "weights' gradient"};
-  snprintf(name, sizeof name, "gemm_linear<%s, %s> %s block, K in %u", p.type == kFloat16 ? "float16" : "bfloat16", kinds[kind],
-           kShapes[p.plan[kind].shape].name, p.plan[kind].parts);
+  const bool together = kind != kOutput && p.together;
+  snprintf(name, sizeof name, "gemm_linear%s<%s, %s> %s block, K in %u%s", together ? "_backward" : "",
+           p.type == kFloat16 ? "float16" : "bfloat16", kinds[kind], kShapes[p.plan[kind].shape].name, p.plan[kind].parts,
+           together ? ", dx and dW in one launch" : "");
   return name;
 }
 
