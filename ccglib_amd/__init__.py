@@ -426,7 +426,8 @@ class FusedLinear(_Handle):
 
     def Backward(self, d_dy, d_z, d_x, d_w, d_dx, d_dw, d_dbias=0, accumulate=False):
         """dz = dy act'(z), dx = dz W, dW (+)= dz^T x, dbias (+)= column sums of dz; 0 for a gradient
-        that is not wanted. dW and dbias are of gradient_type; accumulate: of float32 only."""
+        that is not wanted. dW and dbias are of gradient_type; accumulate: of float32 only. Behind an
+        activation dz is rounded to 16 bits for dx and dW."""
         status = self._lib.ccglib_fused_linear_backward(self._h, int(d_dy), int(d_z), int(d_x), int(d_w),
             int(d_dx), int(d_dw), int(d_dbias), int(bool(accumulate)))
         if status:

@@ -463,12 +463,20 @@ typedef struct ccglib_combine *ccglib_combine_t;
  * (the residual's gradient is dy). bias, residual and z may be null: z is
  * stored where the backward pass is to have it; without an activation that
  * needs none. act is taken of the sum before z is rounded, act' of the z that
- * was stored. dz is rounded to 16 bits, as the matrix instructions want it,
- * dbias is summed without that. dx, dw, dbias: null if not wanted. dw and dbias are of
+ * was stored (relu' is 0 where z is NaN, whose act is NaN). Behind an activation dz is
+ * rounded to 16 bits, as the matrix instructions want it: up to 2^-8 of its value
+ * (bfloat16; float16 2^-11) in dx and dW, also where dW is float32; dbias is summed
+ * without that. dx, dw, dbias: null if not wanted. dw and dbias are of
  * gradient_type, the values' type or float32; float32 ones may be added to
  * (accumulate). training = 0: forward only. x_pitch, w_pitch, y_pitch:
  * elements between rows of x and dx, of W and dW, of y, z, residual and dy (0: K, K, N).
- * kernel_name, product 0 to 2: that of y, of dx, of dW. */
+ * kernel_name, product 0 to 2: that of y, of dx, of dW (small ones are one launch,
+ * where both are wanted).
+ * Up to 2^31 - 1 rows, N, K and distances up to 2^22; for training 65535 blocks of
+ * 64 rows (4.1 million rows; an expert's last block may hold one). A layer for training holds
+ * dz, 2 M N bytes, if it has an activation, and the sums of dbias, 4 N bytes a block of 64 rows (of 16
+ * where there are few). They live for one backward call: forward and backward share nothing but
+ * what the caller hands them. */
 CCGLIB_API int ccglib_fused_linear_create(ccglib_fused_linear_t *linear, size_t M, size_t N, size_t K, int device, void *stream,
                                           int type, int activation, int gradient_type, int training, size_t x_pitch,
                                           size_t w_pitch, size_t y_pitch);

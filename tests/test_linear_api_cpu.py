@@ -61,3 +61,17 @@ def test_null_handles_are_errors_not_crashes():
     assert lib.ccglib_combine_create(None, 1, 1, 1, 0, None, 2, 0, 0, 0) != 0
     for name in ("fused_linear", "grouped_linear", "route", "combine"):
         assert getattr(lib, "ccglib_%s_destroy" % name)(None) == 0
+
+
+@pytest.mark.parametrize("make,rows", [(lambda **a: cc.FusedLinear(**a), 65535 * 64),
+                                       (lambda **a: cc.GroupedLinear(E=4, **a), 65535 * 64 - 4 * 63)])
+def test_rows_of_a_layer_for_training(make, rows):
+    """65535 blocks of 64 rows, the last of each expert with a single one; a layer that has no backward pass takes more."""
+    def refused(**change):
+        try:
+            make(**(dict(M=rows, N=8, K=8, device=0, stream=0) | change))
+        except RuntimeError as e:
+            return "more blocks than a launch" in str(e)
+        return False
+    assert not refused() and not refused(M=rows + 1, training=False)
+    assert refused(M=rows + 64)
