@@ -12,7 +12,8 @@
 //   k contiguous: rows of 128 bytes, chunk c (16 bytes) of row r at c ^ (r & 7); a lane reads its 8 values at once.
 //   k strided: 64 rows of k, the block's columns of each; a 16x16x32 fragment, which wants 8 values along k in a lane,
 //   is read by ds_read_b64_tr_b16, which transposes 4 x 16 values inside 16 lanes. Pieces of the columns are XORed with
-//   bits of k, so that the 4 rows that 16 lanes read lie in different banks.
+//   bits of k, so that the 4 rows that 16 lanes read lie in different banks. 32 lanes read at a time: those of Y, and of X in pieces of 32 bytes
+//   (192 columns), all in different banks; those of X in pieces of 64 bytes, of which a read takes half, two in each of 32 banks.
 // X supplies the instruction's rows, in an order that leaves a lane with 4 NT neighbours in x: wide stores.
 //
 // Ends. Rows beyond an operand are clamped (their sums are never stored), k beyond the end reads zeros. Where a row along k
@@ -23,7 +24,8 @@
 //
 // What bounds it. 8192^3 takes 765 to 805 us in each of the three products (1370 to 1440 TFLOP/s): matrix instructions are busy 67 % of the cycles, at
 // 1.95 to 2.0 GHz; without its copies it would be 646, without the barrier 749. A wave's 128 x 64 of a 256 x 256 block read 96 bytes of LDS
-// a cycle and unit, of 128 that there are; 64 x 64 of the smaller blocks would read 128, which is why they are only for what 256 x 256 leaves idle. A
+// a cycle of matrix instructions and unit, of 128 that there are; 64 x 64 of the smaller blocks would read 128, which is why they are only for what 256 x 256 leaves
+// idle. In dx and dW X's reads take twice their time (40 % of LDS's busy cycles, which are 1.7 times y's), as 160 bytes would: 107 a cycle at 67 %. A
 // block's start and stores take 9 us (12 with an activation) of a round that multiplies 1.5 us a piece: one block a unit, nothing
 // runs beside them. Two blocks of 256 x 128 a unit, in pieces of 32 values, hide them and are slower all the same (8192^3 992; 4096 rows over 32
 // experts of 1024 x 2048 38 for 35).
@@ -246,8 +248,9 @@ template <int KIND, int BY, bool CUT> __device__ __forceinline__ Place place(con
   return p;
 }
 
-// Bits of k that the number of a unit (32 or 64 bytes of columns) is XORed with, for rows of ROW bytes: the 4 rows (and, in steps of 8, the
-// next 16 lanes' 4) that are read together start in different banks (256 bytes of them).
+// Bits of k that the number of a unit (32 or 64 bytes of columns) is XORed with, for rows of ROW bytes: the 4 rows that 16 lanes read
+// start in different banks (256 bytes of them). The next 16 lanes' 4, in steps of 8, lie in the other banks with units of 32 bytes; with units
+// of 64 they lie in the same ones, two ways: a read takes 8 of each 16 bytes, and so half of the banks whatever the order of units.
 template <int ROW, int UNIT> __device__ __forceinline__ unsigned unit_swizzle(unsigned k) {
   if constexpr (ROW % 256 == 0) return UNIT == 32 ? (k & 3) | (k >> 3 & 1) << 2 : k & 3;
   if constexpr (ROW % 128 == 0) return UNIT == 32 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : k >> 1 & 1;
